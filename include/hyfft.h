@@ -289,6 +289,86 @@ HYFFT_API int hyfft_siren_backward(const hyfft_siren_desc* d, const float* coord
                                    float* d_pe_b, float* d_hid_w, float* d_hid_b, float* d_out_w, float* d_out_b,
                                    void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------- decayed linear attention
+ * Linear attention with one decay a = exp(log_decay[h]) for each head:
+ *   S_t = a S_{t-1} + k_t v_t^T,  o_t = scale * S_t^T q_t,  S [Dk, Dv] float32.
+ * q [B, L, H, Dk], k [B, L, Hk, Dk], v [B, L, Hk, Dv] of `dtype`, Hk dividing H (query head h reads
+ * key/value head h / (H / Hk)); any batch, token and head strides, unit stride over the features.
+ * log_decay: float32 [H]. lengths: int32 [B] or NULL (all L): tokens from a sequence's length on are
+ * neither read nor counted, their outputs and gradients are zero (values outside 0 .. L are clamped).
+ * States: float32 contiguous [B, H, Dk, Dv]; initial_state NULL means zero. o and the gradients are
+ * contiguous and overwritten; sums are float32, each output rounded once.
+ * Dk, Dv <= 256 (HYFFT_ERR_UNSUPPORTED above). No counterpart in the reference.               */
+typedef struct hyfft_decay_desc {
+  int32_t batch, heads, kv_heads, dk, dv;
+  int32_t dtype;
+  int64_t length;
+  float scale;
+  int32_t reserved;
+  int64_t q_stride[3]; /* element strides: batch, token, head */
+  int64_t k_stride[3];
+  int64_t v_stride[3];
+  int64_t o_stride[3]; /* of dout in the backward; the forward's o is contiguous */
+} hyfft_decay_desc;
+
+HYFFT_API int hyfft_decay_workspace_size(const hyfft_decay_desc* d, size_t* fwd_bytes, size_t* bwd_bytes);
+/* final_state: the state after each sequence's last token, or NULL to skip it. */
+HYFFT_API int hyfft_decay_forward(const hyfft_decay_desc* d, const void* q, const void* k, const void* v,
+                                  const float* log_decay, const int32_t* lengths, const float* initial_state,
+                                  void* o, float* final_state, void* workspace, size_t workspace_bytes,
+                                  void* stream);
+/* Gradients for dout [B, L, H, Dv] and dfinal_state (NULL: zero). dq, dk, dv have q's, k's and v's shapes
+ * (dk and dv of a shared head are summed over its query heads in a fixed order); dlog_decay float32 [H];
+ * dinitial_state [B, H, Dk, Dv]. Any of them may be NULL to skip it, dv only together with
+ * dinitial_state.                                                                              */
+HYFFT_API int hyfft_decay_backward(const hyfft_decay_desc* d, const void* q, const void* k, const void* v,
+                                   const float* log_decay, const int32_t* lengths, const float* initial_state,
+                                   const void* dout, const float* dfinal_state, void* dq, void* dk, void* dv,
+                                   float* dlog_decay, float* dinitial_state, void* workspace,
+                                   size_t workspace_bytes, void* stream);
+/* One token of each request: q [B, H, Dk], k [B, Hk, Dk], v [B, Hk, Dv] (the token strides and `length` are
+ * not used), o [B, H, Dv] contiguous. state and out_state: [pool, H, Dk, Dv], may be the same memory. Request b
+ * owns slot slots[b] (int32), or slot b where slots is NULL; a slot outside 0 .. pool - 1 marks an idle
+ * request: its output is zero and no state is touched. No two requests may own one slot. */
+HYFFT_API int hyfft_decay_step(const hyfft_decay_desc* d, const void* q, const void* k, const void* v,
+                               const float* log_decay, const int32_t* slots, int64_t pool, const float* state,
+                               float* out_state, void* o, void* stream);
+
+/* ---------------------------------------------------------------- rotary positions
+ * Pair i of the first rot_dim features of every head is turned by position * turns[i] * 2^-64 of a full
+ * turn and scaled by `amplitude`; the other features are copied. Pairs are (2i, 2i + 1) when interleaved,
+ * else (i, i + rot_dim / 2). q [B, L, H, D] and k [B, L, Hk, D] (kv_heads 0: no k) with any batch, token
+ * and head strides; out_q and out_k contiguous. positions: int64 (int32 when pos_int32) read at
+ * b * pos_stride[0] + l * pos_stride[1], NULL: 0 .. L - 1; negative ones are turned backwards.
+ * backward != 0: the transpose (the turn back), which maps output gradients to input gradients. */
+typedef struct hyfft_rotary_desc {
+  int32_t batch, heads, kv_heads, dim, rot_dim, dtype;
+  int32_t interleaved, backward, pos_int32;
+  float amplitude;
+  int64_t length;
+  int64_t q_stride[3]; /* element strides: batch, token, head */
+  int64_t k_stride[3];
+  int64_t pos_stride[2];
+} hyfft_rotary_desc;
+
+HYFFT_API int hyfft_rotary(const hyfft_rotary_desc* d, const void* q, const void* k, const int64_t* turns,
+                           const void* positions, void* out_q, void* out_k, void* stream);
+
+/* ---------------------------------------------------------------- layer norm
+ * y = (x - mean) / sqrt(var + eps) * weight + bias over the last axis of x [rows, C] (row stride x_stride,
+ * unit stride inside a row), var the mean of the centred squares; y contiguous. weight, bias [C] of x's
+ * dtype or float32 (param_dtype), NULL: 1 and 0. mean, rstd: float32 [rows], both NULL to skip them.
+ * The backward overwrites dx (contiguous), dweight and dbias (param_dtype), NULL to skip; the sums over
+ * rows are float32 in a fixed order, rounded once.                                                */
+HYFFT_API int hyfft_layer_norm_workspace_size(int64_t rows, int64_t C, size_t* bwd_bytes);
+HYFFT_API int hyfft_layer_norm_forward(const void* x, const void* weight, const void* bias, void* y, float* mean,
+                                       float* rstd, int64_t rows, int64_t C, int64_t x_stride, float eps,
+                                       int32_t dtype, int32_t param_dtype, void* stream);
+HYFFT_API int hyfft_layer_norm_backward(const void* x, const void* weight, const float* mean, const float* rstd,
+                                        const void* dy, void* dx, void* dweight, void* dbias, int64_t rows,
+                                        int64_t C, int64_t x_stride, int64_t dy_stride, int32_t dtype,
+                                        int32_t param_dtype, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---------------------------------------------------------------- misc */
 /* Message of the most recent error on this thread ("" if none). */
 HYFFT_API const char* hyfft_last_error(void);

@@ -86,6 +86,43 @@ class SirenDesc(ctypes.Structure):
     ]
 
 
+class DecayDesc(ctypes.Structure):
+    _fields_ = [
+        ("batch", ctypes.c_int32),
+        ("heads", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32),
+        ("dk", ctypes.c_int32),
+        ("dv", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("length", ctypes.c_int64),
+        ("scale", ctypes.c_float),
+        ("reserved", ctypes.c_int32),
+        ("q_stride", ctypes.c_int64 * 3),
+        ("k_stride", ctypes.c_int64 * 3),
+        ("v_stride", ctypes.c_int64 * 3),
+        ("o_stride", ctypes.c_int64 * 3),
+    ]
+
+
+class RotaryDesc(ctypes.Structure):
+    _fields_ = [
+        ("batch", ctypes.c_int32),
+        ("heads", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32),
+        ("dim", ctypes.c_int32),
+        ("rot_dim", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32),
+        ("backward", ctypes.c_int32),
+        ("pos_int32", ctypes.c_int32),
+        ("amplitude", ctypes.c_float),
+        ("length", ctypes.c_int64),
+        ("q_stride", ctypes.c_int64 * 3),
+        ("k_stride", ctypes.c_int64 * 3),
+        ("pos_stride", ctypes.c_int64 * 2),
+    ]
+
+
 SIGNATURES = {
     "hyfft_conv_workspace_size": [ctypes.POINTER(ConvDesc), ctypes.POINTER(_sz), ctypes.POINTER(_sz)],
     "hyfft_conv_forward": [ctypes.POINTER(ConvDesc), _vp, _vp, _vp, _vp, _vp, _sz, _vp],
@@ -107,6 +144,14 @@ SIGNATURES = {
     "hyfft_siren_sizes": [ctypes.POINTER(SirenDesc), ctypes.POINTER(_sz), ctypes.POINTER(_sz)],
     "hyfft_siren_forward": [ctypes.POINTER(SirenDesc)] + [_vp] * 10 + [_sz, _vp],
     "hyfft_siren_backward": [ctypes.POINTER(SirenDesc)] + [_vp] * 16 + [_sz, _vp],
+    "hyfft_decay_workspace_size": [ctypes.POINTER(DecayDesc), ctypes.POINTER(_sz), ctypes.POINTER(_sz)],
+    "hyfft_decay_forward": [ctypes.POINTER(DecayDesc)] + [_vp] * 9 + [_sz, _vp],
+    "hyfft_decay_backward": [ctypes.POINTER(DecayDesc)] + [_vp] * 14 + [_sz, _vp],
+    "hyfft_decay_step": [ctypes.POINTER(DecayDesc)] + [_vp] * 5 + [_i64] + [_vp] * 4,
+    "hyfft_rotary": [ctypes.POINTER(RotaryDesc)] + [_vp] * 7,
+    "hyfft_layer_norm_workspace_size": [_i64, _i64, ctypes.POINTER(_sz)],
+    "hyfft_layer_norm_forward": [_vp] * 6 + [_i64, _i64, _i64, ctypes.c_float, _i32, _i32, _vp],
+    "hyfft_layer_norm_backward": [_vp] * 8 + [_i64, _i64, _i64, _i64, _i32, _i32, _vp, _sz, _vp],
     "hyfft_last_error": [],
     "hyfft_version": [],
     "hyfft_launch_count": [],

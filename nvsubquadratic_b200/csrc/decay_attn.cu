@@ -1,0 +1,825 @@
+// Linear attention with one decay for each head, over whole sequences and for single tokens.
+//
+//   S_t = a S_{t-1} + k_t v_t^T,   o_t = scale * S_t^T q_t,   a = exp(log_decay[h]),   S [Dk, Dv] float32
+//
+// The gradients are the same scan with other operands. With G_t = dL/dS_t running backwards,
+//   dq_t = scale * S_t do_t               scan(do, v, k) forwards
+//   dk_t = G_t v_t,  dv_t = G_t^T k_t     scan(v, do, q) and scan(k, q, do) backwards
+//   G_t  = U_{t+1} + scale * q_t do_t^T,  U_t = a G_t,  U_L = dL/dS_L,  dL/dS_0 = U_0
+// and the decay's, with T_t = dS_t / dlog_decay = a (T_{t-1} + S_{t-1}) carried beside S:
+//   dlog_decay = scale * sum_t q_t^T T_t do_t + <dL/dS_L, T_L>.
+//
+// The scan kernel below takes every type and every head size up to 256 and computes in float32
+// multiply-adds. A thread owns one column of S and up to 64 of its rows in registers, so a token
+// costs two packed multiply-adds per pair of state elements (S += k v, o += q S) and no exchange
+// between threads; q and k are read from shared memory as broadcasts. Inside a chunk of 32 tokens the
+// state is kept divided by a^i, which takes the decay out of the inner loop: v is multiplied by a^-i
+// and o by a^i, each from a table, and the chunk's a^n is applied once, as the sum of two floats
+// (a rounded a^n would be off by its rounding error times the number of chunks in a head's memory). Heads that
+// forget more than e^-46 within a chunk, where a^-i would overflow, multiply the state for each token.
+// Few rows and a long axis: the axis is cut into segments; a first pass adds up each segment from a zero
+// state, a small kernel chains the segments' states, and the second pass starts every segment from its own.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <atomic>
+
+#include "../../include/hyfft.h"
+#include "common.cuh"
+
+namespace hyfft {
+
+extern std::atomic<long long> g_launches;
+int set_error(int code, const char* msg);  // engine.cu: the message hyfft_last_error returns
+
+namespace {
+
+constexpr int kTok = 32;        // tokens per chunk
+constexpr int kThreads = 128;   // 4 warps: KW over the state's rows x VW over its columns
+constexpr int kMaxDim = 256;
+constexpr double kFastLimit = 46.0;  // |log_decay| * kTok below this: a^-i stays below 1e20
+
+struct Op {  // strides in elements: batch, token, head
+  const void* p;
+  long long sb, sl, sh;
+  int group;  // query heads that share one head of this operand
+};
+
+struct ScanArgs {
+  Op q, k, v, x;  // x: the output's gradient (learned decays only)
+  void* o;        // nullptr: the pass that adds up each segment from a zero state
+  long long ob, ol, oh;
+  const float* log_decay;
+  const int* lengths;       // [B] or nullptr
+  const float* start;       // state before a row's first token [B, H, ...], nullptr: zero
+  float* finish;            // state after its last
+  float* seg;               // [B * H, nseg, DK, DV] segment sums, then segment start states
+  float* segT;              // the same of T
+  float* dg;                // [B * H, nseg, nslice * VW * KW * 32] partial sums of the decay's gradient
+  float vscale, oscale;
+  int H, L, DK, DV;         // DK: rows of the state in this scan's order, DV: its columns
+  int srow, scol;           // strides of start and finish
+  int nseg, seglen, nslice, reverse;
+  int vec;                  // q, k, v (and x) can be read in 16-byte pieces
+};
+
+__device__ __forceinline__ float2 mul2(float2 a, float b) { return make_float2(a.x * b, a.y * b); }
+__device__ __forceinline__ float2 dup(float a) { return make_float2(a, a); }
+
+// rows [0, n) of an operand, columns [c0, c0 + w) (zeros past D), as floats; token of row i: t0 + i * step
+template <typename T>
+__device__ __forceinline__ void load_tile(float* dst, const T* __restrict__ src, long long sl, int n, int c0, int w,
+                                          int D, long long t0, int step, bool vec, float mul) {
+  if (vec) {
+    constexpr int V = 16 / sizeof(T);
+    const int per = w / V;
+    for (int i = threadIdx.x; i < n * per; i += kThreads) {
+      const int r = i / per, c = (i - r * per) * V;
+      float* d = dst + r * w + c;
+      if (c0 + c < D) {
+        const T* s = src + (t0 + (long long)r * step) * sl + c0 + c;
+        const uint4 raw = *reinterpret_cast<const uint4*>(s);
+        const T* e = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+        for (int u = 0; u < V; ++u) d[u] = DT<T>::load(e + u) * mul;
+      } else {
+#pragma unroll
+        for (int u = 0; u < V; ++u) d[u] = 0.f;
+      }
+    }
+  } else {
+    for (int i = threadIdx.x; i < n * w; i += kThreads) {
+      const int r = i / w, c = i - r * w;
+      dst[i] = c0 + c < D ? DT<T>::load(src + (t0 + (long long)r * step) * sl + c0 + c) * mul : 0.f;
+    }
+  }
+}
+
+// RK rows of the state in each thread, KW warps over its rows, 4 / KW over its columns.
+template <typename T, typename TO, int RK, int KW, bool LEARN>
+__global__ void __launch_bounds__(kThreads) decay_scan_kernel(const ScanArgs A) {
+  constexpr int VW = KW > 2 ? 1 : 4 / KW;
+  constexpr int W = RK * KW, WV = 32 * VW;
+  extern __shared__ __align__(16) float smem[];
+  float* qs = smem;                  // [kTok][W]
+  float* ks = qs + kTok * W;         // [kTok][W]
+  float* vs = ks + kTok * W;         // [kTok][WV]
+  float* xs = vs + kTok * WV;        // [kTok][WV], learned decays only
+  float* os = xs + (LEARN ? kTok * WV : 0);  // [KW][kTok][WV], KW > 1 only
+  __shared__ float apow[kTok], ainv[kTok];
+
+  long long id = blockIdx.x;
+  const int slice = (int)(id % A.nslice);
+  id /= A.nslice;
+  const int seg = (int)(id % A.nseg);
+  const long long bh = id / A.nseg;
+  const int h = (int)(bh % A.H);
+  const long long b = bh / A.H;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int kw = warp % KW, vw = warp / KW;
+  const bool active = warp < KW * VW;
+  const int c0 = slice * WV, col = vw * 32 + lane, row0 = kw * RK;
+  const bool has_col = active && c0 + col < A.DV;
+
+  int len = A.L;
+  if (A.lengths) len = min(max(A.lengths[b], 0), A.L);
+  const long long t_lo = (long long)seg * A.seglen;
+  const long long t_end = min(t_lo + A.seglen, (long long)A.L);  // tokens of the segment
+  const long long t_hi = min(t_end, (long long)len);             // those that count
+  const int n_all = t_hi > t_lo ? (int)(t_hi - t_lo) : 0;
+
+  const float g = A.log_decay[h];
+  const int lag = A.reverse ? 0 : 1;
+  const bool fast = !(fabs((double)g) * kTok > kFastLimit);
+  if (threadIdx.x < kTok) {
+    const int e = threadIdx.x + lag;
+    apow[threadIdx.x] = fast ? (float)(e ? exp((double)g * e) : 1.0) : 1.f;
+    ainv[threadIdx.x] = fast ? (float)(e ? exp(-(double)g * e) : 1.0) : 1.f;
+  }
+  const float a1 = expf(g);
+  const double a32 = exp((double)g * kTok);
+  const float a32hi = (float)a32, a32lo = (float)(a32 - (double)a32hi);
+
+  float2 S[RK / 2], D[LEARN ? RK / 2 : 1];
+#pragma unroll
+  for (int r = 0; r < RK / 2; ++r) S[r] = dup(0.f);
+  if (LEARN)
+#pragma unroll
+    for (int r = 0; r < (LEARN ? RK / 2 : 1); ++r) D[r] = dup(0.f);
+  const long long per_state = (long long)A.DK * A.DV;
+  if (A.o && has_col) {
+    const float* src = nullptr;
+    long long sr = A.DV, sc = 1;
+    if (A.nseg > 1) {
+      src = A.seg + (bh * A.nseg + seg) * per_state;
+    } else if (A.start) {
+      src = A.start + bh * per_state;
+      sr = A.srow, sc = A.scol;
+    }
+    if (src) {
+#pragma unroll
+      for (int r = 0; r < RK; ++r)
+        if (row0 + r < A.DK) (&S[r >> 1].x)[r & 1] = src[(row0 + r) * sr + (c0 + col) * sc];
+    }
+    if (LEARN && A.nseg > 1) {
+      const float* st = A.segT + (bh * A.nseg + seg) * per_state;
+#pragma unroll
+      for (int r = 0; r < RK; ++r)
+        if (row0 + r < A.DK) (&D[LEARN ? r >> 1 : 0].x)[r & 1] = st[(long long)(row0 + r) * A.DV + c0 + col];
+    }
+  }
+
+  const T* qp = static_cast<const T*>(A.q.p) + b * A.q.sb + (long long)(h / A.q.group) * A.q.sh;
+  const T* kp = static_cast<const T*>(A.k.p) + b * A.k.sb + (long long)(h / A.k.group) * A.k.sh;
+  const T* vp = static_cast<const T*>(A.v.p) + b * A.v.sb + (long long)(h / A.v.group) * A.v.sh;
+  const T* xp = LEARN ? static_cast<const T*>(A.x.p) + b * A.x.sb + (long long)(h / A.x.group) * A.x.sh : nullptr;
+  TO* op = static_cast<TO*>(A.o) + (A.o ? b * A.ob + (long long)h * A.oh + c0 : 0);
+  const int step = A.reverse ? -1 : 1;
+  float dg = 0.f;
+
+  for (int i0 = 0; i0 < n_all; i0 += kTok) {
+    const int n = min(kTok, n_all - i0);
+    const long long t0 = A.reverse ? t_hi - 1 - i0 : t_lo + i0;
+    __syncthreads();
+    if (A.o) load_tile(qs, qp, A.q.sl, n, 0, W, A.DK, t0, step, A.vec, 1.f);
+    load_tile(ks, kp, A.k.sl, n, 0, W, A.DK, t0, step, A.vec, 1.f);
+    load_tile(vs, vp, A.v.sl, n, c0, WV, A.DV, t0, step, A.vec, A.vscale);
+    if (LEARN && A.o) load_tile(xs, xp, A.x.sl, n, c0, WV, A.DV, t0, step, A.vec, 1.f);
+    __syncthreads();
+    if (active) {
+      for (int i = 0; i < n; ++i) {
+        const float2 vj = dup(vs[i * WV + col] * ainv[i]);
+        const float4* k4 = reinterpret_cast<const float4*>(ks + i * W + row0);
+        const float4* q4 = reinterpret_cast<const float4*>(qs + i * W + row0);
+        if (!fast && lag) {
+#pragma unroll
+          for (int r = 0; r < RK / 2; ++r) {
+            if (LEARN) D[LEARN ? r : 0] = mul2(cadd(D[LEARN ? r : 0], S[r]), a1);
+            S[r] = mul2(S[r], a1);
+          }
+        }
+        float2 acc0 = dup(0.f), acc1 = dup(0.f), accT = dup(0.f);
+#pragma unroll
+        for (int r = 0; r < RK / 4; ++r) {
+          const float4 kk = k4[r];
+          if (LEARN && fast) {
+            D[LEARN ? 2 * r : 0] = cadd(D[LEARN ? 2 * r : 0], S[2 * r]);
+            D[LEARN ? 2 * r + 1 : 0] = cadd(D[LEARN ? 2 * r + 1 : 0], S[2 * r + 1]);
+          }
+          S[2 * r] = ffma2(make_float2(kk.x, kk.y), vj, S[2 * r]);
+          S[2 * r + 1] = ffma2(make_float2(kk.z, kk.w), vj, S[2 * r + 1]);
+          if (A.o) {
+            const float4 qq = q4[r];
+            acc0 = ffma2(make_float2(qq.x, qq.y), S[2 * r], acc0);
+            acc1 = ffma2(make_float2(qq.z, qq.w), S[2 * r + 1], acc1);
+            if (LEARN) {
+              accT = ffma2(make_float2(qq.x, qq.y), D[LEARN ? 2 * r : 0], accT);
+              accT = ffma2(make_float2(qq.z, qq.w), D[LEARN ? 2 * r + 1 : 0], accT);
+            }
+          }
+        }
+        if (A.o) {
+          if (LEARN) dg = fmaf((accT.x + accT.y) * apow[i], xs[i * WV + col], dg);
+          if (!LEARN) {
+            const float o = ((acc0.x + acc0.y) + (acc1.x + acc1.y)) * (apow[i] * A.oscale);
+            if (KW == 1) {
+              if (has_col) DT<TO>::store(op + (t0 + (long long)i * step) * A.ol + col, o);
+            } else {
+              os[(kw * kTok + i) * WV + col] = o;
+            }
+          }
+        }
+        if (!fast && !lag) {
+#pragma unroll
+          for (int r = 0; r < RK / 2; ++r) S[r] = mul2(S[r], a1);
+        }
+      }
+      if (fast) {
+        float hi = a32hi, lo = a32lo;
+        if (n != kTok) {
+          const double an = exp((double)g * n);
+          hi = (float)an;
+          lo = (float)(an - (double)hi);
+        }
+#pragma unroll
+        for (int r = 0; r < RK / 2; ++r) {
+          S[r] = ffma2(S[r], dup(hi), mul2(S[r], lo));
+          if (LEARN) D[LEARN ? r : 0] = ffma2(D[LEARN ? r : 0], dup(hi), mul2(D[LEARN ? r : 0], lo));
+        }
+      }
+    }
+    if (KW > 1 && A.o && !LEARN) {
+      __syncthreads();
+      for (int i = threadIdx.x; i < n * WV; i += kThreads) {
+        const int r = i / WV, c = i - r * WV;
+        if (c0 + c < A.DV) {
+          float o = 0.f;
+#pragma unroll
+          for (int j = 0; j < KW; ++j) o += os[j * kTok * WV + i];
+          DT<TO>::store(op + (t0 + (long long)r * step) * A.ol + c, o);
+        }
+      }
+    }
+  }
+
+  if (A.o && !LEARN) {  // tokens past the length: zeros
+    const long long z0 = max(t_lo, t_hi);
+    for (long long i = threadIdx.x; i < (t_end - z0) * WV; i += kThreads) {
+      const long long r = i / WV;
+      const int c = (int)(i - r * WV);
+      if (c0 + c < A.DV) DT<TO>::store(op + (z0 + r) * A.ol + c, 0.f);
+    }
+  }
+  if (has_col) {
+    float* dst = nullptr;
+    long long sr = A.DV, sc = 1;
+    if (!A.o) {
+      dst = A.seg + (bh * A.nseg + seg) * per_state;
+    } else if (A.nseg == 1 && A.finish) {
+      dst = A.finish + bh * per_state;
+      sr = A.srow, sc = A.scol;
+    }
+    float* dT = LEARN && (!A.o || A.nseg == 1) ? A.segT + (bh * A.nseg + seg) * per_state : nullptr;
+#pragma unroll
+    for (int r = 0; r < RK; ++r)
+      if (row0 + r < A.DK) {
+        if (dst) dst[(row0 + r) * sr + (c0 + col) * sc] = (&S[r >> 1].x)[r & 1];
+        if (LEARN && dT) dT[(long long)(row0 + r) * A.DV + c0 + col] = (&D[LEARN ? r >> 1 : 0].x)[r & 1];
+      }
+  }
+  if (LEARN && A.o && active)
+    A.dg[((bh * A.nseg + seg) * A.nslice + slice) * (KW * VW * 32) + warp * 32 + lane] = has_col ? dg * A.oscale : 0.f;
+}
+
+// Chains the segments: seg[s] becomes the state before segment s (in scan order), finish the state after the last.
+// T_out = a^n T_in + n a^n S_in + T_segment. With T, segT's last slot keeps the final T (used below).
+__global__ void __launch_bounds__(256) decay_chain_kernel(float* seg, float* segT, float* finalT, const float* start,
+                                                          float* finish, const float* log_decay, const int* lengths,
+                                                          int H, int L, int DK, int DV, int srow, int scol, int nseg,
+                                                          int seglen, int reverse) {
+  const long long bh = blockIdx.y;
+  const int e = blockIdx.x * 256 + threadIdx.x;
+  if (e >= DK * DV) return;
+  const int r = e / DV, c = e - r * DV;
+  const long long per = (long long)DK * DV;
+  const float g = log_decay[bh % H];
+  int len = L;
+  if (lengths) len = min(max(lengths[bh / H], 0), L);
+  const double af = exp((double)g * seglen);
+  float s = start ? start[bh * per + (long long)r * srow + (long long)c * scol] : 0.f, t = 0.f;
+  for (int i = 0; i < nseg; ++i) {
+    const int j = reverse ? nseg - 1 - i : i;
+    const long long lo = (long long)j * seglen;
+    const long long n = max(0ll, min(lo + seglen, (long long)len) - lo);
+    const double an = n == seglen ? af : n ? exp((double)g * (double)n) : 1.0;
+    float* p = seg + (bh * nseg + j) * per + e;
+    const float add = *p;
+    *p = s;
+    if (segT) {
+      float* pt = segT + (bh * nseg + j) * per + e;
+      const float addT = *pt;
+      *pt = t;
+      t = (float)(an * ((double)t + (double)n * (double)s) + (double)addT);
+    }
+    s = (float)(an * (double)s + (double)add);
+  }
+  if (finish) finish[bh * per + (long long)r * srow + (long long)c * scol] = s;
+  if (finalT) finalT[bh * per + e] = t;
+}
+
+// dlog_decay[h] = sum over rows of head h of the partial sums, plus <dfinal, T_final>; one CTA per head, in a fixed order.
+__global__ void __launch_bounds__(256) decay_dg_kernel(const float* part, long long per, const float* finalT,
+                                                       const float* dfinal, long long state, int B, int H, float* out) {
+  const int h = blockIdx.x;
+  double s = 0.0;
+  for (int b = 0; b < B; ++b) {
+    const long long bh = (long long)b * H + h;
+    for (long long i = threadIdx.x; i < per; i += 256) s += (double)part[bh * per + i];
+    if (dfinal)
+      for (long long i = threadIdx.x; i < state; i += 256) s += (double)finalT[bh * state + i] * (double)dfinal[bh * state + i];
+  }
+  __shared__ double red[256];
+  red[threadIdx.x] = s;
+  __syncthreads();
+  for (int w = 128; w > 0; w >>= 1) {
+    if (threadIdx.x < w) red[threadIdx.x] += red[threadIdx.x + w];
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) out[h] = (float)red[0];
+}
+
+// Gradients of a shared head: the sum over its query heads, src [B * L, H, D] float32 -> dst [B * L, Hk, D].
+template <typename T>
+__global__ void __launch_bounds__(256) decay_group_sum_kernel(const float* src, T* dst, long long n, int D, int group) {
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  const long long hk = i / D;
+  const int d = (int)(i - hk * D);
+  float s = 0.f;
+  for (int j = 0; j < group; ++j) s += src[(hk * group + j) * D + d];
+  DT<T>::store(dst + i, s);
+}
+
+// ---------------------------------------------------------------- single tokens
+// One token of each request: a pass over the state, read and written once (8 bytes per element, nothing else of
+// size). A CTA takes one head's state (a slice of 32 columns when there are few heads, so that all SMs have work);
+// a thread reads four neighbouring columns of every (kStepThreads / columns * 4)-th row.
+constexpr int kStepThreads = 256;
+
+struct StepArgs {
+  Op q, k, v;
+  void* o;
+  long long ob, oh;
+  const float* log_decay;
+  const int* slots;
+  const float* state;
+  float* out_state;
+  float scale;
+  long long pool;
+  int H, DK, DV, cols, nslice;
+};
+
+template <typename T, int V>
+__global__ void __launch_bounds__(kStepThreads) decay_step_kernel(const StepArgs A) {
+  extern __shared__ float sm[];
+  float* qs = sm;             // [DK]
+  float* ks = qs + A.DK;      // [DK]
+  float* red = ks + A.DK;     // [rows][cols]
+  const int slice = blockIdx.x % A.nslice;
+  const long long bh = blockIdx.x / A.nslice;
+  const int h = (int)(bh % A.H);
+  const long long b = bh / A.H;
+  const int c0 = slice * A.cols;
+  const int ncol = min(A.cols, A.DV - c0);
+  T* o = static_cast<T*>(A.o) + b * A.ob + (long long)h * A.oh + c0;
+  const long long slot = A.slots ? (long long)A.slots[b] : b;
+  if (slot < 0 || slot >= A.pool) {  // an idle request
+    for (int c = threadIdx.x; c < ncol; c += kStepThreads) DT<T>::store(o + c, 0.f);
+    return;
+  }
+  const T* qp = static_cast<const T*>(A.q.p) + b * A.q.sb + (long long)h * A.q.sh;
+  const T* kp = static_cast<const T*>(A.k.p) + b * A.k.sb + (long long)(h / A.k.group) * A.k.sh;
+  const T* vp = static_cast<const T*>(A.v.p) + b * A.v.sb + (long long)(h / A.v.group) * A.v.sh + c0;
+  for (int i = threadIdx.x; i < A.DK; i += kStepThreads) {
+    qs[i] = DT<T>::load(qp + i) * A.scale;
+    ks[i] = DT<T>::load(kp + i);
+  }
+  const float a = expf(A.log_decay[h]);
+  __syncthreads();
+  const int per = A.cols / V, rows = kStepThreads / per;
+  const int c = (threadIdx.x % per) * V, r0 = threadIdx.x / per;
+  const long long base = (slot * A.H + h) * (long long)A.DK * A.DV + c0 + c;
+  float acc[V], vv[V];
+#pragma unroll
+  for (int u = 0; u < V; ++u) acc[u] = 0.f, vv[u] = 0.f;
+  if (r0 < rows && c < ncol) {
+#pragma unroll
+    for (int u = 0; u < V; ++u) vv[u] = DT<T>::load(vp + c + u);
+#pragma unroll 4
+    for (int r = r0; r < A.DK; r += rows) {
+      const float* src = A.state + base + (long long)r * A.DV;
+      float s[V];
+      if (V == 4) {
+        const float4 x = *reinterpret_cast<const float4*>(src);
+        s[0] = x.x, s[V > 1 ? 1 : 0] = x.y, s[V > 2 ? 2 : 0] = x.z, s[V > 3 ? 3 : 0] = x.w;
+      } else {
+        s[0] = src[0];
+      }
+      const float kk = ks[r], qq = qs[r];
+#pragma unroll
+      for (int u = 0; u < V; ++u) {
+        s[u] = fmaf(a, s[u], kk * vv[u]);
+        acc[u] = fmaf(qq, s[u], acc[u]);
+      }
+      float* dst = A.out_state + base + (long long)r * A.DV;
+      if (V == 4)
+        *reinterpret_cast<float4*>(dst) = make_float4(s[0], s[V > 1 ? 1 : 0], s[V > 2 ? 2 : 0], s[V > 3 ? 3 : 0]);
+      else
+        dst[0] = s[0];
+    }
+  }
+  if (r0 < rows)
+#pragma unroll
+    for (int u = 0; u < V; ++u) red[r0 * A.cols + c + u] = acc[u];
+  __syncthreads();
+  for (int i = threadIdx.x; i < ncol; i += kStepThreads) {
+    float s = 0.f;
+    for (int r = 0; r < rows; ++r) s += red[r * A.cols + i];
+    DT<T>::store(o + i, s);
+  }
+}
+
+// ---------------------------------------------------------------- host
+
+int launched() {
+  if (cudaGetLastError() != cudaSuccess) return set_error(HYFFT_ERR_CUDA, "decay attention: kernel launch failed");
+  g_launches.fetch_add(1, std::memory_order_relaxed);
+  return HYFFT_OK;
+}
+
+// Rows of the state that a thread holds, and warps over them, for a state of DK rows.
+void scan_shape(int DK, int* rk, int* kw) {
+  *kw = DK <= 64 ? 1 : DK <= 128 ? 2 : 4;
+  const int per = (DK + *kw - 1) / *kw;
+  *rk = (per + 15) / 16 * 16;
+}
+
+struct ScanPlan {
+  int rk, kw, nslice, nseg, seglen;
+};
+
+// Segments: enough CTAs for four on each SM, and never shorter than two chunks (a segment costs a state's traffic).
+ScanPlan scan_plan(const hyfft_decay_desc* d, int DK, int DV) {
+  ScanPlan p;
+  scan_shape(DK, &p.rk, &p.kw);
+  const int wv = 32 * (p.kw > 2 ? 1 : 4 / p.kw);
+  p.nslice = (DV + wv - 1) / wv;
+  const long long rows = (long long)d->batch * d->heads * p.nslice;
+  const long long want = std::max<long long>(1, (4 * 148 + rows - 1) / std::max<long long>(rows, 1));
+  const long long most = std::max<long long>(1, (d->length + 2 * kTok - 1) / (2 * kTok));
+  long long n = std::min(want, most);
+  const long long len = std::max<long long>(kTok, ((d->length + n - 1) / n + kTok - 1) / kTok * kTok);
+  p.seglen = (int)std::min<long long>(len, 1ll << 30);
+  p.nseg = (int)std::max<long long>(1, (d->length + p.seglen - 1) / p.seglen);
+  return p;
+}
+
+template <typename T, typename TO, int RK, int KW, bool LEARN>
+int launch_scan_rk(const ScanArgs& A, long long ctas, cudaStream_t st) {
+  constexpr int VW = KW > 2 ? 1 : 4 / KW;
+  const size_t sm = sizeof(float) * kTok * (2 * RK * KW + 32 * VW * (LEARN ? 2 : 1) + (KW > 1 ? KW * 32 * VW : 0));
+  auto kern = decay_scan_kernel<T, TO, RK, KW, LEARN>;
+  if (!kernel_smem_once((const void*)kern, sm)) return set_error(HYFFT_ERR_CUDA, "decay attention: shared memory");
+  kern<<<(unsigned)ctas, kThreads, sm, st>>>(A);
+  return launched();
+}
+
+template <typename T, typename TO, bool LEARN>
+int launch_scan(const ScanArgs& A, int rk, int kw, long long ctas, cudaStream_t st) {
+  if (ctas > 0x7fffffffLL) return set_error(HYFFT_ERR_UNSUPPORTED, "decay attention: too many rows");
+  if (kw == 1) {
+    if (rk == 16) return launch_scan_rk<T, TO, 16, 1, LEARN>(A, ctas, st);
+    if (rk == 32) return launch_scan_rk<T, TO, 32, 1, LEARN>(A, ctas, st);
+    if (rk == 48) return launch_scan_rk<T, TO, 48, 1, LEARN>(A, ctas, st);
+    return launch_scan_rk<T, TO, 64, 1, LEARN>(A, ctas, st);
+  }
+  if (kw == 2) {
+    if (rk == 48) return launch_scan_rk<T, TO, 48, 2, LEARN>(A, ctas, st);
+    return launch_scan_rk<T, TO, 64, 2, LEARN>(A, ctas, st);
+  }
+  if (rk == 48) return launch_scan_rk<T, TO, 48, 4, LEARN>(A, ctas, st);
+  return launch_scan_rk<T, TO, 64, 4, LEARN>(A, ctas, st);
+}
+
+bool op_vec(const Op& o, int D, int es) {
+  const int v = 16 / es;
+  return D % v == 0 && reinterpret_cast<uintptr_t>(o.p) % 16 == 0 && o.sb % v == 0 && o.sl % v == 0 && o.sh % v == 0;
+}
+
+size_t align256(size_t n) { return (n + 255) / 256 * 256; }
+
+size_t seg_bytes(const hyfft_decay_desc* d, const ScanPlan& p) {
+  return p.nseg > 1 ? align256(sizeof(float) * (size_t)d->batch * d->heads * p.nseg * d->dk * d->dv) : 0;
+}
+
+// One scan: segments' sums and their chain where the axis is cut, then the outputs.
+template <typename T, typename TO>
+int run_scan(const hyfft_decay_desc* d, ScanArgs A, float* seg, cudaStream_t st) {
+  const ScanPlan p = scan_plan(d, A.DK, A.DV);
+  A.H = d->heads;
+  A.L = (int)d->length;
+  A.nseg = p.nseg;
+  A.seglen = p.seglen;
+  A.nslice = p.nslice;
+  A.seg = seg;
+  const int es = (int)sizeof(T);
+  A.vec = op_vec(A.q, A.DK, es) && op_vec(A.k, A.DK, es) && op_vec(A.v, A.DV, es);
+  const long long rows = (long long)d->batch * d->heads;
+  const long long ctas = rows * p.nseg * p.nslice;
+  if (p.nseg > 1) {
+    ScanArgs P = A;
+    P.o = nullptr;
+    int rc = launch_scan<T, TO, false>(P, p.rk, p.kw, ctas, st);
+    if (rc != HYFFT_OK) return rc;
+    if (rows > 65535) return set_error(HYFFT_ERR_UNSUPPORTED, "decay attention: too many rows");
+    decay_chain_kernel<<<dim3((A.DK * A.DV + 255) / 256, (unsigned)rows), 256, 0, st>>>(
+        seg, nullptr, nullptr, A.start, A.finish, A.log_decay, A.lengths, A.H, A.L, A.DK, A.DV, A.srow, A.scol, p.nseg,
+        p.seglen, A.reverse);
+    if ((rc = launched()) != HYFFT_OK) return rc;
+  }
+  return launch_scan<T, TO, false>(A, p.rk, p.kw, ctas, st);
+}
+
+// The decay's gradient: the forward scan once more with T beside S.
+template <typename T>
+int run_learn(const hyfft_decay_desc* d, ScanArgs A, const float* dfinal, float* ws, float* out, cudaStream_t st) {
+  const ScanPlan p = scan_plan(d, A.DK, A.DV);
+  A.H = d->heads;
+  A.L = (int)d->length;
+  A.nseg = p.nseg;
+  A.seglen = p.seglen;
+  A.nslice = p.nslice;
+  const int es = (int)sizeof(T);
+  A.vec = op_vec(A.q, A.DK, es) && op_vec(A.k, A.DK, es) && op_vec(A.v, A.DV, es) && op_vec(A.x, A.DV, es);
+  const long long rows = (long long)d->batch * d->heads;
+  const size_t states = (size_t)rows * p.nseg * d->dk * d->dv;
+  float* finalT = ws;
+  A.seg = ws + (size_t)rows * d->dk * d->dv;
+  A.segT = p.nseg > 1 ? A.seg + states : finalT;
+  A.dg = A.seg + (p.nseg > 1 ? 2 * states : 0);
+  A.finish = nullptr;
+  const long long ctas = rows * p.nseg * p.nslice;
+  const int used = p.kw * 32 * (p.kw > 2 ? 1 : 4 / p.kw);
+  if (p.nseg > 1) {
+    ScanArgs P = A;
+    P.o = nullptr;
+    int rc = launch_scan<T, T, true>(P, p.rk, p.kw, ctas, st);
+    if (rc != HYFFT_OK) return rc;
+    if (rows > 65535) return set_error(HYFFT_ERR_UNSUPPORTED, "decay attention: too many rows");
+    decay_chain_kernel<<<dim3((A.DK * A.DV + 255) / 256, (unsigned)rows), 256, 0, st>>>(
+        A.seg, A.segT, finalT, A.start, nullptr, A.log_decay, A.lengths, A.H, A.L, A.DK, A.DV, A.srow, A.scol, p.nseg,
+        p.seglen, 0);
+    if ((rc = launched()) != HYFFT_OK) return rc;
+  }
+  A.o = ws;  // not written by this scan: only says that it is the second pass
+  int rc = launch_scan<T, T, true>(A, p.rk, p.kw, ctas, st);
+  if (rc != HYFFT_OK) return rc;
+  decay_dg_kernel<<<d->heads, 256, 0, st>>>(A.dg, (long long)p.nseg * p.nslice * used, finalT, dfinal,
+                                            (long long)d->dk * d->dv, d->batch, d->heads, out);
+  return launched();
+}
+
+size_t learn_bytes(const hyfft_decay_desc* d) {
+  const ScanPlan p = scan_plan(d, d->dk, d->dv);
+  const size_t rows = (size_t)d->batch * d->heads, per = (size_t)d->dk * d->dv;
+  return align256(sizeof(float) * (rows * per * (1 + (p.nseg > 1 ? 2 * (size_t)p.nseg : 0)) +
+                                   rows * p.nseg * p.nslice * kThreads));
+}
+
+int check_desc(const hyfft_decay_desc* d) {
+  if (!d) return set_error(HYFFT_ERR_INVALID, "decay attention: null descriptor");
+  if (d->batch < 1 || d->length < 0 || d->heads < 1 || d->kv_heads < 1 || d->dk < 1 || d->dv < 1)
+    return set_error(HYFFT_ERR_INVALID, "decay attention: every extent must be positive");
+  if (d->heads % d->kv_heads) return set_error(HYFFT_ERR_INVALID, "decay attention: kv_heads must divide heads");
+  if (d->dtype < HYFFT_F32 || d->dtype > HYFFT_F16) return set_error(HYFFT_ERR_INVALID, "decay attention: bad dtype");
+  if (d->dk > kMaxDim || d->dv > kMaxDim)
+    return set_error(HYFFT_ERR_UNSUPPORTED, "decay attention: head sizes above 256 are not covered");
+  if (d->length > 0x7fffffffLL - 4096) return set_error(HYFFT_ERR_UNSUPPORTED, "decay attention: sequence too long");
+  return HYFFT_OK;
+}
+
+struct Rows {  // strides of a contiguous [B, L, heads, D]
+  long long b, l, h;
+};
+Rows dense(const hyfft_decay_desc* d, int heads, int D) {
+  return {(long long)d->length * heads * D, (long long)heads * D, (long long)D};
+}
+
+template <typename T>
+int forward_t(const hyfft_decay_desc* d, const void* q, const void* k, const void* v, const float* g, const int* lengths,
+              const float* s0, void* o, float* s1, float* ws, cudaStream_t st) {
+  const int r = d->heads / d->kv_heads;
+  const Rows ro = dense(d, d->heads, d->dv);
+  ScanArgs A{};
+  A.q = {q, d->q_stride[0], d->q_stride[1], d->q_stride[2], 1};
+  A.k = {k, d->k_stride[0], d->k_stride[1], d->k_stride[2], r};
+  A.v = {v, d->v_stride[0], d->v_stride[1], d->v_stride[2], r};
+  A.o = o, A.ob = ro.b, A.ol = ro.l, A.oh = ro.h;
+  A.log_decay = g, A.lengths = lengths, A.start = s0, A.finish = s1;
+  A.vscale = 1.f, A.oscale = d->scale;
+  A.DK = d->dk, A.DV = d->dv, A.srow = d->dv, A.scol = 1;
+  return run_scan<T, T>(d, A, ws, st);
+}
+
+// dk or dv: straight to the output where no head is shared, else in float32 per query head and summed.
+template <typename T>
+int shared_scan(const hyfft_decay_desc* d, ScanArgs A, void* out, int D, float* seg, float* per_head, cudaStream_t st) {
+  if (d->heads == d->kv_heads) {
+    const Rows ro = dense(d, d->heads, D);
+    A.o = out, A.ob = ro.b, A.ol = ro.l, A.oh = ro.h;
+    return run_scan<T, T>(d, A, seg, st);
+  }
+  const Rows ro = dense(d, d->heads, D);
+  A.o = per_head, A.ob = ro.b, A.ol = ro.l, A.oh = ro.h;
+  int rc = run_scan<T, float>(d, A, seg, st);
+  if (rc != HYFFT_OK) return rc;
+  const long long n = (long long)d->batch * d->length * d->kv_heads * D;
+  if (n == 0) return HYFFT_OK;
+  decay_group_sum_kernel<T><<<(unsigned)((n + 255) / 256), 256, 0, st>>>(per_head, static_cast<T*>(out), n, D,
+                                                                         d->heads / d->kv_heads);
+  return launched();
+}
+
+template <typename T>
+int backward_t(const hyfft_decay_desc* d, const void* q, const void* k, const void* v, const float* g,
+               const int* lengths, const float* s0, const void* dout, const float* ds1, void* dq, void* dk, void* dv,
+               float* dg, float* ds0, char* ws, size_t seg_size, size_t group_size, cudaStream_t st) {
+  const int r = d->heads / d->kv_heads;
+  const Op oq{q, d->q_stride[0], d->q_stride[1], d->q_stride[2], 1};
+  const Op ok{k, d->k_stride[0], d->k_stride[1], d->k_stride[2], r};
+  const Op ov{v, d->v_stride[0], d->v_stride[1], d->v_stride[2], r};
+  const Op od{dout, d->o_stride[0], d->o_stride[1], d->o_stride[2], 1};
+  float* seg = reinterpret_cast<float*>(ws);
+  float* per_head = reinterpret_cast<float*>(ws + seg_size);
+  float* learn = reinterpret_cast<float*>(ws + seg_size + group_size);
+  ScanArgs A{};
+  A.log_decay = g, A.lengths = lengths;
+  int rc;
+  if (dq) {  // forwards over (do, v, k), the state transposed
+    ScanArgs P = A;
+    const Rows ro = dense(d, d->heads, d->dk);
+    P.q = od, P.k = ov, P.v = ok;
+    P.o = dq, P.ob = ro.b, P.ol = ro.l, P.oh = ro.h;
+    P.start = s0, P.vscale = 1.f, P.oscale = d->scale;
+    P.DK = d->dv, P.DV = d->dk, P.srow = 1, P.scol = d->dv;
+    if ((rc = run_scan<T, T>(d, P, seg, st)) != HYFFT_OK) return rc;
+  }
+  if (dk) {  // backwards over (v, do, q), the state transposed
+    ScanArgs P = A;
+    P.q = ov, P.k = od, P.v = oq;
+    P.start = ds1, P.vscale = d->scale, P.oscale = 1.f, P.reverse = 1;
+    P.DK = d->dv, P.DV = d->dk, P.srow = 1, P.scol = d->dv;
+    if ((rc = shared_scan<T>(d, P, dk, d->dk, seg, per_head, st)) != HYFFT_OK) return rc;
+  }
+  if (dv || ds0) {  // backwards over (k, q, do)
+    ScanArgs P = A;
+    P.q = ok, P.k = oq, P.v = od;
+    P.start = ds1, P.finish = ds0, P.vscale = d->scale, P.oscale = 1.f, P.reverse = 1;
+    P.DK = d->dk, P.DV = d->dv, P.srow = d->dv, P.scol = 1;
+    if ((rc = shared_scan<T>(d, P, dv, d->dv, seg, per_head, st)) != HYFFT_OK) return rc;
+  }
+  if (dg) {
+    ScanArgs P = A;
+    P.q = oq, P.k = ok, P.v = ov, P.x = od;
+    P.start = s0, P.vscale = 1.f, P.oscale = d->scale;
+    P.DK = d->dk, P.DV = d->dv, P.srow = d->dv, P.scol = 1;
+    if ((rc = run_learn<T>(d, P, ds1, learn, dg, st)) != HYFFT_OK) return rc;
+  }
+  return HYFFT_OK;
+}
+
+struct Sizes {
+  size_t fwd, seg, group, learn;
+};
+Sizes sizes(const hyfft_decay_desc* d) {
+  Sizes s;
+  s.fwd = seg_bytes(d, scan_plan(d, d->dk, d->dv));
+  s.seg = std::max(s.fwd, seg_bytes(d, scan_plan(d, d->dv, d->dk)));
+  s.group = d->heads == d->kv_heads
+                ? 0
+                : align256(sizeof(float) * (size_t)d->batch * d->length * d->heads * std::max(d->dk, d->dv));
+  s.learn = learn_bytes(d);
+  return s;
+}
+
+}  // namespace
+}  // namespace hyfft
+
+using namespace hyfft;
+
+extern "C" {
+
+int hyfft_decay_workspace_size(const hyfft_decay_desc* d, size_t* fwd_bytes, size_t* bwd_bytes) {
+  const int rc = check_desc(d);
+  if (rc != HYFFT_OK) return rc;
+  const Sizes s = sizes(d);
+  if (fwd_bytes) *fwd_bytes = s.fwd;
+  if (bwd_bytes) *bwd_bytes = s.seg + s.group + s.learn;
+  return HYFFT_OK;
+}
+
+int hyfft_decay_forward(const hyfft_decay_desc* d, const void* q, const void* k, const void* v, const float* log_decay,
+                        const int32_t* lengths, const float* initial_state, void* o, float* final_state,
+                        void* workspace, size_t workspace_bytes, void* stream) {
+  const int rc = check_desc(d);
+  if (rc != HYFFT_OK) return rc;
+  if (!log_decay || (d->length > 0 && (!q || !k || !v || !o)))
+    return set_error(HYFFT_ERR_INVALID, "decay attention: null tensor");
+  const Sizes s = sizes(d);
+  if (workspace_bytes < s.fwd || (s.fwd && !workspace))
+    return set_error(HYFFT_ERR_WORKSPACE, "decay attention: workspace too small");
+  if (bind_device_of(log_decay) != HYFFT_OK) return set_error(HYFFT_ERR_CUDA, "decay attention: device");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (d->length == 0 && !o) o = const_cast<float*>(log_decay);  // no token writes it
+  float* ws = static_cast<float*>(workspace);
+  if (d->dtype == HYFFT_F32) return forward_t<float>(d, q, k, v, log_decay, lengths, initial_state, o, final_state, ws, st);
+  if (d->dtype == HYFFT_BF16)
+    return forward_t<__nv_bfloat16>(d, q, k, v, log_decay, lengths, initial_state, o, final_state, ws, st);
+  return forward_t<__half>(d, q, k, v, log_decay, lengths, initial_state, o, final_state, ws, st);
+}
+
+int hyfft_decay_backward(const hyfft_decay_desc* d, const void* q, const void* k, const void* v, const float* log_decay,
+                         const int32_t* lengths, const float* initial_state, const void* dout, const float* dfinal_state,
+                         void* dq, void* dk, void* dv, float* dlog_decay, float* dinitial_state, void* workspace,
+                         size_t workspace_bytes, void* stream) {
+  const int rc = check_desc(d);
+  if (rc != HYFFT_OK) return rc;
+  if (!log_decay || (d->length > 0 && (!q || !k || !v || !dout)))
+    return set_error(HYFFT_ERR_INVALID, "decay attention: null tensor in the backward");
+  if (d->length > 0 && dinitial_state && !dv)
+    return set_error(HYFFT_ERR_INVALID, "decay attention: the initial state's gradient comes with dv");
+  const Sizes s = sizes(d);
+  if (workspace_bytes < s.seg + s.group + s.learn || !workspace)
+    return set_error(HYFFT_ERR_WORKSPACE, "decay attention: workspace too small");
+  if (bind_device_of(log_decay) != HYFFT_OK) return set_error(HYFFT_ERR_CUDA, "decay attention: device");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  char* ws = static_cast<char*>(workspace);
+  if (d->length == 0) dq = dk = dv = nullptr;
+  if (d->length == 0 && dinitial_state) dv = ws;  // no token writes it
+  if (d->dtype == HYFFT_F32)
+    return backward_t<float>(d, q, k, v, log_decay, lengths, initial_state, dout, dfinal_state, dq, dk, dv, dlog_decay,
+                             dinitial_state, ws, s.seg, s.group, st);
+  if (d->dtype == HYFFT_BF16)
+    return backward_t<__nv_bfloat16>(d, q, k, v, log_decay, lengths, initial_state, dout, dfinal_state, dq, dk, dv,
+                                     dlog_decay, dinitial_state, ws, s.seg, s.group, st);
+  return backward_t<__half>(d, q, k, v, log_decay, lengths, initial_state, dout, dfinal_state, dq, dk, dv, dlog_decay,
+                            dinitial_state, ws, s.seg, s.group, st);
+}
+
+int hyfft_decay_step(const hyfft_decay_desc* d, const void* q, const void* k, const void* v, const float* log_decay,
+                     const int32_t* slots, int64_t pool, const float* state, float* out_state, void* o, void* stream) {
+  const int rc = check_desc(d);
+  if (rc != HYFFT_OK) return rc;
+  if (!q || !k || !v || !log_decay || !state || !out_state || !o)
+    return set_error(HYFFT_ERR_INVALID, "decay attention step: null tensor");
+  if (bind_device_of(q) != HYFFT_OK) return set_error(HYFFT_ERR_CUDA, "decay attention step: device");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int r = d->heads / d->kv_heads;
+  StepArgs A{};
+  A.q = {q, d->q_stride[0], 0, d->q_stride[2], 1};
+  A.k = {k, d->k_stride[0], 0, d->k_stride[2], r};
+  A.v = {v, d->v_stride[0], 0, d->v_stride[2], r};
+  A.o = o, A.ob = (long long)d->heads * d->dv, A.oh = d->dv;
+  A.log_decay = log_decay, A.slots = slots, A.state = state, A.out_state = out_state, A.scale = d->scale;
+  A.H = d->heads, A.DK = d->dk, A.DV = d->dv, A.pool = pool;
+  const bool vec = d->dv % 4 == 0 && reinterpret_cast<uintptr_t>(state) % 16 == 0 &&
+                   reinterpret_cast<uintptr_t>(out_state) % 16 == 0;
+  const long long rows = (long long)d->batch * d->heads;
+  // all columns in one CTA when the heads fill the machine, slices of 32 otherwise
+  const int whole = vec ? (d->dv + 3) / 4 * 4 : d->dv;
+  A.cols = rows >= 2 * 148 ? whole : std::min(whole, 32);
+  A.nslice = (d->dv + A.cols - 1) / A.cols;
+  const long long ctas = rows * A.nslice;
+  if (ctas > 0x7fffffffLL) return set_error(HYFFT_ERR_UNSUPPORTED, "decay attention step: too many rows");
+  const int per = vec ? A.cols / 4 : A.cols;
+  const size_t sm = sizeof(float) * (2 * (size_t)A.DK + (size_t)(kStepThreads / per) * A.cols);
+#define HYFFT_STEP(T)                                                               \
+  do {                                                                              \
+    if (vec)                                                                        \
+      decay_step_kernel<T, 4><<<(unsigned)ctas, kStepThreads, sm, st>>>(A);         \
+    else                                                                            \
+      decay_step_kernel<T, 1><<<(unsigned)ctas, kStepThreads, sm, st>>>(A);         \
+  } while (0)
+  if (d->dtype == HYFFT_F32)
+    HYFFT_STEP(float);
+  else if (d->dtype == HYFFT_BF16)
+    HYFFT_STEP(__nv_bfloat16);
+  else
+    HYFFT_STEP(__half);
+#undef HYFFT_STEP
+  return launched();
+}
+
+}  // extern "C"
