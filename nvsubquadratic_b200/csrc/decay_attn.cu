@@ -25,9 +25,11 @@
 
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "../../include/hyfft.h"
 #include "common.cuh"
+#include "decay_attn.h"
 
 namespace hyfft {
 
@@ -41,29 +43,7 @@ constexpr int kThreads = 128;   // 4 warps: KW over the state's rows x VW over i
 constexpr int kMaxDim = 256;
 constexpr double kFastLimit = 46.0;  // |log_decay| * kTok below this: a^-i stays below 1e20
 
-struct Op {  // strides in elements: batch, token, head
-  const void* p;
-  long long sb, sl, sh;
-  int group;  // query heads that share one head of this operand
-};
-
-struct ScanArgs {
-  Op q, k, v, x;  // x: the output's gradient (learned decays only)
-  void* o;        // nullptr: the pass that adds up each segment from a zero state
-  long long ob, ol, oh;
-  const float* log_decay;
-  const int* lengths;       // [B] or nullptr
-  const float* start;       // state before a row's first token [B, H, ...], nullptr: zero
-  float* finish;            // state after its last
-  float* seg;               // [B * H, nseg, DK, DV] segment sums, then segment start states
-  float* segT;              // the same of T
-  float* dg;                // [B * H, nseg, nslice * VW * KW * 32] partial sums of the decay's gradient
-  float vscale, oscale;
-  int H, L, DK, DV;         // DK: rows of the state in this scan's order, DV: its columns
-  int srow, scol;           // strides of start and finish
-  int nseg, seglen, nslice, reverse;
-  int vec;                  // q, k, v (and x) can be read in 16-byte pieces
-};
+using Op = ScanOp;
 
 __device__ __forceinline__ float2 mul2(float2 a, float b) { return make_float2(a.x * b, a.y * b); }
 __device__ __forceinline__ float2 dup(float a) { return make_float2(a, a); }
@@ -468,11 +448,31 @@ void scan_shape(int DK, int* rk, int* kw) {
 
 struct ScanPlan {
   int rk, kw, nslice, nseg, seglen;
+  bool mma;
 };
 
+// The tensor cores take every bfloat16 scan whose state has up to 128 rows.
+bool use_mma(const hyfft_decay_desc* d, int DK) { return d->dtype == HYFFT_BF16 && DK <= kMmaMaxDK; }
+
+// Two CTAs for each SM: rows alone where they give every SM one, else as many segments as fit, none shorter than four
+// chunks (a segment costs a second read of k and v and a state's traffic).
+ScanPlan mma_plan(const hyfft_decay_desc* d, int DV) {
+  ScanPlan p{};
+  p.mma = true;
+  p.nslice = (DV + kMmaCols - 1) / kMmaCols;
+  const long long rows = (long long)d->batch * d->heads * p.nslice;
+  const long long want = rows >= 148 ? 1 : 296 / rows;
+  const long long most = std::max<long long>(1, d->length / (4 * kMmaTok));
+  const long long n = std::max<long long>(1, std::min(want, most));
+  const long long len = std::max<long long>(kMmaTok, ((d->length + n - 1) / n + kMmaTok - 1) / kMmaTok * kMmaTok);
+  p.seglen = (int)std::min<long long>(len, 1ll << 30);
+  p.nseg = (int)std::max<long long>(1, (d->length + p.seglen - 1) / p.seglen);
+  return p;
+}
+
 // Segments: enough CTAs for four on each SM, and never shorter than two chunks (a segment costs a state's traffic).
-ScanPlan scan_plan(const hyfft_decay_desc* d, int DK, int DV) {
-  ScanPlan p;
+ScanPlan fma_plan(const hyfft_decay_desc* d, int DK, int DV) {
+  ScanPlan p{};
   scan_shape(DK, &p.rk, &p.kw);
   const int wv = 32 * (p.kw > 2 ? 1 : 4 / p.kw);
   p.nslice = (DV + wv - 1) / wv;
@@ -484,6 +484,10 @@ ScanPlan scan_plan(const hyfft_decay_desc* d, int DK, int DV) {
   p.seglen = (int)std::min<long long>(len, 1ll << 30);
   p.nseg = (int)std::max<long long>(1, (d->length + p.seglen - 1) / p.seglen);
   return p;
+}
+
+ScanPlan scan_plan(const hyfft_decay_desc* d, int DK, int DV) {
+  return use_mma(d, DK) ? mma_plan(d, DV) : fma_plan(d, DK, DV);
 }
 
 template <typename T, typename TO, int RK, int KW, bool LEARN>
@@ -536,12 +540,19 @@ int run_scan(const hyfft_decay_desc* d, ScanArgs A, float* seg, cudaStream_t st)
   A.seg = seg;
   const int es = (int)sizeof(T);
   A.vec = op_vec(A.q, A.DK, es) && op_vec(A.k, A.DK, es) && op_vec(A.v, A.DV, es);
+  A.ovec = A.DV % 8 == 0 && reinterpret_cast<uintptr_t>(A.o) % 16 == 0;
   const long long rows = (long long)d->batch * d->heads;
   const long long ctas = rows * p.nseg * p.nslice;
+  const auto pass = [&](const ScanArgs& P) {
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      if (p.mma) return launch_scan_mma(P, sizeof(TO) == 4, ctas, st);
+    }
+    return launch_scan<T, TO, false>(P, p.rk, p.kw, ctas, st);
+  };
   if (p.nseg > 1) {
     ScanArgs P = A;
     P.o = nullptr;
-    int rc = launch_scan<T, TO, false>(P, p.rk, p.kw, ctas, st);
+    int rc = pass(P);
     if (rc != HYFFT_OK) return rc;
     if (rows > 65535) return set_error(HYFFT_ERR_UNSUPPORTED, "decay attention: too many rows");
     decay_chain_kernel<<<dim3((A.DK * A.DV + 255) / 256, (unsigned)rows), 256, 0, st>>>(
@@ -549,13 +560,13 @@ int run_scan(const hyfft_decay_desc* d, ScanArgs A, float* seg, cudaStream_t st)
         p.seglen, A.reverse);
     if ((rc = launched()) != HYFFT_OK) return rc;
   }
-  return launch_scan<T, TO, false>(A, p.rk, p.kw, ctas, st);
+  return pass(A);
 }
 
 // The decay's gradient: the forward scan once more with T beside S.
 template <typename T>
 int run_learn(const hyfft_decay_desc* d, ScanArgs A, const float* dfinal, float* ws, float* out, cudaStream_t st) {
-  const ScanPlan p = scan_plan(d, A.DK, A.DV);
+  const ScanPlan p = fma_plan(d, A.DK, A.DV);
   A.H = d->heads;
   A.L = (int)d->length;
   A.nseg = p.nseg;
@@ -592,7 +603,7 @@ int run_learn(const hyfft_decay_desc* d, ScanArgs A, const float* dfinal, float*
 }
 
 size_t learn_bytes(const hyfft_decay_desc* d) {
-  const ScanPlan p = scan_plan(d, d->dk, d->dv);
+  const ScanPlan p = fma_plan(d, d->dk, d->dv);
   const size_t rows = (size_t)d->batch * d->heads, per = (size_t)d->dk * d->dv;
   return align256(sizeof(float) * (rows * per * (1 + (p.nseg > 1 ? 2 * (size_t)p.nseg : 0)) +
                                    rows * p.nseg * p.nslice * kThreads));

@@ -1,0 +1,41 @@
+// One scan of the decayed linear attention, as decay_attn.cu plans it and its kernels run it.
+#pragma once
+
+#include <cuda_runtime.h>
+
+namespace hyfft {
+
+struct ScanOp {  // strides in elements: batch, token, head
+  const void* p;
+  long long sb, sl, sh;
+  int group;  // query heads that share one head of this operand
+};
+
+// o_i = oscale * S_i^T q_i with S_i = a S_{i-1} + vscale * k_i v_i^T over a row's tokens, forwards or backwards in time.
+struct ScanArgs {
+  ScanOp q, k, v, x;  // x: the output's gradient (learned decays only)
+  void* o;            // nullptr: the pass that adds up each segment from a zero state
+  long long ob, ol, oh;
+  const float* log_decay;
+  const int* lengths;  // [B] or nullptr
+  const float* start;  // state before a row's first token [B, H, ...], nullptr: zero
+  float* finish;       // state after its last
+  float* seg;          // [B * H, nseg, DK, DV] segment sums, then segment start states
+  float* segT;         // the same of T (learned decays)
+  float* dg;           // [B * H, nseg, ...] partial sums of the decay's gradient
+  float vscale, oscale;
+  int H, L, DK, DV;  // DK: rows of the state in this scan's order, DV: its columns
+  int srow, scol;    // strides of start and finish
+  int nseg, seglen, nslice;
+  int reverse;  // the decay is applied after a token's output instead of before
+  int vec;      // q, k, v (and x) can be read in 16-byte pieces
+  int ovec;     // o can be written in 16-byte pieces
+};
+
+// decay_mma.cu: bfloat16 operands, DK <= 128, columns in slices of 64, segments of whole 64-token chunks.
+constexpr int kMmaTok = 64;
+constexpr int kMmaCols = 64;
+constexpr int kMmaMaxDK = 128;
+int launch_scan_mma(const ScanArgs& A, bool out_f32, long long ctas, cudaStream_t st);
+
+}  // namespace hyfft
