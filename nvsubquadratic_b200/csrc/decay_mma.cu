@@ -15,9 +15,13 @@
 // three products into one accumulator; S lives in registers and takes the chunk's decay as the sum of two floats.
 //
 // Operand tiles sit in shared memory as 8 x 16-byte core matrices, [D / 8][tokens / 8][8][16 B], which the tensor core
-// reads along either axis, so K serves as K^T and V, S as they lie. cp.async brings them in (zeros past a length, a row or a
-// head size), K and V of the next chunk while this one is computed, Q as soon as P and R are done. Two CTAs of 256 threads
-// share an SM (<= 112 KB, 256 TMEM columns each) so that one's products run under the other's epilogues.
+// reads along either axis, so K serves as K^T and V, S as they lie. Twelve warps: three load (cp.async, zeros past a
+// length, a row or a head size; two take turns with K and V, one brings Q), one issues the products, eight compute:
+// they decay P, update the state, split the next chunk's V and write the outputs. Only mbarriers order them, so products
+// and loads run under the computing warps' work; two CTAs share an SM (<= 113 KB, 256 TMEM columns each).
+//
+// The computing warps' instructions are the bound after HBM: 64-row products lie in 16 of a warp's 32 TMEM lanes, and
+// the 16 x 256-bit load shape spreads those over all 32 threads (two rows, pairs of columns).
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -38,29 +42,80 @@ namespace {
 using bf16 = __nv_bfloat16;
 
 constexpr int kT = kMmaTok, kC = kMmaCols;
-constexpr int kThreads = 256;
+constexpr int kThreads = 256;  // computing
+constexpr int kLoader = kThreads / 32, kIssuer = kLoader + 3;  // first loading warp, issuing warp
+constexpr int kAll = kThreads + 4 * 32;
 constexpr int kColP = 0, kColR = 64, kColO = 128, kColS = 192, kTmemCols = 256;
 
-// Bytes of the shared-memory layout for a state of DK (64 or 128) rows.
-template <int DK, bool OUT>
+// What each mbarrier says. "done" by the tensor core, the others by the warps.
+enum Bar {
+  kFull = 0,    // K and V of buffer 0, 1 are in place
+  kFullQ = 2,
+  kEmpty = 3,   // products have read K and V of buffer 0, 1
+  kDoneR = 5,   // Q and the rounded state have been read, R is there
+  kDoneP = 6,
+  kDoneS = 7,
+  kDoneO = 8,
+  kHaveV = 9,   // the decayed V is in place
+  kHaveP = 10,  // P is in place (and its accumulator free)
+  kHaveS = 11,  // the rounded state is in place (and its accumulator free)
+  kReadO = 12,  // R and P V have been read
+  kBars = 13
+};
+
+// Bytes of the shared-memory layout for a state of DK (64 or 128) rows whose update takes TERMS bfloat16 terms.
+// Loaded tiles keep 16 bytes between their 16-byte columns, so that eight lanes that copy one token's columns hit eight banks.
+constexpr int kCol = kT * 16 + 16;
+template <int DK, bool OUT, int TERMS>
 struct Layout {
-  static constexpr int qk = DK * kT * 2, v = kC * kT * 2;
+  static constexpr int qk = DK / 8 * kCol, v = kC / 8 * kCol, term = kC * kT * 2;
+  static constexpr int vbuf = OUT && DK == 128 && TERMS == 3 ? 1 : 2;  // two CTAs must fit an SM
   static constexpr int q = 0;
   static constexpr int k = q + (OUT ? qk : 0);
   static constexpr int vv = k + 2 * qk;
-  static constexpr int w = vv + 2 * v;                 // the decayed V in three terms
-  static constexpr int p = w + 3 * v;                  // P
-  static constexpr int s = p + (OUT ? kT * kT * 2 : 0);  // the rounded state
+  static constexpr int w = vv + vbuf * v;              // the decayed V
+  static constexpr int p = w + TERMS * term;           // P, then the outputs on their way out
+  static constexpr int s = p + (OUT ? kT / 8 * kCol : 0);  // the rounded state
   static constexpr int tab = s + (OUT ? DK * kC * 2 : 0);  // a^d for d = -64 .. 64 (zeros below 0)
   static constexpr int bar = tab + (2 * kT + 4) * 4;
-  static constexpr int bytes = bar + 64;
+  static constexpr int bytes = bar + kBars * 8 + 8;
+  static_assert(2 * (bytes + 1024) <= 228 * 1024, "two CTAs share an SM");
 };
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool valid) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
 }
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
-__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group 0;\n" ::: "memory"); }
+__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_all;\n" ::: "memory"); }
+
+__device__ __forceinline__ void arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(umma::su32(bar)) : "memory");
+}
+// This warp's shared-memory writes and TMEM reads are over; the writes are visible to the tensor core.
+__device__ __forceinline__ void hand_over(uint64_t* bar) {
+  umma::fence_async_smem();
+  umma::fence_before_sync();
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) arrive(bar);
+}
+// Waits for the phase; gives up after about a second (2^16 sleeps of at most 2^14 ns) and returns false.
+__device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity) {
+  const uint32_t a = umma::su32(bar);
+  for (int i = 0; i < (1 << 16); ++i) {
+    uint32_t done;
+    asm volatile(
+        "{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\nselp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(done)
+        : "r"(a), "r"(parity), "r"(1 << 14)
+        : "memory");
+    if (done) return true;
+  }
+  return false;
+}
+__device__ __forceinline__ bool elect() {
+  uint32_t p;
+  asm volatile("{\n.reg .pred q;\nelect.sync _|q, 0xffffffff;\nselp.u32 %0, 1, 0, q;\n}\n" : "=r"(p));
+  return p != 0;
+}
 
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
@@ -71,54 +126,71 @@ __device__ __forceinline__ float2 unpack2(uint32_t u) {
 }
 
 // Columns [c0, c0 + W) of n tokens (scan order from token t0) into a tile of kT tokens, zeros past n and past D.
+// One warp: W / 8 lanes copy a token's columns, so it reads whole 128-byte lines. Addresses advance by constants:
+// recomputed for each copy they held a loading warp up for 180 cycles a copy.
 template <int W>
 __device__ __forceinline__ void load_tile(unsigned char* dst, const bf16* __restrict__ src, long long sl, int n, int c0,
                                           int D, long long t0, int step, bool vec) {
-  // a quarter warp writes 8 tokens of one 16-byte column (128 contiguous bytes); a warp reads 64 bytes of each token
-  for (int i = threadIdx.x; i < kT * W / 8; i += kThreads) {
-    const int r = i & 7, j = ((i >> 3) & 3) | ((i / (kT * 4)) << 2), t = ((i >> 5) % (kT / 8)) * 8 + r;
-    const int c = c0 + j * 8;
-    unsigned char* d = dst + j * (kT * 16) + t * 16;
-    const bool ok = t < n && c < D;
-    const bf16* s = src + (t0 + (long long)(ok ? t : 0) * step) * sl + (ok ? c : 0);
-    if (vec) {
-      cp16(umma::su32(d), s, ok);
-    } else {
+  constexpr int kLanes = W / 8, kRows = 32 / kLanes;
+  const int lane = threadIdx.x & 31, j = lane % kLanes, r = lane / kLanes;
+  const int c = c0 + j * 8;
+  unsigned char* d = dst + j * kCol + r * 16;
+  const bf16* s = src + (t0 + (long long)r * step) * sl + c;
+  const long long jump = kRows * sl * step;
+  if (vec) {
+    const uint32_t du = umma::su32(d);
+    const bool col = c < D;
+#pragma unroll 8
+    for (int t = 0; t < kT; t += kRows) {
+      const bool ok = col && t + r < n;
+      cp16(du + t * 16, ok ? s : src, ok);
+      s += jump;
+    }
+  } else {
+    for (int t = 0; t < kT; t += kRows) {
       uint4 u = make_uint4(0, 0, 0, 0);
       bf16* e = reinterpret_cast<bf16*>(&u);
-      if (ok)
+      if (t + r < n)
 #pragma unroll
-        for (int x = 0; x < 8; ++x)
-          if (c + x < D) e[x] = s[x];
-      *reinterpret_cast<uint4*>(d) = u;
+        for (int y = 0; y < 8; ++y)
+          if (c + y < D) e[y] = s[y];
+      *reinterpret_cast<uint4*>(d + t * 16) = u;
+      s += jump;
     }
   }
 }
 
-__device__ __forceinline__ void tmem_ld32(uint32_t a, float (&v)[32]) {
-  uint32_t r[32];
+// 16 TMEM lanes x 32 columns over a warp: register 4 j + 2 y + x holds row lane / 4 + 8 y, column 8 j + 2 (lane % 4) + x.
+__device__ __forceinline__ void tmem_ld(uint32_t a, uint32_t (&u)[16]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
-      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
       "tcgen05.wait::ld.sync.aligned;\n"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]),
+        "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15])
       : "r"(a)
       : "memory");
-#pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tmem_ld2(uint32_t a, uint32_t b, uint32_t (&u)[16], uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%32];\n"
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%33];\n"
+      "tcgen05.wait::ld.sync.aligned;\n"
+      : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]),
+        "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15]),
+        "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+      : "r"(a), "r"(b)
+      : "memory");
 }
 
 // OUT: the pass with outputs; without it, segments' sums alone (K and V only).
-template <int DK, bool OUT, typename TO>
-__global__ void __launch_bounds__(kThreads, 2) decay_mma_kernel(const ScanArgs A) {
-  using L = Layout<DK, OUT>;
+template <int DK, bool OUT, int TERMS, typename TO>
+__global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A) {
+  using L = Layout<DK, OUT, TERMS>;
   extern __shared__ __align__(1024) unsigned char smem[];
   float* tab = reinterpret_cast<float*>(smem + L::tab);
-  uint64_t* bar = reinterpret_cast<uint64_t*>(smem + L::bar);  // P and R; K^T V; P V
-  uint32_t* tslot = reinterpret_cast<uint32_t*>(smem + L::bar + 32);
+  uint64_t* bar = reinterpret_cast<uint64_t*>(smem + L::bar);
+  uint32_t* tslot = reinterpret_cast<uint32_t*>(smem + L::bar + kBars * 8);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   long long id = blockIdx.x;
@@ -136,232 +208,288 @@ __global__ void __launch_bounds__(kThreads, 2) decay_mma_kernel(const ScanArgs A
   const long long t_end = min(t_lo + A.seglen, (long long)A.L);
   const long long t_hi = min(t_end, (long long)len);
   const int n_all = t_hi > t_lo ? (int)(t_hi - t_lo) : 0;
+  const int chunks = (n_all + kT - 1) / kT;
   const int step = A.reverse ? -1 : 1;
   const long long t_first = A.reverse ? t_hi - 1 : t_lo;
   const int lag = A.reverse ? 0 : 1;
 
-  const bf16* qp = static_cast<const bf16*>(A.q.p) + b * A.q.sb + (long long)(h / A.q.group) * A.q.sh;
-  const bf16* kp = static_cast<const bf16*>(A.k.p) + b * A.k.sb + (long long)(h / A.k.group) * A.k.sh;
-  const bf16* vp = static_cast<const bf16*>(A.v.p) + b * A.v.sb + (long long)(h / A.v.group) * A.v.sh;
-
-  if (n_all > 0) {
-    const int n = min(kT, n_all);
-    if (OUT) load_tile<DK>(smem + L::q, qp, A.q.sl, n, 0, A.DK, t_first, step, A.vec);
-    load_tile<DK>(smem + L::k, kp, A.k.sl, n, 0, A.DK, t_first, step, A.vec);
-    load_tile<kC>(smem + L::vv, vp, A.v.sl, n, c0, A.DV, t_first, step, A.vec);
-  }
-  cp_commit();
   if (warp == 0) umma::tmem_alloc(tslot, kTmemCols);
   if (tid == 0) {
-    for (int i = 0; i < 3; ++i) umma::mbar_init(&bar[i], 1);
+    for (int i = 0; i < kBars; ++i) umma::mbar_init(&bar[i], i < kHaveV ? 1 : kThreads / 32);
     umma::fence_mbar_init();
   }
   const double g = (double)A.log_decay[h];
   if (tid <= 2 * kT) tab[tid] = tid < kT ? 0.f : tid == kT ? 1.f : (float)exp(g * (tid - kT));
-  const float a64hi = (float)exp(g * kT), a64lo = (float)(exp(g * kT) - (double)a64hi);
-
-  // This thread's part of the state: one row and 32 columns. Rows of a 64-row product lie in lanes 0 .. 15 of each warp.
-  const int wq = warp & 3, half = (warp >> 2) * 32;
-  const int srow = DK == 128 ? wq * 32 + lane : wq * 16 + lane;
-  const int trow = wq * 16 + lane;  // and of a 64-token product
-  const bool sact = DK == 128 || lane < 16, tact = lane < 16;
-  float S[32];
-#pragma unroll
-  for (int c = 0; c < 32; ++c) S[c] = 0.f;
-  const long long per_state = (long long)A.DK * A.DV;
-  if (OUT && sact && srow < A.DK) {
-    const float* src = nullptr;
-    long long sr = A.DV, sc = 1;
-    if (A.nseg > 1) {
-      src = A.seg + (bh * A.nseg + seg) * per_state;
-    } else if (A.start) {
-      src = A.start + bh * per_state;
-      sr = A.srow, sc = A.scol;
-    }
-    if (src)
-#pragma unroll
-      for (int c = 0; c < 32; ++c)
-        if (c0 + half + c < A.DV) S[c] = src[srow * sr + (c0 + half + c) * sc];
-  }
-  if (OUT && sact) {
-    unsigned char* d = smem + L::s + srow * 16;
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      *reinterpret_cast<uint4*>(d + (half / 8 + j) * (DK * 16)) =
-          make_uint4(pack2(S[8 * j], S[8 * j + 1]), pack2(S[8 * j + 2], S[8 * j + 3]), pack2(S[8 * j + 4], S[8 * j + 5]),
-                     pack2(S[8 * j + 6], S[8 * j + 7]));
-  }
+  umma::fence_before_sync();
   __syncthreads();
   umma::fence_after_sync();
   const uint32_t tmem = *tslot;
-  const uint32_t lanes = tmem + ((uint32_t)(wq * 32) << 16);
-  const uint32_t sq = umma::su32(smem + L::q), sk0 = umma::su32(smem + L::k), sv0 = umma::su32(smem + L::vv);
-  const uint32_t sw = umma::su32(smem + L::w), sp = umma::su32(smem + L::p), ss = umma::su32(smem + L::s);
-  constexpr uint32_t kIdP = umma::idesc_bf16(kT, kT, 0, 0);
-  constexpr uint32_t kIdR = umma::idesc_bf16(kT, kC, 0, 1);
-  constexpr uint32_t kIdS = umma::idesc_bf16(DK, kC, 1, 1);
-  TO* op = static_cast<TO*>(A.o) + (OUT ? b * A.ob + (long long)h * A.oh + c0 : 0);
-  bool ok = true;
+  bool ok = true;  // false once a wait has run out: no more waits, and NaN in what is written
+  const auto wait = [&](int i, int phase) {
+    ok = ok && wait_phase(&bar[i], phase & 1);
+    umma::fence_after_sync();
+  };
 
-  int it = 0;
-  for (int i0 = 0; i0 < n_all; i0 += kT, ++it) {
-    const int n = min(kT, n_all - i0), buf = it & 1;
-    const uint32_t sk = sk0 + buf * L::qk, sv = sv0 + buf * L::v;
-    const int nn = min(kT, n_all - i0 - kT);  // tokens of the next chunk
-    const long long t0 = t_first + (long long)i0 * step, t1 = t0 + (long long)kT * step;
-    cp_wait();
-    umma::fence_async_smem();
-    umma::fence_before_sync();
-    __syncthreads();  // this chunk's operands and the state are in place; the last chunk's accumulators have been read
-    if (OUT && tid == 0) {
-      umma::fence_after_sync();
-#pragma unroll
-      for (int x = 0; x < DK / 16; ++x)
-        umma::mma(tmem + kColP, umma::sdesc(sq + x * 2 * kT * 16, kT * 16, 128), umma::sdesc(sk + x * 2 * kT * 16, kT * 16, 128),
-                  kIdP, x > 0);
-#pragma unroll
-      for (int x = 0; x < DK / 16; ++x)
-        umma::mma(tmem + kColR, umma::sdesc(sq + x * 2 * kT * 16, kT * 16, 128), umma::sdesc(ss + x * 256, 128, DK * 16), kIdR,
-                  x > 0);
-      umma::commit(&bar[0]);
-    }
-    if (nn > 0) {
-      load_tile<DK>(smem + L::k + (buf ^ 1) * L::qk, kp, A.k.sl, nn, 0, A.DK, t1, step, A.vec);
-      load_tile<kC>(smem + L::vv + (buf ^ 1) * L::v, vp, A.v.sl, nn, c0, A.DV, t1, step, A.vec);
-    }
-    cp_commit();
-    // the decayed V, in three terms
-    for (int i = tid; i < kT * kC / 8; i += kThreads) {
-      const int t = i & (kT - 1);
-      const float w = t < n ? tab[kT + n - t - lag] * A.vscale : 0.f;
-      const uint4 u = *reinterpret_cast<const uint4*>(smem + L::vv + buf * L::v + i * 16);
-      uint4 hi, mid, lo;
-      const uint32_t* up = &u.x;
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        float2 f = unpack2(up[x]);
-        f.x *= w, f.y *= w;
-        const uint32_t a = pack2(f.x, f.y);
-        const float2 fa = unpack2(a);
-        f.x -= fa.x, f.y -= fa.y;
-        const uint32_t c = pack2(f.x, f.y);
-        const float2 fc = unpack2(c);
-        (&hi.x)[x] = a, (&mid.x)[x] = c, (&lo.x)[x] = pack2(f.x - fc.x, f.y - fc.y);
+  if (warp >= kLoader && warp < kIssuer) {
+    const int who = warp - kLoader;
+    if (who < 2) {
+      const bf16* kp = static_cast<const bf16*>(A.k.p) + b * A.k.sb + (long long)(h / A.k.group) * A.k.sh;
+      const bf16* vp = static_cast<const bf16*>(A.v.p) + b * A.v.sb + (long long)(h / A.v.group) * A.v.sh;
+      for (int i = who, use = 0; i < chunks; i += 2, ++use) {
+        const int n = min(kT, n_all - i * kT);
+        const long long t0 = t_first + (long long)i * kT * step;
+        if (use) wait(kEmpty + who, use - 1);
+        load_tile<DK>(smem + L::k + who * L::qk, kp, A.k.sl, n, 0, A.DK, t0, step, A.vec);
+        if (L::vbuf == 1 && i) wait(kDoneO, i - 1);
+        load_tile<kC>(smem + L::vv + (i % L::vbuf) * L::v, vp, A.v.sl, n, c0, A.DV, t0, step, A.vec);
+        cp_wait();
+        hand_over(&bar[kFull + who]);
       }
-      *reinterpret_cast<uint4*>(smem + L::w + i * 16) = hi;
-      *reinterpret_cast<uint4*>(smem + L::w + L::v + i * 16) = mid;
-      *reinterpret_cast<uint4*>(smem + L::w + 2 * L::v + i * 16) = lo;
+    } else if (OUT) {
+      const bf16* qp = static_cast<const bf16*>(A.q.p) + b * A.q.sb + (long long)(h / A.q.group) * A.q.sh;
+      for (int i = 0; i < chunks; ++i) {
+        if (i) wait(kDoneR, i - 1);
+        load_tile<DK>(smem + L::q, qp, A.q.sl, min(kT, n_all - i * kT), 0, A.DK, t_first + (long long)i * kT * step, step,
+                      A.vec);
+        cp_wait();
+        hand_over(&bar[kFullQ]);
+      }
     }
-    umma::fence_async_smem();
-    __syncthreads();
-    if (tid == 0) {
-      umma::fence_after_sync();
+  } else if (warp == kIssuer) {
+    const uint32_t sq = umma::su32(smem + L::q), sw = umma::su32(smem + L::w), sp = umma::su32(smem + L::p);
+    const uint32_t ss = umma::su32(smem + L::s);
+    constexpr uint32_t kIdP = umma::idesc_bf16(kT, kT, 0, 0);
+    constexpr uint32_t kIdR = umma::idesc_bf16(kT, kC, 0, 1);
+    constexpr uint32_t kIdS = umma::idesc_bf16(DK, kC, 1, 1);
+    for (int i = 0; i < chunks; ++i) {
+      const int buf = i & 1;
+      const uint32_t sk = umma::su32(smem + L::k + buf * L::qk), sv = umma::su32(smem + L::vv + (i % L::vbuf) * L::v);
+      wait(kFull + buf, i >> 1);
+      if (OUT) {
+        wait(kFullQ, i);
+        if (elect()) {
 #pragma unroll
-      for (int y = 0; y < 3; ++y)
+          for (int x = 0; x < DK / 16; ++x)
+            umma::mma(tmem + kColP, umma::sdesc(sq + x * 2 * kCol, kCol, 128), umma::sdesc(sk + x * 2 * kCol, kCol, 128),
+                      kIdP, x > 0);
+          umma::commit(&bar[kDoneP]);
+        }
+        __syncwarp();
+      }
+      wait(kHaveS, i);
+      wait(kHaveV, i);
+      if (elect()) {
 #pragma unroll
-        for (int x = 0; x < kT / 16; ++x)
-          umma::mma(tmem + kColS, umma::sdesc(sk + x * 256, 128, kT * 16), umma::sdesc(sw + y * L::v + x * 256, 128, kT * 16),
-                    kIdS, x + y > 0);
-      umma::commit(&bar[1]);
+        for (int y = 0; y < TERMS; ++y)
+#pragma unroll
+          for (int x = 0; x < kT / 16; ++x)
+            umma::mma(tmem + kColS, umma::sdesc(sk + x * 256, 128, kCol),
+                      umma::sdesc(sw + y * L::term + x * 256, 128, kT * 16), kIdS, x + y > 0);
+        umma::commit(&bar[kDoneS]);
+        if (!OUT) umma::commit(&bar[kEmpty + buf]);
+      }
+      __syncwarp();
+      if (OUT) {
+        if (i) wait(kReadO, i - 1);
+        if (elect()) {
+#pragma unroll
+          for (int x = 0; x < DK / 16; ++x)
+            umma::mma(tmem + kColR, umma::sdesc(sq + x * 2 * kCol, kCol, 128), umma::sdesc(ss + x * 256, 128, DK * 16), kIdR,
+                      x > 0);
+          umma::commit(&bar[kDoneR]);
+        }
+        __syncwarp();
+        wait(kHaveP, i);
+        if (elect()) {
+#pragma unroll
+          for (int x = 0; x < kT / 16; ++x)
+            umma::mma(tmem + kColO, umma::sdesc(sp + x * 2 * kCol, kCol, 128), umma::sdesc(sv + x * 256, 128, kCol), kIdR, x > 0);
+          umma::commit(&bar[kDoneO]);
+          umma::commit(&bar[kEmpty + buf]);
+        }
+        __syncwarp();
+      }
     }
-    if (OUT) {
-      ok &= umma::mbar_wait(&bar[0], it & 1);
-      umma::fence_after_sync();
-      if (nn > 0) load_tile<DK>(smem + L::q, qp, A.q.sl, nn, 0, A.DK, t1, step, A.vec);
-      cp_commit();
-      float p[32];
-      tmem_ld32(lanes + kColP + half, p);
-      if (tact) {
-        const float* tb = tab + kT + trow - half;
-        unsigned char* d = smem + L::p + (half / 8) * (kT * 16) + trow * 16;
+  } else {
+    // This thread's part of a 64 x 64 product: rows row and row + 8, columns half + 8 j + pair + {0, 1}, j < 4. Of a
+    // state of 128 rows it has two such parts, 16 TMEM lanes apart (SB).
+    constexpr int SB = DK / 64;
+    const int wq = warp & 3, half = (warp >> 2) * 32;
+    const int row = wq * 16 + (lane >> 2), pair = 2 * (lane & 3);
+    const int srow = SB == 1 ? row : wq * 32 + (lane >> 2);
+    const uint32_t lanes = tmem + ((uint32_t)(wq * 32) << 16) + half;
+    const float a64hi = (float)exp(g * kT), a64lo = (float)(exp(g * kT) - (double)a64hi);
+    const long long per_state = (long long)A.DK * A.DV;
+    const int left = A.DV - c0 - half - pair;  // columns from this thread's first on that exist
+    float S[SB][16];
+    const auto put_state = [&] {  // the rounded state, for R
+#pragma unroll
+      for (int y = 0; y < SB; ++y) {
+        unsigned char* d = smem + L::s + (half / 8) * (DK * 16) + (srow + 16 * y) * 16 + pair * 2;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          uint4 u;
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const int c = 8 * j + 2 * x;
-            (&u.x)[x] = pack2(p[c] * tb[-c], p[c + 1] * tb[-c - 1]);
-          }
-          *reinterpret_cast<uint4*>(d + j * (kT * 16)) = u;
+          *reinterpret_cast<uint32_t*>(d + j * (DK * 16)) = pack2(S[y][4 * j], S[y][4 * j + 1]);
+          *reinterpret_cast<uint32_t*>(d + j * (DK * 16) + 128) = pack2(S[y][4 * j + 2], S[y][4 * j + 3]);
         }
       }
-      umma::fence_async_smem();
-      umma::fence_before_sync();
-      __syncthreads();
-      if (tid == 0) {
-        umma::fence_after_sync();
-#pragma unroll
-        for (int x = 0; x < kT / 16; ++x)
-          umma::mma(tmem + kColO, umma::sdesc(sp + x * 2 * kT * 16, kT * 16, 128), umma::sdesc(sv + x * 256, 128, kT * 16), kIdR,
-                    x > 0);
-        umma::commit(&bar[2]);
-      }
-    }
-    // the state
-    ok &= umma::mbar_wait(&bar[1], it & 1);
-    umma::fence_after_sync();
+    };
     {
-      float d[32];
-      tmem_ld32(lanes + kColS + half, d);
-      float hi = a64hi, lo = a64lo;
-      if (n != kT) {
-        const double an = exp(g * n);
-        hi = (float)an, lo = (float)(an - (double)hi);
+      const float* src = nullptr;
+      long long sr = A.DV, sc = 1;
+      if (OUT && A.nseg > 1) {
+        src = A.seg + (bh * A.nseg + seg) * per_state;
+      } else if (OUT && A.start) {
+        src = A.start + bh * per_state;
+        sr = A.srow, sc = A.scol;
       }
 #pragma unroll
-      for (int c = 0; c < 32; ++c) S[c] = fmaf(S[c], hi, fmaf(S[c], lo, d[c]));
-      if (OUT && sact) {
-        unsigned char* t = smem + L::s + srow * 16;
+      for (int y = 0; y < SB; ++y)
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          *reinterpret_cast<uint4*>(t + (half / 8 + j) * (DK * 16)) =
-              make_uint4(pack2(S[8 * j], S[8 * j + 1]), pack2(S[8 * j + 2], S[8 * j + 3]),
-                         pack2(S[8 * j + 4], S[8 * j + 5]), pack2(S[8 * j + 6], S[8 * j + 7]));
-      }
+        for (int r = 0; r < 16; ++r) {
+          const int c = 8 * (r >> 2) + (r & 1), rw = srow + 16 * y + 8 * ((r >> 1) & 1);
+          S[y][r] = src && rw < A.DK && c < left ? src[rw * sr + (c0 + half + pair + c) * sc] : 0.f;
+        }
+      if (OUT) put_state();
+      hand_over(&bar[kHaveS]);
     }
-    if (OUT) {
-      ok &= umma::mbar_wait(&bar[2], it & 1);
-      umma::fence_after_sync();
-      float r[32], o[32];
-      tmem_ld32(lanes + kColR + half, r);
-      tmem_ld32(lanes + kColO + half, o);
-      if (tact && trow < n) {
-        const float rs = tab[kT + trow + lag] * A.oscale, os = A.vscale * A.oscale;
-        TO* d = op + (t0 + (long long)trow * step) * A.ol + half;
-        const int left = A.DV - c0 - half;
+    // The V of chunk i, decayed, in TERMS terms.
+    const auto split_v = [&](int i) {
+      const int n = min(kT, n_all - i * kT);
+      const unsigned char* v = smem + L::vv + (i % L::vbuf) * L::v;
 #pragma unroll
-        for (int c = 0; c < 32; ++c) o[c] = ok ? fmaf(r[c], rs, o[c] * os) : __int_as_float(0x7fffffff);
-        if (A.ovec && left >= 32) {
-          if constexpr (sizeof(TO) == 2) {
+      for (int x = 0; x < kT * kC / 8 / kThreads; ++x) {
+        const int at = tid + x * kThreads, t = at & (kT - 1);
+        const float w = t < n ? tab[kT + n - t - lag] * A.vscale : 0.f;
+        const uint4 u = *reinterpret_cast<const uint4*>(v + at / kT * kCol + t * 16);
+        uint4 hi, mid, lo;
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-              reinterpret_cast<uint4*>(d)[j] =
-                  make_uint4(pack2(o[8 * j], o[8 * j + 1]), pack2(o[8 * j + 2], o[8 * j + 3]),
-                             pack2(o[8 * j + 4], o[8 * j + 5]), pack2(o[8 * j + 6], o[8 * j + 7]));
-          } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-              reinterpret_cast<float4*>(d)[j] = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+        for (int e = 0; e < 4; ++e) {
+          float2 f = unpack2((&u.x)[e]);
+          f.x *= w, f.y *= w;
+          const uint32_t p = pack2(f.x, f.y);
+          f = csub(f, unpack2(p));
+          const uint32_t q = pack2(f.x, f.y);
+          (&hi.x)[e] = p, (&mid.x)[e] = q;
+          if (TERMS == 3) {
+            f = csub(f, unpack2(q));
+            (&lo.x)[e] = pack2(f.x, f.y);
           }
-        } else {
+        }
+        *reinterpret_cast<uint4*>(smem + L::w + at * 16) = hi;
+        *reinterpret_cast<uint4*>(smem + L::w + L::term + at * 16) = mid;
+        if (TERMS == 3) *reinterpret_cast<uint4*>(smem + L::w + 2 * L::term + at * 16) = lo;
+      }
+    };
+    TO* op = static_cast<TO*>(A.o) + (OUT ? b * A.ob + (long long)h * A.oh + c0 + half + pair : 0);
+    if (chunks) {
+      wait(kFull, 0);
+      split_v(0);
+      hand_over(&bar[kHaveV]);
+    }
+    // a^(i - j) of this thread's part of P: entries 2 m, 2 m + 1 for columns 8 (m - 1), + 1 of its first row. In
+    // registers where there is room.
+    const float* tb = tab + kT + row - half - pair + 8;
+    float dec[SB == 1 ? 10 : 1];
+    if (SB == 1)
 #pragma unroll
-          for (int c = 0; c < 32; ++c)
-            if (c < left) DT<TO>::store(d + c, o[c]);
+      for (int m = 0; m < (SB == 1 ? 10 : 1); ++m) dec[m] = tb[-8 * (m / 2) - (m & 1)];
+    const auto decay = [&](int m) { return SB == 1 ? dec[SB == 1 ? m : 0] : tb[-8 * (m / 2) - (m & 1)]; };
+    const float rs0 = tab[kT + row + lag] * A.oscale, rs1 = tab[kT + row + 8 + lag] * A.oscale;
+    for (int i = 0; i < chunks; ++i) {
+      const int n = min(kT, n_all - i * kT);
+      if (OUT) {  // P
+        wait(kDoneP, i);
+        uint32_t p[16];
+        tmem_ld(lanes + kColP, p);
+        unsigned char* d = smem + L::p + (half / 8) * kCol + row * 16 + pair * 2;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {  // row + 8 at column block j decays like row at block j - 1
+          *reinterpret_cast<uint32_t*>(d + j * kCol) =
+              pack2(__uint_as_float(p[4 * j]) * decay(2 * j + 2), __uint_as_float(p[4 * j + 1]) * decay(2 * j + 3));
+          *reinterpret_cast<uint32_t*>(d + j * kCol + 128) =
+              pack2(__uint_as_float(p[4 * j + 2]) * decay(2 * j), __uint_as_float(p[4 * j + 3]) * decay(2 * j + 1));
+        }
+        hand_over(&bar[kHaveP]);
+      }
+      {  // the state
+        float hi = a64hi, lo = a64lo;
+        if (n != kT) {
+          const double an = exp(g * n);
+          hi = (float)an, lo = (float)(an - (double)hi);
+        }
+        if (OUT) wait(kDoneR, i);
+        wait(kDoneS, i);
+#pragma unroll
+        for (int y = 0; y < SB; ++y) {
+          uint32_t d[16];
+          tmem_ld(lanes + kColS + ((uint32_t)(16 * y) << 16), d);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) S[y][r] = fmaf(S[y][r], hi, fmaf(S[y][r], lo, __uint_as_float(d[r])));
+        }
+        if (OUT) put_state();
+        hand_over(&bar[kHaveS]);
+      }
+      if (OUT) {  // the outputs
+        wait(kDoneO, i);
+        uint32_t r[16], o[16];
+        tmem_ld2(lanes + kColR, lanes + kColO, r, o);
+        umma::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) arrive(&bar[kReadO]);
+        const float os = ok ? A.vscale * A.oscale : __int_as_float(0x7fffffff);
+        // 16-bit outputs go through this warp's own part of P (P V is done with it): 64 bytes of a row by four lanes
+        constexpr bool kStage = sizeof(TO) == 2;
+        const bool stage = kStage && A.ovec;
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          const int rw = row + 8 * y;
+          const float rs = y ? rs1 : rs0;
+          TO* d = op + (t_first + (long long)(i * kT + rw) * step) * A.ol;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int at = 4 * j + 2 * y;
+            const float x0 = fmaf(__uint_as_float(r[at]), rs, __uint_as_float(o[at]) * os);
+            const float x1 = fmaf(__uint_as_float(r[at + 1]), rs, __uint_as_float(o[at + 1]) * os);
+            if (stage) {
+              *reinterpret_cast<uint32_t*>(smem + L::p + (half / 8 + j) * kCol + rw * 16 + pair * 2) = pack2(x0, x1);
+            } else if (rw < n) {
+              if (!kStage && A.ovec && 8 * j < left) {
+                *reinterpret_cast<float2*>(d + 8 * j) = make_float2(x0, x1);
+              } else {
+                if (8 * j < left) DT<TO>::store(d + 8 * j, x0);
+                if (8 * j + 1 < left) DT<TO>::store(d + 8 * j + 1, x1);
+              }
+            }
+          }
+        }
+        if (stage) {
+          __syncwarp();
+          const int c = half + 8 * (lane & 3);
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            const int rw = row + 8 * y;
+            const uint4 u = *reinterpret_cast<const uint4*>(smem + L::p + (c / 8) * kCol + rw * 16);
+            if (rw < n && c0 + c < A.DV)
+              *reinterpret_cast<uint4*>(op - half - pair + (t_first + (long long)(i * kT + rw) * step) * A.ol + c) = u;
+          }
+          __syncwarp();
         }
       }
+      if (i + 1 < chunks) {
+        wait(kFull + ((i + 1) & 1), (i + 1) >> 1);
+        split_v(i + 1);
+        hand_over(&bar[kHaveV]);
+      }
     }
-  }
-  cp_wait();
-
-  if (OUT) {  // tokens past the length: zeros
-    const long long z0 = max(t_lo, t_hi);
-    for (long long i = tid; i < (t_end - z0) * kC; i += kThreads) {
-      const long long r = i / kC;
-      const int c = (int)(i - r * kC);
-      if (c0 + c < A.DV) DT<TO>::store(op + (z0 + r) * A.ol + c, 0.f);
+    if (OUT) {  // tokens past the length: zeros
+      const long long z0 = max(t_lo, t_hi);
+      TO* z = static_cast<TO*>(A.o) + b * A.ob + (long long)h * A.oh + c0;
+      for (long long i = tid; i < (t_end - z0) * kC; i += kThreads) {
+        const long long r = i / kC;
+        const int c = (int)(i - r * kC);
+        if (c0 + c < A.DV) DT<TO>::store(z + (z0 + r) * A.ol + c, 0.f);
+      }
     }
-  }
-  if (sact && srow < A.DK) {
     float* dst = nullptr;
     long long sr = A.DV, sc = 1;
     if (!OUT) {
@@ -372,20 +500,24 @@ __global__ void __launch_bounds__(kThreads, 2) decay_mma_kernel(const ScanArgs A
     }
     if (dst)
 #pragma unroll
-      for (int c = 0; c < 32; ++c)
-        if (c0 + half + c < A.DV) dst[srow * sr + (c0 + half + c) * sc] = ok ? S[c] : __int_as_float(0x7fffffff);
+      for (int y = 0; y < SB; ++y)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int c = 8 * (r >> 2) + (r & 1), rw = srow + 16 * y + 8 * ((r >> 1) & 1);
+          if (rw < A.DK && c < left) dst[rw * sr + (c0 + half + pair + c) * sc] = ok ? S[y][r] : __int_as_float(0x7fffffff);
+        }
   }
   umma::fence_before_sync();
   __syncthreads();
   if (warp == 0) umma::tmem_dealloc(tmem, kTmemCols);
 }
 
-template <int DK, bool OUT, typename TO>
+template <int DK, bool OUT, int TERMS, typename TO>
 int launch(const ScanArgs& A, long long ctas, cudaStream_t st) {
-  auto kern = decay_mma_kernel<DK, OUT, TO>;
-  constexpr size_t sm = Layout<DK, OUT>::bytes;
+  auto kern = decay_mma_kernel<DK, OUT, TERMS, TO>;
+  constexpr size_t sm = Layout<DK, OUT, TERMS>::bytes;
   if (!kernel_smem_once((const void*)kern, sm, true)) return set_error(HYFFT_ERR_CUDA, "decay attention: shared memory");
-  kern<<<(unsigned)ctas, kThreads, sm, st>>>(A);
+  kern<<<(unsigned)ctas, kAll, sm, st>>>(A);
   if (cudaGetLastError() != cudaSuccess) return set_error(HYFFT_ERR_CUDA, "decay attention: kernel launch failed");
   g_launches.fetch_add(1, std::memory_order_relaxed);
   return HYFFT_OK;
@@ -393,8 +525,11 @@ int launch(const ScanArgs& A, long long ctas, cudaStream_t st) {
 
 template <int DK>
 int launch_dk(const ScanArgs& A, bool out_f32, long long ctas, cudaStream_t st) {
-  if (!A.o) return launch<DK, false, bf16>(A, ctas, st);
-  return out_f32 ? launch<DK, true, float>(A, ctas, st) : launch<DK, true, bf16>(A, ctas, st);
+  if (!A.o) return launch<DK, false, 3, bf16>(A, ctas, st);
+  // where segments were added up before, the state only serves this pass's outputs, which read it rounded to 8 bits: 16
+  // bits are enough (not by whether the caller wants the final state, so that asking for it changes no output)
+  if (A.nseg == 1) return out_f32 ? launch<DK, true, 3, float>(A, ctas, st) : launch<DK, true, 3, bf16>(A, ctas, st);
+  return out_f32 ? launch<DK, true, 2, float>(A, ctas, st) : launch<DK, true, 2, bf16>(A, ctas, st);
 }
 
 }  // namespace
