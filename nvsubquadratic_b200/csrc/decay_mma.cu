@@ -14,9 +14,11 @@
 // itself is a result in float32, so the decayed V is not rounded: it is split into three bfloat16 terms (24 bits),
 // three products into one accumulator; S lives in registers and takes the chunk's decay as the sum of two floats.
 //
-// Operand tiles sit in shared memory as 8 x 16-byte core matrices, [D / 8][tokens / 8][8][16 B], which the tensor core
-// reads along either axis, so K serves as K^T and V, S as they lie. Twelve warps: three load (cp.async, zeros past a
-// length, a row or a head size; two take turns with K and V, one brings Q), one issues the products, eight compute:
+// Operand tiles sit in shared memory as rows of 128 bytes (64 columns of a token, or of a row of P or S) whose 16-byte
+// chunks are swizzled by the row's number (chunk ^ row % 8). The tensor core reads such a tile along either axis, so K serves
+// as K^T and V, S as they lie; and both halves of a 32-byte sector stay neighbours, which tiles of 8 x 16-byte core
+// matrices did not give: cp.async then fetched every sector twice. Twelve warps: three load (cp.async, zeros past a
+// length or a head size; two take turns with K and V, one brings Q), one issues the products, eight compute:
 // they decay P, update the state, split the next chunk's V and write the outputs. Only mbarriers order them, so products
 // and loads run under the computing warps' work; two CTAs share an SM (<= 113 KB, 256 TMEM columns each).
 //
@@ -63,24 +65,32 @@ enum Bar {
   kBars = 13
 };
 
-// Bytes of the shared-memory layout for a state of DK (64 or 128) rows whose update takes TERMS bfloat16 terms.
-// Loaded tiles keep 16 bytes between their 16-byte columns, so that eight lanes that copy one token's columns hit eight banks.
-constexpr int kCol = kT * 16 + 16;
+// Bytes of the shared-memory layout for a state of DK (64 or 128) rows whose update takes TERMS bfloat16 terms. Tiles
+// start on 1024 bytes, where the swizzle's pattern does.
+constexpr int kTile = kT * 128;
 template <int DK, bool OUT, int TERMS>
 struct Layout {
-  static constexpr int qk = DK / 8 * kCol, v = kC / 8 * kCol, term = kC * kT * 2;
-  static constexpr int vbuf = OUT && DK == 128 && TERMS == 3 ? 1 : 2;  // two CTAs must fit an SM
+  static constexpr int qk = DK / 64 * kTile;
   static constexpr int q = 0;
   static constexpr int k = q + (OUT ? qk : 0);
-  static constexpr int vv = k + 2 * qk;
-  static constexpr int w = vv + vbuf * v;              // the decayed V
-  static constexpr int p = w + TERMS * term;           // P, then the outputs on their way out
-  static constexpr int s = p + (OUT ? kT / 8 * kCol : 0);  // the rounded state
-  static constexpr int tab = s + (OUT ? DK * kC * 2 : 0);  // a^d for d = -64 .. 64 (zeros below 0)
+  static constexpr int v = k + 2 * qk;
+  static constexpr int w = v + 2 * kTile;              // the decayed V
+  static constexpr int p = w + TERMS * kTile;          // P, then the outputs on their way out
+  static constexpr int s = p + (OUT ? kTile : 0);      // the rounded state
+  static constexpr int tab = s + (OUT ? DK * 128 : 0);  // a^d for d = -64 .. 64 (zeros below 0)
   static constexpr int bar = tab + (2 * kT + 4) * 4;
   static constexpr int bytes = bar + kBars * 8 + 8;
   static_assert(2 * (bytes + 1024) <= 228 * 1024, "two CTAs share an SM");
 };
+// Byte of column c (even) of a row in a swizzled tile of 64 columns.
+__device__ __forceinline__ int swz(int row, int c) { return row * 128 + ((((c >> 3) ^ row) & 7) << 4) + (c & 7) * 2; }
+// Descriptor of a swizzled tile. Rows along M or N, 64 columns along K: groups of 8 rows 1024 bytes apart, 32 bytes for
+// each 16 columns. Rows along K, columns along M or N: groups of 8 rows 1024 bytes apart (2048 for each 16 rows), blocks
+// of 64 columns a tile apart.
+__device__ __forceinline__ uint64_t tile_desc(uint32_t addr) {
+  return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(kTile >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) |
+         (2ull << 61);
+}
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool valid) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
@@ -125,36 +135,41 @@ __device__ __forceinline__ float2 unpack2(uint32_t u) {
   return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
 }
 
-// Columns [c0, c0 + W) of n tokens (scan order from token t0) into a tile of kT tokens, zeros past n and past D.
-// One warp: W / 8 lanes copy a token's columns, so it reads whole 128-byte lines. Addresses advance by constants:
-// recomputed for each copy they held a loading warp up for 180 cycles a copy.
+// Columns [c0, c0 + W) of n tokens (scan order from token t0) into tiles of kT tokens x 64 columns, zeros past n and past D.
+// One warp: eight lanes copy 128 bytes of a token. Addresses advance by constants: recomputed for each copy they held a
+// loading warp up for 180 cycles a copy.
 template <int W>
 __device__ __forceinline__ void load_tile(unsigned char* dst, const bf16* __restrict__ src, long long sl, int n, int c0,
                                           int D, long long t0, int step, bool vec) {
-  constexpr int kLanes = W / 8, kRows = 32 / kLanes;
-  const int lane = threadIdx.x & 31, j = lane % kLanes, r = lane / kLanes;
+  const int lane = threadIdx.x & 31, j = lane & 7, r = lane >> 3;
   const int c = c0 + j * 8;
-  unsigned char* d = dst + j * kCol + r * 16;
   const bf16* s = src + (t0 + (long long)r * step) * sl + c;
-  const long long jump = kRows * sl * step;
+  const long long jump = 4 * sl * step;
+  // rows r + 4 m: their chunk's place alternates between two
+  const int at0 = r * 128 + ((j ^ r) << 4), at1 = (r + 4) * 128 + ((j ^ (r + 4)) << 4);
   if (vec) {
-    const uint32_t du = umma::su32(d);
-    const bool col = c < D;
-#pragma unroll 8
-    for (int t = 0; t < kT; t += kRows) {
-      const bool ok = col && t + r < n;
-      cp16(du + t * 16, ok ? s : src, ok);
+    const uint32_t d0 = umma::su32(dst + at0), d1 = umma::su32(dst + at1);
+#pragma unroll
+    for (int t = 0; t < kT; t += 4) {
+#pragma unroll
+      for (int x = 0; x < W / 64; ++x) {
+        const bool ok = t + r < n && c + 64 * x < D;
+        cp16((t & 4 ? d1 : d0) + (t >> 3) * 1024 + x * kTile, ok ? s + 64 * x : src, ok);
+      }
       s += jump;
     }
   } else {
-    for (int t = 0; t < kT; t += kRows) {
-      uint4 u = make_uint4(0, 0, 0, 0);
-      bf16* e = reinterpret_cast<bf16*>(&u);
-      if (t + r < n)
+    for (int t = 0; t < kT; t += 4) {
 #pragma unroll
-        for (int y = 0; y < 8; ++y)
-          if (c + y < D) e[y] = s[y];
-      *reinterpret_cast<uint4*>(d + t * 16) = u;
+      for (int x = 0; x < W / 64; ++x) {
+        uint4 u = make_uint4(0, 0, 0, 0);
+        bf16* e = reinterpret_cast<bf16*>(&u);
+        if (t + r < n)
+#pragma unroll
+          for (int y = 0; y < 8; ++y)
+            if (c + 64 * x + y < D) e[y] = s[64 * x + y];
+        *reinterpret_cast<uint4*>(dst + (t & 4 ? at1 : at0) + (t >> 3) * 1024 + x * kTile) = u;
+      }
       s += jump;
     }
   }
@@ -224,7 +239,8 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A) {
   __syncthreads();
   umma::fence_after_sync();
   const uint32_t tmem = *tslot;
-  bool ok = true;  // false once a wait has run out: no more waits, and NaN in what is written
+  // false once a wait has run out (or if the tiles lay off the swizzle's pattern): no more waits, and NaN in what is written
+  bool ok = (umma::su32(smem) & 1023) == 0;
   const auto wait = [&](int i, int phase) {
     ok = ok && wait_phase(&bar[i], phase & 1);
     umma::fence_after_sync();
@@ -240,8 +256,7 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A) {
         const long long t0 = t_first + (long long)i * kT * step;
         if (use) wait(kEmpty + who, use - 1);
         load_tile<DK>(smem + L::k + who * L::qk, kp, A.k.sl, n, 0, A.DK, t0, step, A.vec);
-        if (L::vbuf == 1 && i) wait(kDoneO, i - 1);
-        load_tile<kC>(smem + L::vv + (i % L::vbuf) * L::v, vp, A.v.sl, n, c0, A.DV, t0, step, A.vec);
+        load_tile<kC>(smem + L::v + who * kTile, vp, A.v.sl, n, c0, A.DV, t0, step, A.vec);
         cp_wait();
         hand_over(&bar[kFull + who]);
       }
@@ -263,15 +278,15 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A) {
     constexpr uint32_t kIdS = umma::idesc_bf16(DK, kC, 1, 1);
     for (int i = 0; i < chunks; ++i) {
       const int buf = i & 1;
-      const uint32_t sk = umma::su32(smem + L::k + buf * L::qk), sv = umma::su32(smem + L::vv + (i % L::vbuf) * L::v);
+      const uint32_t sk = umma::su32(smem + L::k + buf * L::qk), sv = umma::su32(smem + L::v + buf * kTile);
       wait(kFull + buf, i >> 1);
       if (OUT) {
         wait(kFullQ, i);
         if (elect()) {
 #pragma unroll
           for (int x = 0; x < DK / 16; ++x)
-            umma::mma(tmem + kColP, umma::sdesc(sq + x * 2 * kCol, kCol, 128), umma::sdesc(sk + x * 2 * kCol, kCol, 128),
-                      kIdP, x > 0);
+            umma::mma(tmem + kColP, tile_desc(sq + (x >> 2) * kTile + (x & 3) * 32),
+                      tile_desc(sk + (x >> 2) * kTile + (x & 3) * 32), kIdP, x > 0);
           umma::commit(&bar[kDoneP]);
         }
         __syncwarp();
@@ -283,8 +298,7 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A) {
         for (int y = 0; y < TERMS; ++y)
 #pragma unroll
           for (int x = 0; x < kT / 16; ++x)
-            umma::mma(tmem + kColS, umma::sdesc(sk + x * 256, 128, kCol),
-                      umma::sdesc(sw + y * L::term + x * 256, 128, kT * 16), kIdS, x + y > 0);
+            umma::mma(tmem + kColS, tile_desc(sk + x * 2048), tile_desc(sw + y * kTile + x * 2048), kIdS, x + y > 0);
         umma::commit(&bar[kDoneS]);
         if (!OUT) umma::commit(&bar[kEmpty + buf]);
       }
@@ -294,8 +308,7 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A) {
         if (elect()) {
 #pragma unroll
           for (int x = 0; x < DK / 16; ++x)
-            umma::mma(tmem + kColR, umma::sdesc(sq + x * 2 * kCol, kCol, 128), umma::sdesc(ss + x * 256, 128, DK * 16), kIdR,
-                      x > 0);
+            umma::mma(tmem + kColR, tile_desc(sq + (x >> 2) * kTile + (x & 3) * 32), tile_desc(ss + x * 2048), kIdR, x > 0);
           umma::commit(&bar[kDoneR]);
         }
         __syncwarp();
@@ -303,7 +316,7 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A) {
         if (elect()) {
 #pragma unroll
           for (int x = 0; x < kT / 16; ++x)
-            umma::mma(tmem + kColO, umma::sdesc(sp + x * 2 * kCol, kCol, 128), umma::sdesc(sv + x * 256, 128, kCol), kIdR, x > 0);
+            umma::mma(tmem + kColO, tile_desc(sp + x * 32), tile_desc(sv + x * 2048), kIdR, x > 0);
           umma::commit(&bar[kDoneO]);
           umma::commit(&bar[kEmpty + buf]);
         }
@@ -325,11 +338,12 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A) {
     const auto put_state = [&] {  // the rounded state, for R
 #pragma unroll
       for (int y = 0; y < SB; ++y) {
-        unsigned char* d = smem + L::s + (half / 8) * (DK * 16) + (srow + 16 * y) * 16 + pair * 2;
+        const int rw = srow + 16 * y;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          *reinterpret_cast<uint32_t*>(d + j * (DK * 16)) = pack2(S[y][4 * j], S[y][4 * j + 1]);
-          *reinterpret_cast<uint32_t*>(d + j * (DK * 16) + 128) = pack2(S[y][4 * j + 2], S[y][4 * j + 3]);
+          *reinterpret_cast<uint32_t*>(smem + L::s + swz(rw, half + 8 * j + pair)) = pack2(S[y][4 * j], S[y][4 * j + 1]);
+          *reinterpret_cast<uint32_t*>(smem + L::s + swz(rw, half + 8 * j + pair) + 1024) =
+              pack2(S[y][4 * j + 2], S[y][4 * j + 3]);
         }
       }
     };
@@ -355,12 +369,12 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A) {
     // The V of chunk i, decayed, in TERMS terms.
     const auto split_v = [&](int i) {
       const int n = min(kT, n_all - i * kT);
-      const unsigned char* v = smem + L::vv + (i % L::vbuf) * L::v;
+      const unsigned char* v = smem + L::v + (i & 1) * kTile;
 #pragma unroll
       for (int x = 0; x < kT * kC / 8 / kThreads; ++x) {
-        const int at = tid + x * kThreads, t = at & (kT - 1);
+        const int at = tid + x * kThreads, t = at >> 3;  // V's place in the tile is its terms' place
         const float w = t < n ? tab[kT + n - t - lag] * A.vscale : 0.f;
-        const uint4 u = *reinterpret_cast<const uint4*>(v + at / kT * kCol + t * 16);
+        const uint4 u = *reinterpret_cast<const uint4*>(v + at * 16);
         uint4 hi, mid, lo;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -376,8 +390,8 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A) {
           }
         }
         *reinterpret_cast<uint4*>(smem + L::w + at * 16) = hi;
-        *reinterpret_cast<uint4*>(smem + L::w + L::term + at * 16) = mid;
-        if (TERMS == 3) *reinterpret_cast<uint4*>(smem + L::w + 2 * L::term + at * 16) = lo;
+        *reinterpret_cast<uint4*>(smem + L::w + kTile + at * 16) = mid;
+        if (TERMS == 3) *reinterpret_cast<uint4*>(smem + L::w + 2 * kTile + at * 16) = lo;
       }
     };
     TO* op = static_cast<TO*>(A.o) + (OUT ? b * A.ob + (long long)h * A.oh + c0 + half + pair : 0);
@@ -401,12 +415,12 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A) {
         wait(kDoneP, i);
         uint32_t p[16];
         tmem_ld(lanes + kColP, p);
-        unsigned char* d = smem + L::p + (half / 8) * kCol + row * 16 + pair * 2;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {  // row + 8 at column block j decays like row at block j - 1
-          *reinterpret_cast<uint32_t*>(d + j * kCol) =
+          unsigned char* d = smem + L::p + swz(row, half + 8 * j + pair);
+          *reinterpret_cast<uint32_t*>(d) =
               pack2(__uint_as_float(p[4 * j]) * decay(2 * j + 2), __uint_as_float(p[4 * j + 1]) * decay(2 * j + 3));
-          *reinterpret_cast<uint32_t*>(d + j * kCol + 128) =
+          *reinterpret_cast<uint32_t*>(d + 1024) =
               pack2(__uint_as_float(p[4 * j + 2]) * decay(2 * j), __uint_as_float(p[4 * j + 3]) * decay(2 * j + 1));
         }
         hand_over(&bar[kHaveP]);
@@ -451,7 +465,7 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A) {
             const float x0 = fmaf(__uint_as_float(r[at]), rs, __uint_as_float(o[at]) * os);
             const float x1 = fmaf(__uint_as_float(r[at + 1]), rs, __uint_as_float(o[at + 1]) * os);
             if (stage) {
-              *reinterpret_cast<uint32_t*>(smem + L::p + (half / 8 + j) * kCol + rw * 16 + pair * 2) = pack2(x0, x1);
+              *reinterpret_cast<uint32_t*>(smem + L::p + swz(rw, half + 8 * j + pair)) = pack2(x0, x1);
             } else if (rw < n) {
               if (!kStage && A.ovec && 8 * j < left) {
                 *reinterpret_cast<float2*>(d + 8 * j) = make_float2(x0, x1);
@@ -468,7 +482,7 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A) {
 #pragma unroll
           for (int y = 0; y < 2; ++y) {
             const int rw = row + 8 * y;
-            const uint4 u = *reinterpret_cast<const uint4*>(smem + L::p + (c / 8) * kCol + rw * 16);
+            const uint4 u = *reinterpret_cast<const uint4*>(smem + L::p + swz(rw, c));
             if (rw < n && c0 + c < A.DV)
               *reinterpret_cast<uint4*>(op - half - pair + (t_first + (long long)(i * kT + rw) * step) * A.ol + c) = u;
           }
