@@ -274,7 +274,8 @@ __global__ void __launch_bounds__(kThreads) decay_scan_kernel(const ScanArgs A) 
 }
 
 // Chains the segments: seg[s] becomes the state before segment s (in scan order), finish the state after the last.
-// T_out = a^n T_in + n a^n S_in + T_segment. With T, segT's last slot keeps the final T (used below).
+// T_out = a^n T_in + n a^n S_in + T_segment. 
+constexpr int kChainLoads = 8;
 __global__ void __launch_bounds__(256) decay_chain_kernel(float* seg, float* segT, float* finalT, const float* start,
                                                           float* finish, const float* log_decay, const int* lengths,
                                                           int H, int L, int DK, int DV, int srow, int scol, int nseg,
@@ -289,21 +290,30 @@ __global__ void __launch_bounds__(256) decay_chain_kernel(float* seg, float* seg
   if (lengths) len = min(max(lengths[bh / H], 0), L);
   const double af = exp((double)g * seglen);
   float s = start ? start[bh * per + (long long)r * srow + (long long)c * scol] : 0.f, t = 0.f;
-  for (int i = 0; i < nseg; ++i) {
-    const int j = reverse ? nseg - 1 - i : i;
-    const long long lo = (long long)j * seglen;
-    const long long n = max(0ll, min(lo + seglen, (long long)len) - lo);
-    const double an = n == seglen ? af : n ? exp((double)g * (double)n) : 1.0;
-    float* p = seg + (bh * nseg + j) * per + e;
-    const float add = *p;
-    *p = s;
-    if (segT) {
-      float* pt = segT + (bh * nseg + j) * per + e;
-      const float addT = *pt;
-      *pt = t;
-      t = (float)(an * ((double)t + (double)n * (double)s) + (double)addT);
-    }
-    s = (float)(an * (double)s + (double)add);
+  for (int i0 = 0; i0 < nseg; i0 += kChainLoads) {  // loads of several segments in flight
+    float add[kChainLoads], addT[kChainLoads];
+    const int m = min(kChainLoads, nseg - i0);
+#pragma unroll
+    for (int i = 0; i < kChainLoads; ++i)
+      if (i < m) {
+        const long long at = (bh * nseg + (reverse ? nseg - 1 - i0 - i : i0 + i)) * per + e;
+        add[i] = seg[at];
+        if (segT) addT[i] = segT[at];
+      }
+#pragma unroll
+    for (int i = 0; i < kChainLoads; ++i)
+      if (i < m) {
+        const int j = reverse ? nseg - 1 - i0 - i : i0 + i;
+        const long long at = (bh * nseg + j) * per + e, lo = (long long)j * seglen;
+        const long long n = max(0ll, min(lo + seglen, (long long)len) - lo);
+        const double an = n == seglen ? af : n ? exp((double)g * (double)n) : 1.0;
+        seg[at] = s;
+        if (segT) {
+          segT[at] = t;
+          t = (float)(an * ((double)t + (double)n * (double)s) + (double)addT[i]);
+        }
+        s = (float)(an * (double)s + (double)add[i]);
+      }
   }
   if (finish) finish[bh * per + (long long)r * srow + (long long)c * scol] = s;
   if (finalT) finalT[bh * per + e] = t;
@@ -532,6 +542,7 @@ size_t seg_bytes(const hyfft_decay_desc* d, const ScanPlan& p) {
 template <typename T, typename TO>
 int run_scan(const hyfft_decay_desc* d, ScanArgs A, float* seg, cudaStream_t st) {
   const ScanPlan p = scan_plan(d, A.DK, A.DV);
+  A.B = d->batch;
   A.H = d->heads;
   A.L = (int)d->length;
   A.nseg = p.nseg;
@@ -567,6 +578,7 @@ int run_scan(const hyfft_decay_desc* d, ScanArgs A, float* seg, cudaStream_t st)
 template <typename T>
 int run_learn(const hyfft_decay_desc* d, ScanArgs A, const float* dfinal, float* ws, float* out, cudaStream_t st) {
   const ScanPlan p = fma_plan(d, A.DK, A.DV);
+  A.B = d->batch;
   A.H = d->heads;
   A.L = (int)d->length;
   A.nseg = p.nseg;

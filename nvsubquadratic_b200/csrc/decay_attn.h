@@ -24,7 +24,7 @@ struct ScanArgs {
   float* segT;         // the same of T (learned decays)
   float* dg;           // [B * H, nseg, ...] partial sums of the decay's gradient
   float vscale, oscale;
-  int H, L, DK, DV;  // DK: rows of the state in this scan's order, DV: its columns
+  int B, H, L, DK, DV;  // DK: rows of the state in this scan's order, DV: its columns
   int srow, scol;    // strides of start and finish
   int nseg, seglen, nslice;
   int reverse;  // the decay is applied after a token's output instead of before

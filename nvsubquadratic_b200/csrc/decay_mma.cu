@@ -17,17 +17,21 @@
 // Operand tiles sit in shared memory as rows of 128 bytes (64 columns of a token, or of a row of P or S) whose 16-byte
 // chunks are swizzled by the row's number (chunk ^ row % 8). The tensor core reads such a tile along either axis, so K serves
 // as K^T and V, S as they lie; and both halves of a 32-byte sector stay neighbours, which tiles of 8 x 16-byte core
-// matrices did not give: cp.async then fetched every sector twice. Twelve warps: three load (cp.async, zeros past a
-// length or a head size; two take turns with K and V, one brings Q), one issues the products, eight compute:
-// they decay P, update the state, split the next chunk's V and write the outputs. Only mbarriers order them, so products
-// and loads run under the computing warps' work; two CTAs share an SM (<= 113 KB, 256 TMEM columns each).
+// matrices did not give: cp.async then fetched every sector twice. Rows are in the order of time in either direction.
+// Twelve warps: three load (TMA; the last, partial chunk and tensors that TMA cannot take by cp.async, with zeros past a
+// length or a head size; two take turns with K and V, one brings Q), one issues the products, eight compute: they decay
+// P, update the state, split the next chunk's V and write the outputs. Only mbarriers order them, so products and loads
+// run under the computing warps' work; two CTAs share an SM (<= 113 KB, 256 TMEM columns each).
 //
 // The computing warps' instructions are the bound after HBM: 64-row products lie in 16 of a warp's 32 TMEM lanes, and
 // the 16 x 256-bit load shape spreads those over all 32 threads (two rows, pairs of columns).
+#include <cuda.h>
+#include <cudaTypedefs.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
 #include <atomic>
+#include <mutex>
 
 #include "../../include/hyfft.h"
 #include "common.cuh"
@@ -47,7 +51,7 @@ constexpr int kT = kMmaTok, kC = kMmaCols;
 constexpr int kThreads = 256;  // computing
 constexpr int kLoader = kThreads / 32, kIssuer = kLoader + 3;  // first loading warp, issuing warp
 constexpr int kAll = kThreads + 4 * 32;
-constexpr int kColP = 0, kColR = 64, kColO = 128, kColS = 192, kTmemCols = 256;
+constexpr int kColP = 0, kColR = 64, kColO = 128, kColS = 192, kTmemCols = 256;  // kColS - 64: a second one without outputs
 
 // What each mbarrier says. "done" by the tensor core, the others by the warps.
 enum Bar {
@@ -56,13 +60,13 @@ enum Bar {
   kEmpty = 3,   // products have read K and V of buffer 0, 1
   kDoneR = 5,   // Q and the rounded state have been read, R is there
   kDoneP = 6,
-  kDoneS = 7,
-  kDoneO = 8,
-  kHaveV = 9,   // the decayed V is in place
-  kHaveP = 10,  // P is in place (and its accumulator free)
-  kHaveS = 11,  // the rounded state is in place (and its accumulator free)
-  kReadO = 12,  // R and P V have been read
-  kBars = 13
+  kDoneO = 7,
+  kDoneS = 8,   // K^T V is there, of buffer 0, 1
+  kHaveV = 10,  // the decayed V is in place, of buffer 0, 1
+  kHaveS = 12,  // the rounded state is in place, the accumulator of buffer 0, 1 free
+  kHaveP = 14,  // P is in place (and its accumulator free)
+  kReadO = 15,  // R and P V have been read
+  kBars = 16
 };
 
 // Bytes of the shared-memory layout for a state of DK (64 or 128) rows whose update takes TERMS bfloat16 terms. Tiles
@@ -74,9 +78,10 @@ struct Layout {
   static constexpr int q = 0;
   static constexpr int k = q + (OUT ? qk : 0);
   static constexpr int v = k + 2 * qk;
-  static constexpr int w = v + 2 * kTile;              // the decayed V
-  static constexpr int p = w + TERMS * kTile;          // P, then the outputs on their way out
-  static constexpr int s = p + (OUT ? kTile : 0);      // the rounded state
+  static constexpr int wbuf = OUT ? 1 : 2;
+  static constexpr int w = v + 2 * kTile;               // the decayed V
+  static constexpr int p = w + wbuf * TERMS * kTile;    // P, then the outputs on their way out
+  static constexpr int s = p + (OUT ? kTile : 0);       // the rounded state
   static constexpr int tab = s + (OUT ? DK * 128 : 0);  // a^d for d = -64 .. 64 (zeros below 0)
   static constexpr int bar = tab + (2 * kT + 4) * 4;
   static constexpr int bytes = bar + kBars * 8 + 8;
@@ -135,16 +140,36 @@ __device__ __forceinline__ float2 unpack2(uint32_t u) {
   return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
 }
 
-// Columns [c0, c0 + W) of n tokens (scan order from token t0) into tiles of kT tokens x 64 columns, zeros past n and past D.
+// Maps of q, k, v as [batch, token, head, feature], boxes of 64 tokens x 64 features of one head.
+struct Maps {
+  CUtensorMap q, k, v;
+  int on;
+};
+
+// Columns [c0, c0 + W) of 64 tokens from t0 on, all of them inside the sequence, by TMA; one lane.
+template <int W>
+__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int c0, int head, int t0, int b) {
+#pragma unroll
+  for (int x = 0; x < W / 64; ++x)
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::
+            "r"(dst + x * kTile), "l"(map), "r"(c0 + 64 * x), "r"(head), "r"(t0), "r"(b), "r"(umma::su32(bar))
+        : "memory");
+}
+__device__ __forceinline__ void expect(uint64_t* bar, int bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(umma::su32(bar)), "r"(bytes) : "memory");
+}
+
+// Columns [c0, c0 + W) of n tokens from t0 on into tiles of kT tokens x 64 columns, zeros past n and past D.
 // One warp: eight lanes copy 128 bytes of a token. Addresses advance by constants: recomputed for each copy they held a
 // loading warp up for 180 cycles a copy.
 template <int W>
 __device__ __forceinline__ void load_tile(unsigned char* dst, const bf16* __restrict__ src, long long sl, int n, int c0,
-                                          int D, long long t0, int step, bool vec) {
+                                          int D, long long t0, bool vec) {
   const int lane = threadIdx.x & 31, j = lane & 7, r = lane >> 3;
   const int c = c0 + j * 8;
-  const bf16* s = src + (t0 + (long long)r * step) * sl + c;
-  const long long jump = 4 * sl * step;
+  const bf16* s = src + (t0 + r) * sl + c;
+  const long long jump = 4 * sl;
   // rows r + 4 m: their chunk's place alternates between two
   const int at0 = r * 128 + ((j ^ r) << 4), at1 = (r + 4) * 128 + ((j ^ (r + 4)) << 4);
   if (vec) {
@@ -200,7 +225,7 @@ __device__ __forceinline__ void tmem_ld2(uint32_t a, uint32_t b, uint32_t (&u)[1
 
 // OUT: the pass with outputs; without it, segments' sums alone (K and V only).
 template <int DK, bool OUT, int TERMS, typename TO>
-__global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A) {
+__global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A, const __grid_constant__ Maps M) {
   using L = Layout<DK, OUT, TERMS>;
   extern __shared__ __align__(1024) unsigned char smem[];
   float* tab = reinterpret_cast<float*>(smem + L::tab);
@@ -224,17 +249,15 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A) {
   const long long t_hi = min(t_end, (long long)len);
   const int n_all = t_hi > t_lo ? (int)(t_hi - t_lo) : 0;
   const int chunks = (n_all + kT - 1) / kT;
-  const int step = A.reverse ? -1 : 1;
-  const long long t_first = A.reverse ? t_hi - 1 : t_lo;
-  const int lag = A.reverse ? 0 : 1;
+  const bool rev = A.reverse;
+  const auto tokens = [&](int i) { return min(kT, n_all - i * kT); };  // of chunk i, and the first of them in time
+  const auto first = [&](int i) { return rev ? t_hi - i * kT - tokens(i) : t_lo + i * kT; };
 
   if (warp == 0) umma::tmem_alloc(tslot, kTmemCols);
   if (tid == 0) {
     for (int i = 0; i < kBars; ++i) umma::mbar_init(&bar[i], i < kHaveV ? 1 : kThreads / 32);
     umma::fence_mbar_init();
   }
-  const double g = (double)A.log_decay[h];
-  if (tid <= 2 * kT) tab[tid] = tid < kT ? 0.f : tid == kT ? 1.f : (float)exp(g * (tid - kT));
   umma::fence_before_sync();
   __syncthreads();
   umma::fence_after_sync();
@@ -249,25 +272,42 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A) {
   if (warp >= kLoader && warp < kIssuer) {
     const int who = warp - kLoader;
     if (who < 2) {
-      const bf16* kp = static_cast<const bf16*>(A.k.p) + b * A.k.sb + (long long)(h / A.k.group) * A.k.sh;
-      const bf16* vp = static_cast<const bf16*>(A.v.p) + b * A.v.sb + (long long)(h / A.v.group) * A.v.sh;
+      const int hk = h / A.k.group, hv = h / A.v.group;
+      const bf16* kp = static_cast<const bf16*>(A.k.p) + b * A.k.sb + hk * A.k.sh;
+      const bf16* vp = static_cast<const bf16*>(A.v.p) + b * A.v.sb + hv * A.v.sh;
+      unsigned char *kd = smem + L::k + who * L::qk, *vd = smem + L::v + who * kTile;
       for (int i = who, use = 0; i < chunks; i += 2, ++use) {
-        const int n = min(kT, n_all - i * kT);
-        const long long t0 = t_first + (long long)i * kT * step;
         if (use) wait(kEmpty + who, use - 1);
-        load_tile<DK>(smem + L::k + who * L::qk, kp, A.k.sl, n, 0, A.DK, t0, step, A.vec);
-        load_tile<kC>(smem + L::v + who * kTile, vp, A.v.sl, n, c0, A.DV, t0, step, A.vec);
-        cp_wait();
-        hand_over(&bar[kFull + who]);
+        if (M.on && tokens(i) == kT) {
+          if (lane == 0) {
+            expect(&bar[kFull + who], L::qk + kTile);
+            load_box<DK>(umma::su32(kd), &M.k, &bar[kFull + who], 0, hk, (int)first(i), (int)b);
+            load_box<kC>(umma::su32(vd), &M.v, &bar[kFull + who], c0, hv, (int)first(i), (int)b);
+          }
+          __syncwarp();
+        } else {
+          load_tile<DK>(kd, kp, A.k.sl, tokens(i), 0, A.DK, first(i), A.vec);
+          load_tile<kC>(vd, vp, A.v.sl, tokens(i), c0, A.DV, first(i), A.vec);
+          cp_wait();
+          hand_over(&bar[kFull + who]);
+        }
       }
     } else if (OUT) {
-      const bf16* qp = static_cast<const bf16*>(A.q.p) + b * A.q.sb + (long long)(h / A.q.group) * A.q.sh;
+      const int hq = h / A.q.group;
+      const bf16* qp = static_cast<const bf16*>(A.q.p) + b * A.q.sb + hq * A.q.sh;
       for (int i = 0; i < chunks; ++i) {
         if (i) wait(kDoneR, i - 1);
-        load_tile<DK>(smem + L::q, qp, A.q.sl, min(kT, n_all - i * kT), 0, A.DK, t_first + (long long)i * kT * step, step,
-                      A.vec);
-        cp_wait();
-        hand_over(&bar[kFullQ]);
+        if (M.on && tokens(i) == kT) {
+          if (lane == 0) {
+            expect(&bar[kFullQ], L::qk);
+            load_box<DK>(umma::su32(smem + L::q), &M.q, &bar[kFullQ], 0, hq, (int)first(i), (int)b);
+          }
+          __syncwarp();
+        } else {
+          load_tile<DK>(smem + L::q, qp, A.q.sl, tokens(i), 0, A.DK, first(i), A.vec);
+          cp_wait();
+          hand_over(&bar[kFullQ]);
+        }
       }
     }
   } else if (warp == kIssuer) {
@@ -291,15 +331,17 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A) {
         }
         __syncwarp();
       }
-      wait(kHaveS, i);
-      wait(kHaveV, i);
+      const int wb = i % L::wbuf;
+      wait(kHaveS + wb, i / L::wbuf);
+      wait(kHaveV + wb, i / L::wbuf);
       if (elect()) {
 #pragma unroll
         for (int y = 0; y < TERMS; ++y)
 #pragma unroll
           for (int x = 0; x < kT / 16; ++x)
-            umma::mma(tmem + kColS, tile_desc(sk + x * 2048), tile_desc(sw + y * kTile + x * 2048), kIdS, x + y > 0);
-        umma::commit(&bar[kDoneS]);
+            umma::mma(tmem + kColS - 64 * wb, tile_desc(sk + x * 2048), tile_desc(sw + (wb * TERMS + y) * kTile + x * 2048), kIdS,
+                      x + y > 0);
+        umma::commit(&bar[kDoneS + wb]);
         if (!OUT) umma::commit(&bar[kEmpty + buf]);
       }
       __syncwarp();
@@ -327,11 +369,17 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A) {
     // This thread's part of a 64 x 64 product: rows row and row + 8, columns half + 8 j + pair + {0, 1}, j < 4. Of a
     // state of 128 rows it has two such parts, 16 TMEM lanes apart (SB).
     constexpr int SB = DK / 64;
+    const float g = A.log_decay[h];
+    const auto power = [&](int n) {  // a^n as the sum of two floats
+      const double an = exp((double)g * n);
+      return make_float2((float)an, (float)(an - (double)(float)an));
+    };
+    if (tid <= 2 * kT) tab[tid] = tid < kT ? 0.f : tid == kT ? 1.f : expf(g * (tid - kT));
+    const float2 a64 = power(kT);
     const int wq = warp & 3, half = (warp >> 2) * 32;
     const int row = wq * 16 + (lane >> 2), pair = 2 * (lane & 3);
     const int srow = SB == 1 ? row : wq * 32 + (lane >> 2);
     const uint32_t lanes = tmem + ((uint32_t)(wq * 32) << 16) + half;
-    const float a64hi = (float)exp(g * kT), a64lo = (float)(exp(g * kT) - (double)a64hi);
     const long long per_state = (long long)A.DK * A.DV;
     const int left = A.DV - c0 - half - pair;  // columns from this thread's first on that exist
     float S[SB][16];
@@ -365,15 +413,17 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A) {
         }
       if (OUT) put_state();
       hand_over(&bar[kHaveS]);
+      if (L::wbuf == 2) hand_over(&bar[kHaveS + 1]);
     }
     // The V of chunk i, decayed, in TERMS terms.
     const auto split_v = [&](int i) {
-      const int n = min(kT, n_all - i * kT);
+      unsigned char* terms = smem + L::w + i % L::wbuf * (TERMS * kTile);
+      const int n = tokens(i);
       const unsigned char* v = smem + L::v + (i & 1) * kTile;
 #pragma unroll
       for (int x = 0; x < kT * kC / 8 / kThreads; ++x) {
         const int at = tid + x * kThreads, t = at >> 3;  // V's place in the tile is its terms' place
-        const float w = t < n ? tab[kT + n - t - lag] * A.vscale : 0.f;
+        const float w = t < n ? tab[kT + (rev ? t + 1 : n - 1 - t)] * A.vscale : 0.f;
         const uint4 u = *reinterpret_cast<const uint4*>(v + at * 16);
         uint4 hi, mid, lo;
 #pragma unroll
@@ -389,28 +439,29 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A) {
             (&lo.x)[e] = pack2(f.x, f.y);
           }
         }
-        *reinterpret_cast<uint4*>(smem + L::w + at * 16) = hi;
-        *reinterpret_cast<uint4*>(smem + L::w + kTile + at * 16) = mid;
-        if (TERMS == 3) *reinterpret_cast<uint4*>(smem + L::w + 2 * kTile + at * 16) = lo;
+        *reinterpret_cast<uint4*>(terms + at * 16) = hi;
+        *reinterpret_cast<uint4*>(terms + kTile + at * 16) = mid;
+        if (TERMS == 3) *reinterpret_cast<uint4*>(terms + 2 * kTile + at * 16) = lo;
       }
+      hand_over(&bar[kHaveV + i % L::wbuf]);
     };
     TO* op = static_cast<TO*>(A.o) + (OUT ? b * A.ob + (long long)h * A.oh + c0 + half + pair : 0);
+    asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory");  // the table
     if (chunks) {
       wait(kFull, 0);
       split_v(0);
-      hand_over(&bar[kHaveV]);
     }
-    // a^(i - j) of this thread's part of P: entries 2 m, 2 m + 1 for columns 8 (m - 1), + 1 of its first row. In
-    // registers where there is room.
-    const float* tb = tab + kT + row - half - pair + 8;
+    // a^|row - column| of this thread's part of P, zero where the column is later in scan order: entries 2 m, 2 m + 1 for
+    // columns 8 (m - 1), + 1 of its first row. In registers where there is room.
+    const float* tb = tab + kT + (rev ? half + pair - 8 - row : row - half - pair + 8);
+    const int along = rev ? 1 : -1;
     float dec[SB == 1 ? 10 : 1];
     if (SB == 1)
 #pragma unroll
-      for (int m = 0; m < (SB == 1 ? 10 : 1); ++m) dec[m] = tb[-8 * (m / 2) - (m & 1)];
-    const auto decay = [&](int m) { return SB == 1 ? dec[SB == 1 ? m : 0] : tb[-8 * (m / 2) - (m & 1)]; };
-    const float rs0 = tab[kT + row + lag] * A.oscale, rs1 = tab[kT + row + 8 + lag] * A.oscale;
+      for (int m = 0; m < (SB == 1 ? 10 : 1); ++m) dec[m] = tb[along * (8 * (m / 2) + (m & 1))];
+    const auto decay = [&](int m) { return SB == 1 ? dec[SB == 1 ? m : 0] : tb[along * (8 * (m / 2) + (m & 1))]; };
     for (int i = 0; i < chunks; ++i) {
-      const int n = min(kT, n_all - i * kT);
+      const int n = tokens(i);
       if (OUT) {  // P
         wait(kDoneP, i);
         uint32_t p[16];
@@ -425,24 +476,28 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A) {
         }
         hand_over(&bar[kHaveP]);
       }
-      {  // the state
-        float hi = a64hi, lo = a64lo;
-        if (n != kT) {
-          const double an = exp(g * n);
-          hi = (float)an, lo = (float)(an - (double)hi);
+      const auto next_v = [&] {
+        if (i + 1 < chunks) {
+          wait(kFull + ((i + 1) & 1), (i + 1) >> 1);
+          split_v(i + 1);
         }
+      };
+      if (!OUT) next_v();  // both buffers are in use: the split runs beside the last chunk's product
+      {  // the state
+        const float2 an = n == kT ? a64 : power(n);
         if (OUT) wait(kDoneR, i);
-        wait(kDoneS, i);
+        wait(kDoneS + i % L::wbuf, i / L::wbuf);
 #pragma unroll
         for (int y = 0; y < SB; ++y) {
           uint32_t d[16];
-          tmem_ld(lanes + kColS + ((uint32_t)(16 * y) << 16), d);
+          tmem_ld(lanes + kColS - 64 * (i % L::wbuf) + ((uint32_t)(16 * y) << 16), d);
 #pragma unroll
-          for (int r = 0; r < 16; ++r) S[y][r] = fmaf(S[y][r], hi, fmaf(S[y][r], lo, __uint_as_float(d[r])));
+          for (int r = 0; r < 16; ++r) S[y][r] = fmaf(S[y][r], an.x, fmaf(S[y][r], an.y, __uint_as_float(d[r])));
         }
         if (OUT) put_state();
-        hand_over(&bar[kHaveS]);
+        hand_over(&bar[kHaveS + i % L::wbuf]);
       }
+      if (OUT) next_v();
       if (OUT) {  // the outputs
         wait(kDoneO, i);
         uint32_t r[16], o[16];
@@ -457,8 +512,8 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A) {
 #pragma unroll
         for (int y = 0; y < 2; ++y) {
           const int rw = row + 8 * y;
-          const float rs = y ? rs1 : rs0;
-          TO* d = op + (t_first + (long long)(i * kT + rw) * step) * A.ol;
+          const float rs = tab[kT + (rev ? n - 1 - rw : rw + 1)] * A.oscale;
+          TO* d = op + (first(i) + rw) * A.ol;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int at = 4 * j + 2 * y;
@@ -484,15 +539,10 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A) {
             const int rw = row + 8 * y;
             const uint4 u = *reinterpret_cast<const uint4*>(smem + L::p + swz(rw, c));
             if (rw < n && c0 + c < A.DV)
-              *reinterpret_cast<uint4*>(op - half - pair + (t_first + (long long)(i * kT + rw) * step) * A.ol + c) = u;
+              *reinterpret_cast<uint4*>(op - half - pair + (first(i) + rw) * A.ol + c) = u;
           }
           __syncwarp();
         }
-      }
-      if (i + 1 < chunks) {
-        wait(kFull + ((i + 1) & 1), (i + 1) >> 1);
-        split_v(i + 1);
-        hand_over(&bar[kHaveV]);
       }
     }
     if (OUT) {  // tokens past the length: zeros
@@ -526,31 +576,66 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A) {
   if (warp == 0) umma::tmem_dealloc(tmem, kTmemCols);
 }
 
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+  static std::once_flag once;
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+  });
+  return fn;
+}
+
+// False where TMA cannot address the tensor (a head size, an address or a stride off 16 bytes, a stride of zero).
+bool make_map(CUtensorMap* m, const ScanOp& x, int D, int heads, int L, int B) {
+  PFN_cuTensorMapEncodeTiled_v12000 enc = encode_fn();
+  if (!enc || !x.p) return false;
+  const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)heads, (cuuint64_t)L, (cuuint64_t)B};
+  const long long s[3] = {x.sh, x.sl, x.sb};
+  cuuint64_t strides[3];
+  for (int i = 0; i < 3; ++i) {
+    const long long bytes = dims[i + 1] == 1 ? (long long)((D + 7) / 8 * 16) : 2 * s[i];  // one of them: never stepped over
+    if (bytes <= 0 || bytes % 16 || bytes >= (1ll << 40)) return false;
+    strides[i] = (cuuint64_t)bytes;
+  }
+  const cuuint32_t box[4] = {64, 1, kT, 1}, one[4] = {1, 1, 1, 1};
+  return enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(x.p), dims, strides, box, one,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <int DK, bool OUT, int TERMS, typename TO>
-int launch(const ScanArgs& A, long long ctas, cudaStream_t st) {
+int launch(const ScanArgs& A, const Maps& M, long long ctas, cudaStream_t st) {
   auto kern = decay_mma_kernel<DK, OUT, TERMS, TO>;
   constexpr size_t sm = Layout<DK, OUT, TERMS>::bytes;
   if (!kernel_smem_once((const void*)kern, sm, true)) return set_error(HYFFT_ERR_CUDA, "decay attention: shared memory");
-  kern<<<(unsigned)ctas, kAll, sm, st>>>(A);
+  kern<<<(unsigned)ctas, kAll, sm, st>>>(A, M);
   if (cudaGetLastError() != cudaSuccess) return set_error(HYFFT_ERR_CUDA, "decay attention: kernel launch failed");
   g_launches.fetch_add(1, std::memory_order_relaxed);
   return HYFFT_OK;
 }
 
 template <int DK>
-int launch_dk(const ScanArgs& A, bool out_f32, long long ctas, cudaStream_t st) {
-  if (!A.o) return launch<DK, false, 3, bf16>(A, ctas, st);
+int launch_dk(const ScanArgs& A, const Maps& M, bool out_f32, long long ctas, cudaStream_t st) {
+  if (!A.o) return launch<DK, false, 3, bf16>(A, M, ctas, st);
   // where segments were added up before, the state only serves this pass's outputs, which read it rounded to 8 bits: 16
   // bits are enough (not by whether the caller wants the final state, so that asking for it changes no output)
-  if (A.nseg == 1) return out_f32 ? launch<DK, true, 3, float>(A, ctas, st) : launch<DK, true, 3, bf16>(A, ctas, st);
-  return out_f32 ? launch<DK, true, 2, float>(A, ctas, st) : launch<DK, true, 2, bf16>(A, ctas, st);
+  if (A.nseg == 1) return out_f32 ? launch<DK, true, 3, float>(A, M, ctas, st) : launch<DK, true, 3, bf16>(A, M, ctas, st);
+  return out_f32 ? launch<DK, true, 2, float>(A, M, ctas, st) : launch<DK, true, 2, bf16>(A, M, ctas, st);
 }
 
 }  // namespace
 
 int launch_scan_mma(const ScanArgs& A, bool out_f32, long long ctas, cudaStream_t st) {
   if (ctas > 0x7fffffffLL) return set_error(HYFFT_ERR_UNSUPPORTED, "decay attention: too many rows");
-  return A.DK <= 64 ? launch_dk<64>(A, out_f32, ctas, st) : launch_dk<128>(A, out_f32, ctas, st);
+  Maps M{};
+  M.on = A.L >= kT && A.vec && make_map(&M.k, A.k, A.DK, A.H / A.k.group, A.L, A.B) &&
+         make_map(&M.v, A.v, A.DV, A.H / A.v.group, A.L, A.B) &&
+         (!A.o || make_map(&M.q, A.q, A.DK, A.H / A.q.group, A.L, A.B));
+  return A.DK <= 64 ? launch_dk<64>(A, M, out_f32, ctas, st) : launch_dk<128>(A, M, out_f32, ctas, st);
 }
 
 }  // namespace hyfft
