@@ -6,7 +6,10 @@
 // Both passes are bound by HBM bandwidth: x is read once and y written once forwards, x and dy read and dx written backwards.
 // A row is held in the registers of a group of 32 .. 512 threads (kPer = 8, 16 or 32 elements each), so the mean and
 // then the centred squares are summed from registers: two reductions, no cancellation between E[x^2] and
-// E[x]^2. Groups walk over the rows with the weights in registers and the next row's loads in flight. The weight's and the bias's
+// E[x]^2. Groups walk over the rows with the weights in registers. Rows that start on 16 bytes come through a ring of up
+// to four in shared memory for each group, filled by bulk copies: HBM's latency needs 35 KB in flight on an SM, which
+// registers would not hold (one row ahead in registers: 314 us forwards, 422 backwards for 65536 rows of 4096 bfloat16;
+// ring: @RING@). Other rows are loaded one ahead into registers. The weight's and the bias's
 // gradients stay in each thread's registers over all rows of its group; a CTA adds its groups' sums in shared memory,
 // writes one partial row, and a second kernel adds those rows in a fixed order: no atomics, the same bits every run.
 #include <cuda_bf16.h>
@@ -15,9 +18,13 @@
 
 #include <algorithm>
 #include <atomic>
+#include <map>
+#include <mutex>
+#include <tuple>
 
 #include "../../include/hyfft.h"
 #include "common.cuh"
+#include "umma.cuh"
 
 namespace hyfft {
 
@@ -27,6 +34,7 @@ int set_error(int code, const char* msg);  // engine.cu: the message hyfft_last_
 namespace {
 
 constexpr int kMaxRow = 512 * 32;  // widest row held in registers
+constexpr int kMaxGroups = 8, kMaxWarps = 16, kStages = 4;
 constexpr int kLoopThreads = 512;  // threads of the kernels for wider rows
 
 struct NormArgs {
@@ -36,7 +44,7 @@ struct NormArgs {
   float *part;           // [ctas, 2, C]
   long long rows, xs, ds;  // row strides of x and dy; y and dx are contiguous
   int C, tpr, groups;
-  int w32;  // weight and bias are float32
+  int stages;  // rows in a group's ring
   float eps, invC;
 };
 
@@ -46,42 +54,115 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
-// Sums of (a, b) over the group's threads; `slot` alternates between calls, so one barrier is enough.
-__device__ __forceinline__ float2 group_sum(float2 v, int tpr, int group, float2 (*red)[16], int& slot) {
+// A group's warps leave their sums in shared memory and every thread adds all of them (read as 16-byte broadcasts).
+// `slot` alternates between calls, so that one barrier is enough.
+struct Sums {
+  float4 v[2][kMaxGroups][kMaxWarps / 4];
+};
+__device__ __forceinline__ float read_sums(const float4* r, int warps) {
+  float s = 0.f;
+  for (int i = 0; i < warps; i += 4) {  // the entries past the last warp are zero
+    const float4 q = r[i >> 2];
+    s += (q.x + q.y) + (q.z + q.w);
+  }
+  return s;
+}
+__device__ __forceinline__ float group_sum(float v, int tpr, int group, Sums& sm, int& slot) {
+  v = warp_sum(v);
+  if (tpr == 32) return v;
+  const int t = threadIdx.x - group * tpr;
+  float4* r = sm.v[slot][group];
+  slot ^= 1;
+  if ((t & 31) == 0) reinterpret_cast<float*>(r)[t >> 5] = v;
+  asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(tpr) : "memory");
+  return read_sums(r, tpr >> 5);
+}
+__device__ __forceinline__ float2 group_sum(float2 v, int tpr, int group, Sums& sx, Sums& sy, int& slot) {
   v.x = warp_sum(v.x);
   v.y = warp_sum(v.y);
   if (tpr == 32) return v;
   const int t = threadIdx.x - group * tpr;
-  float2* r = red[group * 3 + slot];
-  slot = slot == 2 ? 0 : slot + 1;
-  if ((t & 31) == 0) r[t >> 5] = v;
+  float4 *x = sx.v[slot][group], *y = sy.v[slot][group];
+  slot ^= 1;
+  if ((t & 31) == 0) reinterpret_cast<float*>(x)[t >> 5] = v.x, reinterpret_cast<float*>(y)[t >> 5] = v.y;
   asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(tpr) : "memory");
-  const int n = tpr >> 5;
-  float2 s = r[0];
-  for (int i = 1; i < n; ++i) s = cadd(s, r[i]);
-  return s;
+  return make_float2(read_sums(x, tpr >> 5), read_sums(y, tpr >> 5));
+}
+// All entries zero, before the first sum.
+__device__ __forceinline__ void clear(Sums& s) {
+  float* f = reinterpret_cast<float*>(&s);
+  for (int i = threadIdx.x; i < (int)(sizeof(Sums) / sizeof(float)); i += blockDim.x) f[i] = 0.f;
 }
 
-// Element e of a thread's kPer: column (t + tpr * (e / V)) * V + e % V.
-template <typename T, int V, int PER>
+// One row (or two, of x and dy) into a place of the ring; one thread.
+__device__ __forceinline__ void bulk_row(unsigned char* dst, const void* src, int bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(umma::su32(dst)),
+               "l"(src), "r"(bytes), "r"(umma::su32(bar))
+               : "memory");
+}
+__device__ __forceinline__ void expect(uint64_t* bar, int bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(umma::su32(bar)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void init_ring(uint64_t (*full)[kStages]) {
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kMaxGroups * kStages; ++i) umma::mbar_init(&full[0][i], 1);
+    umma::fence_mbar_init();
+  }
+}
+
+// A thread's PER elements as PER / 2 pairs, so that the arithmetic runs as packed float32 pairs: element e is column
+// (t + tpr * (e / V)) * V + e % V. Places past C hold zeros (WHOLE: there are none, C = tpr * PER).
+template <typename T>
+__device__ __forceinline__ float2 two(const T* p) {
+  return make_float2(DT<T>::load(p), DT<T>::load(p + 1));
+}
+template <>
+__device__ __forceinline__ float2 two<__nv_bfloat16>(const __nv_bfloat16* p) {
+  const uint32_t u = *reinterpret_cast<const uint32_t*>(p);
+  return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+}
+template <>
+__device__ __forceinline__ float2 two<__half>(const __half* p) {
+  return __half22float2(*reinterpret_cast<const __half2*>(p));
+}
+template <typename T>
+__device__ __forceinline__ void put_two(T* p, float2 v) {
+  DT<T>::store(p, v.x);
+  DT<T>::store(p + 1, v.y);
+}
+template <>
+__device__ __forceinline__ void put_two<__nv_bfloat16>(__nv_bfloat16* p, float2 v) {
+  *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(v.x, v.y);
+}
+template <>
+__device__ __forceinline__ void put_two<__half>(__half* p, float2 v) {
+  *reinterpret_cast<__half2*>(p) = __floats2half2_rn(v.x, v.y);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) { return make_float2(a.x * b.x, a.y * b.y); }
+__device__ __forceinline__ float2 dup(float a) { return make_float2(a, a); }
+
+template <int V>
+__device__ __forceinline__ int column(int e, int t, int tpr) {
+  return (t + tpr * (e / V)) * V + e % V;
+}
+template <typename T, int V, int PER, bool WHOLE>
 __device__ __forceinline__ void load_row(T (&e)[PER], const T* __restrict__ p, int t, int tpr, int C) {
 #pragma unroll
   for (int j = 0; j < PER / V; ++j) {
     const int c = (t + tpr * j) * V;
-    if (c < C) {
-      if constexpr (V > 1)
-        *reinterpret_cast<uint4*>(e + j * V) = *reinterpret_cast<const uint4*>(p + c);
-      else
-        e[j] = p[c];
-    }
+    const bool in = WHOLE || c < C;
+    if constexpr (V > 1)
+      *reinterpret_cast<uint4*>(e + j * V) = in ? *reinterpret_cast<const uint4*>(p + c) : make_uint4(0, 0, 0, 0);
+    else
+      DT<T>::store(e + j, in ? DT<T>::load(p + c) : 0.f);
   }
 }
-template <typename T, int V, int PER>
+template <typename T, int V, int PER, bool WHOLE>
 __device__ __forceinline__ void store_row(T* __restrict__ p, const T (&e)[PER], int t, int tpr, int C) {
 #pragma unroll
   for (int j = 0; j < PER / V; ++j) {
     const int c = (t + tpr * j) * V;
-    if (c < C) {
+    if (WHOLE || c < C) {
       if constexpr (V > 1)
         *reinterpret_cast<uint4*>(p + c) = *reinterpret_cast<const uint4*>(e + j * V);
       else
@@ -89,118 +170,178 @@ __device__ __forceinline__ void store_row(T* __restrict__ p, const T (&e)[PER], 
     }
   }
 }
-template <typename T>
-__device__ __forceinline__ float param(const void* p, int c, int w32) {
-  return w32 ? static_cast<const float*>(p)[c] : DT<T>::load(static_cast<const T*>(p) + c);
+// Pairs that lie past C are zeroed (with V = 1 the two halves of a pair are tpr columns apart).
+template <int V, bool WHOLE>
+__device__ __forceinline__ float2 inside(float2 v, int e, int t, int tpr, int C) {
+  if (WHOLE) return v;
+  const bool a = column<V>(e, t, tpr) < C, b = V > 1 ? a : column<V>(e + 1, t, tpr) < C;
+  return make_float2(a ? v.x : 0.f, b ? v.y : 0.f);
 }
-
-template <typename T, int V, int PER>
-__global__ void __launch_bounds__(512) layer_norm_fwd_kernel(const NormArgs A) {
-  __shared__ float2 red[15 * 3][16];
-  const int group = threadIdx.x / A.tpr, t = threadIdx.x - group * A.tpr;
-  int slot = 0;
-  float w[PER], b[PER];
+template <typename P, int V, int PER>
+__device__ __forceinline__ void load_param(float2 (&f)[PER / 2], const void* p, float none, int t, int tpr, int C) {
 #pragma unroll
   for (int e = 0; e < PER; ++e) {
-    const int c = (t + A.tpr * (e / V)) * V + e % V;
-    w[e] = A.w && c < A.C ? param<T>(A.w, c, A.w32) : 1.f;
-    b[e] = A.b && c < A.C ? param<T>(A.b, c, A.w32) : 0.f;
+    const int c = column<V>(e, t, tpr);
+    (&f[e / 2].x)[e & 1] = p && c < C ? DT<P>::load(static_cast<const P*>(p) + c) : none;
   }
+}
+
+template <typename T, typename P, int V, int PER, bool WHOLE>
+__global__ void __launch_bounds__(512) layer_norm_fwd_kernel(const NormArgs A) {
+  extern __shared__ __align__(16) unsigned char ring[];  // [groups, stages, C]
+  __shared__ uint64_t full[kMaxGroups][kStages];
+  __shared__ Sums sums;
+  clear(sums);
+  init_ring(full);
+  __syncthreads();
+  const int group = threadIdx.x / A.tpr, t = threadIdx.x - group * A.tpr;
+  int slot = 0;
+  float2 w[PER / 2], b[PER / 2];
+  load_param<P, V, PER>(w, A.w, 1.f, t, A.tpr, A.C);
+  load_param<P, V, PER>(b, A.b, 0.f, t, A.tpr, A.C);
   const long long step = (long long)gridDim.x * A.groups;
   long long row = (long long)blockIdx.x * A.groups + group;
   const T* x = static_cast<const T*>(A.x);
   T* y = static_cast<T*>(A.y);
+  constexpr bool kRing = V > 1;
+  const int bytes = A.C * (int)sizeof(T);
+  unsigned char* mine = ring + (size_t)group * A.stages * bytes;
+  const auto fetch = [&](int i, long long r) {
+    expect(&full[group][i], bytes);
+    bulk_row(mine + (size_t)i * bytes, x + r * A.xs, bytes, &full[group][i]);
+  };
   alignas(16) T cur[PER];
-  if (row < A.rows) load_row<T, V, PER>(cur, x + row * A.xs, t, A.tpr, A.C);
+  if (kRing) {
+    if (t == 0)
+      for (int i = 0; i < A.stages; ++i)
+        if (row + i * step < A.rows) fetch(i, row + i * step);
+  } else if (row < A.rows) {
+    load_row<T, V, PER, WHOLE>(cur, x + row * A.xs, t, A.tpr, A.C);
+  }
+  int at = 0, phase = 0;
+  bool ok = true;  // false once a wait has run out: NaN in what is written
   for (; row < A.rows; row += step) {
-    float f[PER];
-    float s = 0.f;
-#pragma unroll
-    for (int e = 0; e < PER; ++e) {
-      const int c = (t + A.tpr * (e / V)) * V + e % V;
-      f[e] = c < A.C ? DT<T>::load(cur + e) : 0.f;
-      s += f[e];
+    if (kRing) {
+      ok = ok && umma::mbar_wait(&full[group][at], phase);
+      load_row<T, V, PER, WHOLE>(cur, reinterpret_cast<const T*>(mine + (size_t)at * bytes), t, A.tpr, A.C);
     }
-    if (row + step < A.rows) load_row<T, V, PER>(cur, x + (row + step) * A.xs, t, A.tpr, A.C);
-    const float mean = group_sum(make_float2(s, 0.f), A.tpr, group, red, slot).x * A.invC;
-    s = 0.f;
+    float2 f[PER / 2], s2 = dup(0.f);
 #pragma unroll
-    for (int e = 0; e < PER; ++e) {
-      const int c = (t + A.tpr * (e / V)) * V + e % V;
-      f[e] -= mean;
-      if (c < A.C) s = fmaf(f[e], f[e], s);
+    for (int p = 0; p < PER / 2; ++p) {
+      f[p] = two<T>(cur + 2 * p);
+      s2 = cadd(s2, f[p]);
     }
-    const float var = group_sum(make_float2(s, 0.f), A.tpr, group, red, slot).x * A.invC;
-    const float rstd = 1.f / sqrtf(var + A.eps);
+    if (!kRing && row + step < A.rows) load_row<T, V, PER, WHOLE>(cur, x + (row + step) * A.xs, t, A.tpr, A.C);
+    const float mean = group_sum(s2.x + s2.y, A.tpr, group, sums, slot) * A.invC;
+    if (kRing) {  // every thread of the group has read its part of the row
+      if (t == 0 && row + A.stages * step < A.rows) fetch(at, row + A.stages * step);
+      if (++at == A.stages) at = 0, phase ^= 1;
+    }
+    s2 = dup(0.f);
+#pragma unroll
+    for (int p = 0; p < PER / 2; ++p) {
+      f[p] = inside<V, WHOLE>(csub(f[p], dup(mean)), 2 * p, t, A.tpr, A.C);
+      s2 = ffma2(f[p], f[p], s2);
+    }
+    const float var = group_sum(s2.x + s2.y, A.tpr, group, sums, slot) * A.invC;
+    const float rstd = ok ? 1.f / sqrtf(var + A.eps) : __int_as_float(0x7fffffff);
     alignas(16) T o[PER];
 #pragma unroll
-    for (int e = 0; e < PER; ++e) DT<T>::store(o + e, fmaf(f[e] * rstd, w[e], b[e]));
-    store_row<T, V, PER>(y + row * A.C, o, t, A.tpr, A.C);
+    for (int p = 0; p < PER / 2; ++p) put_two<T>(o + 2 * p, ffma2(mul2(f[p], dup(rstd)), w[p], b[p]));
+    store_row<T, V, PER, WHOLE>(y + row * A.C, o, t, A.tpr, A.C);
     if (t == 0 && A.mean) A.mean[row] = mean, A.rstd[row] = rstd;
   }
 }
 
-template <typename T, int V, int PER>
+template <typename T, typename P, int V, int PER, bool WHOLE>
 __global__ void __launch_bounds__(512) layer_norm_bwd_kernel(const NormArgs A) {
-  __shared__ float2 red[15 * 3][16];
-  extern __shared__ float sums[];  // [groups, 2, C] where there is more than one group
+  extern __shared__ __align__(16) unsigned char ring[];  // [groups, stages, 2, C]; at the end the groups' sums [groups, 2, C]
+  float* sums = reinterpret_cast<float*>(ring);
+  __shared__ uint64_t full[kMaxGroups][kStages];
+  __shared__ Sums sx, sy;
+  clear(sx);
+  clear(sy);
+  init_ring(full);
+  __syncthreads();
   const int group = threadIdx.x / A.tpr, t = threadIdx.x - group * A.tpr;
   int slot = 0;
-  float w[PER], dw[PER], db[PER];
+  float2 w[PER / 2], dw[PER / 2], db[PER / 2];
+  load_param<P, V, PER>(w, A.w, 1.f, t, A.tpr, A.C);
 #pragma unroll
-  for (int e = 0; e < PER; ++e) {
-    const int c = (t + A.tpr * (e / V)) * V + e % V;
-    w[e] = A.w && c < A.C ? param<T>(A.w, c, A.w32) : 1.f;
-    dw[e] = db[e] = 0.f;
-  }
+  for (int p = 0; p < PER / 2; ++p) dw[p] = db[p] = dup(0.f);
   const long long step = (long long)gridDim.x * A.groups;
   long long row = (long long)blockIdx.x * A.groups + group;
   const T* x = static_cast<const T*>(A.x);
   const T* dy = static_cast<const T*>(A.dy);
+  constexpr bool kRing = V > 1;
+  const int bytes = A.C * (int)sizeof(T);
+  unsigned char* mine = ring + (size_t)group * A.stages * 2 * bytes;
+  const auto fetch = [&](int i, long long r) {
+    expect(&full[group][i], 2 * bytes);
+    bulk_row(mine + (size_t)i * 2 * bytes, x + r * A.xs, bytes, &full[group][i]);
+    bulk_row(mine + ((size_t)i * 2 + 1) * bytes, dy + r * A.ds, bytes, &full[group][i]);
+  };
   alignas(16) T cx[PER];
   alignas(16) T cd[PER];
   float mean = 0.f, rstd = 0.f;
-  if (row < A.rows) {
-    load_row<T, V, PER>(cx, x + row * A.xs, t, A.tpr, A.C);
-    load_row<T, V, PER>(cd, dy + row * A.ds, t, A.tpr, A.C);
-    mean = A.mean[row], rstd = A.rstd[row];
+  if (row < A.rows) mean = A.mean[row], rstd = A.rstd[row];
+  if (kRing) {
+    if (t == 0)
+      for (int i = 0; i < A.stages; ++i)
+        if (row + i * step < A.rows) fetch(i, row + i * step);
+  } else if (row < A.rows) {
+    load_row<T, V, PER, WHOLE>(cx, x + row * A.xs, t, A.tpr, A.C);
+    load_row<T, V, PER, WHOLE>(cd, dy + row * A.ds, t, A.tpr, A.C);
   }
+  int at = 0, phase = 0;
+  bool ok = true;  // false once a wait has run out: NaN in what is written
   for (; row < A.rows; row += step) {
-    float h[PER], g[PER];
-    float2 s = make_float2(0.f, 0.f);
-#pragma unroll
-    for (int e = 0; e < PER; ++e) {
-      const int c = (t + A.tpr * (e / V)) * V + e % V;
-      const float d = c < A.C ? DT<T>::load(cd + e) : 0.f;
-      h[e] = c < A.C ? (DT<T>::load(cx + e) - mean) * rstd : 0.f;
-      g[e] = d * w[e];
-      dw[e] = fmaf(d, h[e], dw[e]);
-      db[e] += d;
-      s.x += g[e];
-      s.y = fmaf(g[e], h[e], s.y);
+    if (kRing) {
+      ok = ok && umma::mbar_wait(&full[group][at], phase);
+      load_row<T, V, PER, WHOLE>(cx, reinterpret_cast<const T*>(mine + (size_t)at * 2 * bytes), t, A.tpr, A.C);
+      load_row<T, V, PER, WHOLE>(cd, reinterpret_cast<const T*>(mine + ((size_t)at * 2 + 1) * bytes), t, A.tpr, A.C);
     }
-    const float r = rstd;
+    const float r = ok ? rstd : __int_as_float(0x7fffffff);
+    float2 h[PER / 2], g[PER / 2], s1 = dup(0.f), s2 = dup(0.f);
+#pragma unroll
+    for (int p = 0; p < PER / 2; ++p) {
+      const float2 d = two<T>(cd + 2 * p);  // zero past C, and so is all that it multiplies
+      h[p] = mul2(csub(two<T>(cx + 2 * p), dup(mean)), dup(r));
+      g[p] = mul2(d, w[p]);
+      dw[p] = ffma2(d, h[p], dw[p]);
+      db[p] = cadd(db[p], d);
+      s1 = cadd(s1, g[p]);
+      s2 = ffma2(g[p], h[p], s2);
+    }
     if (row + step < A.rows) {
-      load_row<T, V, PER>(cx, x + (row + step) * A.xs, t, A.tpr, A.C);
-      load_row<T, V, PER>(cd, dy + (row + step) * A.ds, t, A.tpr, A.C);
+      if (!kRing) {
+        load_row<T, V, PER, WHOLE>(cx, x + (row + step) * A.xs, t, A.tpr, A.C);
+        load_row<T, V, PER, WHOLE>(cd, dy + (row + step) * A.ds, t, A.tpr, A.C);
+      }
       mean = A.mean[row + step], rstd = A.rstd[row + step];
     }
-    s = group_sum(s, A.tpr, group, red, slot);
+    float2 s = group_sum(make_float2(s1.x + s1.y, s2.x + s2.y), A.tpr, group, sx, sy, slot);
+    if (kRing) {  // every thread of the group has read its part of both rows
+      if (t == 0 && row + A.stages * step < A.rows) fetch(at, row + A.stages * step);
+      if (++at == A.stages) at = 0, phase ^= 1;
+    }
     s.x *= A.invC, s.y *= A.invC;
     if (A.dx) {
       alignas(16) T o[PER];
 #pragma unroll
-      for (int e = 0; e < PER; ++e) DT<T>::store(o + e, r * (g[e] - s.x - h[e] * s.y));
-      store_row<T, V, PER>(static_cast<T*>(A.dx) + row * A.C, o, t, A.tpr, A.C);
+      for (int p = 0; p < PER / 2; ++p)
+        put_two<T>(o + 2 * p, mul2(csub(ffma2(h[p], dup(-s.y), g[p]), dup(s.x)), dup(r)));
+      store_row<T, V, PER, WHOLE>(static_cast<T*>(A.dx) + row * A.C, o, t, A.tpr, A.C);
     }
   }
   if (!A.part) return;
+  __syncthreads();  // the ring is read
   float* out = A.part + (long long)blockIdx.x * 2 * A.C;
   float* to = A.groups == 1 ? out : sums + (long long)group * 2 * A.C;
 #pragma unroll
   for (int e = 0; e < PER; ++e) {
-    const int c = (t + A.tpr * (e / V)) * V + e % V;
-    if (c < A.C) to[c] = dw[e], to[A.C + c] = db[e];
+    const int c = column<V>(e, t, A.tpr);
+    if (WHOLE || c < A.C) to[c] = (&dw[e / 2].x)[e & 1], to[A.C + c] = (&db[e / 2].x)[e & 1];
   }
   if (A.groups == 1) return;
   __syncthreads();
@@ -212,25 +353,25 @@ __global__ void __launch_bounds__(512) layer_norm_bwd_kernel(const NormArgs A) {
 }
 
 // Rows wider than the registers of 512 threads: one CTA per row, the row read again for each sum.
-template <typename T>
+template <typename T, typename P>
 __global__ void __launch_bounds__(kLoopThreads) layer_norm_fwd_loop_kernel(const NormArgs A) {
-  __shared__ float2 red[3][16];
+  __shared__ Sums sums;
   int slot = 0;
   for (long long row = blockIdx.x; row < A.rows; row += gridDim.x) {
     const T* x = static_cast<const T*>(A.x) + row * A.xs;
     T* y = static_cast<T*>(A.y) + row * A.C;
     float s = 0.f;
     for (int c = threadIdx.x; c < A.C; c += kLoopThreads) s += DT<T>::load(x + c);
-    const float mean = group_sum(make_float2(s, 0.f), kLoopThreads, 0, red, slot).x * A.invC;
+    const float mean = group_sum(s, kLoopThreads, 0, sums, slot) * A.invC;
     s = 0.f;
     for (int c = threadIdx.x; c < A.C; c += kLoopThreads) {
       const float d = DT<T>::load(x + c) - mean;
       s = fmaf(d, d, s);
     }
-    const float var = group_sum(make_float2(s, 0.f), kLoopThreads, 0, red, slot).x * A.invC;
+    const float var = group_sum(s, kLoopThreads, 0, sums, slot) * A.invC;
     const float rstd = 1.f / sqrtf(var + A.eps);
     for (int c = threadIdx.x; c < A.C; c += kLoopThreads) {
-      const float w = A.w ? param<T>(A.w, c, A.w32) : 1.f, b = A.b ? param<T>(A.b, c, A.w32) : 0.f;
+      const float w = A.w ? DT<P>::load(static_cast<const P*>(A.w) + c) : 1.f, b = A.b ? DT<P>::load(static_cast<const P*>(A.b) + c) : 0.f;
       DT<T>::store(y + c, fmaf((DT<T>::load(x + c) - mean) * rstd, w, b));
     }
     if (threadIdx.x == 0 && A.mean) A.mean[row] = mean, A.rstd[row] = rstd;
@@ -238,9 +379,9 @@ __global__ void __launch_bounds__(kLoopThreads) layer_norm_fwd_loop_kernel(const
 }
 
 // The same backwards; a CTA's sums of dw and db live in its own row of `part`, each column touched by one thread.
-template <typename T>
+template <typename T, typename P>
 __global__ void __launch_bounds__(kLoopThreads) layer_norm_bwd_loop_kernel(const NormArgs A) {
-  __shared__ float2 red[3][16];
+  __shared__ Sums sx, sy;
   int slot = 0;
   float* out = A.part ? A.part + (long long)blockIdx.x * 2 * A.C : nullptr;
   if (out)
@@ -252,7 +393,7 @@ __global__ void __launch_bounds__(kLoopThreads) layer_norm_bwd_loop_kernel(const
     float2 s = make_float2(0.f, 0.f);
     for (int c = threadIdx.x; c < A.C; c += kLoopThreads) {
       const float d = DT<T>::load(dy + c), h = (DT<T>::load(x + c) - mean) * rstd;
-      const float g = A.w ? d * param<T>(A.w, c, A.w32) : d;
+      const float g = A.w ? d * DT<P>::load(static_cast<const P*>(A.w) + c) : d;
       s.x += g;
       s.y = fmaf(g, h, s.y);
       if (out) {
@@ -260,37 +401,39 @@ __global__ void __launch_bounds__(kLoopThreads) layer_norm_bwd_loop_kernel(const
         out[A.C + c] += d;
       }
     }
-    s = group_sum(s, kLoopThreads, 0, red, slot);
+    s = group_sum(s, kLoopThreads, 0, sx, sy, slot);
     s.x *= A.invC, s.y *= A.invC;
     if (A.dx) {
       T* dx = static_cast<T*>(A.dx) + row * A.C;
       for (int c = threadIdx.x; c < A.C; c += kLoopThreads) {
         const float d = DT<T>::load(dy + c), h = (DT<T>::load(x + c) - mean) * rstd;
-        const float g = A.w ? d * param<T>(A.w, c, A.w32) : d;
+        const float g = A.w ? d * DT<P>::load(static_cast<const P*>(A.w) + c) : d;
         DT<T>::store(dx + c, rstd * (g - s.x - h * s.y));
       }
     }
   }
 }
 
-// part [n, 2 C] -> dw, db: 32 columns by 8 strands per CTA, each strand every eighth row, then the strands in order.
+// part [n, 2 C] -> dw, db: 32 columns by 32 strands per CTA, each strand every 32nd row, then the strands in order.
 template <typename P>
-__global__ void __launch_bounds__(256) layer_norm_reduce_kernel(const float* __restrict__ part, int n, int C, P* dw, P* db) {
-  __shared__ float red[8][33];
+__global__ void __launch_bounds__(1024) layer_norm_reduce_kernel(const float* __restrict__ part, int n, int C, P* dw, P* db) {
+  __shared__ float red[32][33];
   const int lane = threadIdx.x & 31, strand = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + lane;
   float s = 0.f;
-  if (c < 2 * C)
-    for (int i = strand; i < n; i += 8) s += part[(long long)i * 2 * C + c];
+  if (c < 2 * C) {
+#pragma unroll 4
+    for (int i = strand; i < n; i += 32) s += part[(long long)i * 2 * C + c];
+  }
   red[strand][lane] = s;
   __syncthreads();
-  if (strand == 0 && c < 2 * C) {
-#pragma unroll
-    for (int i = 1; i < 8; ++i) s += red[i][lane];
-    if (c < C) {
-      if (dw) DT<P>::store(dw + c, s);
+  s = warp_sum(red[lane][strand]);  // column blockIdx.x * 32 + strand, in a fixed order
+  const int d = blockIdx.x * 32 + strand;
+  if (lane == 0 && d < 2 * C) {
+    if (d < C) {
+      if (dw) DT<P>::store(dw + d, s);
     } else if (db) {
-      DT<P>::store(db + c - C, s);
+      DT<P>::store(db + d - C, s);
     }
   }
 }
@@ -305,62 +448,86 @@ struct NormPlan {
   int per, tpr, groups, ctas;  // per 0: the loop kernels
 };
 
-NormPlan plan(long long rows, int C, bool backward) {
+// Few warps for each row (their sums meet at a barrier), enough rows on an SM to keep its share of HBM's latency covered.
+// ctas is an upper bound (and the number of partial rows of the backward): the launch takes what is resident at once.
+NormPlan plan(long long rows, int C) {
   NormPlan p{};
   if (C > kMaxRow) {
     p.tpr = kLoopThreads, p.groups = 1;
     p.ctas = (int)std::min<long long>(rows, 2 * 148);
     return p;
   }
-  p.per = C <= 512 * 8 ? 8 : C <= 512 * 16 ? 16 : 32;
+  p.per = C <= 256 * 8 ? 8 : C <= 512 * 16 ? 16 : 32;
   p.tpr = std::max(32, ((C + p.per - 1) / p.per + 31) / 32 * 32);
-  p.groups = std::max(1, std::min(8, 256 / p.tpr));
-  // rows that stay in flight on an SM: 2048 threads forwards, 1024 backwards, where a thread holds twice as much
-  const int threads = p.tpr * p.groups;
-  const int per_sm = std::max(1, (backward ? 1024 : 2048) / threads / (p.per / 8));
-  p.ctas = (int)std::max<long long>(1, std::min<long long>((rows + p.groups - 1) / p.groups, 148ll * per_sm));
+  p.groups = std::max(1, std::min(kMaxGroups, 256 / p.tpr));
+  p.ctas = (int)std::max<long long>(1, std::min<long long>((rows + p.groups - 1) / p.groups, 148ll * 8));
   return p;
 }
 
-template <typename T, int V, int PER>
-int launch_rows(const NormArgs& A, const NormPlan& p, bool backward, cudaStream_t st) {
+// CTAs of a kernel that fit the device at once, asked once for each kernel, block and device.
+int resident(const void* fn, int threads, size_t smem) {
+  static std::mutex mu;
+  static std::map<std::tuple<const void*, int, size_t, int>, int> known;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  std::lock_guard<std::mutex> lock(mu);
+  auto it = known.find({fn, threads, smem, dev});
+  if (it != known.end()) return it->second;
+  int per_sm = 1, sms = 148;
+  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, fn, threads, smem) != cudaSuccess || per_sm < 1) per_sm = 1;
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  cudaGetLastError();
+  return known[{fn, threads, smem, dev}] = per_sm * sms;
+}
+
+template <typename T, typename P, int V, int PER, bool WHOLE>
+int launch_rows(NormArgs& A, NormPlan& p, bool backward, cudaStream_t st) {
   const int threads = p.tpr * p.groups;
-  if (!backward) {
-    layer_norm_fwd_kernel<T, V, PER><<<p.ctas, threads, 0, st>>>(A);
-  } else {
-    const size_t sm = p.groups > 1 && A.part ? sizeof(float) * 2 * (size_t)p.groups * A.C : 0;
-    auto kern = layer_norm_bwd_kernel<T, V, PER>;
-    if (sm > 32 * 1024 && !kernel_smem_once((const void*)kern, sm)) return set_error(HYFFT_ERR_CUDA, "layer norm: shared memory");
-    kern<<<p.ctas, threads, sm, st>>>(A);
-  }
+  // the ring: as many rows as 64 KB hold (three CTAs on an SM), two at least where 200 KB hold them
+  const size_t row = (size_t)A.C * sizeof(T) * (backward ? 2 : 1) * p.groups;
+  A.stages = (int)std::max<size_t>(2 * row <= 200 * 1024 ? 2 : 1, std::min<size_t>(kStages, 64 * 1024 / row));
+  size_t sm = V > 1 ? row * A.stages : 0;
+  if (backward && A.part && p.groups > 1) sm = std::max(sm, sizeof(float) * 2 * (size_t)p.groups * A.C);
+  const void* fn = backward ? (const void*)layer_norm_bwd_kernel<T, P, V, PER, WHOLE> : (const void*)layer_norm_fwd_kernel<T, P, V, PER, WHOLE>;
+  if (!kernel_smem_once(fn, sm)) return set_error(HYFFT_ERR_CUDA, "layer norm: shared memory");
+  p.ctas = std::min(p.ctas, resident(fn, threads, sm));
+  if (backward)
+    layer_norm_bwd_kernel<T, P, V, PER, WHOLE><<<p.ctas, threads, sm, st>>>(A);
+  else
+    layer_norm_fwd_kernel<T, P, V, PER, WHOLE><<<p.ctas, threads, sm, st>>>(A);
   return launched();
 }
 
-template <typename T, int V>
-int launch_v(const NormArgs& A, const NormPlan& p, bool backward, cudaStream_t st) {
-  if (p.per == 8) return launch_rows<T, V, 8>(A, p, backward, st);
-  if (p.per == 16) return launch_rows<T, V, 16>(A, p, backward, st);
-  return launch_rows<T, V, 32>(A, p, backward, st);
+template <typename T, typename P, int V, int PER>
+int launch_per(NormArgs& A, NormPlan& p, bool backward, cudaStream_t st) {
+  return A.C == p.tpr * PER ? launch_rows<T, P, V, PER, true>(A, p, backward, st)
+                            : launch_rows<T, P, V, PER, false>(A, p, backward, st);
+}
+
+template <typename T, typename P, int V>
+int launch_v(NormArgs& A, NormPlan& p, bool backward, cudaStream_t st) {
+  if (p.per == 8) return launch_per<T, P, V, 8>(A, p, backward, st);
+  if (p.per == 16) return launch_per<T, P, V, 16>(A, p, backward, st);
+  return launch_per<T, P, V, 32>(A, p, backward, st);
 }
 
 bool aligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
-template <typename T>
-int launch_t(NormArgs& A, bool backward, cudaStream_t st) {
-  const NormPlan p = plan(A.rows, A.C, backward);
+template <typename T, typename P>
+int launch_t(NormArgs& A, NormPlan& p, bool backward, cudaStream_t st) {
   A.tpr = p.tpr, A.groups = p.groups;
   A.invC = 1.f / (float)A.C;
   if (p.per == 0) {
     if (backward)
-      layer_norm_bwd_loop_kernel<T><<<p.ctas, kLoopThreads, 0, st>>>(A);
+      layer_norm_bwd_loop_kernel<T, P><<<p.ctas, kLoopThreads, 0, st>>>(A);
     else
-      layer_norm_fwd_loop_kernel<T><<<p.ctas, kLoopThreads, 0, st>>>(A);
+      layer_norm_fwd_loop_kernel<T, P><<<p.ctas, kLoopThreads, 0, st>>>(A);
     return launched();
   }
   constexpr int V = 16 / (int)sizeof(T);
   bool vec = A.C % V == 0 && A.xs % V == 0 && aligned(A.x) && aligned(A.y) && aligned(A.dx);
   if (backward) vec = vec && A.ds % V == 0 && aligned(A.dy);
-  return vec ? launch_v<T, V>(A, p, backward, st) : launch_v<T, 1>(A, p, backward, st);
+  return vec ? launch_v<T, P, V>(A, p, backward, st) : launch_v<T, P, 1>(A, p, backward, st);
 }
 
 int check_args(int64_t rows, int64_t C, int32_t dtype, int32_t param_dtype) {
@@ -371,10 +538,12 @@ int check_args(int64_t rows, int64_t C, int32_t dtype, int32_t param_dtype) {
   return HYFFT_OK;
 }
 
-int run(NormArgs& A, int32_t dtype, bool backward, cudaStream_t st) {
-  if (dtype == HYFFT_F32) return launch_t<float>(A, backward, st);
-  if (dtype == HYFFT_BF16) return launch_t<__nv_bfloat16>(A, backward, st);
-  return launch_t<__half>(A, backward, st);
+int run(NormArgs& A, NormPlan& p, int32_t dtype, int32_t param_dtype, bool backward, cudaStream_t st) {
+  if (dtype == HYFFT_F32) return launch_t<float, float>(A, p, backward, st);
+  if (dtype == HYFFT_BF16)
+    return param_dtype == HYFFT_F32 ? launch_t<__nv_bfloat16, float>(A, p, backward, st)
+                                    : launch_t<__nv_bfloat16, __nv_bfloat16>(A, p, backward, st);
+  return param_dtype == HYFFT_F32 ? launch_t<__half, float>(A, p, backward, st) : launch_t<__half, __half>(A, p, backward, st);
 }
 
 }  // namespace
@@ -387,7 +556,7 @@ extern "C" {
 int hyfft_layer_norm_workspace_size(int64_t rows, int64_t C, size_t* bwd_bytes) {
   const int rc = check_args(rows, C, HYFFT_F32, HYFFT_F32);
   if (rc != HYFFT_OK) return rc;
-  if (bwd_bytes) *bwd_bytes = sizeof(float) * 2 * (size_t)C * plan(rows, (int)C, true).ctas;
+  if (bwd_bytes) *bwd_bytes = sizeof(float) * 2 * (size_t)C * plan(rows, (int)C).ctas;
   return HYFFT_OK;
 }
 
@@ -400,8 +569,9 @@ int hyfft_layer_norm_forward(const void* x, const void* weight, const void* bias
   if (bind_device_of(x) != HYFFT_OK) return set_error(HYFFT_ERR_CUDA, "layer norm: device");
   NormArgs A{};
   A.x = x, A.w = weight, A.b = bias, A.y = y, A.mean = mean, A.rstd = rstd;
-  A.rows = rows, A.C = (int)C, A.xs = x_stride, A.eps = eps, A.w32 = param_dtype == HYFFT_F32;
-  return run(A, dtype, false, static_cast<cudaStream_t>(stream));
+  A.rows = rows, A.C = (int)C, A.xs = x_stride, A.eps = eps;
+  NormPlan p = plan(rows, (int)C);
+  return run(A, p, dtype, param_dtype, false, static_cast<cudaStream_t>(stream));
 }
 
 int hyfft_layer_norm_backward(const void* x, const void* weight, const float* mean, const float* rstd, const void* dy,
@@ -413,25 +583,25 @@ int hyfft_layer_norm_backward(const void* x, const void* weight, const float* me
   if (!x || !dy || !mean || !rstd) return set_error(HYFFT_ERR_INVALID, "layer norm: null tensor in the backward");
   if (bind_device_of(x) != HYFFT_OK) return set_error(HYFFT_ERR_CUDA, "layer norm: device");
   const bool sums = dweight || dbias;
-  const NormPlan p = plan(rows, (int)C, true);
+  NormPlan p = plan(rows, (int)C);
   if (sums && (!workspace || workspace_bytes < sizeof(float) * 2 * (size_t)C * p.ctas))
     return set_error(HYFFT_ERR_WORKSPACE, "layer norm: workspace too small");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   NormArgs A{};
   A.x = x, A.w = weight, A.dy = dy, A.dx = dx;
   A.mean = const_cast<float*>(mean), A.rstd = const_cast<float*>(rstd);
-  A.rows = rows, A.C = (int)C, A.xs = x_stride, A.ds = dy_stride, A.w32 = param_dtype == HYFFT_F32;
+  A.rows = rows, A.C = (int)C, A.xs = x_stride, A.ds = dy_stride;
   A.part = sums ? static_cast<float*>(workspace) : nullptr;
-  int r = run(A, dtype, true, st);
+  int r = run(A, p, dtype, param_dtype, true, st);
   if (r != HYFFT_OK || !sums) return r;
   const unsigned grid = (unsigned)((2 * C + 31) / 32);
   if (param_dtype == HYFFT_F32)
-    layer_norm_reduce_kernel<float><<<grid, 256, 0, st>>>(A.part, p.ctas, (int)C, (float*)dweight, (float*)dbias);
+    layer_norm_reduce_kernel<float><<<grid, 1024, 0, st>>>(A.part, p.ctas, (int)C, (float*)dweight, (float*)dbias);
   else if (dtype == HYFFT_BF16)
-    layer_norm_reduce_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(A.part, p.ctas, (int)C, (__nv_bfloat16*)dweight,
+    layer_norm_reduce_kernel<__nv_bfloat16><<<grid, 1024, 0, st>>>(A.part, p.ctas, (int)C, (__nv_bfloat16*)dweight,
                                                                  (__nv_bfloat16*)dbias);
   else
-    layer_norm_reduce_kernel<__half><<<grid, 256, 0, st>>>(A.part, p.ctas, (int)C, (__half*)dweight, (__half*)dbias);
+    layer_norm_reduce_kernel<__half><<<grid, 1024, 0, st>>>(A.part, p.ctas, (int)C, (__half*)dweight, (__half*)dbias);
   return launched();
 }
 
