@@ -7,10 +7,10 @@
 // A row is held in the registers of a group of 32 .. 512 threads (kPer = 8, 16 or 32 elements each), so the mean and
 // then the centred squares are summed from registers: two reductions, no cancellation between E[x^2] and
 // E[x]^2. Groups walk over the rows with the weights in registers. Rows that start on 16 bytes come through a ring of up
-// to four in shared memory for each group, filled by bulk copies: HBM's latency needs 35 KB in flight on an SM, which
-// registers would not hold (one row ahead in registers: 314 us forwards, 422 backwards for 65536 rows of 4096 bfloat16;
-// ring: @RING@). Other rows are loaded one ahead into registers. The weight's and the bias's
-// gradients stay in each thread's registers over all rows of its group; a CTA adds its groups' sums in shared memory,
+// to four in shared memory for each group, filled by bulk copies (65536 rows of 4096 bfloat16: 228 us forwards, 278
+// backwards; with the next row's loads in registers instead 246 and 330). Other rows are loaded one ahead into registers.
+// Everything per element runs on packed pairs (element by element, with a test of the column for each, it was 314 and
+// 422 us: instructions were the bound). The weight's and the bias's gradients stay in each thread's registers over all rows of its group; a CTA adds its groups' sums in shared memory,
 // writes one partial row, and a second kernel adds those rows in a fixed order: no atomics, the same bits every run.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

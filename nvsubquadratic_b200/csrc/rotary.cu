@@ -18,6 +18,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "../../include/hyfft.h"
 #include "common.cuh"
@@ -64,34 +65,68 @@ __device__ __forceinline__ void copy_run(T* dst, const T* src) {
   }
 }
 
-// V: pairs per thread. INTER: the pairs are neighbours.
-template <typename T, int V, bool INTER>
+// Two neighbouring elements as float32 and back; the packed forms where V > 1 says that they lie on an even place.
+template <typename T, bool PACKED>
+__device__ __forceinline__ float2 two(const T* p) {
+  if constexpr (PACKED && sizeof(T) == 2) {
+    if constexpr (std::is_same<T, __half>::value) {
+      return __half22float2(*reinterpret_cast<const __half2*>(p));
+    } else {
+      const uint32_t u = *reinterpret_cast<const uint32_t*>(p);
+      return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+    }
+  }
+  return make_float2(DT<T>::load(p), DT<T>::load(p + 1));
+}
+template <typename T, bool PACKED>
+__device__ __forceinline__ void put_two(T* p, float2 v) {
+  if constexpr (PACKED && sizeof(T) == 2) {
+    if constexpr (std::is_same<T, __half>::value)
+      *reinterpret_cast<__half2*>(p) = __floats2half2_rn(v.x, v.y);
+    else
+      *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(v.x, v.y);
+  } else {
+    DT<T>::store(p, v.x);
+    DT<T>::store(p + 1, v.y);
+  }
+}
+
+// V: pairs per thread. INTER: the pairs are neighbours. ID: the type that counts threads (64-bit divisions would cost as
+// much as four heads do).
+template <typename T, int V, bool INTER, typename ID>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotArgs A) {
-  const long long id = (long long)blockIdx.x * kThreads + threadIdx.x;
-  if (id >= A.items) return;
-  const int all = A.units + A.tail;
+  const ID id = (ID)blockIdx.x * kThreads + threadIdx.x;
+  if (id >= (ID)A.items) return;
+  const ID all = (ID)(A.units + A.tail);
   const int unit = (int)(id % all);
-  const long long rest = id / all;
-  const int grp = (int)(rest % A.groups);
-  const long long tok = rest / A.groups;
-  const long long b = tok / A.L, l = tok - b * A.L;
+  const ID rest = id / all;
+  const int grp = (int)(rest % (ID)A.groups);
+  const long long tok = (long long)(rest / (ID)A.groups);
+  const long long b = (long long)((ID)tok / (ID)A.L), l = tok - b * A.L;
   const int nh = A.heads[0] + A.heads[1];
   constexpr int R = INTER ? 2 * V : V;  // elements of one run
+  const T* src[2];
+  T* dst[2];
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    src[w] = static_cast<const T*>(A.x[w]) + b * A.xb[w] + l * A.xl[w];
+    dst[w] = static_cast<T*>(A.y[w]) + tok * A.heads[w] * (long long)A.D;
+  }
+  // head h of q and k counted through
+  const auto from = [&](int h) { return h < A.heads[0] ? src[0] + h * A.xh[0] : src[1] + (h - A.heads[0]) * A.xh[1]; };
+  const auto to = [&](int h) {
+    return h < A.heads[0] ? dst[0] + (long long)h * A.D : dst[1] + (long long)(h - A.heads[0]) * A.D;
+  };
 
   if (unit >= A.units) {  // features that are not turned
     const int c = 2 * A.half + (unit - A.units) * R;
     for (int h = grp; h < nh; h += A.groups) {
-      const int w = h >= A.heads[0];
-      const int hh = w ? h - A.heads[0] : h;
-      const T* src = static_cast<const T*>(w ? A.x[1] : A.x[0]) + b * (w ? A.xb[1] : A.xb[0]) +
-                     l * (w ? A.xl[1] : A.xl[0]) + hh * (w ? A.xh[1] : A.xh[0]) + c;
-      T* dst = static_cast<T*>(w ? A.y[1] : A.y[0]) + (tok * (w ? A.heads[1] : A.heads[0]) + hh) * (long long)A.D + c;
-      alignas(16) T e[R];
+      const T* s = from(h) + c;
+      T* d = to(h) + c;
       if (c + R <= A.D) {
-        copy_run<T, R>(e, src);
-        copy_run<T, R>(dst, e);
+        copy_run<T, R>(d, s);
       } else {
-        for (int u = 0; c + u < A.D; ++u) dst[u] = src[u];
+        for (int u = 0; c + u < A.D; ++u) d[u] = s[u];
       }
     }
     return;
@@ -120,15 +155,12 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotArgs A) {
     for (int j = 0; j < 4; ++j) {
       const int h = h0 + j * A.groups;
       if (h < nh) {
-        const int w = h >= A.heads[0];
-        const int hh = w ? h - A.heads[0] : h;
-        const T* src = static_cast<const T*>(w ? A.x[1] : A.x[0]) + b * (w ? A.xb[1] : A.xb[0]) +
-                       l * (w ? A.xl[1] : A.xl[0]) + hh * (w ? A.xh[1] : A.xh[0]);
+        const T* s = from(h);
         if constexpr (INTER) {
-          copy_run<T, 2 * V>(d[j].e, src + c0);
+          copy_run<T, 2 * V>(d[j].e, s + c0);
         } else {
-          copy_run<T, V>(d[j].e, src + c0);
-          copy_run<T, V>(d[j].e + V, src + c1);
+          copy_run<T, V>(d[j].e, s + c0);
+          copy_run<T, V>(d[j].e + V, s + c1);
         }
       }
     }
@@ -136,21 +168,31 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotArgs A) {
     for (int j = 0; j < 4; ++j) {
       const int h = h0 + j * A.groups;
       if (h < nh) {
-        const int w = h >= A.heads[0];
-        const int hh = w ? h - A.heads[0] : h;
-        T* dst = static_cast<T*>(w ? A.y[1] : A.y[0]) + (tok * (w ? A.heads[1] : A.heads[0]) + hh) * (long long)A.D;
-#pragma unroll
-        for (int u = 0; u < V; ++u) {
-          const int ia = INTER ? 2 * u : u, ib = INTER ? 2 * u + 1 : V + u;
-          const float a = DT<T>::load(&d[j].e[ia]), bb = DT<T>::load(&d[j].e[ib]);
-          DT<T>::store(&d[j].e[ia], fmaf(a, cs[u], -bb * sn[u]));
-          DT<T>::store(&d[j].e[ib], fmaf(a, sn[u], bb * cs[u]));
-        }
+        T* o = to(h);
         if constexpr (INTER) {
-          copy_run<T, 2 * V>(dst + c0, d[j].e);
+#pragma unroll
+          for (int u = 0; u < V; ++u) {
+            const float2 ab = two<T, (V > 1)>(d[j].e + 2 * u);
+            put_two<T, (V > 1)>(d[j].e + 2 * u, ffma2(make_float2(ab.y, ab.x), make_float2(-sn[u], sn[u]), cscale(ab, cs[u])));
+          }
+          copy_run<T, 2 * V>(o + c0, d[j].e);
         } else {
-          copy_run<T, V>(dst + c0, d[j].e);
-          copy_run<T, V>(dst + c1, d[j].e + V);
+          if constexpr (V == 1) {
+            const float a = DT<T>::load(d[j].e), bb = DT<T>::load(d[j].e + 1);
+            DT<T>::store(d[j].e, fmaf(a, cs[0], -bb * sn[0]));
+            DT<T>::store(d[j].e + 1, fmaf(a, sn[0], bb * cs[0]));
+          } else {
+#pragma unroll
+            for (int u = 0; u < V; u += 2) {
+              const float2 a = two<T, true>(d[j].e + u), bb = two<T, true>(d[j].e + V + u);
+              const float2 c = make_float2(cs[u], cs[u + 1]), s = make_float2(sn[u], sn[u + 1]);
+              const float2 n = make_float2(-sn[u], -sn[u + 1]);
+              put_two<T, true>(d[j].e + u, ffma2(bb, n, make_float2(a.x * c.x, a.y * c.y)));
+              put_two<T, true>(d[j].e + V + u, ffma2(a, s, make_float2(bb.x * c.x, bb.y * c.y)));
+            }
+          }
+          copy_run<T, V>(o + c0, d[j].e);
+          copy_run<T, V>(o + c1, d[j].e + V);
         }
       }
     }
@@ -170,7 +212,10 @@ int launch(RotArgs A, long long tokens, cudaStream_t st) {
   A.items = tokens * (A.units + A.tail) * A.groups;
   const long long ctas = (A.items + kThreads - 1) / kThreads;
   if (ctas > 0x7fffffffLL) return set_error(HYFFT_ERR_UNSUPPORTED, "rotary: too many elements");
-  rotary_kernel<T, V, INTER><<<(unsigned)ctas, kThreads, 0, st>>>(A);
+  if (ctas * kThreads < (1ll << 32))
+    rotary_kernel<T, V, INTER, unsigned><<<(unsigned)ctas, kThreads, 0, st>>>(A);
+  else
+    rotary_kernel<T, V, INTER, unsigned long long><<<(unsigned)ctas, kThreads, 0, st>>>(A);
   if (cudaGetLastError() != cudaSuccess) return set_error(HYFFT_ERR_CUDA, "rotary: kernel launch failed");
   g_launches.fetch_add(1, std::memory_order_relaxed);
   return HYFFT_OK;
