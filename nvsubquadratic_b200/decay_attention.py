@@ -48,6 +48,23 @@ def _unit(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
+_PLANS: dict = {}
+
+
+def _plan(q, k, v, scale, dout=None):
+    """(descriptor, (forward, backward) workspace bytes) of a call, built once for each set of shapes and strides."""
+    key = (q.shape, q.stride(), q.dtype, k.shape, k.stride(), v.shape, v.stride(), scale,
+           None if dout is None else dout.stride())
+    hit = _PLANS.get(key)
+    if hit is None:
+        d = _desc(q, k, v, scale, dout)
+        hit = (d, _workspaces(d))
+        if len(_PLANS) >= 256:
+            _PLANS.clear()
+        _PLANS[key] = hit
+    return hit
+
+
 def _desc(q, k, v, scale, dout=None) -> _lib.DecayDesc:
     d = _lib.DecayDesc()
     d.batch, d.length = q.shape[0], q.shape[1] if q.ndim == 4 else 1
@@ -68,29 +85,33 @@ def _workspaces(d) -> tuple[int, int]:
     return f.value, b.value
 
 
-class _DecayFunction(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, log_decay, initial_state, lengths, scale, want_state):
-        dev = _lib.require_cuda(q, k, v, log_decay, initial_state, lengths)
-        q, k, v = _unit(q), _unit(k), _unit(v)
-        g = log_decay.detach().to(torch.float32).contiguous()
-        s0 = initial_state.contiguous() if initial_state is not None else None
-        B, L, H, Dk = q.shape
-        Dv = v.shape[-1]
-        o = torch.empty((B, L, H, Dv), dtype=q.dtype, device=dev)
-        state = torch.empty((B, H, Dk, Dv), dtype=torch.float32, device=dev) if want_state else None
-        ctx.set_materialize_grads(False)
-        ctx.save_for_backward(q, k, v, g, s0, lengths)
-        ctx.scale, ctx.decay_dtype = scale, log_decay.dtype
-        if B == 0:
-            return o, state
-        d = _desc(q, k, v, scale)
-        need, _ = _workspaces(d)
+def _forward(q, k, v, log_decay, initial_state, lengths, scale, want_state):
+    """(o, state or None, the tensors as the library read them)."""
+    dev = _lib.require_cuda(q, k, v, log_decay, initial_state, lengths)
+    q, k, v = _unit(q), _unit(k), _unit(v)
+    g = log_decay.detach().to(torch.float32).contiguous()
+    s0 = initial_state.contiguous() if initial_state is not None else None
+    B, L, H, Dk = q.shape
+    Dv = v.shape[-1]
+    o = q.new_empty((B, L, H, Dv))
+    state = g.new_empty((B, H, Dk, Dv)) if want_state else None
+    if B:
+        d, (need, _) = _plan(q, k, v, scale)
         ws = _lib.workspace(need, dev)
         rc = _lib.load().hyfft_decay_forward(ctypes.byref(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(),
                                              _lib.ptr(lengths), _lib.ptr(s0), o.data_ptr(), _lib.ptr(state),
                                              ws.data_ptr(), ws.numel(), _lib.stream_ptr(dev))
         _lib.check(rc, "hyfft_decay_forward")
+    return o, state, (q, k, v, g, s0)
+
+
+class _DecayFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, log_decay, initial_state, lengths, scale, want_state):
+        o, state, read = _forward(q, k, v, log_decay, initial_state, lengths, scale, want_state)
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(*read, lengths)
+        ctx.scale, ctx.decay_dtype = scale, log_decay.dtype
         return o, state
 
     @staticmethod
@@ -108,15 +129,14 @@ class _DecayFunction(torch.autograd.Function):
         do = _unit(do.to(q.dtype))
         if dstate is not None:
             dstate = dstate.to(torch.float32).contiguous()
-        dq = torch.empty(q.shape, dtype=q.dtype, device=dev) if want[0] else None
-        dk = torch.empty(k.shape, dtype=q.dtype, device=dev) if want[1] else None
+        dq = q.new_empty(q.shape) if want[0] else None
+        dk = k.new_empty(k.shape) if want[1] else None
         ds0 = torch.empty_like(s0) if s0 is not None and want[4] else None
-        dv = torch.empty(v.shape, dtype=q.dtype, device=dev) if want[2] or ds0 is not None else None
+        dv = v.new_empty(v.shape) if want[2] or ds0 is not None else None
         dg = torch.empty_like(g) if want[3] else None
         if B == 0:
             return dq, dk, dv, (torch.zeros_like(g).to(ctx.decay_dtype) if want[3] else None), ds0, *none
-        d = _desc(q, k, v, ctx.scale, do)
-        _, need = _workspaces(d)
+        d, (_, need) = _plan(q, k, v, ctx.scale, do)
         ws = _lib.workspace(need, dev)
         rc = _lib.load().hyfft_decay_backward(ctypes.byref(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(),
                                               _lib.ptr(lengths), _lib.ptr(s0), do.data_ptr(), _lib.ptr(dstate),
@@ -155,7 +175,11 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay
         assert lengths.dtype == torch.int32, f"lengths must be int32; got {lengths.dtype}"
         lengths = lengths.contiguous()
     scale = Dk ** -0.5 if scale is None else float(scale)
-    o, state = _DecayFunction.apply(q, k, v, log_decay, initial_state, lengths, scale, bool(return_state))
+    args = (q, k, v, log_decay, initial_state, lengths, scale, bool(return_state))
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:5]):
+        o, state = _DecayFunction.apply(*args)
+    else:
+        o, state, _ = _forward(*args)
     return (o, state) if return_state else o
 
 
@@ -194,10 +218,10 @@ def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_
     dev = _lib.require_cuda(q, k, v, log_decay, state, out_state, slots)
     q, k, v = _unit(q), _unit(k), _unit(v)
     g = log_decay.to(torch.float32).contiguous()
-    o = torch.empty((B, H, v.shape[-1]), dtype=q.dtype, device=dev)
+    o = q.new_empty((B, H, v.shape[-1]))
     if B == 0:
         return o
-    d = _desc(q, k, v, Dk ** -0.5 if scale is None else float(scale))
+    d, _ = _plan(q, k, v, Dk ** -0.5 if scale is None else float(scale))
     rc = _lib.load().hyfft_decay_step(ctypes.byref(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(),
                                       _lib.ptr(slots), N, state.data_ptr(), out_state.data_ptr(), o.data_ptr(),
                                       _lib.stream_ptr(dev))

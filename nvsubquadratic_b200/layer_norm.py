@@ -6,6 +6,7 @@
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -16,8 +17,17 @@ __all__ = ["layer_norm", "LayerNormB200"]
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """t as ``[rows, C]`` with unit stride inside a row: a view where its rows have one stride, else a copy."""
-    t = t.reshape(-1, t.shape[-1])
+    if t.ndim != 2:
+        t = t.reshape(-1, t.shape[-1])
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_size(rows: int, C: int) -> int:
+    size = ctypes.c_size_t()
+    _lib.check(_lib.load().hyfft_layer_norm_workspace_size(rows, C, ctypes.byref(size)),
+               "hyfft_layer_norm_workspace_size")
+    return size.value
 
 
 def _param_code(x, weight, bias) -> int:
@@ -25,28 +35,31 @@ def _param_code(x, weight, bias) -> int:
     return _lib.DTYPE_CODE[p.dtype] if p is not None else _lib.F32
 
 
+def _forward(x, weight, bias, eps, keep):
+    """(y, x as rows, weight, statistics [2, rows]: means, then reciprocal deviations; None unless kept)."""
+    dev = _lib.require_cuda(x, weight, bias)
+    x2 = _rows(x)
+    w = weight.contiguous() if weight is not None else None
+    b = bias.contiguous() if bias is not None else None
+    rows, C = x2.shape
+    y = x.new_empty(x.shape)
+    stats = x.new_empty((2, rows), dtype=torch.float32) if keep else None
+    if rows:
+        mean = stats.data_ptr() if keep else None
+        rc = _lib.load().hyfft_layer_norm_forward(
+            x2.data_ptr(), _lib.ptr(w), _lib.ptr(b), y.data_ptr(), mean, mean + 4 * rows if keep else None, rows, C,
+            x2.stride(0), eps, _lib.DTYPE_CODE[x.dtype], _param_code(x, w, b), _lib.stream_ptr(dev))
+        _lib.check(rc, "hyfft_layer_norm_forward")
+    return y, x2, w, stats
+
+
 class _LayerNormFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
-        dev = _lib.require_cuda(x, weight, bias)
-        shape = x.shape
-        x2 = _rows(x)
-        w = weight.contiguous() if weight is not None else None
-        b = bias.contiguous() if bias is not None else None
-        rows, C = x2.shape
-        y = torch.empty(shape, dtype=x.dtype, device=dev)
-        keep = any(ctx.needs_input_grad[:3])
-        stats = torch.empty((2, rows), dtype=torch.float32, device=dev) if keep else None
-        if rows:
-            rc = _lib.load().hyfft_layer_norm_forward(
-                x2.data_ptr(), _lib.ptr(w), _lib.ptr(b), y.data_ptr(), stats[0].data_ptr() if keep else None,
-                stats[1].data_ptr() if keep else None, rows, C, x2.stride(0), eps, _lib.DTYPE_CODE[x.dtype],
-                _param_code(x, w, b), _lib.stream_ptr(dev))
-            _lib.check(rc, "hyfft_layer_norm_forward")
-        if keep:
-            ctx.save_for_backward(x2, w, stats)
-            ctx.shape = shape
-            ctx.bias = (b.dtype, b.shape) if b is not None else None
+        y, x2, w, stats = _forward(x, weight, bias, eps, True)
+        ctx.save_for_backward(x2, w, stats)
+        ctx.shape = x.shape
+        ctx.bias = bias.dtype if bias is not None else None
         return y
 
     @staticmethod
@@ -56,22 +69,20 @@ class _LayerNormFunction(torch.autograd.Function):
         rows, C = x2.shape
         want = ctx.needs_input_grad
         dy2 = _rows(dy.to(x2.dtype))
-        dx = torch.empty(ctx.shape, dtype=x2.dtype, device=dev) if want[0] else None
-        dw = torch.empty_like(w) if w is not None and want[1] else None
-        db = torch.empty(ctx.bias[1], dtype=ctx.bias[0], device=dev) if ctx.bias is not None and want[2] else None
+        dx = x2.new_empty(ctx.shape) if want[0] else None
+        dw = w.new_empty(C) if w is not None and want[1] else None
+        db = x2.new_empty(C, dtype=ctx.bias) if ctx.bias is not None and want[2] else None
         if not rows:
             return dx, dw.zero_() if dw is not None else None, db.zero_() if db is not None else None, None
         lib = _lib.load()
         ws, need = None, 0
         if dw is not None or db is not None:
-            size = ctypes.c_size_t()
-            _lib.check(lib.hyfft_layer_norm_workspace_size(rows, C, ctypes.byref(size)),
-                       "hyfft_layer_norm_workspace_size")
-            need = size.value
+            need = _workspace_size(rows, C)
             ws = _lib.workspace(need, dev)
         code = _lib.DTYPE_CODE[w.dtype] if w is not None else (
-            _lib.DTYPE_CODE[ctx.bias[0]] if ctx.bias is not None else _lib.F32)
-        rc = lib.hyfft_layer_norm_backward(x2.data_ptr(), _lib.ptr(w), stats[0].data_ptr(), stats[1].data_ptr(),
+            _lib.DTYPE_CODE[ctx.bias] if ctx.bias is not None else _lib.F32)
+        mean = stats.data_ptr()
+        rc = lib.hyfft_layer_norm_backward(x2.data_ptr(), _lib.ptr(w), mean, mean + 4 * rows,
                                            dy2.data_ptr(), _lib.ptr(dx), _lib.ptr(dw), _lib.ptr(db), rows, C,
                                            x2.stride(0), dy2.stride(0), _lib.DTYPE_CODE[x2.dtype], code,
                                            _lib.ptr(ws), need, _lib.stream_ptr(dev))
@@ -94,7 +105,9 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
         assert weight.dtype == bias.dtype, f"weight and bias must share a dtype; got {weight.dtype} and {bias.dtype}"
     if x.dtype not in _lib.DTYPE_CODE:
         raise NotImplementedError(f"dtype {x.dtype} is not supported (float32, bfloat16, float16)")
-    return _LayerNormFunction.apply(x, weight, bias, float(eps))
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+        return _LayerNormFunction.apply(x, weight, bias, float(eps))
+    return _forward(x, weight, bias, float(eps), False)[0]
 
 
 class LayerNormB200(torch.nn.Module):

@@ -67,13 +67,17 @@ def _unit(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
-def _call(q, k, turns, positions, amplitude, interleaved, backward):
-    dev = _lib.require_cuda(q, k, turns, positions)
-    q, k = _unit(q), _unit(k) if k is not None else None
-    oq = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    ok = torch.empty(k.shape, dtype=k.dtype, device=dev) if k is not None else None
-    if q.shape[0] == 0 or q.shape[1] == 0:
-        return oq, ok
+_DESCS: dict = {}
+
+
+def _desc(q, k, turns, positions, amplitude, interleaved, backward):
+    """The descriptor of a call, built once for each set of shapes and strides."""
+    key = (q.shape, q.stride(), q.dtype, None if k is None else (k.shape, k.stride()), turns.shape,
+           None if positions is None else (positions.shape, positions.stride(), positions.dtype), amplitude, interleaved,
+           backward)
+    d = _DESCS.get(key)
+    if d is not None:
+        return d
     d = _lib.RotaryDesc()
     d.batch, d.length, d.heads, d.dim = q.shape
     d.kv_heads = k.shape[2] if k is not None else 0
@@ -88,6 +92,20 @@ def _call(q, k, turns, positions, amplitude, interleaved, backward):
         d.pos_int32 = int(positions.dtype == torch.int32)
         d.pos_stride[0] = positions.stride(0) if positions.ndim == 2 else 0
         d.pos_stride[1] = positions.stride(-1)
+    if len(_DESCS) >= 256:
+        _DESCS.clear()
+    _DESCS[key] = d
+    return d
+
+
+def _call(q, k, turns, positions, amplitude, interleaved, backward):
+    dev = _lib.require_cuda(q, k, turns, positions)
+    q, k = _unit(q), _unit(k) if k is not None else None
+    oq = q.new_empty(q.shape)
+    ok = k.new_empty(k.shape) if k is not None else None
+    if oq.numel() == 0:
+        return oq, ok
+    d = _desc(q, k, turns, positions, amplitude, interleaved, backward)
     rc = _lib.load().hyfft_rotary(ctypes.byref(d), q.data_ptr(), _lib.ptr(k), turns.data_ptr(), _lib.ptr(positions),
                                   oq.data_ptr(), _lib.ptr(ok), _lib.stream_ptr(dev))
     _lib.check(rc, "hyfft_rotary")
@@ -141,4 +159,7 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, turns: torch.Tensor, *, posi
         assert tuple(positions.shape) in ((L,), (B, L)), f"positions must be [{L}] or [{B}, {L}]; got {tuple(positions.shape)}"
     if q.dtype not in _lib.DTYPE_CODE:
         raise NotImplementedError(f"dtype {q.dtype} is not supported (float32, bfloat16, float16)")
-    return _RotaryFunction.apply(q, k, turns.contiguous(), positions, float(amplitude), bool(interleaved))
+    args = (q, k, turns.contiguous(), positions, float(amplitude), bool(interleaved))
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        return _RotaryFunction.apply(*args)
+    return _call(*args, False)
