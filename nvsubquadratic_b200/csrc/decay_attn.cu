@@ -9,14 +9,17 @@
 // and the decay's, with T_t = dS_t / dlog_decay = a (T_{t-1} + S_{t-1}) carried beside S:
 //   dlog_decay = scale * sum_t q_t^T T_t do_t + <dL/dS_L, T_L>.
 //
-// The scan kernel below takes every type and every head size up to 256 and computes in float32
-// multiply-adds. A thread owns one column of S and up to 64 of its rows in registers, so a token
-// costs two packed multiply-adds per pair of state elements (S += k v, o += q S) and no exchange
-// between threads; q and k are read from shared memory as broadcasts. Inside a chunk of 32 tokens the
-// state is kept divided by a^i, which takes the decay out of the inner loop: v is multiplied by a^-i
-// and o by a^i, each from a table, and the chunk's a^n is applied once, as the sum of two floats
+// The scan kernel below takes every type and every head size up to 256 and computes in float32 multiply-adds. A thread
+// owns four columns of the state and up to 32 of its rows in registers, packed in pairs of rows: a token costs two packed
+// multiply-adds per pair (S += k v, o += q S). q and k are read from shared memory as broadcasts, which the register
+// file takes at 128 bytes a cycle: one 16-byte read serves 16 multiply-adds here (with one column per thread it served four
+// and the reads were the bound: 2.08 ms for 16 x 4096 tokens, 12 heads of 64, float16, instead of @SCAN@). The two halves of a
+// warp hold two parts of the rows, their sums meet in one shuffle; states of more than 64 rows take more warps.
+// Inside a chunk of 16 tokens the state is kept divided by a^i, which takes the decay out of the inner loop: v is
+// multiplied by a^-i and o by a^i, each from a table, and the chunk's a^n is applied once, as the sum of two floats
 // (a rounded a^n would be off by its rounding error times the number of chunks in a head's memory). Heads that
 // forget more than e^-46 within a chunk, where a^-i would overflow, multiply the state for each token.
+// bfloat16 states of up to 128 rows go to the tensor cores instead (decay_mma.cu).
 // Few rows and a long axis: the axis is cut into segments; a first pass adds up each segment from a zero
 // state, a small kernel chains the segments' states, and the second pass starts every segment from its own.
 #include <cuda_bf16.h>
@@ -38,8 +41,8 @@ int set_error(int code, const char* msg);  // engine.cu: the message hyfft_last_
 
 namespace {
 
-constexpr int kTok = 32;        // tokens per chunk
-constexpr int kThreads = 128;   // 4 warps: KW over the state's rows x VW over its columns
+constexpr int kTok = 16;   // tokens per chunk
+constexpr int kCols = 64;  // columns per CTA: 16 lanes x 4
 constexpr int kMaxDim = 256;
 constexpr double kFastLimit = 46.0;  // |log_decay| * kTok below this: a^-i stays below 1e20
 
@@ -48,46 +51,59 @@ using Op = ScanOp;
 __device__ __forceinline__ float2 mul2(float2 a, float b) { return make_float2(a.x * b, a.y * b); }
 __device__ __forceinline__ float2 dup(float a) { return make_float2(a, a); }
 
-// rows [0, n) of an operand, columns [c0, c0 + w) (zeros past D), as floats; token of row i: t0 + i * step
-template <typename T>
-__device__ __forceinline__ void load_tile(float* dst, const T* __restrict__ src, long long sl, int n, int c0, int w,
-                                          int D, long long t0, int step, bool vec, float mul) {
-  if (vec) {
-    constexpr int V = 16 / sizeof(T);
-    const int per = w / V;
-    for (int i = threadIdx.x; i < n * per; i += kThreads) {
-      const int r = i / per, c = (i - r * per) * V;
-      float* d = dst + r * w + c;
-      if (c0 + c < D) {
-        const T* s = src + (t0 + (long long)r * step) * sl + c0 + c;
-        const uint4 raw = *reinterpret_cast<const uint4*>(s);
-        const T* e = reinterpret_cast<const T*>(&raw);
-#pragma unroll
-        for (int u = 0; u < V; ++u) d[u] = DT<T>::load(e + u) * mul;
-      } else {
-#pragma unroll
-        for (int u = 0; u < V; ++u) d[u] = 0.f;
-      }
-    }
-  } else {
-    for (int i = threadIdx.x; i < n * w; i += kThreads) {
-      const int r = i / w, c = i - r * w;
-      dst[i] = c0 + c < D ? DT<T>::load(src + (t0 + (long long)r * step) * sl + c0 + c) * mul : 0.f;
-    }
+// Columns [c0, c0 + W) of n tokens (zeros past D); token of row i: t0 + i * step. Left in flight.
+template <typename T, int W>
+__device__ __forceinline__ void fetch_tile(T* dst, const T* __restrict__ src, long long sl, int n, int c0, int D,
+                                           long long t0, int step) {
+  constexpr int V = 16 / sizeof(T), kPer = W / V;
+  for (int i = threadIdx.x; i < n * kPer; i += blockDim.x) {
+    const int r = i / kPer, c = (i - r * kPer) * V;
+    const bool ok = c0 + c < D;
+    const T* s = ok ? src + (t0 + (long long)r * step) * sl + c0 + c : src;
+    const unsigned d = (unsigned)__cvta_generic_to_shared(dst + r * W + c);
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(d), "l"(s), "r"(ok ? 16 : 0) : "memory");
+  }
+}
+// The same as floats, from any address, at once.
+template <typename T, int W>
+__device__ __forceinline__ void load_tile(float* dst, const T* __restrict__ src, long long sl, int n, int c0, int D,
+                                          long long t0, int step) {
+  for (int i = threadIdx.x; i < n * W; i += blockDim.x) {
+    const int r = i / W, c = i - r * W;
+    dst[i] = c0 + c < D ? DT<T>::load(src + (t0 + (long long)r * step) * sl + c0 + c) : 0.f;
+  }
+}
+// n rows of a 16-bit tile to floats.
+template <typename T, int W>
+__device__ __forceinline__ void widen_tile(float* dst, const T* src, int n) {
+  for (int i = threadIdx.x; i < n * W / 8; i += blockDim.x) {
+    const uint4 raw = reinterpret_cast<const uint4*>(src)[i];
+    const T* e = reinterpret_cast<const T*>(&raw);
+    float4* d = reinterpret_cast<float4*>(dst) + 2 * i;
+    d[0] = make_float4(DT<T>::load(e), DT<T>::load(e + 1), DT<T>::load(e + 2), DT<T>::load(e + 3));
+    d[1] = make_float4(DT<T>::load(e + 4), DT<T>::load(e + 5), DT<T>::load(e + 6), DT<T>::load(e + 7));
   }
 }
 
-// RK rows of the state in each thread, KW warps over its rows, 4 / KW over its columns.
-template <typename T, typename TO, int RK, int KW, bool LEARN>
-__global__ void __launch_bounds__(kThreads) decay_scan_kernel(const ScanArgs A) {
-  constexpr int VW = KW > 2 ? 1 : 4 / KW;
-  constexpr int W = RK * KW, WV = 32 * VW;
+// Floats of shared memory: tiles as the inner loop reads them, two chunks as they arrive (16-bit types; a float32 chunk is
+// read where it arrived), the parts of o where warps share a row.
+template <typename T, int RH, int KW, bool LEARN>
+struct Smem {
+  static constexpr int W = 2 * RH * KW;
+  static constexpr int chunk = kTok * (2 * W + kCols * (LEARN ? 2 : 1));  // elements
+  static constexpr bool wide = sizeof(T) == 4;
+  static constexpr int raw = wide ? 0 : chunk;                           // where the arriving chunks begin, in floats
+  static constexpr int os = raw + (wide ? 2 * chunk : chunk);
+  static constexpr int floats = os + (KW > 1 ? KW * kTok * kCols : 0);
+};
+
+// RH rows of the state in each thread (two halves of a warp: 2 RH rows), KW warps over its rows.
+template <typename T, typename TO, int RH, int KW, bool LEARN>
+__global__ void __launch_bounds__(32 * KW) decay_scan_kernel(const ScanArgs A) {
+  using M = Smem<T, RH, KW, LEARN>;
+  constexpr int W = M::W;
   extern __shared__ __align__(16) float smem[];
-  float* qs = smem;                  // [kTok][W]
-  float* ks = qs + kTok * W;         // [kTok][W]
-  float* vs = ks + kTok * W;         // [kTok][WV]
-  float* xs = vs + kTok * WV;        // [kTok][WV], learned decays only
-  float* os = xs + (LEARN ? kTok * WV : 0);  // [KW][kTok][WV], KW > 1 only
+  float* os = smem + M::os;  // [KW][kTok][kCols]
   __shared__ float apow[kTok], ainv[kTok];
 
   long long id = blockIdx.x;
@@ -98,10 +114,8 @@ __global__ void __launch_bounds__(kThreads) decay_scan_kernel(const ScanArgs A) 
   const int h = (int)(bh % A.H);
   const long long b = bh / A.H;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int kw = warp % KW, vw = warp / KW;
-  const bool active = warp < KW * VW;
-  const int c0 = slice * WV, col = vw * 32 + lane, row0 = kw * RK;
-  const bool has_col = active && c0 + col < A.DV;
+  const int c0 = slice * kCols, col = (lane & 15) * 4, row0 = (warp * 2 + (lane >> 4)) * RH;
+  const int left = A.DV - c0 - col;  // columns from this thread's first on that exist
 
   int len = A.L;
   if (A.lengths) len = min(max(A.lengths[b], 0), A.L);
@@ -116,20 +130,23 @@ __global__ void __launch_bounds__(kThreads) decay_scan_kernel(const ScanArgs A) 
   if (threadIdx.x < kTok) {
     const int e = threadIdx.x + lag;
     apow[threadIdx.x] = fast ? (float)(e ? exp((double)g * e) : 1.0) : 1.f;
-    ainv[threadIdx.x] = fast ? (float)(e ? exp(-(double)g * e) : 1.0) : 1.f;
+    ainv[threadIdx.x] = (fast ? (float)(e ? exp(-(double)g * e) : 1.0) : 1.f) * A.vscale;
   }
   const float a1 = expf(g);
-  const double a32 = exp((double)g * kTok);
-  const float a32hi = (float)a32, a32lo = (float)(a32 - (double)a32hi);
+  const double ac = exp((double)g * kTok);
+  const float achi = (float)ac, aclo = (float)(ac - (double)achi);
 
-  float2 S[RK / 2], D[LEARN ? RK / 2 : 1];
+  // rows row0 + 2 p, row0 + 2 p + 1 of column col + c; D: the same of T
+  float2 S[RH / 2][4], D[LEARN ? RH / 2 : 1][4];
 #pragma unroll
-  for (int r = 0; r < RK / 2; ++r) S[r] = dup(0.f);
-  if (LEARN)
+  for (int p = 0; p < RH / 2; ++p)
 #pragma unroll
-    for (int r = 0; r < (LEARN ? RK / 2 : 1); ++r) D[r] = dup(0.f);
+    for (int c = 0; c < 4; ++c) {
+      S[p][c] = dup(0.f);
+      if (LEARN) D[LEARN ? p : 0][c] = dup(0.f);
+    }
   const long long per_state = (long long)A.DK * A.DV;
-  if (A.o && has_col) {
+  if (A.o) {
     const float* src = nullptr;
     long long sr = A.DV, sc = 1;
     if (A.nseg > 1) {
@@ -138,17 +155,15 @@ __global__ void __launch_bounds__(kThreads) decay_scan_kernel(const ScanArgs A) 
       src = A.start + bh * per_state;
       sr = A.srow, sc = A.scol;
     }
-    if (src) {
+    const float* srcT = LEARN && A.nseg > 1 ? A.segT + (bh * A.nseg + seg) * per_state : nullptr;
 #pragma unroll
-      for (int r = 0; r < RK; ++r)
-        if (row0 + r < A.DK) (&S[r >> 1].x)[r & 1] = src[(row0 + r) * sr + (c0 + col) * sc];
-    }
-    if (LEARN && A.nseg > 1) {
-      const float* st = A.segT + (bh * A.nseg + seg) * per_state;
+    for (int r = 0; r < RH; ++r)
 #pragma unroll
-      for (int r = 0; r < RK; ++r)
-        if (row0 + r < A.DK) (&D[LEARN ? r >> 1 : 0].x)[r & 1] = st[(long long)(row0 + r) * A.DV + c0 + col];
-    }
+      for (int c = 0; c < 4; ++c)
+        if (row0 + r < A.DK && c < left) {
+          if (src) (&S[r >> 1][c].x)[r & 1] = src[(row0 + r) * sr + (c0 + col + c) * sc];
+          if (LEARN && srcT) (&D[LEARN ? r >> 1 : 0][c].x)[r & 1] = srcT[(long long)(row0 + r) * A.DV + c0 + col + c];
+        }
   }
 
   const T* qp = static_cast<const T*>(A.q.p) + b * A.q.sb + (long long)(h / A.q.group) * A.q.sh;
@@ -159,85 +174,145 @@ __global__ void __launch_bounds__(kThreads) decay_scan_kernel(const ScanArgs A) 
   const int step = A.reverse ? -1 : 1;
   float dg = 0.f;
 
+  // A chunk's tiles: q [kTok][W], k [kTok][W], v [kTok][kCols], x [kTok][kCols].
+  const auto fetch = [&](int i0) {
+    const int n = min(kTok, n_all - i0);
+    const long long t0 = A.reverse ? t_hi - 1 - i0 : t_lo + i0;
+    T* raw = reinterpret_cast<T*>(smem + M::raw) + (i0 / kTok & 1) * M::chunk;
+    if (A.o) fetch_tile<T, W>(raw, qp, A.q.sl, n, 0, A.DK, t0, step);
+    fetch_tile<T, W>(raw + kTok * W, kp, A.k.sl, n, 0, A.DK, t0, step);
+    fetch_tile<T, kCols>(raw + 2 * kTok * W, vp, A.v.sl, n, c0, A.DV, t0, step);
+    if (LEARN && A.o) fetch_tile<T, kCols>(raw + 2 * kTok * W + kTok * kCols, xp, A.x.sl, n, c0, A.DV, t0, step);
+  };
+  if (A.vec) {
+    if (n_all > 0) fetch(0);
+    asm volatile("cp.async.commit_group;\n" ::: "memory");
+  }
   for (int i0 = 0; i0 < n_all; i0 += kTok) {
     const int n = min(kTok, n_all - i0);
     const long long t0 = A.reverse ? t_hi - 1 - i0 : t_lo + i0;
+    float* tile = smem + (M::wide ? (i0 / kTok & 1) * M::chunk : 0);
+    __syncthreads();  // the last chunk has been read
+    if (A.vec) {
+      if (i0 + kTok < n_all) fetch(i0 + kTok);
+      asm volatile("cp.async.commit_group;\ncp.async.wait_group 1;\n" ::: "memory");
+      if constexpr (!M::wide) {
+        __syncthreads();
+        const T* raw = reinterpret_cast<const T*>(smem + M::raw) + (i0 / kTok & 1) * M::chunk;
+        if (A.o) widen_tile<T, W>(tile, raw, n);
+        widen_tile<T, W>(tile + kTok * W, raw + kTok * W, n);
+        widen_tile<T, kCols>(tile + 2 * kTok * W, raw + 2 * kTok * W, n);
+        if (LEARN && A.o) widen_tile<T, kCols>(tile + 2 * kTok * W + kTok * kCols, raw + 2 * kTok * W + kTok * kCols, n);
+      }
+    } else {
+      if (A.o) load_tile<T, W>(tile, qp, A.q.sl, n, 0, A.DK, t0, step);
+      load_tile<T, W>(tile + kTok * W, kp, A.k.sl, n, 0, A.DK, t0, step);
+      load_tile<T, kCols>(tile + 2 * kTok * W, vp, A.v.sl, n, c0, A.DV, t0, step);
+      if (LEARN && A.o) load_tile<T, kCols>(tile + 2 * kTok * W + kTok * kCols, xp, A.x.sl, n, c0, A.DV, t0, step);
+    }
     __syncthreads();
-    if (A.o) load_tile(qs, qp, A.q.sl, n, 0, W, A.DK, t0, step, A.vec, 1.f);
-    load_tile(ks, kp, A.k.sl, n, 0, W, A.DK, t0, step, A.vec, 1.f);
-    load_tile(vs, vp, A.v.sl, n, c0, WV, A.DV, t0, step, A.vec, A.vscale);
-    if (LEARN && A.o) load_tile(xs, xp, A.x.sl, n, c0, WV, A.DV, t0, step, A.vec, 1.f);
-    __syncthreads();
-    if (active) {
-      for (int i = 0; i < n; ++i) {
-        const float2 vj = dup(vs[i * WV + col] * ainv[i]);
-        const float4* k4 = reinterpret_cast<const float4*>(ks + i * W + row0);
-        const float4* q4 = reinterpret_cast<const float4*>(qs + i * W + row0);
-        if (!fast && lag) {
+    const float *qs = tile, *ks = tile + kTok * W, *vs = ks + kTok * W, *xs = vs + kTok * kCols;
+    for (int i = 0; i < n; ++i) {
+      const float4 v4 = *reinterpret_cast<const float4*>(vs + i * kCols + col);
+      const float ai = ainv[i];
+      const float2 vj[4] = {dup(v4.x * ai), dup(v4.y * ai), dup(v4.z * ai), dup(v4.w * ai)};
+      const float4* k4 = reinterpret_cast<const float4*>(ks + i * W + row0);
+      const float4* q4 = reinterpret_cast<const float4*>(qs + i * W + row0);
+      if (!fast && lag) {
 #pragma unroll
-          for (int r = 0; r < RK / 2; ++r) {
-            if (LEARN) D[LEARN ? r : 0] = mul2(cadd(D[LEARN ? r : 0], S[r]), a1);
-            S[r] = mul2(S[r], a1);
+        for (int p = 0; p < RH / 2; ++p)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            if (LEARN) D[LEARN ? p : 0][c] = mul2(cadd(D[LEARN ? p : 0][c], S[p][c]), a1);
+            S[p][c] = mul2(S[p][c], a1);
           }
-        }
-        float2 acc0 = dup(0.f), acc1 = dup(0.f), accT = dup(0.f);
+      }
+      float2 acc[4] = {dup(0.f), dup(0.f), dup(0.f), dup(0.f)};  // of o, or of q T
 #pragma unroll
-        for (int r = 0; r < RK / 4; ++r) {
-          const float4 kk = k4[r];
+      for (int r = 0; r < RH / 4; ++r) {
+        const float4 kk = k4[r];
+        const float2 ka = make_float2(kk.x, kk.y), kb = make_float2(kk.z, kk.w);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
           if (LEARN && fast) {
-            D[LEARN ? 2 * r : 0] = cadd(D[LEARN ? 2 * r : 0], S[2 * r]);
-            D[LEARN ? 2 * r + 1 : 0] = cadd(D[LEARN ? 2 * r + 1 : 0], S[2 * r + 1]);
+            D[LEARN ? 2 * r : 0][c] = cadd(D[LEARN ? 2 * r : 0][c], S[2 * r][c]);
+            D[LEARN ? 2 * r + 1 : 0][c] = cadd(D[LEARN ? 2 * r + 1 : 0][c], S[2 * r + 1][c]);
           }
-          S[2 * r] = ffma2(make_float2(kk.x, kk.y), vj, S[2 * r]);
-          S[2 * r + 1] = ffma2(make_float2(kk.z, kk.w), vj, S[2 * r + 1]);
-          if (A.o) {
-            const float4 qq = q4[r];
-            acc0 = ffma2(make_float2(qq.x, qq.y), S[2 * r], acc0);
-            acc1 = ffma2(make_float2(qq.z, qq.w), S[2 * r + 1], acc1);
-            if (LEARN) {
-              accT = ffma2(make_float2(qq.x, qq.y), D[LEARN ? 2 * r : 0], accT);
-              accT = ffma2(make_float2(qq.z, qq.w), D[LEARN ? 2 * r + 1 : 0], accT);
-            }
-          }
+          S[2 * r][c] = ffma2(ka, vj[c], S[2 * r][c]);
+          S[2 * r + 1][c] = ffma2(kb, vj[c], S[2 * r + 1][c]);
         }
         if (A.o) {
-          if (LEARN) dg = fmaf((accT.x + accT.y) * apow[i], xs[i * WV + col], dg);
-          if (!LEARN) {
-            const float o = ((acc0.x + acc0.y) + (acc1.x + acc1.y)) * (apow[i] * A.oscale);
-            if (KW == 1) {
-              if (has_col) DT<TO>::store(op + (t0 + (long long)i * step) * A.ol + col, o);
+          const float4 qq = q4[r];
+          const float2 qa = make_float2(qq.x, qq.y), qb = make_float2(qq.z, qq.w);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            acc[c] = ffma2(qa, LEARN ? D[LEARN ? 2 * r : 0][c] : S[2 * r][c], acc[c]);
+            acc[c] = ffma2(qb, LEARN ? D[LEARN ? 2 * r + 1 : 0][c] : S[2 * r + 1][c], acc[c]);
+          }
+        }
+      }
+      if (A.o) {
+        if (LEARN) {
+          const float4 x4 = *reinterpret_cast<const float4*>(xs + i * kCols + col);
+          float s = (acc[0].x + acc[0].y) * x4.x;
+          s = fmaf(acc[1].x + acc[1].y, x4.y, s);
+          s = fmaf(acc[2].x + acc[2].y, x4.z, s);
+          s = fmaf(acc[3].x + acc[3].y, x4.w, s);
+          dg = fmaf(s, apow[i], dg);
+        } else {
+          const float as = apow[i] * A.oscale;
+          float o[4];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            o[c] = acc[c].x + acc[c].y;
+            o[c] = (o[c] + __shfl_xor_sync(0xffffffffu, o[c], 16)) * as;
+          }
+          if (lane < 16) {
+            if (KW > 1) {
+              *reinterpret_cast<float4*>(os + (warp * kTok + i) * kCols + col) = make_float4(o[0], o[1], o[2], o[3]);
             } else {
-              os[(kw * kTok + i) * WV + col] = o;
+              TO* d = op + (t0 + (long long)i * step) * A.ol + col;
+              if (sizeof(TO) == 4 && A.ovec && left > 0) {
+                *reinterpret_cast<float4*>(d) = make_float4(o[0], o[1], o[2], o[3]);
+              } else {
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                  if (c < left) DT<TO>::store(d + c, o[c]);
+              }
             }
           }
         }
-        if (!fast && !lag) {
-#pragma unroll
-          for (int r = 0; r < RK / 2; ++r) S[r] = mul2(S[r], a1);
-        }
       }
-      if (fast) {
-        float hi = a32hi, lo = a32lo;
-        if (n != kTok) {
-          const double an = exp((double)g * n);
-          hi = (float)an;
-          lo = (float)(an - (double)hi);
-        }
+      if (!fast && !lag) {
 #pragma unroll
-        for (int r = 0; r < RK / 2; ++r) {
-          S[r] = ffma2(S[r], dup(hi), mul2(S[r], lo));
-          if (LEARN) D[LEARN ? r : 0] = ffma2(D[LEARN ? r : 0], dup(hi), mul2(D[LEARN ? r : 0], lo));
-        }
+        for (int p = 0; p < RH / 2; ++p)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) S[p][c] = mul2(S[p][c], a1);
       }
+    }
+    if (fast) {
+      float hi = achi, lo = aclo;
+      if (n != kTok) {
+        const double an = exp((double)g * n);
+        hi = (float)an;
+        lo = (float)(an - (double)hi);
+      }
+#pragma unroll
+      for (int p = 0; p < RH / 2; ++p)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          S[p][c] = ffma2(S[p][c], dup(hi), mul2(S[p][c], lo));
+          if (LEARN) D[LEARN ? p : 0][c] = ffma2(D[LEARN ? p : 0][c], dup(hi), mul2(D[LEARN ? p : 0][c], lo));
+        }
     }
     if (KW > 1 && A.o && !LEARN) {
       __syncthreads();
-      for (int i = threadIdx.x; i < n * WV; i += kThreads) {
-        const int r = i / WV, c = i - r * WV;
+      for (int i = threadIdx.x; i < n * kCols; i += 32 * KW) {
+        const int r = i / kCols, c = i - r * kCols;
         if (c0 + c < A.DV) {
           float o = 0.f;
 #pragma unroll
-          for (int j = 0; j < KW; ++j) o += os[j * kTok * WV + i];
+          for (int j = 0; j < KW; ++j) o += os[j * kTok * kCols + i];
           DT<TO>::store(op + (t0 + (long long)r * step) * A.ol + c, o);
         }
       }
@@ -246,31 +321,30 @@ __global__ void __launch_bounds__(kThreads) decay_scan_kernel(const ScanArgs A) 
 
   if (A.o && !LEARN) {  // tokens past the length: zeros
     const long long z0 = max(t_lo, t_hi);
-    for (long long i = threadIdx.x; i < (t_end - z0) * WV; i += kThreads) {
-      const long long r = i / WV;
-      const int c = (int)(i - r * WV);
+    for (long long i = threadIdx.x; i < (t_end - z0) * kCols; i += 32 * KW) {
+      const long long r = i / kCols;
+      const int c = (int)(i - r * kCols);
       if (c0 + c < A.DV) DT<TO>::store(op + (z0 + r) * A.ol + c, 0.f);
     }
   }
-  if (has_col) {
-    float* dst = nullptr;
-    long long sr = A.DV, sc = 1;
-    if (!A.o) {
-      dst = A.seg + (bh * A.nseg + seg) * per_state;
-    } else if (A.nseg == 1 && A.finish) {
-      dst = A.finish + bh * per_state;
-      sr = A.srow, sc = A.scol;
-    }
-    float* dT = LEARN && (!A.o || A.nseg == 1) ? A.segT + (bh * A.nseg + seg) * per_state : nullptr;
-#pragma unroll
-    for (int r = 0; r < RK; ++r)
-      if (row0 + r < A.DK) {
-        if (dst) dst[(row0 + r) * sr + (c0 + col) * sc] = (&S[r >> 1].x)[r & 1];
-        if (LEARN && dT) dT[(long long)(row0 + r) * A.DV + c0 + col] = (&D[LEARN ? r >> 1 : 0].x)[r & 1];
-      }
+  float* dst = nullptr;
+  long long sr = A.DV, sc = 1;
+  if (!A.o) {
+    dst = A.seg + (bh * A.nseg + seg) * per_state;
+  } else if (A.nseg == 1 && A.finish) {
+    dst = A.finish + bh * per_state;
+    sr = A.srow, sc = A.scol;
   }
-  if (LEARN && A.o && active)
-    A.dg[((bh * A.nseg + seg) * A.nslice + slice) * (KW * VW * 32) + warp * 32 + lane] = has_col ? dg * A.oscale : 0.f;
+  float* dT = LEARN && (!A.o || A.nseg == 1) ? A.segT + (bh * A.nseg + seg) * per_state : nullptr;
+#pragma unroll
+  for (int r = 0; r < RH; ++r)
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      if (row0 + r < A.DK && c < left) {
+        if (dst) dst[(row0 + r) * sr + (c0 + col + c) * sc] = (&S[r >> 1][c].x)[r & 1];
+        if (LEARN && dT) dT[(long long)(row0 + r) * A.DV + c0 + col + c] = (&D[LEARN ? r >> 1 : 0][c].x)[r & 1];
+      }
+  if (LEARN && A.o) A.dg[((bh * A.nseg + seg) * A.nslice + slice) * (32 * KW) + threadIdx.x] = dg * A.oscale;
 }
 
 // Chains the segments: seg[s] becomes the state before segment s (in scan order), finish the state after the last.
@@ -450,14 +524,14 @@ int launched() {
 }
 
 // Rows of the state that a thread holds, and warps over them, for a state of DK rows.
-void scan_shape(int DK, int* rk, int* kw) {
-  *kw = DK <= 64 ? 1 : DK <= 128 ? 2 : 4;
-  const int per = (DK + *kw - 1) / *kw;
-  *rk = (per + 15) / 16 * 16;
+void scan_shape(int DK, int* rh, int* kw) {
+  *kw = 1;
+  while (*kw * 32 < DK) *kw *= 2;
+  *rh = DK <= 16 ? 8 : 16;
 }
 
 struct ScanPlan {
-  int rk, kw, nslice, nseg, seglen;
+  int rh, kw, nslice, nseg, seglen;
   bool mma;
 };
 
@@ -480,16 +554,15 @@ ScanPlan mma_plan(const hyfft_decay_desc* d, int DV) {
   return p;
 }
 
-// Segments: enough CTAs for four on each SM, and never shorter than two chunks (a segment costs a state's traffic).
+// Segments: enough for twelve warps on each SM, and never shorter than four chunks (a segment costs a state's traffic).
 ScanPlan fma_plan(const hyfft_decay_desc* d, int DK, int DV) {
   ScanPlan p{};
-  scan_shape(DK, &p.rk, &p.kw);
-  const int wv = 32 * (p.kw > 2 ? 1 : 4 / p.kw);
-  p.nslice = (DV + wv - 1) / wv;
-  const long long rows = (long long)d->batch * d->heads * p.nslice;
-  const long long want = std::max<long long>(1, (4 * 148 + rows - 1) / std::max<long long>(rows, 1));
-  const long long most = std::max<long long>(1, (d->length + 2 * kTok - 1) / (2 * kTok));
-  long long n = std::min(want, most);
+  scan_shape(DK, &p.rh, &p.kw);
+  p.nslice = (DV + kCols - 1) / kCols;
+  const long long warps = (long long)d->batch * d->heads * p.nslice * p.kw;
+  const long long want = std::max<long long>(1, (12 * 148 + warps - 1) / warps);
+  const long long most = std::max<long long>(1, (d->length + 4 * kTok - 1) / (4 * kTok));
+  const long long n = std::min(want, most);
   const long long len = std::max<long long>(kTok, ((d->length + n - 1) / n + kTok - 1) / kTok * kTok);
   p.seglen = (int)std::min<long long>(len, 1ll << 30);
   p.nseg = (int)std::max<long long>(1, (d->length + p.seglen - 1) / p.seglen);
@@ -500,31 +573,25 @@ ScanPlan scan_plan(const hyfft_decay_desc* d, int DK, int DV) {
   return use_mma(d, DK) ? mma_plan(d, DV) : fma_plan(d, DK, DV);
 }
 
-template <typename T, typename TO, int RK, int KW, bool LEARN>
-int launch_scan_rk(const ScanArgs& A, long long ctas, cudaStream_t st) {
-  constexpr int VW = KW > 2 ? 1 : 4 / KW;
-  const size_t sm = sizeof(float) * kTok * (2 * RK * KW + 32 * VW * (LEARN ? 2 : 1) + (KW > 1 ? KW * 32 * VW : 0));
-  auto kern = decay_scan_kernel<T, TO, RK, KW, LEARN>;
-  if (!kernel_smem_once((const void*)kern, sm)) return set_error(HYFFT_ERR_CUDA, "decay attention: shared memory");
-  kern<<<(unsigned)ctas, kThreads, sm, st>>>(A);
+template <typename T, typename TO, int RH, int KW, bool LEARN>
+int launch_scan_rh(const ScanArgs& A, long long ctas, cudaStream_t st) {
+  const size_t sm = sizeof(float) * Smem<T, RH, KW, LEARN>::floats;
+  auto kern = decay_scan_kernel<T, TO, RH, KW, LEARN>;
+  if (!kernel_smem_once((const void*)kern, sm, true)) return set_error(HYFFT_ERR_CUDA, "decay attention: shared memory");
+  kern<<<(unsigned)ctas, 32 * KW, sm, st>>>(A);
   return launched();
 }
 
 template <typename T, typename TO, bool LEARN>
-int launch_scan(const ScanArgs& A, int rk, int kw, long long ctas, cudaStream_t st) {
+int launch_scan(const ScanArgs& A, int rh, int kw, long long ctas, cudaStream_t st) {
   if (ctas > 0x7fffffffLL) return set_error(HYFFT_ERR_UNSUPPORTED, "decay attention: too many rows");
-  if (kw == 1) {
-    if (rk == 16) return launch_scan_rk<T, TO, 16, 1, LEARN>(A, ctas, st);
-    if (rk == 32) return launch_scan_rk<T, TO, 32, 1, LEARN>(A, ctas, st);
-    if (rk == 48) return launch_scan_rk<T, TO, 48, 1, LEARN>(A, ctas, st);
-    return launch_scan_rk<T, TO, 64, 1, LEARN>(A, ctas, st);
+  if constexpr (LEARN || !std::is_same<T, __nv_bfloat16>::value) {  // up to 128 rows of bfloat16 run on the tensor cores
+    if (rh == 8) return launch_scan_rh<T, TO, 8, 1, LEARN>(A, ctas, st);
+    if (kw == 1) return launch_scan_rh<T, TO, 16, 1, LEARN>(A, ctas, st);
+    if (kw == 2) return launch_scan_rh<T, TO, 16, 2, LEARN>(A, ctas, st);
+    if (kw == 4) return launch_scan_rh<T, TO, 16, 4, LEARN>(A, ctas, st);
   }
-  if (kw == 2) {
-    if (rk == 48) return launch_scan_rk<T, TO, 48, 2, LEARN>(A, ctas, st);
-    return launch_scan_rk<T, TO, 64, 2, LEARN>(A, ctas, st);
-  }
-  if (rk == 48) return launch_scan_rk<T, TO, 48, 4, LEARN>(A, ctas, st);
-  return launch_scan_rk<T, TO, 64, 4, LEARN>(A, ctas, st);
+  return launch_scan_rh<T, TO, 16, 8, LEARN>(A, ctas, st);
 }
 
 bool op_vec(const Op& o, int D, int es) {
@@ -558,7 +625,7 @@ int run_scan(const hyfft_decay_desc* d, ScanArgs A, float* seg, cudaStream_t st)
     if constexpr (std::is_same<T, __nv_bfloat16>::value) {
       if (p.mma) return launch_scan_mma(P, sizeof(TO) == 4, ctas, st);
     }
-    return launch_scan<T, TO, false>(P, p.rk, p.kw, ctas, st);
+    return launch_scan<T, TO, false>(P, p.rh, p.kw, ctas, st);
   };
   if (p.nseg > 1) {
     ScanArgs P = A;
@@ -594,11 +661,10 @@ int run_learn(const hyfft_decay_desc* d, ScanArgs A, const float* dfinal, float*
   A.dg = A.seg + (p.nseg > 1 ? 2 * states : 0);
   A.finish = nullptr;
   const long long ctas = rows * p.nseg * p.nslice;
-  const int used = p.kw * 32 * (p.kw > 2 ? 1 : 4 / p.kw);
   if (p.nseg > 1) {
     ScanArgs P = A;
     P.o = nullptr;
-    int rc = launch_scan<T, T, true>(P, p.rk, p.kw, ctas, st);
+    int rc = launch_scan<T, T, true>(P, p.rh, p.kw, ctas, st);
     if (rc != HYFFT_OK) return rc;
     if (rows > 65535) return set_error(HYFFT_ERR_UNSUPPORTED, "decay attention: too many rows");
     decay_chain_kernel<<<dim3((A.DK * A.DV + 255) / 256, (unsigned)rows), 256, 0, st>>>(
@@ -607,9 +673,9 @@ int run_learn(const hyfft_decay_desc* d, ScanArgs A, const float* dfinal, float*
     if ((rc = launched()) != HYFFT_OK) return rc;
   }
   A.o = ws;  // not written by this scan: only says that it is the second pass
-  int rc = launch_scan<T, T, true>(A, p.rk, p.kw, ctas, st);
+  int rc = launch_scan<T, T, true>(A, p.rh, p.kw, ctas, st);
   if (rc != HYFFT_OK) return rc;
-  decay_dg_kernel<<<d->heads, 256, 0, st>>>(A.dg, (long long)p.nseg * p.nslice * used, finalT, dfinal,
+  decay_dg_kernel<<<d->heads, 256, 0, st>>>(A.dg, (long long)p.nseg * p.nslice * 32 * p.kw, finalT, dfinal,
                                             (long long)d->dk * d->dv, d->batch, d->heads, out);
   return launched();
 }
@@ -618,7 +684,7 @@ size_t learn_bytes(const hyfft_decay_desc* d) {
   const ScanPlan p = fma_plan(d, d->dk, d->dv);
   const size_t rows = (size_t)d->batch * d->heads, per = (size_t)d->dk * d->dv;
   return align256(sizeof(float) * (rows * per * (1 + (p.nseg > 1 ? 2 * (size_t)p.nseg : 0)) +
-                                   rows * p.nseg * p.nslice * kThreads));
+                                   rows * p.nseg * p.nslice * 32 * p.kw));
 }
 
 int check_desc(const hyfft_decay_desc* d) {
