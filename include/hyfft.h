@@ -312,7 +312,8 @@ typedef struct hyfft_decay_desc {
 } hyfft_decay_desc;
 
 HYFFT_API int hyfft_decay_workspace_size(const hyfft_decay_desc* d, size_t* fwd_bytes, size_t* bwd_bytes);
-/* final_state: the state after each sequence's last token, or NULL to skip it. */
+/* final_state: the state after each sequence's last token, or NULL to skip it. What the forward leaves in its workspace
+ * can be given to the backward of the same call as `saved` (fwd_bytes of it). */
 HYFFT_API int hyfft_decay_forward(const hyfft_decay_desc* d, const void* q, const void* k, const void* v,
                                   const float* log_decay, const int32_t* lengths, const float* initial_state,
                                   void* o, float* final_state, void* workspace, size_t workspace_bytes,
@@ -320,10 +321,10 @@ HYFFT_API int hyfft_decay_forward(const hyfft_decay_desc* d, const void* q, cons
 /* Gradients for dout [B, L, H, Dv] and dfinal_state (NULL: zero). dq, dk, dv have q's, k's and v's shapes
  * (dk and dv of a shared head are summed over its query heads in a fixed order); dlog_decay float32 [H];
  * dinitial_state [B, H, Dk, Dv]. Any of them may be NULL to skip it, dv only together with
- * dinitial_state.                                                                              */
+ * dinitial_state. saved: the forward's workspace, or NULL to compute its contents again.         */
 HYFFT_API int hyfft_decay_backward(const hyfft_decay_desc* d, const void* q, const void* k, const void* v,
                                    const float* log_decay, const int32_t* lengths, const float* initial_state,
-                                   const void* dout, const float* dfinal_state, void* dq, void* dk, void* dv,
+                                   const void* saved, const void* dout, const float* dfinal_state, void* dq, void* dk, void* dv,
                                    float* dlog_decay, float* dinitial_state, void* workspace,
                                    size_t workspace_bytes, void* stream);
 /* One token of each request: q [B, H, Dk], k [B, Hk, Dk], v [B, Hk, Dv] (the token strides and `length` are

@@ -151,6 +151,7 @@ __global__ void __launch_bounds__(32 * KW) decay_scan_kernel(const ScanArgs A) {
     long long sr = A.DV, sc = 1;
     if (A.nseg > 1) {
       src = A.seg + (bh * A.nseg + seg) * per_state;
+      sr = A.segrow, sc = A.segcol;
     } else if (A.start) {
       src = A.start + bh * per_state;
       sr = A.srow, sc = A.scol;
@@ -530,47 +531,41 @@ void scan_shape(int DK, int* rh, int* kw) {
   *rh = DK <= 16 ? 8 : 16;
 }
 
-struct ScanPlan {
-  int rh, kw, nslice, nseg, seglen;
-  bool mma;
-};
-
 // The tensor cores take every bfloat16 scan whose state has up to 128 rows.
 bool use_mma(const hyfft_decay_desc* d, int DK) { return d->dtype == HYFFT_BF16 && DK <= kMmaMaxDK; }
 
-// Two CTAs for each SM: rows alone where they give every SM one, else as many segments as fit, none shorter than four
-// chunks (a segment costs a second read of k and v and a state's traffic).
-ScanPlan mma_plan(const hyfft_decay_desc* d, int DV) {
-  ScanPlan p{};
-  p.mma = true;
-  p.nslice = (DV + kMmaCols - 1) / kMmaCols;
-  const long long rows = (long long)d->batch * d->heads * p.nslice;
-  const long long want = rows >= 148 ? 1 : 296 / rows;
-  const long long most = std::max<long long>(1, d->length / (4 * kMmaTok));
+int slices(int DV) { return (DV + kCols - 1) / kCols; }  // 64 columns a CTA on either path
+static_assert(kCols == kMmaCols && kMmaTok % kTok == 0, "one plan for both paths");
+
+struct Segments {
+  int n, len;
+};
+
+// All scans of a call cut the axis at the same places, so that one pass over the segments serves several. Tensor
+// cores: two CTAs for each SM; rows alone where they give every SM one, else as many segments as fit, none shorter than
+// four chunks (a segment costs a second read of k and v and a state's traffic). Else: twelve warps for each SM, segments of one
+// chunk at least.
+Segments segments(const hyfft_decay_desc* d, bool learn) {
+  const long long rows = (long long)d->batch * d->heads;
+  long long want, most;
+  if (!learn && use_mma(d, d->dk) && use_mma(d, d->dv)) {
+    const long long ctas = rows * std::max(slices(d->dk), slices(d->dv));
+    want = ctas >= 148 ? 1 : 296 / ctas;
+    most = d->length / (4 * kMmaTok);
+  } else {
+    int rh, kw, rh2, kw2;
+    scan_shape(d->dk, &rh, &kw);
+    scan_shape(d->dv, &rh2, &kw2);
+    const long long warps = rows * (learn ? slices(d->dv) * kw : std::max(slices(d->dv) * kw, slices(d->dk) * kw2));
+    want = (12 * 148 + warps - 1) / warps;
+    most = (d->length + kMmaTok - 1) / kMmaTok;
+  }
   const long long n = std::max<long long>(1, std::min(want, most));
   const long long len = std::max<long long>(kMmaTok, ((d->length + n - 1) / n + kMmaTok - 1) / kMmaTok * kMmaTok);
-  p.seglen = (int)std::min<long long>(len, 1ll << 30);
-  p.nseg = (int)std::max<long long>(1, (d->length + p.seglen - 1) / p.seglen);
-  return p;
-}
-
-// Segments: enough for twelve warps on each SM, and never shorter than four chunks (a segment costs a state's traffic).
-ScanPlan fma_plan(const hyfft_decay_desc* d, int DK, int DV) {
-  ScanPlan p{};
-  scan_shape(DK, &p.rh, &p.kw);
-  p.nslice = (DV + kCols - 1) / kCols;
-  const long long warps = (long long)d->batch * d->heads * p.nslice * p.kw;
-  const long long want = std::max<long long>(1, (12 * 148 + warps - 1) / warps);
-  const long long most = std::max<long long>(1, (d->length + 4 * kTok - 1) / (4 * kTok));
-  const long long n = std::min(want, most);
-  const long long len = std::max<long long>(kTok, ((d->length + n - 1) / n + kTok - 1) / kTok * kTok);
-  p.seglen = (int)std::min<long long>(len, 1ll << 30);
-  p.nseg = (int)std::max<long long>(1, (d->length + p.seglen - 1) / p.seglen);
-  return p;
-}
-
-ScanPlan scan_plan(const hyfft_decay_desc* d, int DK, int DV) {
-  return use_mma(d, DK) ? mma_plan(d, DV) : fma_plan(d, DK, DV);
+  Segments g;
+  g.len = (int)std::min<long long>(len, 1ll << 30);
+  g.n = (int)std::max<long long>(1, (d->length + g.len - 1) / g.len);
+  return g;
 }
 
 template <typename T, typename TO, int RH, int KW, bool LEARN>
@@ -601,90 +596,105 @@ bool op_vec(const Op& o, int D, int es) {
 
 size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
-size_t seg_bytes(const hyfft_decay_desc* d, const ScanPlan& p) {
-  return p.nseg > 1 ? align256(sizeof(float) * (size_t)d->batch * d->heads * p.nseg * d->dk * d->dv) : 0;
+// Bytes of the segments' states; 0 where the axis is not cut.
+size_t seg_bytes(const hyfft_decay_desc* d) {
+  const Segments g = segments(d, false);
+  return g.n > 1 ? align256(sizeof(float) * (size_t)d->batch * d->heads * g.n * d->dk * d->dv) : 0;
 }
 
-// One scan: segments' sums and their chain where the axis is cut, then the outputs.
-template <typename T, typename TO>
-int run_scan(const hyfft_decay_desc* d, ScanArgs A, float* seg, cudaStream_t st) {
-  const ScanPlan p = scan_plan(d, A.DK, A.DV);
+void set_segments(const hyfft_decay_desc* d, ScanArgs& A, bool learn) {
+  const Segments g = segments(d, learn);
   A.B = d->batch;
   A.H = d->heads;
   A.L = (int)d->length;
-  A.nseg = p.nseg;
-  A.seglen = p.seglen;
-  A.nslice = p.nslice;
-  A.seg = seg;
+  A.nseg = g.n;
+  A.seglen = g.len;
+  A.nslice = slices(A.DV);
+}
+
+template <typename T, typename TO>
+int run_pass(const hyfft_decay_desc* d, ScanArgs A, cudaStream_t st) {
   const int es = (int)sizeof(T);
-  A.vec = op_vec(A.q, A.DK, es) && op_vec(A.k, A.DK, es) && op_vec(A.v, A.DV, es);
+  A.vec = (!A.o || op_vec(A.q, A.DK, es)) && op_vec(A.k, A.DK, es) && op_vec(A.v, A.DV, es);
   A.ovec = A.DV % 8 == 0 && reinterpret_cast<uintptr_t>(A.o) % 16 == 0;
-  const long long rows = (long long)d->batch * d->heads;
-  const long long ctas = rows * p.nseg * p.nslice;
-  const auto pass = [&](const ScanArgs& P) {
-    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-      if (p.mma) return launch_scan_mma(P, sizeof(TO) == 4, ctas, st);
-    }
-    return launch_scan<T, TO, false>(P, p.rh, p.kw, ctas, st);
-  };
-  if (p.nseg > 1) {
-    ScanArgs P = A;
-    P.o = nullptr;
-    int rc = pass(P);
-    if (rc != HYFFT_OK) return rc;
-    if (rows > 65535) return set_error(HYFFT_ERR_UNSUPPORTED, "decay attention: too many rows");
-    decay_chain_kernel<<<dim3((A.DK * A.DV + 255) / 256, (unsigned)rows), 256, 0, st>>>(
-        seg, nullptr, nullptr, A.start, A.finish, A.log_decay, A.lengths, A.H, A.L, A.DK, A.DV, A.srow, A.scol, p.nseg,
-        p.seglen, A.reverse);
-    if ((rc = launched()) != HYFFT_OK) return rc;
+  const long long ctas = (long long)d->batch * d->heads * A.nseg * A.nslice;
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    if (use_mma(d, A.DK)) return launch_scan_mma(A, sizeof(TO) == 4, ctas, st);
   }
-  return pass(A);
+  int rh, kw;
+  scan_shape(A.DK, &rh, &kw);
+  return launch_scan<T, TO, false>(A, rh, kw, ctas, st);
+}
+
+// The segments' start states, [B * H, nseg, dk, dv], and the state after the last one; nothing where the axis is not cut.
+template <typename T>
+int run_states(const hyfft_decay_desc* d, ScanArgs A, float* seg, cudaStream_t st) {
+  set_segments(d, A, false);
+  if (A.nseg == 1) return HYFFT_OK;
+  A.o = nullptr;
+  A.seg = seg;
+  const long long rows = (long long)d->batch * d->heads;
+  if (rows > 65535) return set_error(HYFFT_ERR_UNSUPPORTED, "decay attention: too many rows");
+  const int rc = run_pass<T, T>(d, A, st);
+  if (rc != HYFFT_OK) return rc;
+  decay_chain_kernel<<<dim3((A.DK * A.DV + 255) / 256, (unsigned)rows), 256, 0, st>>>(
+      seg, nullptr, nullptr, A.start, A.finish, A.log_decay, A.lengths, A.H, A.L, A.DK, A.DV, A.srow, A.scol, A.nseg,
+      A.seglen, A.reverse);
+  return launched();
+}
+
+// The outputs, from segment states of either orientation (`turned`: the states' rows are this scan's columns).
+template <typename T, typename TO>
+int run_outputs(const hyfft_decay_desc* d, ScanArgs A, const float* seg, bool turned, cudaStream_t st) {
+  set_segments(d, A, false);
+  A.seg = const_cast<float*>(seg);
+  A.segrow = turned ? 1 : A.DV;
+  A.segcol = turned ? A.DK : 1;
+  return run_pass<T, TO>(d, A, st);
 }
 
 // The decay's gradient: the forward scan once more with T beside S.
 template <typename T>
 int run_learn(const hyfft_decay_desc* d, ScanArgs A, const float* dfinal, float* ws, float* out, cudaStream_t st) {
-  const ScanPlan p = fma_plan(d, A.DK, A.DV);
-  A.B = d->batch;
-  A.H = d->heads;
-  A.L = (int)d->length;
-  A.nseg = p.nseg;
-  A.seglen = p.seglen;
-  A.nslice = p.nslice;
+  set_segments(d, A, true);
+  int rh, kw;
+  scan_shape(A.DK, &rh, &kw);
+  A.segrow = A.DV, A.segcol = 1;
   const int es = (int)sizeof(T);
   A.vec = op_vec(A.q, A.DK, es) && op_vec(A.k, A.DK, es) && op_vec(A.v, A.DV, es) && op_vec(A.x, A.DV, es);
   const long long rows = (long long)d->batch * d->heads;
-  const size_t states = (size_t)rows * p.nseg * d->dk * d->dv;
+  const size_t states = (size_t)rows * A.nseg * d->dk * d->dv;
   float* finalT = ws;
   A.seg = ws + (size_t)rows * d->dk * d->dv;
-  A.segT = p.nseg > 1 ? A.seg + states : finalT;
-  A.dg = A.seg + (p.nseg > 1 ? 2 * states : 0);
+  A.segT = A.nseg > 1 ? A.seg + states : finalT;
+  A.dg = A.seg + (A.nseg > 1 ? 2 * states : 0);
   A.finish = nullptr;
-  const long long ctas = rows * p.nseg * p.nslice;
-  if (p.nseg > 1) {
+  const long long ctas = rows * A.nseg * A.nslice;
+  if (A.nseg > 1) {
     ScanArgs P = A;
     P.o = nullptr;
-    int rc = launch_scan<T, T, true>(P, p.rh, p.kw, ctas, st);
+    int rc = launch_scan<T, T, true>(P, rh, kw, ctas, st);
     if (rc != HYFFT_OK) return rc;
     if (rows > 65535) return set_error(HYFFT_ERR_UNSUPPORTED, "decay attention: too many rows");
     decay_chain_kernel<<<dim3((A.DK * A.DV + 255) / 256, (unsigned)rows), 256, 0, st>>>(
-        A.seg, A.segT, finalT, A.start, nullptr, A.log_decay, A.lengths, A.H, A.L, A.DK, A.DV, A.srow, A.scol, p.nseg,
-        p.seglen, 0);
+        A.seg, A.segT, finalT, A.start, nullptr, A.log_decay, A.lengths, A.H, A.L, A.DK, A.DV, A.srow, A.scol, A.nseg,
+        A.seglen, 0);
     if ((rc = launched()) != HYFFT_OK) return rc;
   }
   A.o = ws;  // not written by this scan: only says that it is the second pass
-  int rc = launch_scan<T, T, true>(A, p.rh, p.kw, ctas, st);
+  int rc = launch_scan<T, T, true>(A, rh, kw, ctas, st);
   if (rc != HYFFT_OK) return rc;
-  decay_dg_kernel<<<d->heads, 256, 0, st>>>(A.dg, (long long)p.nseg * p.nslice * 32 * p.kw, finalT, dfinal,
+  decay_dg_kernel<<<d->heads, 256, 0, st>>>(A.dg, (long long)A.nseg * A.nslice * 32 * kw, finalT, dfinal,
                                             (long long)d->dk * d->dv, d->batch, d->heads, out);
   return launched();
 }
 
 size_t learn_bytes(const hyfft_decay_desc* d) {
-  const ScanPlan p = fma_plan(d, d->dk, d->dv);
+  const Segments g = segments(d, true);
+  int rh, kw;
+  scan_shape(d->dk, &rh, &kw);
   const size_t rows = (size_t)d->batch * d->heads, per = (size_t)d->dk * d->dv;
-  return align256(sizeof(float) * (rows * per * (1 + (p.nseg > 1 ? 2 * (size_t)p.nseg : 0)) +
-                                   rows * p.nseg * p.nslice * 32 * p.kw));
+  return align256(sizeof(float) * (rows * per * (1 + (g.n > 1 ? 2 * (size_t)g.n : 0)) + rows * g.n * slices(d->dv) * 32 * kw));
 }
 
 int check_desc(const hyfft_decay_desc* d) {
@@ -719,20 +729,22 @@ int forward_t(const hyfft_decay_desc* d, const void* q, const void* k, const voi
   A.log_decay = g, A.lengths = lengths, A.start = s0, A.finish = s1;
   A.vscale = 1.f, A.oscale = d->scale;
   A.DK = d->dk, A.DV = d->dv, A.srow = d->dv, A.scol = 1;
-  return run_scan<T, T>(d, A, ws, st);
+  const int rc = run_states<T>(d, A, ws, st);
+  return rc == HYFFT_OK ? run_outputs<T, T>(d, A, ws, false, st) : rc;
 }
 
 // dk or dv: straight to the output where no head is shared, else in float32 per query head and summed.
 template <typename T>
-int shared_scan(const hyfft_decay_desc* d, ScanArgs A, void* out, int D, float* seg, float* per_head, cudaStream_t st) {
+int shared_scan(const hyfft_decay_desc* d, ScanArgs A, void* out, int D, const float* seg, bool turned, float* per_head,
+                cudaStream_t st) {
   if (d->heads == d->kv_heads) {
     const Rows ro = dense(d, d->heads, D);
     A.o = out, A.ob = ro.b, A.ol = ro.l, A.oh = ro.h;
-    return run_scan<T, T>(d, A, seg, st);
+    return run_outputs<T, T>(d, A, seg, turned, st);
   }
   const Rows ro = dense(d, d->heads, D);
   A.o = per_head, A.ob = ro.b, A.ol = ro.l, A.oh = ro.h;
-  int rc = run_scan<T, float>(d, A, seg, st);
+  int rc = run_outputs<T, float>(d, A, seg, turned, st);
   if (rc != HYFFT_OK) return rc;
   const long long n = (long long)d->batch * d->length * d->kv_heads * D;
   if (n == 0) return HYFFT_OK;
@@ -743,7 +755,8 @@ int shared_scan(const hyfft_decay_desc* d, ScanArgs A, void* out, int D, float* 
 
 template <typename T>
 int backward_t(const hyfft_decay_desc* d, const void* q, const void* k, const void* v, const float* g,
-               const int* lengths, const float* s0, const void* dout, const float* ds1, void* dq, void* dk, void* dv,
+               const int* lengths, const float* s0, const float* saved, const void* dout, const float* ds1, void* dq,
+               void* dk, void* dv,
                float* dg, float* ds0, char* ws, size_t seg_size, size_t group_size, cudaStream_t st) {
   const int r = d->heads / d->kv_heads;
   const Op oq{q, d->q_stride[0], d->q_stride[1], d->q_stride[2], 1};
@@ -757,28 +770,34 @@ int backward_t(const hyfft_decay_desc* d, const void* q, const void* k, const vo
   A.log_decay = g, A.lengths = lengths;
   int rc;
   if (dq) {  // forwards over (do, v, k), the state transposed
+    if (!saved) {
+      ScanArgs P = A;
+      P.k = ok, P.v = ov, P.start = s0, P.vscale = 1.f;
+      P.DK = d->dk, P.DV = d->dv, P.srow = d->dv, P.scol = 1;
+      if ((rc = run_states<T>(d, P, seg, st)) != HYFFT_OK) return rc;
+      saved = seg;
+    }
     ScanArgs P = A;
     const Rows ro = dense(d, d->heads, d->dk);
     P.q = od, P.k = ov, P.v = ok;
     P.o = dq, P.ob = ro.b, P.ol = ro.l, P.oh = ro.h;
     P.start = s0, P.vscale = 1.f, P.oscale = d->scale;
     P.DK = d->dv, P.DV = d->dk, P.srow = 1, P.scol = d->dv;
-    if ((rc = run_scan<T, T>(d, P, seg, st)) != HYFFT_OK) return rc;
+    if ((rc = run_outputs<T, T>(d, P, saved, true, st)) != HYFFT_OK) return rc;
   }
-  if (dk) {  // backwards over (v, do, q), the state transposed
+  ScanArgs G = A;  // backwards over (k, q, do): the state's gradient, in the state's own orientation
+  G.q = ok, G.k = oq, G.v = od;
+  G.start = ds1, G.finish = ds0, G.vscale = d->scale, G.oscale = 1.f, G.reverse = 1;
+  G.DK = d->dk, G.DV = d->dv, G.srow = d->dv, G.scol = 1;
+  if ((dk || dv) && (rc = run_states<T>(d, G, seg, st)) != HYFFT_OK) return rc;
+  if (dk) {  // and over (v, do, q), transposed
     ScanArgs P = A;
     P.q = ov, P.k = od, P.v = oq;
     P.start = ds1, P.vscale = d->scale, P.oscale = 1.f, P.reverse = 1;
     P.DK = d->dv, P.DV = d->dk, P.srow = 1, P.scol = d->dv;
-    if ((rc = shared_scan<T>(d, P, dk, d->dk, seg, per_head, st)) != HYFFT_OK) return rc;
+    if ((rc = shared_scan<T>(d, P, dk, d->dk, seg, true, per_head, st)) != HYFFT_OK) return rc;
   }
-  if (dv || ds0) {  // backwards over (k, q, do)
-    ScanArgs P = A;
-    P.q = ok, P.k = oq, P.v = od;
-    P.start = ds1, P.finish = ds0, P.vscale = d->scale, P.oscale = 1.f, P.reverse = 1;
-    P.DK = d->dk, P.DV = d->dv, P.srow = d->dv, P.scol = 1;
-    if ((rc = shared_scan<T>(d, P, dv, d->dv, seg, per_head, st)) != HYFFT_OK) return rc;
-  }
+  if (dv && (rc = shared_scan<T>(d, G, dv, d->dv, seg, false, per_head, st)) != HYFFT_OK) return rc;
   if (dg) {
     ScanArgs P = A;
     P.q = oq, P.k = ok, P.v = ov, P.x = od;
@@ -790,12 +809,11 @@ int backward_t(const hyfft_decay_desc* d, const void* q, const void* k, const vo
 }
 
 struct Sizes {
-  size_t fwd, seg, group, learn;
+  size_t seg, group, learn;
 };
 Sizes sizes(const hyfft_decay_desc* d) {
   Sizes s;
-  s.fwd = seg_bytes(d, scan_plan(d, d->dk, d->dv));
-  s.seg = std::max(s.fwd, seg_bytes(d, scan_plan(d, d->dv, d->dk)));
+  s.seg = seg_bytes(d);
   s.group = d->heads == d->kv_heads
                 ? 0
                 : align256(sizeof(float) * (size_t)d->batch * d->length * d->heads * std::max(d->dk, d->dv));
@@ -814,7 +832,7 @@ int hyfft_decay_workspace_size(const hyfft_decay_desc* d, size_t* fwd_bytes, siz
   const int rc = check_desc(d);
   if (rc != HYFFT_OK) return rc;
   const Sizes s = sizes(d);
-  if (fwd_bytes) *fwd_bytes = s.fwd;
+  if (fwd_bytes) *fwd_bytes = s.seg;
   if (bwd_bytes) *bwd_bytes = s.seg + s.group + s.learn;
   return HYFFT_OK;
 }
@@ -827,7 +845,7 @@ int hyfft_decay_forward(const hyfft_decay_desc* d, const void* q, const void* k,
   if (!log_decay || (d->length > 0 && (!q || !k || !v || !o)))
     return set_error(HYFFT_ERR_INVALID, "decay attention: null tensor");
   const Sizes s = sizes(d);
-  if (workspace_bytes < s.fwd || (s.fwd && !workspace))
+  if (workspace_bytes < s.seg || (s.seg && !workspace))
     return set_error(HYFFT_ERR_WORKSPACE, "decay attention: workspace too small");
   if (bind_device_of(log_decay) != HYFFT_OK) return set_error(HYFFT_ERR_CUDA, "decay attention: device");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -840,7 +858,8 @@ int hyfft_decay_forward(const hyfft_decay_desc* d, const void* q, const void* k,
 }
 
 int hyfft_decay_backward(const hyfft_decay_desc* d, const void* q, const void* k, const void* v, const float* log_decay,
-                         const int32_t* lengths, const float* initial_state, const void* dout, const float* dfinal_state,
+                         const int32_t* lengths, const float* initial_state, const void* saved, const void* dout,
+                         const float* dfinal_state,
                          void* dq, void* dk, void* dv, float* dlog_decay, float* dinitial_state, void* workspace,
                          size_t workspace_bytes, void* stream) {
   const int rc = check_desc(d);
@@ -858,12 +877,12 @@ int hyfft_decay_backward(const hyfft_decay_desc* d, const void* q, const void* k
   if (d->length == 0) dq = dk = dv = nullptr;
   if (d->length == 0 && dinitial_state) dv = ws;  // no token writes it
   if (d->dtype == HYFFT_F32)
-    return backward_t<float>(d, q, k, v, log_decay, lengths, initial_state, dout, dfinal_state, dq, dk, dv, dlog_decay,
+    return backward_t<float>(d, q, k, v, log_decay, lengths, initial_state, static_cast<const float*>(saved), dout, dfinal_state, dq, dk, dv, dlog_decay,
                              dinitial_state, ws, s.seg, s.group, st);
   if (d->dtype == HYFFT_BF16)
-    return backward_t<__nv_bfloat16>(d, q, k, v, log_decay, lengths, initial_state, dout, dfinal_state, dq, dk, dv,
+    return backward_t<__nv_bfloat16>(d, q, k, v, log_decay, lengths, initial_state, static_cast<const float*>(saved), dout, dfinal_state, dq, dk, dv,
                                      dlog_decay, dinitial_state, ws, s.seg, s.group, st);
-  return backward_t<__half>(d, q, k, v, log_decay, lengths, initial_state, dout, dfinal_state, dq, dk, dv, dlog_decay,
+  return backward_t<__half>(d, q, k, v, log_decay, lengths, initial_state, static_cast<const float*>(saved), dout, dfinal_state, dq, dk, dv, dlog_decay,
                             dinitial_state, ws, s.seg, s.group, st);
 }
 

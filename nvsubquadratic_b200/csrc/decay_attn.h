@@ -25,7 +25,8 @@ struct ScanArgs {
   float* dg;           // [B * H, nseg, ...] partial sums of the decay's gradient
   float vscale, oscale;
   int B, H, L, DK, DV;  // DK: rows of the state in this scan's order, DV: its columns
-  int srow, scol;    // strides of start and finish
+  int srow, scol;        // strides of start and finish
+  int segrow, segcol;    // strides of a segment's start state as it is read
   int nseg, seglen, nslice;
   int reverse;  // the decay is applied after a token's output instead of before
   int vec;      // q, k, v (and x) can be read in 16-byte pieces

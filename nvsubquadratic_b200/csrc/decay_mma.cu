@@ -400,6 +400,7 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A, co
       long long sr = A.DV, sc = 1;
       if (OUT && A.nseg > 1) {
         src = A.seg + (bh * A.nseg + seg) * per_state;
+        sr = A.segrow, sc = A.segcol;
       } else if (OUT && A.start) {
         src = A.start + bh * per_state;
         sr = A.srow, sc = A.scol;

@@ -86,7 +86,7 @@ def _workspaces(d) -> tuple[int, int]:
 
 
 def _forward(q, k, v, log_decay, initial_state, lengths, scale, want_state):
-    """(o, state or None, the tensors as the library read them)."""
+    """(o, state or None, the tensors as the library read them and what it leaves for the backward)."""
     dev = _lib.require_cuda(q, k, v, log_decay, initial_state, lengths)
     q, k, v = _unit(q), _unit(k), _unit(v)
     g = log_decay.detach().to(torch.float32).contiguous()
@@ -95,14 +95,16 @@ def _forward(q, k, v, log_decay, initial_state, lengths, scale, want_state):
     Dv = v.shape[-1]
     o = q.new_empty((B, L, H, Dv))
     state = g.new_empty((B, H, Dk, Dv)) if want_state else None
+    saved = None
     if B:
         d, (need, _) = _plan(q, k, v, scale)
         ws = _lib.workspace(need, dev)
+        saved = ws if need else None
         rc = _lib.load().hyfft_decay_forward(ctypes.byref(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(),
                                              _lib.ptr(lengths), _lib.ptr(s0), o.data_ptr(), _lib.ptr(state),
                                              ws.data_ptr(), ws.numel(), _lib.stream_ptr(dev))
         _lib.check(rc, "hyfft_decay_forward")
-    return o, state, (q, k, v, g, s0)
+    return o, state, (q, k, v, g, s0, saved)
 
 
 class _DecayFunction(torch.autograd.Function):
@@ -116,7 +118,7 @@ class _DecayFunction(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, do, dstate):
-        q, k, v, g, s0, lengths = ctx.saved_tensors
+        q, k, v, g, s0, saved, lengths = ctx.saved_tensors
         dev = q.device
         want = ctx.needs_input_grad
         B, L, H, Dk = q.shape
@@ -139,7 +141,7 @@ class _DecayFunction(torch.autograd.Function):
         d, (_, need) = _plan(q, k, v, ctx.scale, do)
         ws = _lib.workspace(need, dev)
         rc = _lib.load().hyfft_decay_backward(ctypes.byref(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(),
-                                              _lib.ptr(lengths), _lib.ptr(s0), do.data_ptr(), _lib.ptr(dstate),
+                                              _lib.ptr(lengths), _lib.ptr(s0), _lib.ptr(saved), do.data_ptr(), _lib.ptr(dstate),
                                               _lib.ptr(dq), _lib.ptr(dk), _lib.ptr(dv), _lib.ptr(dg), _lib.ptr(ds0),
                                               ws.data_ptr(), ws.numel(), _lib.stream_ptr(dev))
         _lib.check(rc, "hyfft_decay_backward")
