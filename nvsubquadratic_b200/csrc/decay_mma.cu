@@ -18,12 +18,13 @@
 // chunks are swizzled by the row's number (chunk ^ row % 8). The tensor core reads such a tile along either axis, so K serves
 // as K^T and V, S as they lie; and both halves of a 32-byte sector stay neighbours, which tiles of 8 x 16-byte core
 // matrices did not give: cp.async then fetched every sector twice. Rows are in the order of time in either direction.
-// Twelve warps: three load (TMA; the last, partial chunk and tensors that TMA cannot take by cp.async, with zeros past a
-// length or a head size; two take turns with K and V, one brings Q), one issues the products, eight compute: they decay
-// P, update the state, split the next chunk's V and write the outputs. Only mbarriers order them, so products and loads
-// run under the computing warps' work; two CTAs share an SM (<= 113 KB, 256 TMEM columns each).
+// Sixteen warps: three load (TMA; the last, partial chunk and tensors that TMA cannot take by cp.async, with zeros past a
+// length or a head size; two take turns with K and V, one brings Q), one issues the products, eight compute: they decay P,
+// update the state and split the next chunk's V; four write the outputs. Only mbarriers order them. The computing warps' chain
+// of TMEM reads, shared-memory writes and barriers sets the pace, so what need not be in it is not: @WRITERS@.
+// Registers move from the loading to the computing warps. Two CTAs share an SM (<= 113 KB, 256 TMEM columns each).
 //
-// The computing warps' instructions are the bound after HBM: 64-row products lie in 16 of a warp's 32 TMEM lanes, and
+// 64-row products lie in 16 of a warp's 32 TMEM lanes, and
 // the 16 x 256-bit load shape spreads those over all 32 threads (two rows, pairs of columns).
 #include <cuda.h>
 #include <cudaTypedefs.h>
@@ -50,23 +51,33 @@ using bf16 = __nv_bfloat16;
 constexpr int kT = kMmaTok, kC = kMmaCols;
 constexpr int kThreads = 256;  // computing
 constexpr int kLoader = kThreads / 32, kIssuer = kLoader + 3;  // first loading warp, issuing warp
-constexpr int kAll = kThreads + 4 * 32;
+constexpr int kWriter = kIssuer + 1, kWriters = 4;
+constexpr int kAll = 32 * (kWriter + kWriters);
+// Registers of a thread: computing, loading and issuing, writing; together those of the launch (64 for each of 512).
+template <int DK>
+struct Regs {
+  static constexpr int compute = DK == 64 ? 72 : 88, load = DK == 64 ? 40 : 32, write = DK == 64 ? 72 : 48;
+  static_assert(kThreads * compute + 128 * load + 128 * write <= 64 * kAll, "setmaxnreg would wait forever");
+};
 constexpr int kColP = 0, kColR = 64, kColO = 128, kColS = 192, kTmemCols = 256;  // kColS - 64: a second one without outputs
 
-// What each mbarrier says. "done" by the tensor core, the others by the warps.
+// What each mbarrier says: full and empty for the loads, done by the tensor core, the others by the warps.
+// A barrier with two phases behind its waiter cannot be told from one with none: where a waiter may fall behind (two
+// buffers in use), each buffer has its own.
 enum Bar {
-  kFull = 0,    // K and V of buffer 0, 1 are in place
-  kFullQ = 2,
-  kEmpty = 3,   // products have read K and V of buffer 0, 1
-  kDoneR = 5,   // Q and the rounded state have been read, R is there
-  kDoneP = 6,
-  kDoneO = 7,
-  kDoneS = 8,   // K^T V is there, of buffer 0, 1
-  kHaveV = 10,  // the decayed V is in place, of buffer 0, 1
-  kHaveS = 12,  // the rounded state is in place, the accumulator of buffer 0, 1 free
-  kHaveP = 14,  // P is in place (and its accumulator free)
-  kReadO = 15,  // R and P V have been read
-  kBars = 16
+  kFull = 0,     // K and V of buffer 0, 1 are in place
+  kFullQ = 2,    // Q of buffer 0, 1
+  kEmpty = 4,    // products have read K and V of buffer 0, 1
+  kEmptyQ = 6,   // and Q of buffer 0, 1
+  kDoneR = 8,    // R is there, the rounded state has been read
+  kDoneP = 9,
+  kDoneO = 10,
+  kDoneS = 11,   // K^T V is there, of buffer 0, 1
+  kHaveV = 13,   // the decayed V is in place, of buffer 0, 1
+  kHaveS = 15,   // the rounded state is in place, the accumulator of buffer 0, 1 free
+  kHaveP = 17,   // P is in place (and its accumulator free)
+  kReadO = 18,   // R and P V have been read, by the writing warps
+  kBars = 19
 };
 
 // Bytes of the shared-memory layout for a state of DK (64 or 128) rows whose update takes TERMS bfloat16 terms. Tiles
@@ -76,11 +87,12 @@ template <int DK, bool OUT, int TERMS>
 struct Layout {
   static constexpr int qk = DK / 64 * kTile;
   static constexpr int q = 0;
-  static constexpr int k = q + (OUT ? qk : 0);
+  static constexpr int qbuf = DK == 64 ? 2 : 1;  // as many as two CTAs on an SM leave room for
+  static constexpr int k = q + (OUT ? qbuf * qk : 0);
   static constexpr int v = k + 2 * qk;
   static constexpr int wbuf = OUT ? 1 : 2;
   static constexpr int w = v + 2 * kTile;               // the decayed V
-  static constexpr int p = w + wbuf * TERMS * kTile;    // P, then the outputs on their way out
+  static constexpr int p = w + wbuf * TERMS * kTile;    // P
   static constexpr int s = p + (OUT ? kTile : 0);       // the rounded state
   static constexpr int tab = s + (OUT ? DK * 128 : 0);  // a^d for d = -64 .. 64 (zeros below 0)
   static constexpr int bar = tab + (2 * kT + 4) * 4;
@@ -89,12 +101,20 @@ struct Layout {
 };
 // Byte of column c (even) of a row in a swizzled tile of 64 columns.
 __device__ __forceinline__ int swz(int row, int c) { return row * 128 + ((((c >> 3) ^ row) & 7) << 4) + (c & 7) * 2; }
-// Descriptor of a swizzled tile. Rows along M or N, 64 columns along K: groups of 8 rows 1024 bytes apart, 32 bytes for
-// each 16 columns. Rows along K, columns along M or N: groups of 8 rows 1024 bytes apart (2048 for each 16 rows), blocks
-// of 64 columns a tile apart.
-__device__ __forceinline__ uint64_t tile_desc(uint32_t addr) {
-  return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(kTile >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) |
-         (2ull << 61);
+// Descriptor of a swizzled tile, as two words of which only the low one depends on the address. Rows along M or N, 64
+// columns along K: groups of 8 rows 1024 bytes apart, 32 bytes for each 16 columns. Rows along K, columns along M or N:
+// groups of 8 rows 1024 bytes apart (2048 for each 16 rows), blocks of 64 columns a tile apart.
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_low(const void* p) {
+  return (umma::su32(p) >> 4) | ((uint32_t)(kTile >> 4) << 16);
+}
+constexpr int kAlongK = 32 >> 4, kAlongRows = 2048 >> 4, kNextTile = kTile >> 4;  // steps of the low word
+__device__ __forceinline__ void mma(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n.reg .pred p;\n.reg .b64 da, db;\nmov.b64 da, {%1, %5};\nmov.b64 db, {%2, %5};\nsetp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)add), "n"(kDescHigh)
+      : "memory");
 }
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool valid) {
@@ -112,24 +132,39 @@ __device__ __forceinline__ void hand_over(uint64_t* bar) {
   __syncwarp();
   if ((threadIdx.x & 31) == 0) arrive(bar);
 }
-// Waits for the phase; gives up after about a second (2^16 sleeps of at most 2^14 ns) and returns false.
+// Waits for the phase; gives up after about a second and returns false. No time hint: with one, try_wait becomes a loop of
+// short sleeps (128 x 128 grid training: 71 us a pass with outputs, without the hint 69).
+__device__ __forceinline__ bool try_phase(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(done)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return done != 0;
+}
 __device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity) {
   const uint32_t a = umma::su32(bar);
-  for (int i = 0; i < (1 << 16); ++i) {
-    uint32_t done;
-    asm volatile(
-        "{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\nselp.u32 %0, 1, 0, p;\n}\n"
-        : "=r"(done)
-        : "r"(a), "r"(parity), "r"(1 << 14)
-        : "memory");
-    if (done) return true;
-  }
-  return false;
+  if (try_phase(a, parity)) return true;
+  const long long t0 = clock64();
+  while (!try_phase(a, parity))
+    if (clock64() - t0 > (1ll << 31)) return false;
+  return true;
 }
 __device__ __forceinline__ bool elect() {
   uint32_t p;
   asm volatile("{\n.reg .pred q;\nelect.sync _|q, 0xffffffff;\nselp.u32 %0, 1, 0, q;\n}\n" : "=r"(p));
   return p != 0;
+}
+
+// Lanes `by` apart exchange: the lane whose bit is clear keeps a and gives b, the other keeps b and gives a.
+__device__ __forceinline__ void swap_pairs(uint32_t& a, uint32_t& b, int by, int lane) {
+  const bool up = lane & by;
+  const uint32_t got = __shfl_xor_sync(0xffffffffu, up ? a : b, by);
+  if (up)
+    a = got;
+  else
+    b = got;
 }
 
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
@@ -255,7 +290,8 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A, co
 
   if (warp == 0) umma::tmem_alloc(tslot, kTmemCols);
   if (tid == 0) {
-    for (int i = 0; i < kBars; ++i) umma::mbar_init(&bar[i], i < kHaveV ? 1 : kThreads / 32);
+    for (int i = 0; i < kBars; ++i)
+      umma::mbar_init(&bar[i], i < kHaveV ? 1 : i == kReadO ? kWriters : kThreads / 32);
     umma::fence_mbar_init();
   }
   umma::fence_before_sync();
@@ -269,6 +305,15 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A, co
     umma::fence_after_sync();
   };
 
+  const float g = A.log_decay[h];
+  // a^d, d = -64 .. 64, by the computing and writing warps for themselves
+  const auto fill_table = [&](int i) {
+    if (i <= 2 * kT) tab[i] = i < kT ? 0.f : i == kT ? 1.f : expf(g * (i - kT));
+    asm volatile("bar.sync 1, %0;" ::"n"(kThreads + 32 * kWriters) : "memory");
+  };
+  if (warp >= kLoader && warp < kWriter) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Regs<DK>::load));
+  }
   if (warp >= kLoader && warp < kIssuer) {
     const int who = warp - kLoader;
     if (who < 2) {
@@ -296,42 +341,45 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A, co
       const int hq = h / A.q.group;
       const bf16* qp = static_cast<const bf16*>(A.q.p) + b * A.q.sb + hq * A.q.sh;
       for (int i = 0; i < chunks; ++i) {
-        if (i) wait(kDoneR, i - 1);
+        const int qb = i % L::qbuf;
+        unsigned char* qd = smem + L::q + qb * L::qk;
+        if (i >= L::qbuf) wait(kEmptyQ + qb, i / L::qbuf - 1);
         if (M.on && tokens(i) == kT) {
           if (lane == 0) {
-            expect(&bar[kFullQ], L::qk);
-            load_box<DK>(umma::su32(smem + L::q), &M.q, &bar[kFullQ], 0, hq, (int)first(i), (int)b);
+            expect(&bar[kFullQ + qb], L::qk);
+            load_box<DK>(umma::su32(qd), &M.q, &bar[kFullQ + qb], 0, hq, (int)first(i), (int)b);
           }
           __syncwarp();
         } else {
-          load_tile<DK>(smem + L::q, qp, A.q.sl, tokens(i), 0, A.DK, first(i), A.vec);
+          load_tile<DK>(qd, qp, A.q.sl, tokens(i), 0, A.DK, first(i), A.vec);
           cp_wait();
-          hand_over(&bar[kFullQ]);
+          hand_over(&bar[kFullQ + qb]);
         }
       }
     }
   } else if (warp == kIssuer) {
-    const uint32_t sq = umma::su32(smem + L::q), sw = umma::su32(smem + L::w), sp = umma::su32(smem + L::p);
-    const uint32_t ss = umma::su32(smem + L::s);
+    // every descriptor is one of these plus a constant: built anew for each product, they held the issue up
+    const uint32_t dq = desc_low(smem + L::q), dw = desc_low(smem + L::w), dp = desc_low(smem + L::p), ds = desc_low(smem + L::s);
+    const uint32_t dk0 = desc_low(smem + L::k), dv0 = desc_low(smem + L::v);
     constexpr uint32_t kIdP = umma::idesc_bf16(kT, kT, 0, 0);
     constexpr uint32_t kIdR = umma::idesc_bf16(kT, kC, 0, 1);
     constexpr uint32_t kIdS = umma::idesc_bf16(DK, kC, 1, 1);
     for (int i = 0; i < chunks; ++i) {
-      const int buf = i & 1;
-      const uint32_t sk = umma::su32(smem + L::k + buf * L::qk), sv = umma::su32(smem + L::v + buf * kTile);
+      const int buf = i & 1, wb = i % L::wbuf;
+      const uint32_t dk = dk0 + buf * (L::qk >> 4), dv = dv0 + buf * kNextTile;
       wait(kFull + buf, i >> 1);
       if (OUT) {
-        wait(kFullQ, i);
+        const uint32_t dqi = dq + i % L::qbuf * (L::qk >> 4);
+        wait(kFullQ + i % L::qbuf, i / L::qbuf);
         if (elect()) {
 #pragma unroll
           for (int x = 0; x < DK / 16; ++x)
-            umma::mma(tmem + kColP, tile_desc(sq + (x >> 2) * kTile + (x & 3) * 32),
-                      tile_desc(sk + (x >> 2) * kTile + (x & 3) * 32), kIdP, x > 0);
+            mma(tmem + kColP, dqi + (x >> 2) * kNextTile + (x & 3) * kAlongK, dk + (x >> 2) * kNextTile + (x & 3) * kAlongK, kIdP,
+                x > 0);
           umma::commit(&bar[kDoneP]);
         }
         __syncwarp();
       }
-      const int wb = i % L::wbuf;
       wait(kHaveS + wb, i / L::wbuf);
       wait(kHaveV + wb, i / L::wbuf);
       if (elect()) {
@@ -339,42 +387,106 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A, co
         for (int y = 0; y < TERMS; ++y)
 #pragma unroll
           for (int x = 0; x < kT / 16; ++x)
-            umma::mma(tmem + kColS - 64 * wb, tile_desc(sk + x * 2048), tile_desc(sw + (wb * TERMS + y) * kTile + x * 2048), kIdS,
-                      x + y > 0);
+            mma(tmem + kColS - 64 * wb, dk + x * kAlongRows, dw + (wb * TERMS + y) * kNextTile + x * kAlongRows, kIdS, x + y > 0);
         umma::commit(&bar[kDoneS + wb]);
         if (!OUT) umma::commit(&bar[kEmpty + buf]);
       }
       __syncwarp();
       if (OUT) {
+        const uint32_t dqi = dq + i % L::qbuf * (L::qk >> 4);
         if (i) wait(kReadO, i - 1);
         if (elect()) {
 #pragma unroll
           for (int x = 0; x < DK / 16; ++x)
-            umma::mma(tmem + kColR, tile_desc(sq + (x >> 2) * kTile + (x & 3) * 32), tile_desc(ss + x * 2048), kIdR, x > 0);
+            mma(tmem + kColR, dqi + (x >> 2) * kNextTile + (x & 3) * kAlongK, ds + x * kAlongRows, kIdR, x > 0);
           umma::commit(&bar[kDoneR]);
+          umma::commit(&bar[kEmptyQ + i % L::qbuf]);
         }
         __syncwarp();
         wait(kHaveP, i);
         if (elect()) {
 #pragma unroll
-          for (int x = 0; x < kT / 16; ++x)
-            umma::mma(tmem + kColO, tile_desc(sp + x * 32), tile_desc(sv + x * 2048), kIdR, x > 0);
+          for (int x = 0; x < kT / 16; ++x) mma(tmem + kColO, dp + x * kAlongK, dv + x * kAlongRows, kIdR, x > 0);
           umma::commit(&bar[kDoneO]);
           umma::commit(&bar[kEmpty + buf]);
         }
         __syncwarp();
       }
     }
+  } else if (warp >= kWriter) {
+    if (Regs<DK>::write > 64)
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Regs<DK>::write));
+    else
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Regs<DK>::write));
+    fill_table(2 * kT + 1);
+    if (OUT) {
+      const int wq = warp & 3, row = wq * 16 + (lane >> 2), quad = lane & 3;
+      const uint32_t lanes = tmem + ((uint32_t)(wq * 32) << 16);
+      TO* op = static_cast<TO*>(A.o) + b * A.ob + (long long)h * A.oh + c0;
+      for (int i = 0; i < chunks; ++i) {
+        const int n = tokens(i);
+        wait(kDoneO, i);
+        const float os = ok ? A.vscale * A.oscale : __int_as_float(0x7fffffff);
+#pragma unroll
+        for (int half = 0; half < kC; half += 32) {
+          uint32_t r[16], o[16];
+          tmem_ld2(lanes + kColR + half, lanes + kColO + half, r, o);
+          if (half) {  // all of it has been read
+            umma::fence_before_sync();
+            __syncwarp();
+            if (lane == 0) arrive(&bar[kReadO]);
+          }
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            const int rw = row + 8 * y;
+            const float rs = tab[kT + (rev ? n - 1 - rw : rw + 1)] * A.oscale;
+            TO* d = op + (first(i) + rw) * A.ol + half;
+            float2 f[4];  // columns half + 8 j + 2 quad, + 1
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int at = 4 * j + 2 * y;
+              f[j] = make_float2(fmaf(__uint_as_float(r[at]), rs, __uint_as_float(o[at]) * os),
+                                 fmaf(__uint_as_float(r[at + 1]), rs, __uint_as_float(o[at + 1]) * os));
+            }
+            if (sizeof(TO) == 2 && A.ovec) {
+              // transposed among four lanes: each stores 16 bytes of the row, together 64
+              uint4 u = make_uint4(pack2(f[0].x, f[0].y), pack2(f[1].x, f[1].y), pack2(f[2].x, f[2].y), pack2(f[3].x, f[3].y));
+              swap_pairs(u.x, u.y, 1, quad);
+              swap_pairs(u.z, u.w, 1, quad);
+              swap_pairs(u.x, u.z, 2, quad);
+              swap_pairs(u.y, u.w, 2, quad);
+              if (rw < n && c0 + half + 8 * quad < A.DV) *reinterpret_cast<uint4*>(d + 8 * quad) = u;
+            } else if (rw < n) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const int c = 8 * j + 2 * quad, left = A.DV - c0 - half - c;
+                if (sizeof(TO) == 4 && A.ovec && left > 0) {
+                  *reinterpret_cast<float2*>(d + c) = f[j];
+                } else {
+                  if (left > 0) DT<TO>::store(d + c, f[j].x);
+                  if (left > 1) DT<TO>::store(d + c + 1, f[j].y);
+                }
+              }
+            }
+          }
+        }
+      }
+      const long long z0 = max(t_lo, t_hi);  // tokens past the length: zeros
+      for (long long i = tid - 32 * kWriter; i < (t_end - z0) * kC; i += 32 * kWriters) {
+        const long long r = i / kC;
+        const int c = (int)(i - r * kC);
+        if (c0 + c < A.DV) DT<TO>::store(op + (z0 + r) * A.ol + c, 0.f);
+      }
+    }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Regs<DK>::compute));
     // This thread's part of a 64 x 64 product: rows row and row + 8, columns half + 8 j + pair + {0, 1}, j < 4. Of a
     // state of 128 rows it has two such parts, 16 TMEM lanes apart (SB).
     constexpr int SB = DK / 64;
-    const float g = A.log_decay[h];
     const auto power = [&](int n) {  // a^n as the sum of two floats
       const double an = exp((double)g * n);
       return make_float2((float)an, (float)(an - (double)(float)an));
     };
-    if (tid <= 2 * kT) tab[tid] = tid < kT ? 0.f : tid == kT ? 1.f : expf(g * (tid - kT));
     const float2 a64 = power(kT);
     const int wq = warp & 3, half = (warp >> 2) * 32;
     const int row = wq * 16 + (lane >> 2), pair = 2 * (lane & 3);
@@ -418,9 +530,10 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A, co
     }
     // The V of chunk i, decayed, in TERMS terms.
     const auto split_v = [&](int i) {
-      unsigned char* terms = smem + L::w + i % L::wbuf * (TERMS * kTile);
-      const int n = tokens(i);
+      const int wb = i % L::wbuf, n = tokens(i);
       const unsigned char* v = smem + L::v + (i & 1) * kTile;
+      unsigned char* terms = smem + L::w + wb * (TERMS * kTile);
+      wait(kFull + (i & 1), i >> 1);
 #pragma unroll
       for (int x = 0; x < kT * kC / 8 / kThreads; ++x) {
         const int at = tid + x * kThreads, t = at >> 3;  // V's place in the tile is its terms' place
@@ -444,14 +557,9 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A, co
         *reinterpret_cast<uint4*>(terms + kTile + at * 16) = mid;
         if (TERMS == 3) *reinterpret_cast<uint4*>(terms + 2 * kTile + at * 16) = lo;
       }
-      hand_over(&bar[kHaveV + i % L::wbuf]);
+      hand_over(&bar[kHaveV + wb]);
     };
-    TO* op = static_cast<TO*>(A.o) + (OUT ? b * A.ob + (long long)h * A.oh + c0 + half + pair : 0);
-    asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory");  // the table
-    if (chunks) {
-      wait(kFull, 0);
-      split_v(0);
-    }
+    fill_table(tid);
     // a^|row - column| of this thread's part of P, zero where the column is later in scan order: entries 2 m, 2 m + 1 for
     // columns 8 (m - 1), + 1 of its first row. In registers where there is room.
     const float* tb = tab + kT + (rev ? half + pair - 8 - row : row - half - pair + 8);
@@ -461,8 +569,10 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A, co
 #pragma unroll
       for (int m = 0; m < (SB == 1 ? 10 : 1); ++m) dec[m] = tb[along * (8 * (m / 2) + (m & 1))];
     const auto decay = [&](int m) { return SB == 1 ? dec[SB == 1 ? m : 0] : tb[along * (8 * (m / 2) + (m & 1))]; };
+    if (chunks) split_v(0);
     for (int i = 0; i < chunks; ++i) {
       const int n = tokens(i);
+      if (!OUT && i + 1 < chunks) split_v(i + 1);  // both buffers are in use: beside the last chunk's product
       if (OUT) {  // P
         wait(kDoneP, i);
         uint32_t p[16];
@@ -477,13 +587,6 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A, co
         }
         hand_over(&bar[kHaveP]);
       }
-      const auto next_v = [&] {
-        if (i + 1 < chunks) {
-          wait(kFull + ((i + 1) & 1), (i + 1) >> 1);
-          split_v(i + 1);
-        }
-      };
-      if (!OUT) next_v();  // both buffers are in use: the split runs beside the last chunk's product
       {  // the state
         const float2 an = n == kT ? a64 : power(n);
         if (OUT) wait(kDoneR, i);
@@ -498,62 +601,7 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A, co
         if (OUT) put_state();
         hand_over(&bar[kHaveS + i % L::wbuf]);
       }
-      if (OUT) next_v();
-      if (OUT) {  // the outputs
-        wait(kDoneO, i);
-        uint32_t r[16], o[16];
-        tmem_ld2(lanes + kColR, lanes + kColO, r, o);
-        umma::fence_before_sync();
-        __syncwarp();
-        if (lane == 0) arrive(&bar[kReadO]);
-        const float os = ok ? A.vscale * A.oscale : __int_as_float(0x7fffffff);
-        // 16-bit outputs go through this warp's own part of P (P V is done with it): 64 bytes of a row by four lanes
-        constexpr bool kStage = sizeof(TO) == 2;
-        const bool stage = kStage && A.ovec;
-#pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          const int rw = row + 8 * y;
-          const float rs = tab[kT + (rev ? n - 1 - rw : rw + 1)] * A.oscale;
-          TO* d = op + (first(i) + rw) * A.ol;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int at = 4 * j + 2 * y;
-            const float x0 = fmaf(__uint_as_float(r[at]), rs, __uint_as_float(o[at]) * os);
-            const float x1 = fmaf(__uint_as_float(r[at + 1]), rs, __uint_as_float(o[at + 1]) * os);
-            if (stage) {
-              *reinterpret_cast<uint32_t*>(smem + L::p + swz(rw, half + 8 * j + pair)) = pack2(x0, x1);
-            } else if (rw < n) {
-              if (!kStage && A.ovec && 8 * j < left) {
-                *reinterpret_cast<float2*>(d + 8 * j) = make_float2(x0, x1);
-              } else {
-                if (8 * j < left) DT<TO>::store(d + 8 * j, x0);
-                if (8 * j + 1 < left) DT<TO>::store(d + 8 * j + 1, x1);
-              }
-            }
-          }
-        }
-        if (stage) {
-          __syncwarp();
-          const int c = half + 8 * (lane & 3);
-#pragma unroll
-          for (int y = 0; y < 2; ++y) {
-            const int rw = row + 8 * y;
-            const uint4 u = *reinterpret_cast<const uint4*>(smem + L::p + swz(rw, c));
-            if (rw < n && c0 + c < A.DV)
-              *reinterpret_cast<uint4*>(op - half - pair + (first(i) + rw) * A.ol + c) = u;
-          }
-          __syncwarp();
-        }
-      }
-    }
-    if (OUT) {  // tokens past the length: zeros
-      const long long z0 = max(t_lo, t_hi);
-      TO* z = static_cast<TO*>(A.o) + b * A.ob + (long long)h * A.oh + c0;
-      for (long long i = tid; i < (t_end - z0) * kC; i += kThreads) {
-        const long long r = i / kC;
-        const int c = (int)(i - r * kC);
-        if (c0 + c < A.DV) DT<TO>::store(z + (z0 + r) * A.ol + c, 0.f);
-      }
+      if (OUT && i + 1 < chunks) split_v(i + 1);
     }
     float* dst = nullptr;
     long long sr = A.DV, sc = 1;
