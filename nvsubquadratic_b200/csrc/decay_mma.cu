@@ -53,31 +53,31 @@ constexpr int kThreads = 256;  // computing
 constexpr int kLoader = kThreads / 32, kIssuer = kLoader + 3;  // first loading warp, issuing warp
 constexpr int kWriter = kIssuer + 1, kWriters = 4;
 constexpr int kAll = 32 * (kWriter + kWriters);
-// Registers of a thread: computing, loading and issuing, writing; together those of the launch (64 for each of 512).
-template <int DK>
+// Registers of a thread: computing, loading and issuing, writing; together those of the launch (64 for each of 512). Chosen
+// so that nothing spills: with the shared memory that is taken here a spilled register comes back from L2.
+template <int DK, bool OUT>
 struct Regs {
-  static constexpr int compute = DK == 64 ? 72 : 88, load = DK == 64 ? 40 : 32, write = DK == 64 ? 72 : 48;
+  static constexpr int compute = DK == 64 && OUT ? 72 : 80, load = DK == 64 && OUT ? 56 : 48, write = load;
   static_assert(kThreads * compute + 128 * load + 128 * write <= 64 * kAll, "setmaxnreg would wait forever");
 };
 constexpr int kColP = 0, kColR = 64, kColO = 128, kColS = 192, kTmemCols = 256;  // kColS - 64: a second one without outputs
 
-// What each mbarrier says: full and empty for the loads, done by the tensor core, the others by the warps.
+// What each mbarrier says: full for the loads, done by the tensor core, the others by the warps. One commit tells all that
+// wait for a product, the loading warps too: a second commit behind it held the issuing warp for a thousand cycles.
 // A barrier with two phases behind its waiter cannot be told from one with none: where a waiter may fall behind (two
-// buffers in use), each buffer has its own.
+// buffers in use), each buffer, or each of two successive chunks, has its own.
 enum Bar {
-  kFull = 0,     // K and V of buffer 0, 1 are in place
-  kFullQ = 2,    // Q of buffer 0, 1
-  kEmpty = 4,    // products have read K and V of buffer 0, 1
-  kEmptyQ = 6,   // and Q of buffer 0, 1
-  kDoneR = 8,    // R is there, the rounded state has been read
-  kDoneP = 9,
-  kDoneO = 10,
-  kDoneS = 11,   // K^T V is there, of buffer 0, 1
-  kHaveV = 13,   // the decayed V is in place, of buffer 0, 1
-  kHaveS = 15,   // the rounded state is in place, the accumulator of buffer 0, 1 free
-  kHaveP = 17,   // P is in place (and its accumulator free)
-  kReadO = 18,   // R and P V have been read, by the writing warps
-  kBars = 19
+  kFull = 0,    // K and V of buffer 0, 1 are in place
+  kFullQ = 2,   // Q of buffer 0, 1
+  kDoneR = 4,   // R is there, Q and the rounded state have been read; even chunks, odd chunks
+  kDoneO = 6,   // P V is there, K and V have been read; even, odd
+  kDoneS = 8,   // K^T V is there (without outputs: K and V have been read); buffer 0, 1
+  kDoneP = 10,
+  kHaveV = 11,  // the decayed V is in place, of buffer 0, 1
+  kHaveS = 13,  // the rounded state is in place, the accumulator of buffer 0, 1 free
+  kHaveP = 15,  // P is in place (and its accumulator free)
+  kReadO = 16,  // R and P V have been read, by the writing warps
+  kBars = 17
 };
 
 // Bytes of the shared-memory layout for a state of DK (64 or 128) rows whose update takes TERMS bfloat16 terms. Tiles
@@ -312,7 +312,7 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A, co
     asm volatile("bar.sync 1, %0;" ::"n"(kThreads + 32 * kWriters) : "memory");
   };
   if (warp >= kLoader && warp < kWriter) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Regs<DK>::load));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Regs<DK, OUT>::load));
   }
   if (warp >= kLoader && warp < kIssuer) {
     const int who = warp - kLoader;
@@ -322,7 +322,7 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A, co
       const bf16* vp = static_cast<const bf16*>(A.v.p) + b * A.v.sb + hv * A.v.sh;
       unsigned char *kd = smem + L::k + who * L::qk, *vd = smem + L::v + who * kTile;
       for (int i = who, use = 0; i < chunks; i += 2, ++use) {
-        if (use) wait(kEmpty + who, use - 1);
+        if (use) wait((OUT ? kDoneO : kDoneS) + who, use - 1);
         if (M.on && tokens(i) == kT) {
           if (lane == 0) {
             expect(&bar[kFull + who], L::qk + kTile);
@@ -343,7 +343,7 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A, co
       for (int i = 0; i < chunks; ++i) {
         const int qb = i % L::qbuf;
         unsigned char* qd = smem + L::q + qb * L::qk;
-        if (i >= L::qbuf) wait(kEmptyQ + qb, i / L::qbuf - 1);
+        if (i >= L::qbuf) wait(kDoneR + ((i - L::qbuf) & 1), (i - L::qbuf) >> 1);
         if (M.on && tokens(i) == kT) {
           if (lane == 0) {
             expect(&bar[kFullQ + qb], L::qk);
@@ -389,7 +389,6 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A, co
           for (int x = 0; x < kT / 16; ++x)
             mma(tmem + kColS - 64 * wb, dk + x * kAlongRows, dw + (wb * TERMS + y) * kNextTile + x * kAlongRows, kIdS, x + y > 0);
         umma::commit(&bar[kDoneS + wb]);
-        if (!OUT) umma::commit(&bar[kEmpty + buf]);
       }
       __syncwarp();
       if (OUT) {
@@ -399,25 +398,20 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A, co
 #pragma unroll
           for (int x = 0; x < DK / 16; ++x)
             mma(tmem + kColR, dqi + (x >> 2) * kNextTile + (x & 3) * kAlongK, ds + x * kAlongRows, kIdR, x > 0);
-          umma::commit(&bar[kDoneR]);
-          umma::commit(&bar[kEmptyQ + i % L::qbuf]);
+          umma::commit(&bar[kDoneR + buf]);
         }
         __syncwarp();
         wait(kHaveP, i);
         if (elect()) {
 #pragma unroll
           for (int x = 0; x < kT / 16; ++x) mma(tmem + kColO, dp + x * kAlongK, dv + x * kAlongRows, kIdR, x > 0);
-          umma::commit(&bar[kDoneO]);
-          umma::commit(&bar[kEmpty + buf]);
+          umma::commit(&bar[kDoneO + buf]);
         }
         __syncwarp();
       }
     }
   } else if (warp >= kWriter) {
-    if (Regs<DK>::write > 64)
-      asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Regs<DK>::write));
-    else
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Regs<DK>::write));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Regs<DK, OUT>::write));
     fill_table(2 * kT + 1);
     if (OUT) {
       const int wq = warp & 3, row = wq * 16 + (lane >> 2), quad = lane & 3;
@@ -425,7 +419,7 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A, co
       TO* op = static_cast<TO*>(A.o) + b * A.ob + (long long)h * A.oh + c0;
       for (int i = 0; i < chunks; ++i) {
         const int n = tokens(i);
-        wait(kDoneO, i);
+        wait(kDoneO + (i & 1), i >> 1);
         const float os = ok ? A.vscale * A.oscale : __int_as_float(0x7fffffff);
 #pragma unroll
         for (int half = 0; half < kC; half += 32) {
@@ -479,7 +473,7 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A, co
       }
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Regs<DK>::compute));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Regs<DK, OUT>::compute));
     // This thread's part of a 64 x 64 product: rows row and row + 8, columns half + 8 j + pair + {0, 1}, j < 4. Of a
     // state of 128 rows it has two such parts, 16 TMEM lanes apart (SB).
     constexpr int SB = DK / 64;
@@ -589,7 +583,7 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A, co
       }
       {  // the state
         const float2 an = n == kT ? a64 : power(n);
-        if (OUT) wait(kDoneR, i);
+        if (OUT) wait(kDoneR + (i & 1), i >> 1);
         wait(kDoneS + i % L::wbuf, i / L::wbuf);
 #pragma unroll
         for (int y = 0; y < SB; ++y) {
