@@ -13,7 +13,7 @@
 // owns four columns of the state and up to 32 of its rows in registers, packed in pairs of rows: a token costs two packed
 // multiply-adds per pair (S += k v, o += q S). q and k are read from shared memory as broadcasts, which the register
 // file takes at 128 bytes a cycle: one 16-byte read serves 16 multiply-adds here (with one column per thread it served four
-// and the reads were the bound: 2.08 ms for 16 x 4096 tokens, 12 heads of 64, float16, instead of @SCAN@). The two halves of a
+// and the reads were the bound: 2.08 ms for 16 x 4096 tokens, 12 heads of 64, float16, instead of 1.00). The two halves of a
 // warp hold two parts of the rows, their sums meet in one shuffle; states of more than 64 rows take more warps.
 // Inside a chunk of 16 tokens the state is kept divided by a^i, which takes the decay out of the inner loop: v is
 // multiplied by a^-i and o by a^i, each from a table, and the chunk's a^n is applied once, as the sum of two floats

@@ -21,7 +21,10 @@
 // Sixteen warps: three load (TMA; the last, partial chunk and tensors that TMA cannot take by cp.async, with zeros past a
 // length or a head size; two take turns with K and V, one brings Q), one issues the products, eight compute: they decay P,
 // update the state and split the next chunk's V; four write the outputs. Only mbarriers order them. The computing warps' chain
-// of TMEM reads, shared-memory writes and barriers sets the pace, so what need not be in it is not: @WRITERS@.
+// of TMEM reads, shared-memory writes and barriers sets the pace, so what need not be in it is not (a pass with outputs
+// over the 128 x 128 grid, 32 rows of 16384 tokens of 64: 134 us with eight warps doing everything, 69 with loads and products
+// issued by others, 58 with the outputs written by others too, Q in several buffers and no register spilled; its traffic
+// at the copy's rate takes 41).
 // Registers move from the loading to the computing warps. Two CTAs share an SM (<= 113 KB, 256 TMEM columns each).
 //
 // 64-row products lie in 16 of a warp's 32 TMEM lanes, and
@@ -64,20 +67,20 @@ constexpr int kColP = 0, kColR = 64, kColO = 128, kColS = 192, kTmemCols = 256; 
 
 // What each mbarrier says: full for the loads, done by the tensor core, the others by the warps. One commit tells all that
 // wait for a product, the loading warps too: a second commit behind it held the issuing warp for a thousand cycles.
-// A barrier with two phases behind its waiter cannot be told from one with none: where a waiter may fall behind (two
-// buffers in use), each buffer, or each of two successive chunks, has its own.
+// A barrier with two phases behind its waiter cannot be told from one with none: where a waiter may fall behind (several
+// buffers in use), each buffer has its own.
 enum Bar {
-  kFull = 0,    // K and V of buffer 0, 1 are in place
-  kFullQ = 2,   // Q of buffer 0, 1
-  kDoneR = 4,   // R is there, Q and the rounded state have been read; even chunks, odd chunks
-  kDoneO = 6,   // P V is there, K and V have been read; even, odd
-  kDoneS = 8,   // K^T V is there (without outputs: K and V have been read); buffer 0, 1
-  kDoneP = 10,
-  kHaveV = 11,  // the decayed V is in place, of buffer 0, 1
-  kHaveS = 13,  // the rounded state is in place, the accumulator of buffer 0, 1 free
-  kHaveP = 15,  // P is in place (and its accumulator free)
-  kReadO = 16,  // R and P V have been read, by the writing warps
-  kBars = 17
+  kFull = 0,     // K and V of a buffer are in place
+  kFullQ = 4,    // Q of a buffer
+  kDoneR = 7,    // R is there, Q (of a buffer) and the rounded state have been read
+  kDoneO = 10,   // P V is there, K and V of a buffer have been read
+  kDoneS = 14,   // K^T V is there (without outputs: K and V of a buffer have been read)
+  kDoneP = 18,
+  kHaveV = 19,   // the decayed V is in place, of buffer 0, 1
+  kHaveS = 21,   // the rounded state is in place, the accumulator of buffer 0, 1 free
+  kHaveP = 23,   // P is in place (and its accumulator free)
+  kReadO = 24,   // R and P V have been read, by the writing warps
+  kBars = 25
 };
 
 // Bytes of the shared-memory layout for a state of DK (64 or 128) rows whose update takes TERMS bfloat16 terms. Tiles
@@ -86,12 +89,14 @@ constexpr int kTile = kT * 128;
 template <int DK, bool OUT, int TERMS>
 struct Layout {
   static constexpr int qk = DK / 64 * kTile;
+  // as many buffers of K and V, of Q and of the decayed V as two CTAs on an SM leave room for
+  static constexpr int nbuf = OUT ? (DK == 64 ? 3 : 2) : (DK == 64 ? 4 : 2);
+  static constexpr int qbuf = DK == 64 ? 3 : 1;
+  static constexpr int wbuf = OUT ? 1 : DK == 64 ? 2 : 2;
   static constexpr int q = 0;
-  static constexpr int qbuf = DK == 64 ? 2 : 1;  // as many as two CTAs on an SM leave room for
   static constexpr int k = q + (OUT ? qbuf * qk : 0);
-  static constexpr int v = k + 2 * qk;
-  static constexpr int wbuf = OUT ? 1 : 2;
-  static constexpr int w = v + 2 * kTile;               // the decayed V
+  static constexpr int v = k + nbuf * qk;
+  static constexpr int w = v + nbuf * kTile;            // the decayed V
   static constexpr int p = w + wbuf * TERMS * kTile;    // P
   static constexpr int s = p + (OUT ? kTile : 0);       // the rounded state
   static constexpr int tab = s + (OUT ? DK * 128 : 0);  // a^d for d = -64 .. 64 (zeros below 0)
@@ -320,21 +325,22 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A, co
       const int hk = h / A.k.group, hv = h / A.v.group;
       const bf16* kp = static_cast<const bf16*>(A.k.p) + b * A.k.sb + hk * A.k.sh;
       const bf16* vp = static_cast<const bf16*>(A.v.p) + b * A.v.sb + hv * A.v.sh;
-      unsigned char *kd = smem + L::k + who * L::qk, *vd = smem + L::v + who * kTile;
-      for (int i = who, use = 0; i < chunks; i += 2, ++use) {
-        if (use) wait((OUT ? kDoneO : kDoneS) + who, use - 1);
+      for (int i = who; i < chunks; i += 2) {
+        const int nb = i % L::nbuf;
+        unsigned char *kd = smem + L::k + nb * L::qk, *vd = smem + L::v + nb * kTile;
+        if (i >= L::nbuf) wait((OUT ? kDoneO : kDoneS) + nb, i / L::nbuf - 1);
         if (M.on && tokens(i) == kT) {
           if (lane == 0) {
-            expect(&bar[kFull + who], L::qk + kTile);
-            load_box<DK>(umma::su32(kd), &M.k, &bar[kFull + who], 0, hk, (int)first(i), (int)b);
-            load_box<kC>(umma::su32(vd), &M.v, &bar[kFull + who], c0, hv, (int)first(i), (int)b);
+            expect(&bar[kFull + nb], L::qk + kTile);
+            load_box<DK>(umma::su32(kd), &M.k, &bar[kFull + nb], 0, hk, (int)first(i), (int)b);
+            load_box<kC>(umma::su32(vd), &M.v, &bar[kFull + nb], c0, hv, (int)first(i), (int)b);
           }
           __syncwarp();
         } else {
           load_tile<DK>(kd, kp, A.k.sl, tokens(i), 0, A.DK, first(i), A.vec);
           load_tile<kC>(vd, vp, A.v.sl, tokens(i), c0, A.DV, first(i), A.vec);
           cp_wait();
-          hand_over(&bar[kFull + who]);
+          hand_over(&bar[kFull + nb]);
         }
       }
     } else if (OUT) {
@@ -343,7 +349,7 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A, co
       for (int i = 0; i < chunks; ++i) {
         const int qb = i % L::qbuf;
         unsigned char* qd = smem + L::q + qb * L::qk;
-        if (i >= L::qbuf) wait(kDoneR + ((i - L::qbuf) & 1), (i - L::qbuf) >> 1);
+        if (i >= L::qbuf) wait(kDoneR + qb, i / L::qbuf - 1);
         if (M.on && tokens(i) == kT) {
           if (lane == 0) {
             expect(&bar[kFullQ + qb], L::qk);
@@ -365,9 +371,9 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A, co
     constexpr uint32_t kIdR = umma::idesc_bf16(kT, kC, 0, 1);
     constexpr uint32_t kIdS = umma::idesc_bf16(DK, kC, 1, 1);
     for (int i = 0; i < chunks; ++i) {
-      const int buf = i & 1, wb = i % L::wbuf;
-      const uint32_t dk = dk0 + buf * (L::qk >> 4), dv = dv0 + buf * kNextTile;
-      wait(kFull + buf, i >> 1);
+      const int nb = i % L::nbuf, wb = i % L::wbuf;
+      const uint32_t dk = dk0 + nb * (L::qk >> 4), dv = dv0 + nb * kNextTile;
+      wait(kFull + nb, i / L::nbuf);
       if (OUT) {
         const uint32_t dqi = dq + i % L::qbuf * (L::qk >> 4);
         wait(kFullQ + i % L::qbuf, i / L::qbuf);
@@ -388,7 +394,7 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A, co
 #pragma unroll
           for (int x = 0; x < kT / 16; ++x)
             mma(tmem + kColS - 64 * wb, dk + x * kAlongRows, dw + (wb * TERMS + y) * kNextTile + x * kAlongRows, kIdS, x + y > 0);
-        umma::commit(&bar[kDoneS + wb]);
+        umma::commit(&bar[kDoneS + (OUT ? 0 : nb)]);
       }
       __syncwarp();
       if (OUT) {
@@ -398,14 +404,14 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A, co
 #pragma unroll
           for (int x = 0; x < DK / 16; ++x)
             mma(tmem + kColR, dqi + (x >> 2) * kNextTile + (x & 3) * kAlongK, ds + x * kAlongRows, kIdR, x > 0);
-          umma::commit(&bar[kDoneR + buf]);
+          umma::commit(&bar[kDoneR + i % L::qbuf]);
         }
         __syncwarp();
         wait(kHaveP, i);
         if (elect()) {
 #pragma unroll
           for (int x = 0; x < kT / 16; ++x) mma(tmem + kColO, dp + x * kAlongK, dv + x * kAlongRows, kIdR, x > 0);
-          umma::commit(&bar[kDoneO + buf]);
+          umma::commit(&bar[kDoneO + nb]);
         }
         __syncwarp();
       }
@@ -419,7 +425,7 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A, co
       TO* op = static_cast<TO*>(A.o) + b * A.ob + (long long)h * A.oh + c0;
       for (int i = 0; i < chunks; ++i) {
         const int n = tokens(i);
-        wait(kDoneO + (i & 1), i >> 1);
+        wait(kDoneO + i % L::nbuf, i / L::nbuf);
         const float os = ok ? A.vscale * A.oscale : __int_as_float(0x7fffffff);
 #pragma unroll
         for (int half = 0; half < kC; half += 32) {
@@ -525,9 +531,9 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A, co
     // The V of chunk i, decayed, in TERMS terms.
     const auto split_v = [&](int i) {
       const int wb = i % L::wbuf, n = tokens(i);
-      const unsigned char* v = smem + L::v + (i & 1) * kTile;
+      const unsigned char* v = smem + L::v + i % L::nbuf * kTile;
       unsigned char* terms = smem + L::w + wb * (TERMS * kTile);
-      wait(kFull + (i & 1), i >> 1);
+      wait(kFull + i % L::nbuf, i / L::nbuf);
 #pragma unroll
       for (int x = 0; x < kT * kC / 8 / kThreads; ++x) {
         const int at = tid + x * kThreads, t = at >> 3;  // V's place in the tile is its terms' place
@@ -566,7 +572,7 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A, co
     if (chunks) split_v(0);
     for (int i = 0; i < chunks; ++i) {
       const int n = tokens(i);
-      if (!OUT && i + 1 < chunks) split_v(i + 1);  // both buffers are in use: beside the last chunk's product
+      if (L::wbuf == 2 && i + 1 < chunks) split_v(i + 1);  // both buffers are in use: beside the last chunk's product
       if (OUT) {  // P
         wait(kDoneP, i);
         uint32_t p[16];
@@ -583,8 +589,8 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A, co
       }
       {  // the state
         const float2 an = n == kT ? a64 : power(n);
-        if (OUT) wait(kDoneR + (i & 1), i >> 1);
-        wait(kDoneS + i % L::wbuf, i / L::wbuf);
+        if (OUT) wait(kDoneR + i % L::qbuf, i / L::qbuf);
+        wait(kDoneS + (OUT ? 0 : i % L::nbuf), OUT ? i : i / L::nbuf);
 #pragma unroll
         for (int y = 0; y < SB; ++y) {
           uint32_t d[16];
@@ -595,7 +601,7 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A, co
         if (OUT) put_state();
         hand_over(&bar[kHaveS + i % L::wbuf]);
       }
-      if (OUT && i + 1 < chunks) split_v(i + 1);
+      if (L::wbuf == 1 && i + 1 < chunks) split_v(i + 1);
     }
     float* dst = nullptr;
     long long sr = A.DV, sc = 1;
