@@ -312,8 +312,9 @@ typedef struct hyfft_decay_desc {
 } hyfft_decay_desc;
 
 HYFFT_API int hyfft_decay_workspace_size(const hyfft_decay_desc* d, size_t* fwd_bytes, size_t* bwd_bytes);
-/* final_state: the state after each sequence's last token, or NULL to skip it. What the forward leaves in its workspace
- * can be given to the backward of the same call as `saved` (fwd_bytes of it). */
+HYFFT_API int hyfft_decay_saved_size(const hyfft_decay_desc* d, size_t* saved_bytes);
+/* final_state: the state after each sequence's last token, or NULL to skip it. The first
+ * saved_bytes that the forward leaves in its workspace can be given to the backward of the same call as `saved`. */
 HYFFT_API int hyfft_decay_forward(const hyfft_decay_desc* d, const void* q, const void* k, const void* v,
                                   const float* log_decay, const int32_t* lengths, const float* initial_state,
                                   void* o, float* final_state, void* workspace, size_t workspace_bytes,
@@ -321,7 +322,7 @@ HYFFT_API int hyfft_decay_forward(const hyfft_decay_desc* d, const void* q, cons
 /* Gradients for dout [B, L, H, Dv] and dfinal_state (NULL: zero). dq, dk, dv have q's, k's and v's shapes
  * (dk and dv of a shared head are summed over its query heads in a fixed order); dlog_decay float32 [H];
  * dinitial_state [B, H, Dk, Dv]. Any of them may be NULL to skip it, dv only together with
- * dinitial_state. saved: the forward's workspace, or NULL to compute its contents again.         */
+ * dinitial_state. saved: what the forward left, or NULL to compute it again.                      */
 HYFFT_API int hyfft_decay_backward(const hyfft_decay_desc* d, const void* q, const void* k, const void* v,
                                    const float* log_decay, const int32_t* lengths, const float* initial_state,
                                    const void* saved, const void* dout, const float* dfinal_state, void* dq, void* dk, void* dv,

@@ -145,6 +145,7 @@ SIGNATURES = {
     "hyfft_siren_forward": [ctypes.POINTER(SirenDesc)] + [_vp] * 10 + [_sz, _vp],
     "hyfft_siren_backward": [ctypes.POINTER(SirenDesc)] + [_vp] * 16 + [_sz, _vp],
     "hyfft_decay_workspace_size": [ctypes.POINTER(DecayDesc), ctypes.POINTER(_sz), ctypes.POINTER(_sz)],
+    "hyfft_decay_saved_size": [ctypes.POINTER(DecayDesc), ctypes.POINTER(_sz)],
     "hyfft_decay_forward": [ctypes.POINTER(DecayDesc)] + [_vp] * 9 + [_sz, _vp],
     "hyfft_decay_backward": [ctypes.POINTER(DecayDesc)] + [_vp] * 15 + [_sz, _vp],
     "hyfft_decay_step": [ctypes.POINTER(DecayDesc)] + [_vp] * 5 + [_i64] + [_vp] * 4,

@@ -19,7 +19,7 @@
 // multiplied by a^-i and o by a^i, each from a table, and the chunk's a^n is applied once, as the sum of two floats
 // (a rounded a^n would be off by its rounding error times the number of chunks in a head's memory). Heads that
 // forget more than e^-46 within a chunk, where a^-i would overflow, multiply the state for each token.
-// bfloat16 states of up to 128 rows go to the tensor cores instead (decay_mma.cu).
+// What of this runs on the tensor cores instead (decay_mma.cu) says use_mma below.
 // Few rows and a long axis: the axis is cut into segments; a first pass adds up each segment from a zero
 // state, a small kernel chains the segments' states, and the second pass starts every segment from its own.
 #include <cuda_bf16.h>
@@ -531,8 +531,17 @@ void scan_shape(int DK, int* rh, int* kw) {
   *rh = DK <= 16 ? 8 : 16;
 }
 
-// The tensor cores take every bfloat16 scan whose state has up to 128 rows.
-bool use_mma(const hyfft_decay_desc* d, int DK) { return d->dtype == HYFFT_BF16 && DK <= kMmaMaxDK; }
+// The tensor cores take every bfloat16 scan whose state has up to 128 rows, and float16 and float32 ones (as sums of
+// bfloat16 terms) from half a chunk of tokens on: below, the scan's time is latency either way and laying out the terms is one
+// launch more (12 heads of 64, float32, multiply-adds: 11 us for 16 tokens, 27 for 64; tensor cores: 10 for 64). All
+// scans of a call go one way.
+bool use_mma(const hyfft_decay_desc* d, int DK) {
+  if (d->dtype == HYFFT_BF16) return DK <= kMmaMaxDK;
+  return std::max(d->dk, d->dv) <= kMmaMaxDK && d->length >= kMmaTok / 2;
+}
+int terms(const hyfft_decay_desc* d) {  // bfloat16 terms of an operand, 0: none are laid out
+  return d->dtype == HYFFT_BF16 || !use_mma(d, d->dk) ? 0 : d->dtype == HYFFT_F16 ? 2 : 3;
+}
 
 int slices(int DV) { return (DV + kCols - 1) / kCols; }  // 64 columns a CTA on either path
 static_assert(kCols == kMmaCols && kMmaTok % kTok == 0, "one plan for both paths");
@@ -550,7 +559,9 @@ Segments segments(const hyfft_decay_desc* d, bool learn) {
   long long want, most;
   if (!learn && use_mma(d, d->dk) && use_mma(d, d->dv)) {
     const long long ctas = rows * std::max(slices(d->dk), slices(d->dv));
-    want = ctas >= 148 ? 1 : 296 / ctas;
+    // two CTAs share an SM but where the terms of float32, or of heads above 64, fill it
+    const int fit = terms(d) == 3 || (terms(d) == 2 && std::max(d->dk, d->dv) > 64) ? 148 : 296;
+    want = ctas >= 148 ? 1 : fit / ctas;
     most = d->length / (4 * kMmaTok);
   } else {
     int rh, kw, rh2, kw2;
@@ -580,7 +591,7 @@ int launch_scan_rh(const ScanArgs& A, long long ctas, cudaStream_t st) {
 template <typename T, typename TO, bool LEARN>
 int launch_scan(const ScanArgs& A, int rh, int kw, long long ctas, cudaStream_t st) {
   if (ctas > 0x7fffffffLL) return set_error(HYFFT_ERR_UNSUPPORTED, "decay attention: too many rows");
-  if constexpr (LEARN || !std::is_same<T, __nv_bfloat16>::value) {  // up to 128 rows of bfloat16 run on the tensor cores
+  if constexpr (LEARN || !std::is_same<T, __nv_bfloat16>::value) {  // bfloat16 states of up to 128 rows run on the tensor cores
     if (rh == 8) return launch_scan_rh<T, TO, 8, 1, LEARN>(A, ctas, st);
     if (kw == 1) return launch_scan_rh<T, TO, 16, 1, LEARN>(A, ctas, st);
     if (kw == 2) return launch_scan_rh<T, TO, 16, 2, LEARN>(A, ctas, st);
@@ -618,8 +629,9 @@ int run_pass(const hyfft_decay_desc* d, ScanArgs A, cudaStream_t st) {
   A.vec = (!A.o || op_vec(A.q, A.DK, es)) && op_vec(A.k, A.DK, es) && op_vec(A.v, A.DV, es);
   A.ovec = A.DV % 8 == 0 && reinterpret_cast<uintptr_t>(A.o) % 16 == 0;
   const long long ctas = (long long)d->batch * d->heads * A.nseg * A.nslice;
-  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-    if (use_mma(d, A.DK)) return launch_scan_mma(A, sizeof(TO) == 4, ctas, st);
+  if (use_mma(d, A.DK)) {
+    if (terms(d)) A.vec = 1;  // laid out so
+    return launch_scan_mma(A, d->dtype, sizeof(TO) == 4, ctas, st);
   }
   int rh, kw;
   scan_shape(A.DK, &rh, &kw);
@@ -729,7 +741,15 @@ int forward_t(const hyfft_decay_desc* d, const void* q, const void* k, const voi
   A.log_decay = g, A.lengths = lengths, A.start = s0, A.finish = s1;
   A.vscale = 1.f, A.oscale = d->scale;
   A.DK = d->dk, A.DV = d->dv, A.srow = d->dv, A.scol = 1;
-  const int rc = run_states<T>(d, A, ws, st);
+  int rc = HYFFT_OK;
+  if (terms(d)) {
+    ScanOp ops[3] = {A.q, A.k, A.v};
+    const int heads[3] = {d->heads, d->kv_heads, d->kv_heads}, D[3] = {d->dk, d->dk, d->dv};
+    rc = launch_split_terms(ops, heads, D, 3, d->batch, d->length, d->dtype, terms(d),
+                            reinterpret_cast<char*>(ws) + seg_bytes(d), st);
+    A.q = ops[0], A.k = ops[1], A.v = ops[2];
+  }
+  if (rc == HYFFT_OK) rc = run_states<T>(d, A, ws, st);
   return rc == HYFFT_OK ? run_outputs<T, T>(d, A, ws, false, st) : rc;
 }
 
@@ -759,16 +779,25 @@ int backward_t(const hyfft_decay_desc* d, const void* q, const void* k, const vo
                void* dk, void* dv,
                float* dg, float* ds0, char* ws, size_t seg_size, size_t group_size, cudaStream_t st) {
   const int r = d->heads / d->kv_heads;
-  const Op oq{q, d->q_stride[0], d->q_stride[1], d->q_stride[2], 1};
-  const Op ok{k, d->k_stride[0], d->k_stride[1], d->k_stride[2], r};
-  const Op ov{v, d->v_stride[0], d->v_stride[1], d->v_stride[2], r};
-  const Op od{dout, d->o_stride[0], d->o_stride[1], d->o_stride[2], 1};
+  Op oq{q, d->q_stride[0], d->q_stride[1], d->q_stride[2], 1};
+  Op ok{k, d->k_stride[0], d->k_stride[1], d->k_stride[2], r};
+  Op ov{v, d->v_stride[0], d->v_stride[1], d->v_stride[2], r};
+  Op od{dout, d->o_stride[0], d->o_stride[1], d->o_stride[2], 1};
   float* seg = reinterpret_cast<float*>(ws);
   float* per_head = reinterpret_cast<float*>(ws + seg_size);
   float* learn = reinterpret_cast<float*>(ws + seg_size + group_size);
+  const Op plain[4] = {oq, ok, ov, od};
   ScanArgs A{};
   A.log_decay = g, A.lengths = lengths;
   int rc;
+  if (terms(d) && (dq || dk || dv)) {
+    Op ops[4] = {oq, ok, ov, od};
+    const int heads[4] = {d->heads, d->kv_heads, d->kv_heads, d->heads}, D[4] = {d->dk, d->dk, d->dv, d->dv};
+    if ((rc = launch_split_terms(ops, heads, D, 4, d->batch, d->length, d->dtype, terms(d),
+                                 ws + seg_size + group_size + learn_bytes(d), st)) != HYFFT_OK)
+      return rc;
+    oq = ops[0], ok = ops[1], ov = ops[2], od = ops[3];
+  }
   if (dq) {  // forwards over (do, v, k), the state transposed
     if (!saved) {
       ScanArgs P = A;
@@ -800,7 +829,7 @@ int backward_t(const hyfft_decay_desc* d, const void* q, const void* k, const vo
   if (dv && (rc = shared_scan<T>(d, G, dv, d->dv, seg, false, per_head, st)) != HYFFT_OK) return rc;
   if (dg) {
     ScanArgs P = A;
-    P.q = oq, P.k = ok, P.v = ov, P.x = od;
+    P.q = plain[0], P.k = plain[1], P.v = plain[2], P.x = plain[3];
     P.start = s0, P.vscale = 1.f, P.oscale = d->scale;
     P.DK = d->dk, P.DV = d->dv, P.srow = d->dv, P.scol = 1;
     if ((rc = run_learn<T>(d, P, ds1, learn, dg, st)) != HYFFT_OK) return rc;
@@ -809,7 +838,7 @@ int backward_t(const hyfft_decay_desc* d, const void* q, const void* k, const vo
 }
 
 struct Sizes {
-  size_t seg, group, learn;
+  size_t seg, group, learn, terms3, terms4;  // the terms of q, k, v, and those with the output's gradient
 };
 Sizes sizes(const hyfft_decay_desc* d) {
   Sizes s;
@@ -818,6 +847,13 @@ Sizes sizes(const hyfft_decay_desc* d) {
                 ? 0
                 : align256(sizeof(float) * (size_t)d->batch * d->length * d->heads * std::max(d->dk, d->dv));
   s.learn = learn_bytes(d);
+  s.terms3 = s.terms4 = 0;
+  if (const int t = terms(d)) {
+    s.terms3 = mma_terms_bytes(d->batch, d->length, d->heads, d->dk, t) +
+               mma_terms_bytes(d->batch, d->length, d->kv_heads, d->dk, t) +
+               mma_terms_bytes(d->batch, d->length, d->kv_heads, d->dv, t);
+    s.terms4 = s.terms3 + mma_terms_bytes(d->batch, d->length, d->heads, d->dv, t);
+  }
   return s;
 }
 
@@ -832,8 +868,16 @@ int hyfft_decay_workspace_size(const hyfft_decay_desc* d, size_t* fwd_bytes, siz
   const int rc = check_desc(d);
   if (rc != HYFFT_OK) return rc;
   const Sizes s = sizes(d);
-  if (fwd_bytes) *fwd_bytes = s.seg;
-  if (bwd_bytes) *bwd_bytes = s.seg + s.group + s.learn;
+  if (fwd_bytes) *fwd_bytes = s.seg + s.terms3;
+  if (bwd_bytes) *bwd_bytes = s.seg + s.group + s.learn + s.terms4;
+  return HYFFT_OK;
+}
+
+int hyfft_decay_saved_size(const hyfft_decay_desc* d, size_t* saved_bytes) {
+  const int rc = check_desc(d);
+  if (rc != HYFFT_OK) return rc;
+  if (!saved_bytes) return set_error(HYFFT_ERR_INVALID, "decay attention: null size");
+  *saved_bytes = sizes(d).seg;
   return HYFFT_OK;
 }
 
@@ -845,7 +889,7 @@ int hyfft_decay_forward(const hyfft_decay_desc* d, const void* q, const void* k,
   if (!log_decay || (d->length > 0 && (!q || !k || !v || !o)))
     return set_error(HYFFT_ERR_INVALID, "decay attention: null tensor");
   const Sizes s = sizes(d);
-  if (workspace_bytes < s.seg || (s.seg && !workspace))
+  if (workspace_bytes < s.seg + s.terms3 || (s.seg + s.terms3 && !workspace))
     return set_error(HYFFT_ERR_WORKSPACE, "decay attention: workspace too small");
   if (bind_device_of(log_decay) != HYFFT_OK) return set_error(HYFFT_ERR_CUDA, "decay attention: device");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -869,7 +913,7 @@ int hyfft_decay_backward(const hyfft_decay_desc* d, const void* q, const void* k
   if (d->length > 0 && dinitial_state && !dv)
     return set_error(HYFFT_ERR_INVALID, "decay attention: the initial state's gradient comes with dv");
   const Sizes s = sizes(d);
-  if (workspace_bytes < s.seg + s.group + s.learn || !workspace)
+  if (workspace_bytes < s.seg + s.group + s.learn + s.terms4 || !workspace)
     return set_error(HYFFT_ERR_WORKSPACE, "decay attention: workspace too small");
   if (bind_device_of(log_decay) != HYFFT_OK) return set_error(HYFFT_ERR_CUDA, "decay attention: device");
   cudaStream_t st = static_cast<cudaStream_t>(stream);

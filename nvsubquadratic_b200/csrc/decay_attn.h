@@ -8,7 +8,8 @@ namespace hyfft {
 struct ScanOp {  // strides in elements: batch, token, head
   const void* p;
   long long sb, sl, sh;
-  int group;  // query heads that share one head of this operand
+  int group;         // query heads that share one head of this operand
+  long long st = 0;  // between the bfloat16 terms of a split operand
 };
 
 // o_i = oscale * S_i^T q_i with S_i = a S_{i-1} + vscale * k_i v_i^T over a row's tokens, forwards or backwards in time.
@@ -33,10 +34,15 @@ struct ScanArgs {
   int ovec;     // o can be written in 16-byte pieces
 };
 
-// decay_mma.cu: bfloat16 operands, DK <= 128, columns in slices of 64, segments of whole 64-token chunks.
+// decay_mma.cu: DK <= 128, columns in slices of 64, segments of whole 64-token chunks. float16 and float32 operands are
+// first split into bfloat16 terms (2, 3): launch_split_terms does up to four tensors [B, L, heads[w], D[w]] into `ws` and makes
+// the ops point there.
 constexpr int kMmaTok = 64;
 constexpr int kMmaCols = 64;
 constexpr int kMmaMaxDK = 128;
-int launch_scan_mma(const ScanArgs& A, bool out_f32, long long ctas, cudaStream_t st);
+int launch_scan_mma(const ScanArgs& A, int dtype, bool out_f32, long long ctas, cudaStream_t st);
+size_t mma_terms_bytes(int B, long long L, int heads, int D, int terms);
+int launch_split_terms(ScanOp* ops, const int* heads, const int* D, int n, int B, long long L, int dtype, int terms, char* ws,
+                       cudaStream_t st);
 
 }  // namespace hyfft

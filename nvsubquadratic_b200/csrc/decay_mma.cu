@@ -1,5 +1,11 @@
 // The decayed linear attention's scan on the tensor cores (tcgen05), bfloat16 operands, float32 state.
 //
+// float16 and float32 operands come as sums of NT = 2 and 3 bfloat16 terms (8 bits each; a small kernel lays them out
+// first, NT = 1 below is bfloat16 itself). A product of two sums runs the pairs of terms whose order is below NT, 3 or 6 of
+// them, into one float32 accumulator, and what the kernel rounds for a product (P, the state's copy) it keeps to NT terms too, so
+// float32 results are float32's (16 x 4096 tokens, 12 heads of 64: 0.62 ms, multiply-adds take 1.03; float16 0.48 and 1.00).
+// The tensor cores' own float16 would do with fewer products but not hold a state beyond 65504.
+//
 // A CTA walks over one row's tokens (or a segment of them) in chunks of 64 and keeps 64 columns of the state. With
 // i, j the tokens of a chunk in scan order, n of them valid, S the state before it (e = 1 forwards, 0 backwards, where
 // the decay is applied after a token's output):
@@ -32,10 +38,12 @@
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <cuda_bf16.h>
+#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include <atomic>
 #include <mutex>
+#include <type_traits>
 
 #include "../../include/hyfft.h"
 #include "common.cuh"
@@ -83,26 +91,28 @@ enum Bar {
   kBars = 25
 };
 
-// Bytes of the shared-memory layout for a state of DK (64 or 128) rows whose update takes TERMS bfloat16 terms. Tiles
-// start on 1024 bytes, where the swizzle's pattern does.
+// Bytes of the shared-memory layout for a state of DK (64 or 128) rows, operands of NT terms, a state update from TERMS
+// terms of the decayed V. Tiles start on 1024 bytes, where the swizzle's pattern does.
 constexpr int kTile = kT * 128;
-template <int DK, bool OUT, int TERMS>
+template <int DK, bool OUT, int NT, int TERMS>
 struct Layout {
-  static constexpr int qk = DK / 64 * kTile;
-  // as many buffers of K and V, of Q and of the decayed V as two CTAs on an SM leave room for
-  static constexpr int nbuf = OUT ? (DK == 64 ? 3 : 2) : (DK == 64 ? 4 : 2);
-  static constexpr int qbuf = DK == 64 ? 3 : 1;
-  static constexpr int wbuf = OUT ? 1 : DK == 64 ? 2 : 2;
+  static constexpr bool two = NT == 1 || (NT == 2 && DK == 64);  // CTAs on an SM
+  static constexpr int qk = NT * DK / 64 * kTile, vt = NT * kTile;
+  // as many buffers of K and V, of Q and of the decayed V as there is room for
+  static constexpr int nbuf = NT == 1 ? (OUT ? (DK == 64 ? 3 : 2) : (DK == 64 ? 4 : 2))
+                                      : (OUT ? (NT == 3 && DK == 64 ? 2 : 1) : (NT == 3 && DK == 64 ? 3 : 2));
+  static constexpr int qbuf = NT == 1 && DK == 64 ? 3 : 1;
+  static constexpr int wbuf = OUT || (NT == 2 && DK == 64) ? 1 : 2;
   static constexpr int q = 0;
   static constexpr int k = q + (OUT ? qbuf * qk : 0);
   static constexpr int v = k + nbuf * qk;
-  static constexpr int w = v + nbuf * kTile;            // the decayed V
-  static constexpr int p = w + wbuf * TERMS * kTile;    // P
-  static constexpr int s = p + (OUT ? kTile : 0);       // the rounded state
-  static constexpr int tab = s + (OUT ? DK * 128 : 0);  // a^d for d = -64 .. 64 (zeros below 0)
+  static constexpr int w = v + nbuf * vt;                    // the decayed V
+  static constexpr int p = w + wbuf * TERMS * kTile;         // P
+  static constexpr int s = p + (OUT ? NT * kTile : 0);       // the state in NT terms
+  static constexpr int tab = s + (OUT ? NT * DK * 128 : 0);  // a^d for d = -64 .. 64 (zeros below 0)
   static constexpr int bar = tab + (2 * kT + 4) * 4;
   static constexpr int bytes = bar + kBars * 8 + 8;
-  static_assert(2 * (bytes + 1024) <= 228 * 1024, "two CTAs share an SM");
+  static_assert((two ? 2 : 1) * (bytes + 1024) <= 228 * 1024 && bytes <= 227 * 1024, "does not fit an SM");
 };
 // Byte of column c (even) of a row in a swizzled tile of 64 columns.
 __device__ __forceinline__ int swz(int row, int c) { return row * 128 + ((((c >> 3) ^ row) & 7) << 4) + (c & 7) * 2; }
@@ -176,6 +186,14 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
+template <typename TO>
+__device__ __forceinline__ uint32_t pack_out(float2 f) {
+  if constexpr (std::is_same<TO, __half>::value) {
+    const __half2 h = __floats2half2_rn(f.x, f.y);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  return pack2(f.x, f.y);
+}
 __device__ __forceinline__ float2 unpack2(uint32_t u) {
   return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
 }
@@ -240,6 +258,16 @@ __device__ __forceinline__ void load_tile(unsigned char* dst, const bf16* __rest
   }
 }
 
+// Two neighbouring values of a tile row in NT terms, the terms `apart` bytes from each other.
+template <int NT>
+__device__ __forceinline__ void put_terms(unsigned char* d, int apart, float2 f) {
+#pragma unroll
+  for (int y = 0; y < NT; ++y) {
+    const uint32_t u = pack2(f.x, f.y);
+    *reinterpret_cast<uint32_t*>(d + y * apart) = u;
+    if (y + 1 < NT) f = csub(f, unpack2(u));
+  }
+}
 // 16 TMEM lanes x 32 columns over a warp: register 4 j + 2 y + x holds row lane / 4 + 8 y, column 8 j + 2 (lane % 4) + x.
 __device__ __forceinline__ void tmem_ld(uint32_t a, uint32_t (&u)[16]) {
   asm volatile(
@@ -263,10 +291,31 @@ __device__ __forceinline__ void tmem_ld2(uint32_t a, uint32_t b, uint32_t (&u)[1
       : "memory");
 }
 
+// The products of a sum of na terms and one of nb: the pairs whose order (the terms' numbers added) is below `orders`, the
+// smallest products first. The accumulator cuts off below its last bit at every step, so steps at the full size are to be few
+// (largest first, float32 outputs were off by 1.2e-6 of their norm instead of 1.3e-7).
+constexpr int term_a(int y, int na, int nb, int orders) {
+  for (int o = orders - 1; o >= 0; --o)
+    for (int a = 0; a < na; ++a)
+      if (o - a >= 0 && o - a < nb && y-- == 0) return a;
+  return -1;
+}
+constexpr int term_b(int y, int na, int nb, int orders) {
+  for (int o = orders - 1; o >= 0; --o)
+    for (int a = 0; a < na; ++a)
+      if (o - a >= 0 && o - a < nb && y-- == 0) return o - a;
+  return -1;
+}
+constexpr int pairs(int na, int nb, int orders) {
+  int n = 0;
+  while (term_a(n, na, nb, orders) >= 0) ++n;
+  return n;
+}
+
 // OUT: the pass with outputs; without it, segments' sums alone (K and V only).
-template <int DK, bool OUT, int TERMS, typename TO>
+template <int DK, bool OUT, int NT, int TERMS, typename TO>
 __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A, const __grid_constant__ Maps M) {
-  using L = Layout<DK, OUT, TERMS>;
+  using L = Layout<DK, OUT, NT, TERMS>;
   extern __shared__ __align__(1024) unsigned char smem[];
   float* tab = reinterpret_cast<float*>(smem + L::tab);
   uint64_t* bar = reinterpret_cast<uint64_t*>(smem + L::bar);
@@ -325,20 +374,29 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A, co
       const int hk = h / A.k.group, hv = h / A.v.group;
       const bf16* kp = static_cast<const bf16*>(A.k.p) + b * A.k.sb + hk * A.k.sh;
       const bf16* vp = static_cast<const bf16*>(A.v.p) + b * A.v.sb + hv * A.v.sh;
-      for (int i = who; i < chunks; i += 2) {
+      // one buffer: one warp fills it. A warp that skips a buffer's phase could take the one before for the one that it waits
+      // for; with more buffers each wait is preceded by one for a later chunk than the phase that was skipped.
+      constexpr int kTurns = L::nbuf == 1 ? 1 : 2;
+      for (int i = who < kTurns ? who : chunks; i < chunks; i += kTurns) {
         const int nb = i % L::nbuf;
-        unsigned char *kd = smem + L::k + nb * L::qk, *vd = smem + L::v + nb * kTile;
+        unsigned char *kd = smem + L::k + nb * L::qk, *vd = smem + L::v + nb * L::vt;
         if (i >= L::nbuf) wait((OUT ? kDoneO : kDoneS) + nb, i / L::nbuf - 1);
         if (M.on && tokens(i) == kT) {
           if (lane == 0) {
-            expect(&bar[kFull + nb], L::qk + kTile);
-            load_box<DK>(umma::su32(kd), &M.k, &bar[kFull + nb], 0, hk, (int)first(i), (int)b);
-            load_box<kC>(umma::su32(vd), &M.v, &bar[kFull + nb], c0, hv, (int)first(i), (int)b);
+            expect(&bar[kFull + nb], L::qk + L::vt);
+#pragma unroll
+            for (int y = 0; y < NT; ++y) {
+              load_box<DK>(umma::su32(kd + y * L::qk / NT), &M.k, &bar[kFull + nb], 0, hk, (int)first(i), (int)b + y * A.B);
+              load_box<kC>(umma::su32(vd + y * kTile), &M.v, &bar[kFull + nb], c0, hv, (int)first(i), (int)b + y * A.B);
+            }
           }
           __syncwarp();
         } else {
-          load_tile<DK>(kd, kp, A.k.sl, tokens(i), 0, A.DK, first(i), A.vec);
-          load_tile<kC>(vd, vp, A.v.sl, tokens(i), c0, A.DV, first(i), A.vec);
+#pragma unroll
+          for (int y = 0; y < NT; ++y) {
+            load_tile<DK>(kd + y * L::qk / NT, kp + y * A.k.st, A.k.sl, tokens(i), 0, A.DK, first(i), A.vec);
+            load_tile<kC>(vd + y * kTile, vp + y * A.v.st, A.v.sl, tokens(i), c0, A.DV, first(i), A.vec);
+          }
           cp_wait();
           hand_over(&bar[kFull + nb]);
         }
@@ -353,11 +411,15 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A, co
         if (M.on && tokens(i) == kT) {
           if (lane == 0) {
             expect(&bar[kFullQ + qb], L::qk);
-            load_box<DK>(umma::su32(qd), &M.q, &bar[kFullQ + qb], 0, hq, (int)first(i), (int)b);
+#pragma unroll
+            for (int y = 0; y < NT; ++y)
+              load_box<DK>(umma::su32(qd + y * L::qk / NT), &M.q, &bar[kFullQ + qb], 0, hq, (int)first(i), (int)b + y * A.B);
           }
           __syncwarp();
         } else {
-          load_tile<DK>(qd, qp, A.q.sl, tokens(i), 0, A.DK, first(i), A.vec);
+#pragma unroll
+          for (int y = 0; y < NT; ++y)
+            load_tile<DK>(qd + y * L::qk / NT, qp + y * A.q.st, A.q.sl, tokens(i), 0, A.DK, first(i), A.vec);
           cp_wait();
           hand_over(&bar[kFullQ + qb]);
         }
@@ -372,16 +434,20 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A, co
     constexpr uint32_t kIdS = umma::idesc_bf16(DK, kC, 1, 1);
     for (int i = 0; i < chunks; ++i) {
       const int nb = i % L::nbuf, wb = i % L::wbuf;
-      const uint32_t dk = dk0 + nb * (L::qk >> 4), dv = dv0 + nb * kNextTile;
+      const uint32_t dk = dk0 + nb * (L::qk >> 4), dv = dv0 + nb * (L::vt >> 4);
       wait(kFull + nb, i / L::nbuf);
       if (OUT) {
         const uint32_t dqi = dq + i % L::qbuf * (L::qk >> 4);
         wait(kFullQ + i % L::qbuf, i / L::qbuf);
         if (elect()) {
 #pragma unroll
-          for (int x = 0; x < DK / 16; ++x)
-            mma(tmem + kColP, dqi + (x >> 2) * kNextTile + (x & 3) * kAlongK, dk + (x >> 2) * kNextTile + (x & 3) * kAlongK, kIdP,
-                x > 0);
+          for (int y = 0; y < pairs(NT, NT, NT); ++y)
+#pragma unroll
+            for (int x = 0; x < DK / 16; ++x) {
+              const int at = (x >> 2) * kNextTile + (x & 3) * kAlongK;
+              mma(tmem + kColP, dqi + term_a(y, NT, NT, NT) * (L::qk / NT >> 4) + at,
+                  dk + term_b(y, NT, NT, NT) * (L::qk / NT >> 4) + at, kIdP, x + y > 0);
+            }
           umma::commit(&bar[kDoneP]);
         }
         __syncwarp();
@@ -390,10 +456,11 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A, co
       wait(kHaveV + wb, i / L::wbuf);
       if (elect()) {
 #pragma unroll
-        for (int y = 0; y < TERMS; ++y)
+        for (int y = 0; y < pairs(NT, TERMS, TERMS); ++y)
 #pragma unroll
           for (int x = 0; x < kT / 16; ++x)
-            mma(tmem + kColS - 64 * wb, dk + x * kAlongRows, dw + (wb * TERMS + y) * kNextTile + x * kAlongRows, kIdS, x + y > 0);
+            mma(tmem + kColS - 64 * wb, dk + term_a(y, NT, TERMS, TERMS) * (L::qk / NT >> 4) + x * kAlongRows,
+                dw + (wb * TERMS + term_b(y, NT, TERMS, TERMS)) * kNextTile + x * kAlongRows, kIdS, x + y > 0);
         umma::commit(&bar[kDoneS + (OUT ? 0 : nb)]);
       }
       __syncwarp();
@@ -402,15 +469,22 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A, co
         if (i) wait(kReadO, i - 1);
         if (elect()) {
 #pragma unroll
-          for (int x = 0; x < DK / 16; ++x)
-            mma(tmem + kColR, dqi + (x >> 2) * kNextTile + (x & 3) * kAlongK, ds + x * kAlongRows, kIdR, x > 0);
+          for (int y = 0; y < pairs(NT, NT, NT); ++y)
+#pragma unroll
+            for (int x = 0; x < DK / 16; ++x)
+              mma(tmem + kColR, dqi + term_a(y, NT, NT, NT) * (L::qk / NT >> 4) + (x >> 2) * kNextTile + (x & 3) * kAlongK,
+                  ds + term_b(y, NT, NT, NT) * (DK * 128 >> 4) + x * kAlongRows, kIdR, x + y > 0);
           umma::commit(&bar[kDoneR + i % L::qbuf]);
         }
         __syncwarp();
         wait(kHaveP, i);
         if (elect()) {
 #pragma unroll
-          for (int x = 0; x < kT / 16; ++x) mma(tmem + kColO, dp + x * kAlongK, dv + x * kAlongRows, kIdR, x > 0);
+          for (int y = 0; y < pairs(NT, NT, NT); ++y)
+#pragma unroll
+            for (int x = 0; x < kT / 16; ++x)
+              mma(tmem + kColO, dp + term_a(y, NT, NT, NT) * kNextTile + x * kAlongK,
+                  dv + term_b(y, NT, NT, NT) * kNextTile + x * kAlongRows, kIdR, x + y > 0);
           umma::commit(&bar[kDoneO + nb]);
         }
         __syncwarp();
@@ -450,7 +524,7 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A, co
             }
             if (sizeof(TO) == 2 && A.ovec) {
               // transposed among four lanes: each stores 16 bytes of the row, together 64
-              uint4 u = make_uint4(pack2(f[0].x, f[0].y), pack2(f[1].x, f[1].y), pack2(f[2].x, f[2].y), pack2(f[3].x, f[3].y));
+              uint4 u = make_uint4(pack_out<TO>(f[0]), pack_out<TO>(f[1]), pack_out<TO>(f[2]), pack_out<TO>(f[3]));
               swap_pairs(u.x, u.y, 1, quad);
               swap_pairs(u.z, u.w, 1, quad);
               swap_pairs(u.x, u.z, 2, quad);
@@ -501,9 +575,9 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A, co
         const int rw = srow + 16 * y;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          *reinterpret_cast<uint32_t*>(smem + L::s + swz(rw, half + 8 * j + pair)) = pack2(S[y][4 * j], S[y][4 * j + 1]);
-          *reinterpret_cast<uint32_t*>(smem + L::s + swz(rw, half + 8 * j + pair) + 1024) =
-              pack2(S[y][4 * j + 2], S[y][4 * j + 3]);
+          unsigned char* d = smem + L::s + swz(rw, half + 8 * j + pair);
+          put_terms<NT>(d, DK * 128, make_float2(S[y][4 * j], S[y][4 * j + 1]));
+          put_terms<NT>(d + 1024, DK * 128, make_float2(S[y][4 * j + 2], S[y][4 * j + 3]));
         }
       }
     };
@@ -531,18 +605,21 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A, co
     // The V of chunk i, decayed, in TERMS terms.
     const auto split_v = [&](int i) {
       const int wb = i % L::wbuf, n = tokens(i);
-      const unsigned char* v = smem + L::v + i % L::nbuf * kTile;
+      const unsigned char* v = smem + L::v + i % L::nbuf * L::vt;
       unsigned char* terms = smem + L::w + wb * (TERMS * kTile);
       wait(kFull + i % L::nbuf, i / L::nbuf);
 #pragma unroll
       for (int x = 0; x < kT * kC / 8 / kThreads; ++x) {
         const int at = tid + x * kThreads, t = at >> 3;  // V's place in the tile is its terms' place
         const float w = t < n ? tab[kT + (rev ? t + 1 : n - 1 - t)] * A.vscale : 0.f;
-        const uint4 u = *reinterpret_cast<const uint4*>(v + at * 16);
-        uint4 hi, mid, lo;
+        uint4 u[NT], hi, mid, lo;
+#pragma unroll
+        for (int y = 0; y < NT; ++y) u[y] = *reinterpret_cast<const uint4*>(v + y * kTile + at * 16);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          float2 f = unpack2((&u.x)[e]);
+          float2 f = unpack2((&u[NT - 1].x)[e]);  // the terms from the least on: exact
+#pragma unroll
+          for (int y = NT - 2; y >= 0; --y) f = cadd(f, unpack2((&u[y].x)[e]));
           f.x *= w, f.y *= w;
           const uint32_t p = pack2(f.x, f.y);
           f = csub(f, unpack2(p));
@@ -580,10 +657,10 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A, co
 #pragma unroll
         for (int j = 0; j < 4; ++j) {  // row + 8 at column block j decays like row at block j - 1
           unsigned char* d = smem + L::p + swz(row, half + 8 * j + pair);
-          *reinterpret_cast<uint32_t*>(d) =
-              pack2(__uint_as_float(p[4 * j]) * decay(2 * j + 2), __uint_as_float(p[4 * j + 1]) * decay(2 * j + 3));
-          *reinterpret_cast<uint32_t*>(d + 1024) =
-              pack2(__uint_as_float(p[4 * j + 2]) * decay(2 * j), __uint_as_float(p[4 * j + 3]) * decay(2 * j + 1));
+          put_terms<NT>(d, kTile, make_float2(__uint_as_float(p[4 * j]) * decay(2 * j + 2),
+                                              __uint_as_float(p[4 * j + 1]) * decay(2 * j + 3)));
+          put_terms<NT>(d + 1024, kTile, make_float2(__uint_as_float(p[4 * j + 2]) * decay(2 * j),
+                                                     __uint_as_float(p[4 * j + 3]) * decay(2 * j + 1)));
         }
         hand_over(&bar[kHaveP]);
       }
@@ -639,7 +716,7 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
 }
 
 // False where TMA cannot address the tensor (a head size, an address or a stride off 16 bytes, a stride of zero).
-bool make_map(CUtensorMap* m, const ScanOp& x, int D, int heads, int L, int B) {
+bool make_map(CUtensorMap* m, const ScanOp& x, int D, int heads, int L, int B) {  // B: batches times terms
   PFN_cuTensorMapEncodeTiled_v12000 enc = encode_fn();
   if (!enc || !x.p) return false;
   const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)heads, (cuuint64_t)L, (cuuint64_t)B};
@@ -656,10 +733,10 @@ bool make_map(CUtensorMap* m, const ScanOp& x, int D, int heads, int L, int B) {
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int DK, bool OUT, int TERMS, typename TO>
+template <int DK, bool OUT, int NT, int TERMS, typename TO>
 int launch(const ScanArgs& A, const Maps& M, long long ctas, cudaStream_t st) {
-  auto kern = decay_mma_kernel<DK, OUT, TERMS, TO>;
-  constexpr size_t sm = Layout<DK, OUT, TERMS>::bytes;
+  auto kern = decay_mma_kernel<DK, OUT, NT, TERMS, TO>;
+  constexpr size_t sm = Layout<DK, OUT, NT, TERMS>::bytes;
   if (!kernel_smem_once((const void*)kern, sm, true)) return set_error(HYFFT_ERR_CUDA, "decay attention: shared memory");
   kern<<<(unsigned)ctas, kAll, sm, st>>>(A, M);
   if (cudaGetLastError() != cudaSuccess) return set_error(HYFFT_ERR_CUDA, "decay attention: kernel launch failed");
@@ -667,24 +744,107 @@ int launch(const ScanArgs& A, const Maps& M, long long ctas, cudaStream_t st) {
   return HYFFT_OK;
 }
 
-template <int DK>
+template <int DK, int NT, typename T>
 int launch_dk(const ScanArgs& A, const Maps& M, bool out_f32, long long ctas, cudaStream_t st) {
-  if (!A.o) return launch<DK, false, 3, bf16>(A, M, ctas, st);
-  // where segments were added up before, the state only serves this pass's outputs, which read it rounded to 8 bits: 16
-  // bits are enough (not by whether the caller wants the final state, so that asking for it changes no output)
-  if (A.nseg == 1) return out_f32 ? launch<DK, true, 3, float>(A, M, ctas, st) : launch<DK, true, 3, bf16>(A, M, ctas, st);
-  return out_f32 ? launch<DK, true, 2, float>(A, M, ctas, st) : launch<DK, true, 2, bf16>(A, M, ctas, st);
+  if (!A.o) return launch<DK, false, NT, 3, T>(A, M, ctas, st);
+  // where segments were added up before, the state only serves this pass's outputs: those of bfloat16 read it rounded
+  // to 8 bits, and 16 are enough (not by whether the caller wants the final state, so that asking for it changes no output)
+  if (NT == 1 && A.nseg > 1)
+    return out_f32 ? launch<DK, true, NT, NT == 1 ? 2 : 3, float>(A, M, ctas, st)
+                   : launch<DK, true, NT, NT == 1 ? 2 : 3, T>(A, M, ctas, st);
+  return out_f32 ? launch<DK, true, NT, 3, float>(A, M, ctas, st) : launch<DK, true, NT, 3, T>(A, M, ctas, st);
+}
+
+// ---------------------------------------------------------------- terms
+struct SplitArgs {
+  const void* src[4];
+  bf16* dst[4];
+  long long sb[4], sl[4], sh[4], begin[5];  // strides; where each tensor's work begins, in runs of eight features
+  int heads[4], D[4], n;
+  int B, L, terms;
+};
+
+// x = sum of bfloat16 terms, largest first; an infinity or NaN is the first term alone.
+template <typename T>
+__global__ void __launch_bounds__(256) decay_split_kernel(const SplitArgs A) {
+  const long long id = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (id >= A.begin[A.n]) return;
+  int w = 0;
+  while (id >= A.begin[w + 1]) ++w;
+  const int D = A.D[w], runs = (D + 7) / 8;
+  long long i = id - A.begin[w];
+  const int c = (int)(i % runs) * 8;
+  i /= runs;
+  const int h = (int)(i % A.heads[w]);
+  i /= A.heads[w];  // b * L + l
+  const long long b = i / A.L, l = i - b * A.L;
+  const T* src = static_cast<const T*>(A.src[w]) + b * A.sb[w] + l * A.sl[w] + h * A.sh[w] + c;
+  float f[8];
+#pragma unroll
+  for (int u = 0; u < 8; ++u) f[u] = c + u < D ? DT<T>::load(src + u) : 0.f;
+  const long long per = (long long)A.B * A.L * A.heads[w] * runs * 8;
+  bf16* dst = A.dst[w] + ((i * A.heads[w] + h) * runs * 8 + c);
+  for (int t = 0; t < A.terms; ++t) {
+    uint4 out;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const uint32_t p = pack2(f[2 * u], f[2 * u + 1]);
+      (&out.x)[u] = p;
+      const float2 r = unpack2(p);
+      f[2 * u] = isfinite(r.x) ? f[2 * u] - r.x : 0.f;
+      f[2 * u + 1] = isfinite(r.y) ? f[2 * u + 1] - r.y : 0.f;
+    }
+    *reinterpret_cast<uint4*>(dst + t * per) = out;
+  }
+}
+
+size_t term_elements(int B, long long L, int heads, int D, int terms) {
+  return (size_t)terms * B * L * heads * ((D + 7) / 8 * 8);
 }
 
 }  // namespace
 
-int launch_scan_mma(const ScanArgs& A, bool out_f32, long long ctas, cudaStream_t st) {
+size_t mma_terms_bytes(int B, long long L, int heads, int D, int terms) {
+  return (sizeof(bf16) * term_elements(B, L, heads, D, terms) + 255) / 256 * 256;
+}
+
+int launch_split_terms(ScanOp* ops, const int* heads, const int* D, int n, int B, long long L, int dtype, int terms,
+                       char* ws, cudaStream_t st) {
+  SplitArgs A{};
+  A.B = B, A.L = (int)L, A.terms = terms, A.n = n;
+  for (int w = 0; w < n; ++w) {
+    const int runs = (D[w] + 7) / 8;
+    A.src[w] = ops[w].p, A.sb[w] = ops[w].sb, A.sl[w] = ops[w].sl, A.sh[w] = ops[w].sh;
+    A.heads[w] = heads[w], A.D[w] = D[w];
+    A.dst[w] = reinterpret_cast<bf16*>(ws);
+    ws += mma_terms_bytes(B, L, heads[w], D[w], terms);
+    A.begin[w + 1] = A.begin[w] + (long long)B * L * heads[w] * runs;
+    ops[w].p = A.dst[w];
+    ops[w].sh = runs * 8, ops[w].sl = (long long)heads[w] * runs * 8, ops[w].sb = L * ops[w].sl, ops[w].st = B * ops[w].sb;
+  }
+  const long long ctas = (A.begin[n] + 255) / 256;
+  if (ctas > 0x7fffffffLL) return set_error(HYFFT_ERR_UNSUPPORTED, "decay attention: too many elements");
+  if (dtype == HYFFT_F32)
+    decay_split_kernel<float><<<(unsigned)ctas, 256, 0, st>>>(A);
+  else
+    decay_split_kernel<__half><<<(unsigned)ctas, 256, 0, st>>>(A);
+  if (cudaGetLastError() != cudaSuccess) return set_error(HYFFT_ERR_CUDA, "decay attention: kernel launch failed");
+  g_launches.fetch_add(1, std::memory_order_relaxed);
+  return HYFFT_OK;
+}
+
+int launch_scan_mma(const ScanArgs& A, int dtype, bool out_f32, long long ctas, cudaStream_t st) {
   if (ctas > 0x7fffffffLL) return set_error(HYFFT_ERR_UNSUPPORTED, "decay attention: too many rows");
+  const int nt = dtype == HYFFT_BF16 ? 1 : dtype == HYFFT_F16 ? 2 : 3;
   Maps M{};
-  M.on = A.L >= kT && A.vec && make_map(&M.k, A.k, A.DK, A.H / A.k.group, A.L, A.B) &&
-         make_map(&M.v, A.v, A.DV, A.H / A.v.group, A.L, A.B) &&
-         (!A.o || make_map(&M.q, A.q, A.DK, A.H / A.q.group, A.L, A.B));
-  return A.DK <= 64 ? launch_dk<64>(A, M, out_f32, ctas, st) : launch_dk<128>(A, M, out_f32, ctas, st);
+  M.on = A.L >= kT && A.vec && make_map(&M.k, A.k, A.DK, A.H / A.k.group, A.L, A.B * nt) &&
+         make_map(&M.v, A.v, A.DV, A.H / A.v.group, A.L, A.B * nt) &&
+         (!A.o || make_map(&M.q, A.q, A.DK, A.H / A.q.group, A.L, A.B * nt));
+  const bool wide = A.DK > 64;
+  if (nt == 1) return wide ? launch_dk<128, 1, bf16>(A, M, out_f32, ctas, st) : launch_dk<64, 1, bf16>(A, M, out_f32, ctas, st);
+  if (nt == 2)
+    return wide ? launch_dk<128, 2, __half>(A, M, out_f32, ctas, st) : launch_dk<64, 2, __half>(A, M, out_f32, ctas, st);
+  return wide ? launch_dk<128, 3, float>(A, M, true, ctas, st) : launch_dk<64, 3, float>(A, M, true, ctas, st);
 }
 
 }  // namespace hyfft

@@ -52,7 +52,7 @@ _PLANS: dict = {}
 
 
 def _plan(q, k, v, scale, dout=None):
-    """(descriptor, (forward, backward) workspace bytes) of a call, built once for each set of shapes and strides."""
+    """(descriptor, (forward, saved, backward) workspace bytes) of a call, built once for each set of shapes and strides."""
     key = (q.shape, q.stride(), q.dtype, k.shape, k.stride(), v.shape, v.stride(), scale,
            None if dout is None else dout.stride())
     hit = _PLANS.get(key)
@@ -78,14 +78,15 @@ def _desc(q, k, v, scale, dout=None) -> _lib.DecayDesc:
     return d
 
 
-def _workspaces(d) -> tuple[int, int]:
-    f, b = ctypes.c_size_t(), ctypes.c_size_t()
-    _lib.check(_lib.load().hyfft_decay_workspace_size(ctypes.byref(d), ctypes.byref(f), ctypes.byref(b)),
-               "hyfft_decay_workspace_size")
-    return f.value, b.value
+def _workspaces(d) -> tuple[int, int, int]:
+    f, s, b = ctypes.c_size_t(), ctypes.c_size_t(), ctypes.c_size_t()
+    lib = _lib.load()
+    _lib.check(lib.hyfft_decay_workspace_size(ctypes.byref(d), ctypes.byref(f), ctypes.byref(b)), "hyfft_decay_workspace_size")
+    _lib.check(lib.hyfft_decay_saved_size(ctypes.byref(d), ctypes.byref(s)), "hyfft_decay_saved_size")
+    return f.value, s.value, b.value
 
 
-def _forward(q, k, v, log_decay, initial_state, lengths, scale, want_state):
+def _forward(q, k, v, log_decay, initial_state, lengths, scale, want_state, want_saved):
     """(o, state or None, the tensors as the library read them and what it leaves for the backward)."""
     dev = _lib.require_cuda(q, k, v, log_decay, initial_state, lengths)
     q, k, v = _unit(q), _unit(k), _unit(v)
@@ -97,20 +98,21 @@ def _forward(q, k, v, log_decay, initial_state, lengths, scale, want_state):
     state = g.new_empty((B, H, Dk, Dv)) if want_state else None
     saved = None
     if B:
-        d, (need, _) = _plan(q, k, v, scale)
+        d, (need, keep, _) = _plan(q, k, v, scale)
         ws = _lib.workspace(need, dev)
-        saved = ws if need else None
         rc = _lib.load().hyfft_decay_forward(ctypes.byref(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(),
                                              _lib.ptr(lengths), _lib.ptr(s0), o.data_ptr(), _lib.ptr(state),
                                              ws.data_ptr(), ws.numel(), _lib.stream_ptr(dev))
         _lib.check(rc, "hyfft_decay_forward")
+        if keep and want_saved:  # without the rest of the workspace, which is as large as the inputs
+            saved = ws if keep == need else ws[:keep].clone()
     return o, state, (q, k, v, g, s0, saved)
 
 
 class _DecayFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, log_decay, initial_state, lengths, scale, want_state):
-        o, state, read = _forward(q, k, v, log_decay, initial_state, lengths, scale, want_state)
+        o, state, read = _forward(q, k, v, log_decay, initial_state, lengths, scale, want_state, True)
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(*read, lengths)
         ctx.scale, ctx.decay_dtype = scale, log_decay.dtype
@@ -138,7 +140,7 @@ class _DecayFunction(torch.autograd.Function):
         dg = torch.empty_like(g) if want[3] else None
         if B == 0:
             return dq, dk, dv, (torch.zeros_like(g).to(ctx.decay_dtype) if want[3] else None), ds0, *none
-        d, (_, need) = _plan(q, k, v, ctx.scale, do)
+        d, (_, _, need) = _plan(q, k, v, ctx.scale, do)
         ws = _lib.workspace(need, dev)
         rc = _lib.load().hyfft_decay_backward(ctypes.byref(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(),
                                               _lib.ptr(lengths), _lib.ptr(s0), _lib.ptr(saved), do.data_ptr(), _lib.ptr(dstate),
@@ -181,7 +183,7 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:5]):
         o, state = _DecayFunction.apply(*args)
     else:
-        o, state, _ = _forward(*args)
+        o, state, _ = _forward(*args, False)
     return (o, state) if return_state else o
 
 
