@@ -826,6 +826,8 @@ int launch_split_terms(ScanOp* ops, const int* heads, const int* D, int n, int B
   if (ctas > 0x7fffffffLL) return set_error(HYFFT_ERR_UNSUPPORTED, "decay attention: too many elements");
   if (dtype == HYFFT_F32)
     decay_split_kernel<float><<<(unsigned)ctas, 256, 0, st>>>(A);
+  else if (dtype == HYFFT_BF16)
+    decay_split_kernel<bf16><<<(unsigned)ctas, 256, 0, st>>>(A);
   else
     decay_split_kernel<__half><<<(unsigned)ctas, 256, 0, st>>>(A);
   if (cudaGetLastError() != cudaSuccess) return set_error(HYFFT_ERR_CUDA, "decay attention: kernel launch failed");

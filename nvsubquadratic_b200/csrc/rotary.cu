@@ -11,7 +11,8 @@
 //
 // Every element is read once and written once (that is all the traffic; bound by HBM bandwidth). A thread computes the sines
 // and cosines of one vector of pairs at one token and applies them to several heads of q and of k in one launch, so
-// their cost is shared; no table is stored or read.
+// their cost is shared; no table is stored or read. 65536 tokens of 32 + 32 heads of 128, bfloat16: 319 us either way, 6.6
+// TB/s, the rate of a copy (470 us with elements converted one by one and 64-bit divisions for the thread's place).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
