@@ -430,7 +430,7 @@ __global__ void __launch_bounds__(256) decay_group_sum_kernel(const float* src, 
 // ---------------------------------------------------------------- single tokens
 // One token of each request: a pass over the state, read and written once (8 bytes per element, nothing else of
 // size). A CTA takes one head's state (a slice of 32 columns when there are few heads, so that all SMs have work);
-// a thread reads four neighbouring columns of every (kStepThreads / columns * 4)-th row. 171 requests of 32 heads of
+// a thread reads four neighbouring columns of every (kStepThreads / columns * 4)-th row. 172 requests of 32 heads of
 // 128 x 128: 133 us, 5.5 TB/s (84% of a copy's rate); one request of 12 heads of 64 x 64: 3 us.
 constexpr int kStepThreads = 256;
 

@@ -33,8 +33,8 @@
 // at the copy's rate takes 41).
 // Registers move from the loading to the computing warps. Two CTAs share an SM (<= 113 KB, 256 TMEM columns each).
 //
-// 64-row products lie in 16 of a warp's 32 TMEM lanes, and
-// the 16 x 256-bit load shape spreads those over all 32 threads (two rows, pairs of columns).
+// 64-row products lie in 16 of a warp's 32 TMEM lanes, and the 16 x 256-bit load shape spreads those over all 32 threads
+// (two rows, pairs of columns).
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <cuda_bf16.h>
