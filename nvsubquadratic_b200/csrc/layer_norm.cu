@@ -7,11 +7,13 @@
 // A row is held in the registers of a group of 32 .. 512 threads (kPer = 8, 16 or 32 elements each), so the mean and
 // then the centred squares are summed from registers: two reductions, no cancellation between E[x^2] and
 // E[x]^2. Groups walk over the rows with the weights in registers. Rows that start on 16 bytes come through a ring of up
-// to four in shared memory for each group, filled by bulk copies (65536 rows of 4096 bfloat16: 228 us forwards, 278
+// to four in shared memory for each group, filled by bulk copies (65536 rows of 4096 bfloat16: 205 us forwards, 277
 // backwards; with the next row's loads in registers instead 246 and 330). Other rows are loaded one ahead into registers.
+// Forwards 16-bit weights stay packed, which leaves room for four CTAs an SM instead of three (205 against 227 us); joining
+// the warps' own means and squares with one barrier instead of two cost more instructions than it saved (251).
 // Everything per element runs on packed pairs (element by element, with a test of the column for each, it was 314 and
-// 422 us: instructions were the bound). The weight's and the bias's gradients stay in each thread's registers over all rows of its group; a CTA adds its groups' sums in shared memory,
-// writes one partial row, and a second kernel adds those rows in a fixed order: no atomics, the same bits every run.
+// 422 us: instructions were the bound). The weight's and the bias's gradients stay in each thread's registers over
+// all rows of its group; a CTA adds its groups' sums in shared memory, writes one partial row, and a second kernel adds those rows in a fixed order: no atomics, the same bits every run.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -186,6 +188,26 @@ __device__ __forceinline__ void load_param(float2 (&f)[PER / 2], const void* p, 
   }
 }
 
+// Keeps 16-bit parameters packed: what is converted inside the loop must not be moved out of it.
+template <typename P, int PER>
+__device__ __forceinline__ void opaque(P (&f)[PER]) {
+  if constexpr (sizeof(P) == 2) {
+    uint32_t* u = reinterpret_cast<uint32_t*>(f);
+#pragma unroll
+    for (int i = 0; i < PER / 2; ++i) asm volatile("" : "+r"(u[i]));
+  }
+}
+
+// The same in the parameters' own type: half the registers for 16-bit ones.
+template <typename P, int V, int PER>
+__device__ __forceinline__ void keep_param(P (&f)[PER], const void* p, float none, int t, int tpr, int C) {
+#pragma unroll
+  for (int e = 0; e < PER; ++e) {
+    const int c = column<V>(e, t, tpr);
+    DT<P>::store(f + e, p && c < C ? DT<P>::load(static_cast<const P*>(p) + c) : none);
+  }
+}
+
 template <typename T, typename P, int V, int PER, bool WHOLE>
 __global__ void __launch_bounds__(512) layer_norm_fwd_kernel(const NormArgs A) {
   extern __shared__ __align__(16) unsigned char ring[];  // [groups, stages, C]
@@ -196,9 +218,9 @@ __global__ void __launch_bounds__(512) layer_norm_fwd_kernel(const NormArgs A) {
   __syncthreads();
   const int group = threadIdx.x / A.tpr, t = threadIdx.x - group * A.tpr;
   int slot = 0;
-  float2 w[PER / 2], b[PER / 2];
-  load_param<P, V, PER>(w, A.w, 1.f, t, A.tpr, A.C);
-  load_param<P, V, PER>(b, A.b, 0.f, t, A.tpr, A.C);
+  alignas(16) P w[PER], b[PER];
+  keep_param<P, V, PER>(w, A.w, 1.f, t, A.tpr, A.C);
+  keep_param<P, V, PER>(b, A.b, 0.f, t, A.tpr, A.C);
   const long long step = (long long)gridDim.x * A.groups;
   long long row = (long long)blockIdx.x * A.groups + group;
   const T* x = static_cast<const T*>(A.x);
@@ -245,9 +267,11 @@ __global__ void __launch_bounds__(512) layer_norm_fwd_kernel(const NormArgs A) {
     }
     const float var = group_sum(s2.x + s2.y, A.tpr, group, sums, slot) * A.invC;
     const float rstd = ok ? 1.f / sqrtf(var + A.eps) : __int_as_float(0x7fffffff);
+    opaque(w);
+    opaque(b);
     alignas(16) T o[PER];
 #pragma unroll
-    for (int p = 0; p < PER / 2; ++p) put_two<T>(o + 2 * p, ffma2(mul2(f[p], dup(rstd)), w[p], b[p]));
+    for (int p = 0; p < PER / 2; ++p) put_two<T>(o + 2 * p, ffma2(mul2(f[p], dup(rstd)), two<P>(w + 2 * p), two<P>(b + 2 * p)));
     store_row<T, V, PER, WHOLE>(y + row * A.C, o, t, A.tpr, A.C);
     if (t == 0 && A.mean) A.mean[row] = mean, A.rstd[row] = rstd;
   }
