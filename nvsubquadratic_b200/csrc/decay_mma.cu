@@ -15,8 +15,9 @@
 //   o_i = a^(i+e) R_i + (P V)_i
 //   S  <- a^n S + K^T (a^(n-j-e) V_j)
 //
-// All four products accumulate in float32 in TMEM. P and the copy of S that R reads are rounded to bfloat16 (each is
-// one operand of one product: together with the output's own rounding the error is 1.4 times that of one rounding). The state
+// All four products accumulate in float32 in TMEM. P and the copy of S that R reads are operands of bfloat16 products too: of
+// bfloat16 tensors they are kept as two terms (16 bits), so that the one error that shows in an output is its own
+// rounding (one term each made it 1.4 times as large). The state
 // itself is a result in float32, so the decayed V is not rounded: it is split into three bfloat16 terms (24 bits),
 // three products into one accumulator; S lives in registers and takes the chunk's decay as the sum of two floats.
 //
@@ -94,22 +95,26 @@ enum Bar {
 // Bytes of the shared-memory layout for a state of DK (64 or 128) rows, operands of NT terms, a state update from TERMS
 // terms of the decayed V. Tiles start on 1024 bytes, where the swizzle's pattern does.
 constexpr int kTile = kT * 128;
+// Terms of what a pass rounds itself, P and the state's copy: 16 bits at least.
+constexpr int round_terms(int nt) { return nt == 1 ? 2 : nt; }
 template <int DK, bool OUT, int NT, int TERMS>
 struct Layout {
+  static constexpr int RT = round_terms(NT);
   static constexpr bool two = NT == 1 || (NT == 2 && DK == 64);  // CTAs on an SM
   static constexpr int qk = NT * DK / 64 * kTile, vt = NT * kTile;
-  // as many buffers of K and V, of Q and of the decayed V as there is room for
-  static constexpr int nbuf = NT == 1 ? (OUT ? (DK == 64 ? 3 : 2) : (DK == 64 ? 4 : 2))
+  // as many buffers of K and V, of Q and of the decayed V as there is room for (bfloat16 heads of 128 with outputs: one of each
+  // and two CTAs; one CTA with four is slower, 8 heads of 65536 tokens 303 us against 295)
+  static constexpr int nbuf = NT == 1 ? (OUT ? (DK == 64 ? (TERMS == 2 ? 3 : 2) : 1) : (DK == 64 ? 4 : 2))
                                       : (OUT ? (NT == 3 && DK == 64 ? 2 : 1) : (NT == 3 && DK == 64 ? 3 : 2));
-  static constexpr int qbuf = NT == 1 && DK == 64 ? 3 : 1;
+  static constexpr int qbuf = NT == 1 && DK == 64 ? (TERMS == 2 ? 2 : 3) : 1;
   static constexpr int wbuf = OUT || (NT == 2 && DK == 64) ? 1 : 2;
   static constexpr int q = 0;
   static constexpr int k = q + (OUT ? qbuf * qk : 0);
   static constexpr int v = k + nbuf * qk;
   static constexpr int w = v + nbuf * vt;                    // the decayed V
   static constexpr int p = w + wbuf * TERMS * kTile;         // P
-  static constexpr int s = p + (OUT ? NT * kTile : 0);       // the state in NT terms
-  static constexpr int tab = s + (OUT ? NT * DK * 128 : 0);  // a^d for d = -64 .. 64 (zeros below 0)
+  static constexpr int s = p + (OUT ? RT * kTile : 0);       // the state in RT terms
+  static constexpr int tab = s + (OUT ? RT * DK * 128 : 0);  // a^d for d = -64 .. 64 (zeros below 0)
   static constexpr int bar = tab + (2 * kT + 4) * 4;
   static constexpr int bytes = bar + kBars * 8 + 8;
   static_assert((two ? 2 : 1) * (bytes + 1024) <= 228 * 1024 && bytes <= 227 * 1024, "does not fit an SM");
@@ -316,6 +321,7 @@ constexpr int pairs(int na, int nb, int orders) {
 template <int DK, bool OUT, int NT, int TERMS, typename TO>
 __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A, const __grid_constant__ Maps M) {
   using L = Layout<DK, OUT, NT, TERMS>;
+  constexpr int RT = L::RT;
   extern __shared__ __align__(1024) unsigned char smem[];
   float* tab = reinterpret_cast<float*>(smem + L::tab);
   uint64_t* bar = reinterpret_cast<uint64_t*>(smem + L::bar);
@@ -469,22 +475,22 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A, co
         if (i) wait(kReadO, i - 1);
         if (elect()) {
 #pragma unroll
-          for (int y = 0; y < pairs(NT, NT, NT); ++y)
+          for (int y = 0; y < pairs(NT, RT, RT); ++y)
 #pragma unroll
             for (int x = 0; x < DK / 16; ++x)
-              mma(tmem + kColR, dqi + term_a(y, NT, NT, NT) * (L::qk / NT >> 4) + (x >> 2) * kNextTile + (x & 3) * kAlongK,
-                  ds + term_b(y, NT, NT, NT) * (DK * 128 >> 4) + x * kAlongRows, kIdR, x + y > 0);
+              mma(tmem + kColR, dqi + term_a(y, NT, RT, RT) * (L::qk / NT >> 4) + (x >> 2) * kNextTile + (x & 3) * kAlongK,
+                  ds + term_b(y, NT, RT, RT) * (DK * 128 >> 4) + x * kAlongRows, kIdR, x + y > 0);
           umma::commit(&bar[kDoneR + i % L::qbuf]);
         }
         __syncwarp();
         wait(kHaveP, i);
         if (elect()) {
 #pragma unroll
-          for (int y = 0; y < pairs(NT, NT, NT); ++y)
+          for (int y = 0; y < pairs(RT, NT, RT); ++y)
 #pragma unroll
             for (int x = 0; x < kT / 16; ++x)
-              mma(tmem + kColO, dp + term_a(y, NT, NT, NT) * kNextTile + x * kAlongK,
-                  dv + term_b(y, NT, NT, NT) * kNextTile + x * kAlongRows, kIdR, x + y > 0);
+              mma(tmem + kColO, dp + term_a(y, RT, NT, RT) * kNextTile + x * kAlongK,
+                  dv + term_b(y, RT, NT, RT) * kNextTile + x * kAlongRows, kIdR, x + y > 0);
           umma::commit(&bar[kDoneO + nb]);
         }
         __syncwarp();
@@ -576,8 +582,8 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A, co
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           unsigned char* d = smem + L::s + swz(rw, half + 8 * j + pair);
-          put_terms<NT>(d, DK * 128, make_float2(S[y][4 * j], S[y][4 * j + 1]));
-          put_terms<NT>(d + 1024, DK * 128, make_float2(S[y][4 * j + 2], S[y][4 * j + 3]));
+          put_terms<RT>(d, DK * 128, make_float2(S[y][4 * j], S[y][4 * j + 1]));
+          put_terms<RT>(d + 1024, DK * 128, make_float2(S[y][4 * j + 2], S[y][4 * j + 3]));
         }
       }
     };
@@ -657,9 +663,9 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A, co
 #pragma unroll
         for (int j = 0; j < 4; ++j) {  // row + 8 at column block j decays like row at block j - 1
           unsigned char* d = smem + L::p + swz(row, half + 8 * j + pair);
-          put_terms<NT>(d, kTile, make_float2(__uint_as_float(p[4 * j]) * decay(2 * j + 2),
+          put_terms<RT>(d, kTile, make_float2(__uint_as_float(p[4 * j]) * decay(2 * j + 2),
                                               __uint_as_float(p[4 * j + 1]) * decay(2 * j + 3)));
-          put_terms<NT>(d + 1024, kTile, make_float2(__uint_as_float(p[4 * j + 2]) * decay(2 * j),
+          put_terms<RT>(d + 1024, kTile, make_float2(__uint_as_float(p[4 * j + 2]) * decay(2 * j),
                                                      __uint_as_float(p[4 * j + 3]) * decay(2 * j + 1)));
         }
         hand_over(&bar[kHaveP]);
@@ -747,8 +753,8 @@ int launch(const ScanArgs& A, const Maps& M, long long ctas, cudaStream_t st) {
 template <int DK, int NT, typename T>
 int launch_dk(const ScanArgs& A, const Maps& M, bool out_f32, long long ctas, cudaStream_t st) {
   if (!A.o) return launch<DK, false, NT, 3, T>(A, M, ctas, st);
-  // where segments were added up before, the state only serves this pass's outputs: those of bfloat16 read it rounded
-  // to 8 bits, and 16 are enough (not by whether the caller wants the final state, so that asking for it changes no output)
+  // where segments were added up before, the state only serves this pass's outputs: those of bfloat16 read it in 16 bits,
+  // and as many of the decayed V are enough (not by whether the caller wants the final state, so that asking for it changes no output)
   if (NT == 1 && A.nseg > 1)
     return out_f32 ? launch<DK, true, NT, NT == 1 ? 2 : 3, float>(A, M, ctas, st)
                    : launch<DK, true, NT, NT == 1 ? 2 : 3, T>(A, M, ctas, st);

@@ -420,3 +420,27 @@ def test_steps_follow_the_sequence():
     for t in range(60, L):
         got.append(decay_attention_step(q[:, t], k[:, t], v[:, t], g, s).unsqueeze(1))
     assert rel_l2(want, torch.cat(got, 1)) <= 2 * TOL[F32] and rel_l2(ws, s) <= 2 * TOL[F32]
+
+
+# ---------------------------------------------------------------- one rounding
+
+# A bfloat16 value m 2^e, 1 <= m < 2, is off by a uniform error of spacing 2^(e-7): rms 2^(e-7) / sqrt(12), so a tensor that is
+# rounded to nearest once is off by at most 2^-7 / sqrt(12) of its norm. What the scan itself rounds, it keeps in 16 bits
+# (2^-17 of an operand); four times that is allowed beside.
+ONE_ROUNDING = 2.0 ** -7 / 12 ** 0.5 + 2.0 ** -15
+
+# uncut rows, cut ones, head sizes of both widths, shared heads
+ROUNDED = [(40, 200, 4, 4, 64, 64), (40, 200, 4, 2, 128, 128), (2, 1500, 2, 1, 64, 64), (1, 1500, 2, 2, 128, 128),
+           (1, 700, 2, 2, 96, 40)]
+
+
+@gpu
+@pytest.mark.parametrize("shape", ROUNDED, ids=str)
+def test_bfloat16_results_are_rounded_once(shape):
+    args = _inputs(*shape, BF16)
+    o, _, grads = _run(*args, learn=False)
+    q, k, v, g, s0, do, ds = args
+    errs = {"o": rel_l2(oracle_forward(q, k, v, g, initial_state=s0)[0], o)}
+    ref = decay_attention_grads(q, k, v, g, do, ds, initial_state=s0)
+    errs.update({n: rel_l2(r, x) for n, r, x in zip(("dq", "dk", "dv"), ref, grads)})
+    assert all(e <= ONE_ROUNDING for e in errs.values()), errs
