@@ -22,6 +22,7 @@ HYFFT_ERR_INVALID = 1
 HYFFT_ERR_UNSUPPORTED = 2
 HYFFT_ERR_WORKSPACE = 3
 HYFFT_ERR_CUDA = 4
+HYFFT_ERR_WAIT = 5
 
 F32, BF16, F16 = 0, 1, 2
 LAYOUT_BHL, LAYOUT_BLH = 0, 1
@@ -156,6 +157,8 @@ SIGNATURES = {
     "hyfft_last_error": [],
     "hyfft_version": [],
     "hyfft_launch_count": [],
+    "hyfft_wait_status": [_i32, _i32],
+    "hyfft_set_wait_clocks": [ctypes.c_longlong],
 }
 _STR_FUNCS = {"hyfft_last_error", "hyfft_version"}
 
@@ -187,6 +190,7 @@ def load() -> ctypes.CDLL:
             fn.argtypes = args
             fn.restype = ctypes.c_char_p if name in _STR_FUNCS else ctypes.c_int
         lib.hyfft_launch_count.restype = ctypes.c_longlong
+        lib.hyfft_set_wait_clocks.restype = ctypes.c_longlong
         _lib = lib
         return lib
 
@@ -241,6 +245,13 @@ def ptr(t: torch.Tensor | None) -> int | None:
 
 def workspace(nbytes: int, device: torch.device) -> torch.Tensor:
     return torch.empty(max(int(nbytes), 1), dtype=torch.uint8, device=device)
+
+
+def check_waits(device: torch.device | int = 0, clear: bool = True) -> None:
+    """Waits for the device and raises ``HyfftError`` if a wait inside one of its kernels has run out since the last
+    such check (the results of that call hold NaN)."""
+    index = device if isinstance(device, int) else torch.device(device).index or 0
+    check(load().hyfft_wait_status(index, int(clear)), "hyfft_wait_status")
 
 
 def launch_count() -> int:

@@ -32,6 +32,7 @@ struct ScanArgs {
   int reverse;  // the decay is applied after a token's output instead of before
   int vec;      // q, k, v (and x) can be read in 16-byte pieces
   int ovec;     // o can be written in 16-byte pieces
+  unsigned patience;   // clocks after which a wait inside the kernel gives up
 };
 
 // decay_mma.cu: DK <= 128, columns in slices of 64, segments of whole 64-token chunks. float16 and float32 operands are
@@ -40,8 +41,9 @@ struct ScanArgs {
 constexpr int kMmaTok = 64;
 constexpr int kMmaCols = 64;
 constexpr int kMmaMaxDK = 128;
-int launch_scan_mma(const ScanArgs& A, int dtype, bool out_f32, long long ctas, cudaStream_t st);
+int launch_scan_mma(ScanArgs A, int dtype, bool out_f32, long long ctas, cudaStream_t st);
 size_t mma_terms_bytes(int B, long long L, int heads, int D, int terms);
+int decay_wait_status(bool clear, unsigned* ran_out);
 int launch_split_terms(ScanOp* ops, const int* heads, const int* D, int n, int B, long long L, int dtype, int terms, char* ws,
                        cudaStream_t st);
 

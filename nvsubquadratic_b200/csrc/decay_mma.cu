@@ -50,6 +50,7 @@
 #include "common.cuh"
 #include "decay_attn.h"
 #include "umma.cuh"
+#include "waits.cuh"
 
 namespace hyfft {
 
@@ -67,10 +68,13 @@ constexpr int kWriter = kIssuer + 1, kWriters = 4;
 constexpr int kAll = 32 * (kWriter + kWriters);
 // Registers of a thread: computing, loading and issuing, writing; together those of the launch (64 for each of 512). Chosen
 // so that nothing spills: with the shared memory that is taken here a spilled register comes back from L2.
+// Where all warps have something to run at the end, they take the launch's 64 again: after a barrier, since a warp that
+// did so before the computing warps have got their registers would leave them waiting forever.
 template <int DK, bool OUT>
 struct Regs {
   static constexpr int compute = DK == 64 && OUT ? 72 : 80, load = DK == 64 && OUT ? 56 : 48, write = load;
-  static_assert(kThreads * compute + 128 * load + 128 * write <= 64 * kAll, "setmaxnreg would wait forever");
+  static constexpr int launch = 64;
+  static_assert(kThreads * compute + 128 * load + 128 * write <= launch * kAll, "setmaxnreg would wait forever");
 };
 constexpr int kColP = 0, kColR = 64, kColO = 128, kColS = 192, kTmemCols = 256;  // kColS - 64: a second one without outputs
 
@@ -89,8 +93,12 @@ enum Bar {
   kHaveS = 21,   // the rounded state is in place, the accumulator of buffer 0, 1 free
   kHaveP = 23,   // P is in place (and its accumulator free)
   kReadO = 24,   // R and P V have been read, by the writing warps
-  kBars = 25
+  kDrain = 25,   // all products are over; after a wait that ran out
+  kBars = 26
 };
+// Words behind the barriers: the TMEM address, whether a wait has run out (or the tiles lie off the swizzle's pattern), and the
+// last chunk that each loading warp brought (two of K and V, one of Q; -1: none).
+enum Word { kTmem = 0, kFailed = 1, kLast = 2, kWords = 6 };
 
 // Bytes of the shared-memory layout for a state of DK (64 or 128) rows, operands of NT terms, a state update from TERMS
 // terms of the decayed V. Tiles start on 1024 bytes, where the swizzle's pattern does.
@@ -116,7 +124,7 @@ struct Layout {
   static constexpr int s = p + (OUT ? RT * kTile : 0);       // the state in RT terms
   static constexpr int tab = s + (OUT ? RT * DK * 128 : 0);  // a^d for d = -64 .. 64 (zeros below 0)
   static constexpr int bar = tab + (2 * kT + 4) * 4;
-  static constexpr int bytes = bar + kBars * 8 + 8;
+  static constexpr int bytes = bar + kBars * 8 + kWords * 4;
   static_assert((two ? 2 : 1) * (bytes + 1024) <= 228 * 1024 && bytes <= 227 * 1024, "does not fit an SM");
 };
 // Byte of column c (even) of a row in a swizzled tile of 64 columns.
@@ -151,25 +159,6 @@ __device__ __forceinline__ void hand_over(uint64_t* bar) {
   umma::fence_before_sync();
   __syncwarp();
   if ((threadIdx.x & 31) == 0) arrive(bar);
-}
-// Waits for the phase; gives up after about a second and returns false. No time hint: with one, try_wait becomes a loop of
-// short sleeps (128 x 128 grid training: 71 us a pass with outputs, without the hint 69).
-__device__ __forceinline__ bool try_phase(uint32_t bar, uint32_t parity) {
-  uint32_t done;
-  asm volatile(
-      "{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n"
-      : "=r"(done)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  return done != 0;
-}
-__device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity) {
-  const uint32_t a = umma::su32(bar);
-  if (try_phase(a, parity)) return true;
-  const long long t0 = clock64();
-  while (!try_phase(a, parity))
-    if (clock64() - t0 > (1ll << 31)) return false;
-  return true;
 }
 __device__ __forceinline__ bool elect() {
   uint32_t p;
@@ -317,6 +306,27 @@ constexpr int pairs(int na, int nb, int orders) {
   return n;
 }
 
+// What a CTA works on.
+struct Place {
+  int slice, seg, h, n;      // n: tokens that count
+  long long bh, b, lo, hi, end;  // tokens of the segment: lo .. end, up to hi they count
+  __device__ __forceinline__ Place(const ScanArgs& A, unsigned cta) {
+    long long id = cta;
+    slice = (int)(id % A.nslice);
+    id /= A.nslice;
+    seg = (int)(id % A.nseg);
+    bh = id / A.nseg;
+    h = (int)(bh % A.H);
+    b = bh / A.H;
+    int len = A.L;
+    if (A.lengths) len = min(max(A.lengths[b], 0), A.L);
+    lo = (long long)seg * A.seglen;
+    end = min(lo + A.seglen, (long long)A.L);
+    hi = min(end, (long long)len);
+    n = hi > lo ? (int)(hi - lo) : 0;
+  }
+};
+
 // OUT: the pass with outputs; without it, segments' sums alone (K and V only).
 template <int DK, bool OUT, int NT, int TERMS, typename TO>
 __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A, const __grid_constant__ Maps M) {
@@ -325,45 +335,47 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A, co
   extern __shared__ __align__(1024) unsigned char smem[];
   float* tab = reinterpret_cast<float*>(smem + L::tab);
   uint64_t* bar = reinterpret_cast<uint64_t*>(smem + L::bar);
-  uint32_t* tslot = reinterpret_cast<uint32_t*>(smem + L::bar + kBars * 8);
+  volatile int* word = reinterpret_cast<volatile int*>(smem + L::bar + kBars * 8);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
-  long long id = blockIdx.x;
-  const int slice = (int)(id % A.nslice);
-  id /= A.nslice;
-  const int seg = (int)(id % A.nseg);
-  const long long bh = id / A.nseg;
-  const int h = (int)(bh % A.H);
-  const long long b = bh / A.H;
-  const int c0 = slice * kC;
-
-  int len = A.L;
-  if (A.lengths) len = min(max(A.lengths[b], 0), A.L);
-  const long long t_lo = (long long)seg * A.seglen;
-  const long long t_end = min(t_lo + A.seglen, (long long)A.L);
-  const long long t_hi = min(t_end, (long long)len);
-  const int n_all = t_hi > t_lo ? (int)(t_hi - t_lo) : 0;
+  const Place at(A, blockIdx.x);
+  const int h = at.h, c0 = at.slice * kC, seg = at.seg, n_all = at.n;
+  const long long b = at.b, bh = at.bh, t_lo = at.lo, t_hi = at.hi, t_end = at.end;
   const int chunks = (n_all + kT - 1) / kT;
   const bool rev = A.reverse;
   const auto tokens = [&](int i) { return min(kT, n_all - i * kT); };  // of chunk i, and the first of them in time
   const auto first = [&](int i) { return rev ? t_hi - i * kT - tokens(i) : t_lo + i * kT; };
 
-  if (warp == 0) umma::tmem_alloc(tslot, kTmemCols);
+  if (warp == 0) umma::tmem_alloc(reinterpret_cast<uint32_t*>(smem + L::bar + kBars * 8), kTmemCols);
   if (tid == 0) {
     for (int i = 0; i < kBars; ++i)
-      umma::mbar_init(&bar[i], i < kHaveV ? 1 : i == kReadO ? kWriters : kThreads / 32);
+      umma::mbar_init(&bar[i], i < kHaveV || i == kDrain ? 1 : i == kReadO ? kWriters : kThreads / 32);
     umma::fence_mbar_init();
+    word[kFailed] = (umma::su32(smem) & 1023) != 0;
+    for (int i = kLast; i < kWords; ++i) word[i] = -1;
   }
   umma::fence_before_sync();
   __syncthreads();
   umma::fence_after_sync();
-  const uint32_t tmem = *tslot;
-  // false once a wait has run out (or if the tiles lay off the swizzle's pattern): no more waits, and NaN in what is written
-  bool ok = (umma::su32(smem) & 1023) == 0;
+  const uint32_t tmem = (uint32_t)word[kTmem];
+  // False once a wait of this thread has run out: no more waits. A loading or issuing warp then copies nothing and issues no
+  // product any more, the others go on over what there is; warps that wait for it run out themselves. What is in flight is
+  // waited for at the end, and all results of the CTA become NaN there.
+  bool ok = !word[kFailed];
   const auto wait = [&](int i, int phase) {
-    ok = ok && wait_phase(&bar[i], phase & 1);
+    ok = ok && wait_phase(&bar[i], phase & 1, A.patience);
     umma::fence_after_sync();
   };
+  // The same for the loading warps. Where they have one buffer a chunk's loads begin when the last chunk's products end, and
+  // being woken takes longer than seeing it (8 heads of 128, 65536 tokens: 309 us, 295; with more buffers 382, 391).
+  const auto wait_free = [&](int i, int phase) {
+    if (L::nbuf > 1) return wait(i, phase);
+    const uint32_t a = umma::su32(&bar[i]);
+    const unsigned t0 = (unsigned)clock64();
+    while (ok && !test_phase(a, phase & 1)) ok = (unsigned)clock64() - t0 < A.patience;
+    umma::fence_after_sync();
+  };
+  const auto stopped = [&] { return __any_sync(0xffffffffu, !ok) != 0; };  // the same for the whole warp
 
   const float g = A.log_decay[h];
   // a^d, d = -64 .. 64, by the computing and writing warps for themselves
@@ -376,6 +388,7 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A, co
   }
   if (warp >= kLoader && warp < kIssuer) {
     const int who = warp - kLoader;
+    int last = -1;  // chunk brought
     if (who < 2) {
       const int hk = h / A.k.group, hv = h / A.v.group;
       const bf16* kp = static_cast<const bf16*>(A.k.p) + b * A.k.sb + hk * A.k.sh;
@@ -386,9 +399,10 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A, co
       for (int i = who < kTurns ? who : chunks; i < chunks; i += kTurns) {
         const int nb = i % L::nbuf;
         unsigned char *kd = smem + L::k + nb * L::qk, *vd = smem + L::v + nb * L::vt;
-        if (i >= L::nbuf) wait((OUT ? kDoneO : kDoneS) + nb, i / L::nbuf - 1);
+        if (i >= L::nbuf) wait_free((OUT ? kDoneO : kDoneS) + nb, i / L::nbuf - 1);
         if (M.on && tokens(i) == kT) {
-          if (lane == 0) {
+          if (lane == 0 && ok) {
+            last = i;
             expect(&bar[kFull + nb], L::qk + L::vt);
 #pragma unroll
             for (int y = 0; y < NT; ++y) {
@@ -397,7 +411,8 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A, co
             }
           }
           __syncwarp();
-        } else {
+        } else if (!stopped()) {
+          last = i;
 #pragma unroll
           for (int y = 0; y < NT; ++y) {
             load_tile<DK>(kd + y * L::qk / NT, kp + y * A.k.st, A.k.sl, tokens(i), 0, A.DK, first(i), A.vec);
@@ -413,16 +428,18 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A, co
       for (int i = 0; i < chunks; ++i) {
         const int qb = i % L::qbuf;
         unsigned char* qd = smem + L::q + qb * L::qk;
-        if (i >= L::qbuf) wait(kDoneR + qb, i / L::qbuf - 1);
+        if (i >= L::qbuf) wait_free(kDoneR + qb, i / L::qbuf - 1);
         if (M.on && tokens(i) == kT) {
-          if (lane == 0) {
+          if (lane == 0 && ok) {
+            last = i;
             expect(&bar[kFullQ + qb], L::qk);
 #pragma unroll
             for (int y = 0; y < NT; ++y)
               load_box<DK>(umma::su32(qd + y * L::qk / NT), &M.q, &bar[kFullQ + qb], 0, hq, (int)first(i), (int)b + y * A.B);
           }
           __syncwarp();
-        } else {
+        } else if (!stopped()) {
+          last = i;
 #pragma unroll
           for (int y = 0; y < NT; ++y)
             load_tile<DK>(qd + y * L::qk / NT, qp + y * A.q.st, A.q.sl, tokens(i), 0, A.DK, first(i), A.vec);
@@ -431,6 +448,7 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A, co
         }
       }
     }
+    if (lane == 0) word[kLast + who] = last;
   } else if (warp == kIssuer) {
     // every descriptor is one of these plus a constant: built anew for each product, they held the issue up
     const uint32_t dq = desc_low(smem + L::q), dw = desc_low(smem + L::w), dp = desc_low(smem + L::p), ds = desc_low(smem + L::s);
@@ -439,13 +457,14 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A, co
     constexpr uint32_t kIdR = umma::idesc_bf16(kT, kC, 0, 1);
     constexpr uint32_t kIdS = umma::idesc_bf16(DK, kC, 1, 1);
     for (int i = 0; i < chunks; ++i) {
+      if (stopped()) break;
       const int nb = i % L::nbuf, wb = i % L::wbuf;
       const uint32_t dk = dk0 + nb * (L::qk >> 4), dv = dv0 + nb * (L::vt >> 4);
       wait(kFull + nb, i / L::nbuf);
       if (OUT) {
         const uint32_t dqi = dq + i % L::qbuf * (L::qk >> 4);
         wait(kFullQ + i % L::qbuf, i / L::qbuf);
-        if (elect()) {
+        if (elect() && ok) {
 #pragma unroll
           for (int y = 0; y < pairs(NT, NT, NT); ++y)
 #pragma unroll
@@ -460,7 +479,7 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A, co
       }
       wait(kHaveS + wb, i / L::wbuf);
       wait(kHaveV + wb, i / L::wbuf);
-      if (elect()) {
+      if (elect() && ok) {
 #pragma unroll
         for (int y = 0; y < pairs(NT, TERMS, TERMS); ++y)
 #pragma unroll
@@ -473,7 +492,7 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A, co
       if (OUT) {
         const uint32_t dqi = dq + i % L::qbuf * (L::qk >> 4);
         if (i) wait(kReadO, i - 1);
-        if (elect()) {
+        if (elect() && ok) {
 #pragma unroll
           for (int y = 0; y < pairs(NT, RT, RT); ++y)
 #pragma unroll
@@ -484,7 +503,7 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A, co
         }
         __syncwarp();
         wait(kHaveP, i);
-        if (elect()) {
+        if (elect() && ok) {
 #pragma unroll
           for (int y = 0; y < pairs(RT, NT, RT); ++y)
 #pragma unroll
@@ -506,7 +525,7 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A, co
       for (int i = 0; i < chunks; ++i) {
         const int n = tokens(i);
         wait(kDoneO + i % L::nbuf, i / L::nbuf);
-        const float os = ok ? A.vscale * A.oscale : __int_as_float(0x7fffffff);
+        const float os = A.vscale * A.oscale;
 #pragma unroll
         for (int half = 0; half < kC; half += 32) {
           uint32_t r[16], o[16];
@@ -700,11 +719,51 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A, co
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int c = 8 * (r >> 2) + (r & 1), rw = srow + 16 * y + 8 * ((r >> 1) & 1);
-          if (rw < A.DK && c < left) dst[rw * sr + (c0 + half + pair + c) * sc] = ok ? S[y][r] : __int_as_float(0x7fffffff);
+          if (rw < A.DK && c < left) dst[rw * sr + (c0 + half + pair + c) * sc] = S[y][r];
         }
   }
+  if (!ok) word[kFailed] = 1;
   umma::fence_before_sync();
   __syncthreads();
+  if (word[kFailed]) {
+    if (warp < kLoader)
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Regs<DK, OUT>::launch));
+    else
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Regs<DK, OUT>::launch));
+    // products and copies in flight end by themselves; shared memory and TMEM are given back after them
+    if (warp == kIssuer) {
+      if (elect()) umma::commit(&bar[kDrain]);
+      wait_phase(&bar[kDrain], 0, kWaitClocks);
+    } else if (warp == kLoader && lane < L::nbuf) {
+      constexpr int kTurns = L::nbuf == 1 ? 1 : 2;
+      const int i = max(word[kLast], word[kLast + 1]) - lane;  // the last chunk of one of the buffers
+      if (i >= 0 && i <= word[kLast + i % kTurns]) wait_phase(&bar[kFull + i % L::nbuf], i / L::nbuf & 1, kWaitClocks);
+    } else if (OUT && warp == kLoader + 2 && lane < L::qbuf) {
+      const int i = word[kLast + 2] - lane;
+      if (i >= 0) wait_phase(&bar[kFullQ + i % L::qbuf], i / L::qbuf & 1, kWaitClocks);
+    }
+    umma::fence_before_sync();
+    __syncthreads();
+    // asked anew: kept in registers all along, the place cost the loops some of theirs
+    unsigned cta;
+    asm volatile("mov.u32 %0, %%ctaid.x;" : "=r"(cta));
+    const Place z(A, cta);
+    const int col = z.slice * kC, DV = A.DV;
+    const float nan = __int_as_float(0x7fffffff);
+    if (OUT)
+      for (long long i = threadIdx.x; i < (long long)z.n * kC; i += kAll) {
+        const int c = col + (int)(i % kC);
+        if (c < DV) DT<TO>::store(static_cast<TO*>(A.o) + z.b * A.ob + (long long)z.h * A.oh + (z.lo + i / kC) * A.ol + c, nan);
+      }
+    float* dst = !OUT ? A.seg + (z.bh * A.nseg + z.seg) * A.DK * DV
+                      : A.nseg == 1 && A.finish ? A.finish + z.bh * A.DK * DV : nullptr;
+    if (dst)
+      for (int i = threadIdx.x; i < A.DK * kC; i += kAll) {
+        const int c = col + i % kC;
+        if (c < DV) dst[(long long)(i / kC) * (OUT ? A.srow : DV) + (long long)c * (OUT ? A.scol : 1)] = nan;
+      }
+    if (threadIdx.x == 0) atomicExch(&g_ran_out, 1u);
+  }
   if (warp == 0) umma::tmem_dealloc(tmem, kTmemCols);
 }
 
@@ -841,10 +900,13 @@ int launch_split_terms(ScanOp* ops, const int* heads, const int* D, int n, int B
   return HYFFT_OK;
 }
 
-int launch_scan_mma(const ScanArgs& A, int dtype, bool out_f32, long long ctas, cudaStream_t st) {
+int decay_wait_status(bool clear, unsigned* ran_out) { return read_ran_out(clear, ran_out) == cudaSuccess ? HYFFT_OK : HYFFT_ERR_CUDA; }
+
+int launch_scan_mma(ScanArgs A, int dtype, bool out_f32, long long ctas, cudaStream_t st) {
   if (ctas > 0x7fffffffLL) return set_error(HYFFT_ERR_UNSUPPORTED, "decay attention: too many rows");
   const int nt = dtype == HYFFT_BF16 ? 1 : dtype == HYFFT_F16 ? 2 : 3;
   Maps M{};
+  A.patience = g_wait_clocks.load(std::memory_order_relaxed);
   M.on = A.L >= kT && A.vec && make_map(&M.k, A.k, A.DK, A.H / A.k.group, A.L, A.B * nt) &&
          make_map(&M.v, A.v, A.DV, A.H / A.v.group, A.L, A.B * nt) &&
          (!A.o || make_map(&M.q, A.q, A.DK, A.H / A.q.group, A.L, A.B * nt));

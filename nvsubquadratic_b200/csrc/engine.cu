@@ -53,6 +53,8 @@ static int fail(int code, const char* fmt, ...) {
 int set_error(int code, const char* msg) { return fail(code, "%s", msg); }
 
 std::atomic<long long> g_launches{0};
+std::atomic<unsigned> g_wait_clocks{1u << 31};  // kWaitClocks of waits.cuh
+int decay_wait_status(bool clear, unsigned* ran_out);  // decay_mma.cu
 
 static int check_launch(const char* what) {
   cudaError_t e = cudaGetLastError();
@@ -1230,6 +1232,24 @@ extern "C" {
 
 const char* hyfft_last_error(void) { return g_last_error.c_str(); }
 const char* hyfft_version(void) { return "hyfft 0.1 (sm_100a)"; }
+long long hyfft_set_wait_clocks(long long clocks) {
+  return clocks < 0 ? g_wait_clocks.load() : g_wait_clocks.exchange((unsigned)std::min(clocks, 1ll << 31));
+}
+
+int hyfft_wait_status(int32_t device, int32_t clear) {
+  int cur = -1;
+  if (cudaGetDevice(&cur) != cudaSuccess || cudaSetDevice(device) != cudaSuccess) {
+    cudaGetLastError();
+    return fail(HYFFT_ERR_CUDA, "wait status: device %d", (int)device);
+  }
+  unsigned scan = 0;
+  const bool read = cudaDeviceSynchronize() == cudaSuccess && decay_wait_status(clear != 0, &scan) == HYFFT_OK;
+  cudaSetDevice(cur);
+  if (!read) return fail(HYFFT_ERR_CUDA, "wait status: %s", cudaGetErrorString(cudaGetLastError()));
+  if (scan) return fail(HYFFT_ERR_WAIT, "a wait inside a kernel ran out: decayed linear attention left NaN in its results");
+  return HYFFT_OK;
+}
+
 long long hyfft_launch_count(void) { return g_launches.load(std::memory_order_relaxed); }
 
 int hyfft_conv_workspace_size(const hyfft_conv_desc* d, size_t* fwd_bytes, size_t* bwd_bytes) {

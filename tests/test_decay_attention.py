@@ -444,3 +444,46 @@ def test_bfloat16_results_are_rounded_once(shape):
     ref = decay_attention_grads(q, k, v, g, do, ds, initial_state=s0)
     errs.update({n: rel_l2(r, x) for n, r, x in zip(("dq", "dk", "dv"), ref, grads)})
     assert all(e <= ONE_ROUNDING for e in errs.values()), errs
+
+
+# ---------------------------------------------------------------- waits that run out
+
+
+def test_wait_limit_is_kept():
+    from nvsubquadratic_b200 import _lib
+
+    lib = _lib.load()
+    before = lib.hyfft_set_wait_clocks(1000)
+    assert lib.hyfft_set_wait_clocks(-1) == 1000 and lib.hyfft_set_wait_clocks(before) == 1000
+    assert lib.hyfft_set_wait_clocks(-1) == before == 1 << 31
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("shape", [(2, 700, 4, 2, 64, 64), (2, 700, 2, 2, 128, 128), (40, 300, 4, 4, 64, 64), (1, 300, 2, 2, 65, 33)],
+                         ids=str)
+def test_waits_that_run_out_leave_nan_and_a_status(shape, dtype):
+    """With no patience at all some wait inside the tensor-core scan runs out: every value is the right one or NaN, the host
+    can tell, and the next call is as ever."""
+    from nvsubquadratic_b200 import _lib
+
+    args = _inputs(*shape, dtype)
+    want = _run(*args)
+    _lib.check_waits(0)
+    lib = _lib.load()
+    before = lib.hyfft_set_wait_clocks(0)
+    try:
+        got = _run(*args)
+        torch.cuda.synchronize()
+    finally:
+        lib.hyfft_set_wait_clocks(before)
+    with pytest.raises(_lib.HyfftError, match="ran out"):
+        _lib.check_waits(0)
+    _lib.check_waits(0)  # it was cleared
+    for a, b in zip((want[0], want[1], *want[2]), (got[0], got[1], *got[2])):
+        assert ((a == b) | b.isnan()).all()
+    assert got[0].isnan().any()
+    again = _run(*args)
+    for a, b in zip((want[0], want[1], *want[2]), (again[0], again[1], *again[2])):
+        assert torch.equal(a, b)
+    _lib.check_waits(0)
