@@ -299,6 +299,8 @@ HYFFT_API int hyfft_siren_backward(const hyfft_siren_desc* d, const float* coord
  * neither read nor counted, their outputs and gradients are zero (values outside 0 .. L are clamped).
  * States: float32 contiguous [B, H, Dk, Dv]; initial_state NULL means zero. o and the gradients are
  * contiguous and overwritten; sums are float32, each output rounded once.
+ * An infinity or a NaN reaches what the recurrence lets it reach (no earlier token, no other head); what it reaches is
+ * computed token by token and takes longer.
  * Dk, Dv <= 256 (HYFFT_ERR_UNSUPPORTED above). No counterpart in the reference.               */
 typedef struct hyfft_decay_desc {
   int32_t batch, heads, kv_heads, dk, dv;

@@ -134,7 +134,8 @@ __global__ void __launch_bounds__(32 * KW) decay_scan_kernel(const ScanArgs A) {
   }
   const float a1 = expf(g);
   const double ac = exp((double)g * kTok);
-  const float achi = (float)ac, aclo = (float)(ac - (double)achi);
+  float achi, aclo;
+  two_floats(ac, &achi, &aclo);
 
   // rows row0 + 2 p, row0 + 2 p + 1 of column col + c; D: the same of T
   float2 S[RH / 2][4], D[LEARN ? RH / 2 : 1][4];
@@ -294,9 +295,7 @@ __global__ void __launch_bounds__(32 * KW) decay_scan_kernel(const ScanArgs A) {
     if (fast) {
       float hi = achi, lo = aclo;
       if (n != kTok) {
-        const double an = exp((double)g * n);
-        hi = (float)an;
-        lo = (float)(an - (double)hi);
+        two_floats(exp((double)g * n), &hi, &lo);
       }
 #pragma unroll
       for (int p = 0; p < RH / 2; ++p)
@@ -363,7 +362,9 @@ __global__ void __launch_bounds__(256) decay_chain_kernel(float* seg, float* seg
   const float g = log_decay[bh % H];
   int len = L;
   if (lengths) len = min(max(lengths[bh / H], 0), L);
-  const double af = exp((double)g * seglen);
+  // a power that is too small even for a double is not zero all the same: an infinite state stays infinite
+  const double least = g > -INFINITY ? 1e-300 : 0.0;
+  const double af = fmax(exp((double)g * seglen), least);
   float s = start ? start[bh * per + (long long)r * srow + (long long)c * scol] : 0.f, t = 0.f;
   for (int i0 = 0; i0 < nseg; i0 += kChainLoads) {  // loads of several segments in flight
     float add[kChainLoads], addT[kChainLoads];
@@ -381,7 +382,7 @@ __global__ void __launch_bounds__(256) decay_chain_kernel(float* seg, float* seg
         const int j = reverse ? nseg - 1 - i0 - i : i0 + i;
         const long long at = (bh * nseg + j) * per + e, lo = (long long)j * seglen;
         const long long n = max(0ll, min(lo + seglen, (long long)len) - lo);
-        const double an = n == seglen ? af : n ? exp((double)g * (double)n) : 1.0;
+        const double an = n == seglen ? af : n ? fmax(exp((double)g * (double)n), least) : 1.0;
         seg[at] = s;
         if (segT) {
           segT[at] = t;

@@ -35,6 +35,13 @@ struct ScanArgs {
   unsigned patience;   // clocks after which a wait inside the kernel gives up
 };
 
+// a as the sum of two floats, both of a's sign and neither zero, so that infinity times a is infinity plus infinity.
+__device__ __forceinline__ void two_floats(double a, float* hi, float* lo) {
+  *hi = __double2float_rz(a);
+  *lo = (float)(a - (double)*hi);
+  if (*hi > 0.f) *lo = fmaxf(*lo, 1.1754944e-38f);
+}
+
 // decay_mma.cu: DK <= 128, columns in slices of 64, segments of whole 64-token chunks. float16 and float32 operands are
 // first split into bfloat16 terms (2, 3): launch_split_terms does up to four tensors [B, L, heads[w], D[w]] into `ws` and makes
 // the ops point there.

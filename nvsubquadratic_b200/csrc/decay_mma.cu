@@ -32,6 +32,7 @@
 // over the 128 x 128 grid, 32 rows of 16384 tokens of 64: 134 us with eight warps doing everything, 69 with loads and products
 // issued by others, 58 with the outputs written by others too, Q in several buffers and no register spilled; its traffic
 // at the copy's rate takes 41).
+// A result that is infinite or NaN is computed again at the end, token by token in scan order (scan_by_token).
 // Registers move from the loading to the computing warps. Two CTAs share an SM (<= 113 KB, 256 TMEM columns each).
 //
 // 64-row products lie in 16 of a warp's 32 TMEM lanes, and the 16 x 256-bit load shape spreads those over all 32 threads
@@ -98,7 +99,7 @@ enum Bar {
 };
 // Words behind the barriers: the TMEM address, whether a wait has run out (or the tiles lie off the swizzle's pattern), and the
 // last chunk that each loading warp brought (two of K and V, one of Q; -1: none).
-enum Word { kTmem = 0, kFailed = 1, kLast = 2, kWords = 6 };
+enum Word { kTmem = 0, kFailed = 1, kLast = 2, kOdd = 5, kWords = 6 };  // kOdd: a result is infinite or NaN
 
 // Bytes of the shared-memory layout for a state of DK (64 or 128) rows, operands of NT terms, a state update from TERMS
 // terms of the decayed V. Tiles start on 1024 bytes, where the swizzle's pattern does.
@@ -327,6 +328,79 @@ struct Place {
   }
 };
 
+// The CTA's work once more, strictly token by token, for results that are infinite or NaN. The products above run over
+// all pairs of a chunk's tokens and multiply what is masked by zero, so an infinity or a NaN in one token reaches earlier ones, and
+// a difference of two terms makes a NaN of an infinity. Here neither happens: a value reaches what the recurrence lets it reach.
+// A thread holds DK / 8 rows of one column; slow (about 16 tokens in 2 us), and only such results pay for it.
+template <int DK, bool OUT, int NT, typename TO>
+__device__ __forceinline__ void scan_by_token(const ScanArgs& A, const Place& z, float* sm) {
+  constexpr int kN = 16, kG = kAll / kC, kR = DK / kG;
+  float *qs = sm, *ks = qs + kN * DK, *vs = ks + kN * DK, *red = vs + kN * kC;
+  const int tid = threadIdx.x, col = z.slice * kC, c = tid % kC, grp = tid / kC;
+  const int rows = min(kR, A.DK - grp * kR);
+  float hi, lo;
+  two_floats(exp((double)A.log_decay[z.h]), &hi, &lo);
+  const long long per = (long long)A.DK * A.DV;
+  const float* src = nullptr;
+  long long sr = A.DV, sc = 1;
+  if (OUT && A.nseg > 1)
+    src = A.seg + (z.bh * A.nseg + z.seg) * per, sr = A.segrow, sc = A.segcol;
+  else if (OUT && A.start)
+    src = A.start + z.bh * per, sr = A.srow, sc = A.scol;
+  float S[kR];
+#pragma unroll
+  for (int r = 0; r < kR; ++r) S[r] = src && r < rows && col + c < A.DV ? src[(grp * kR + r) * sr + (col + c) * sc] : 0.f;
+  const auto get = [&](const ScanOp& x, int d, long long t) {
+    const bf16* p = static_cast<const bf16*>(x.p) + z.b * x.sb + (long long)(z.h / x.group) * x.sh + t * x.sl + d;
+    float f = __bfloat162float(p[(NT - 1) * x.st]);
+#pragma unroll
+    for (int y = NT - 2; y >= 0; --y) f += __bfloat162float(p[y * x.st]);
+    return f;
+  };
+  const auto when = [&](int i) { return A.reverse ? z.hi - 1 - i : z.lo + i; };
+  for (int i0 = 0; i0 < z.n; i0 += kN) {
+    const int n = min(kN, z.n - i0);
+    for (int i = tid; i < n * DK; i += kAll) {
+      const int d = i % DK;
+      const bool in = d < A.DK;
+      ks[i] = in ? get(A.k, d, when(i0 + i / DK)) : 0.f;
+      if (OUT) qs[i] = in ? get(A.q, d, when(i0 + i / DK)) : 0.f;
+    }
+    for (int i = tid; i < n * kC; i += kAll)
+      vs[i] = col + i % kC < A.DV ? get(A.v, col + i % kC, when(i0 + i / kC)) * A.vscale : 0.f;
+    __syncthreads();
+    for (int t = 0; t < n; ++t) {
+      const float v = vs[t * kC + c];
+      float o = 0.f;
+#pragma unroll
+      for (int r = 0; r < kR; ++r)
+        if (r < rows) {
+          const int at = t * DK + grp * kR + r;
+          if (!A.reverse) S[r] = fmaf(S[r], hi, S[r] * lo);
+          S[r] = fmaf(ks[at], v, S[r]);
+          if (OUT) o = fmaf(qs[at], S[r], o);
+          if (A.reverse) S[r] = fmaf(S[r], hi, S[r] * lo);
+        }
+      if (OUT) red[(t * kG + grp) * kC + c] = o;
+    }
+    __syncthreads();
+    if (OUT)
+      for (int i = tid; i < n * kC; i += kAll) {
+        const int t = i / kC, d = col + i % kC;
+        float o = 0.f;
+        for (int y = 0; y < kG; ++y) o += red[(t * kG + y) * kC + i % kC];
+        if (d < A.DV)
+          DT<TO>::store(static_cast<TO*>(A.o) + z.b * A.ob + (long long)z.h * A.oh + when(i0 + t) * A.ol + d, o * A.oscale);
+      }
+  }
+  float* dst = !OUT ? A.seg + (z.bh * A.nseg + z.seg) * per : A.nseg == 1 && A.finish ? A.finish + z.bh * per : nullptr;
+  if (dst)
+#pragma unroll
+    for (int r = 0; r < kR; ++r)
+      if (r < rows && col + c < A.DV)
+        dst[(long long)(grp * kR + r) * (OUT ? A.srow : A.DV) + (long long)(col + c) * (OUT ? A.scol : 1)] = S[r];
+}
+
 // OUT: the pass with outputs; without it, segments' sums alone (K and V only).
 template <int DK, bool OUT, int NT, int TERMS, typename TO>
 __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A, const __grid_constant__ Maps M) {
@@ -352,7 +426,8 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A, co
       umma::mbar_init(&bar[i], i < kHaveV || i == kDrain ? 1 : i == kReadO ? kWriters : kThreads / 32);
     umma::fence_mbar_init();
     word[kFailed] = (umma::su32(smem) & 1023) != 0;
-    for (int i = kLast; i < kWords; ++i) word[i] = -1;
+    for (int i = kLast; i < kOdd; ++i) word[i] = -1;
+    word[kOdd] = 0;
   }
   umma::fence_before_sync();
   __syncthreads();
@@ -522,6 +597,7 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A, co
       const int wq = warp & 3, row = wq * 16 + (lane >> 2), quad = lane & 3;
       const uint32_t lanes = tmem + ((uint32_t)(wq * 32) << 16);
       TO* op = static_cast<TO*>(A.o) + b * A.ob + (long long)h * A.oh + c0;
+      float2 odd = make_float2(0.f, 0.f);  // NaN once a result was infinite or NaN
       for (int i = 0; i < chunks; ++i) {
         const int n = tokens(i);
         wait(kDoneO + i % L::nbuf, i / L::nbuf);
@@ -546,6 +622,7 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A, co
               const int at = 4 * j + 2 * y;
               f[j] = make_float2(fmaf(__uint_as_float(r[at]), rs, __uint_as_float(o[at]) * os),
                                  fmaf(__uint_as_float(r[at + 1]), rs, __uint_as_float(o[at + 1]) * os));
+              odd = ffma2(f[j], make_float2(0.f, 0.f), odd);
             }
             if (sizeof(TO) == 2 && A.ovec) {
               // transposed among four lanes: each stores 16 bytes of the row, together 64
@@ -570,6 +647,7 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A, co
           }
         }
       }
+      if (odd.x != 0.f || odd.y != 0.f) word[kOdd] = 1;
       const long long z0 = max(t_lo, t_hi);  // tokens past the length: zeros
       for (long long i = tid - 32 * kWriter; i < (t_end - z0) * kC; i += 32 * kWriters) {
         const long long r = i / kC;
@@ -713,56 +791,64 @@ __global__ void __launch_bounds__(kAll, 2) decay_mma_kernel(const ScanArgs A, co
       dst = A.finish + bh * per_state;
       sr = A.srow, sc = A.scol;
     }
-    if (dst)
+    if (dst) {
+      float odd = 0.f;
 #pragma unroll
       for (int y = 0; y < SB; ++y)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int c = 8 * (r >> 2) + (r & 1), rw = srow + 16 * y + 8 * ((r >> 1) & 1);
+          odd = fmaf(S[y][r], 0.f, odd);
           if (rw < A.DK && c < left) dst[rw * sr + (c0 + half + pair + c) * sc] = S[y][r];
         }
+      if (odd != 0.f) word[kOdd] = 1;
+    }
   }
   if (!ok) word[kFailed] = 1;
   umma::fence_before_sync();
   __syncthreads();
-  if (word[kFailed]) {
+  if (word[kFailed] || word[kOdd]) {
     if (warp < kLoader)
       asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Regs<DK, OUT>::launch));
     else
       asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Regs<DK, OUT>::launch));
-    // products and copies in flight end by themselves; shared memory and TMEM are given back after them
-    if (warp == kIssuer) {
-      if (elect()) umma::commit(&bar[kDrain]);
-      wait_phase(&bar[kDrain], 0, kWaitClocks);
-    } else if (warp == kLoader && lane < L::nbuf) {
-      constexpr int kTurns = L::nbuf == 1 ? 1 : 2;
-      const int i = max(word[kLast], word[kLast + 1]) - lane;  // the last chunk of one of the buffers
-      if (i >= 0 && i <= word[kLast + i % kTurns]) wait_phase(&bar[kFull + i % L::nbuf], i / L::nbuf & 1, kWaitClocks);
-    } else if (OUT && warp == kLoader + 2 && lane < L::qbuf) {
-      const int i = word[kLast + 2] - lane;
-      if (i >= 0) wait_phase(&bar[kFullQ + i % L::qbuf], i / L::qbuf & 1, kWaitClocks);
-    }
-    umma::fence_before_sync();
-    __syncthreads();
     // asked anew: kept in registers all along, the place cost the loops some of theirs
     unsigned cta;
     asm volatile("mov.u32 %0, %%ctaid.x;" : "=r"(cta));
     const Place z(A, cta);
-    const int col = z.slice * kC, DV = A.DV;
-    const float nan = __int_as_float(0x7fffffff);
-    if (OUT)
-      for (long long i = threadIdx.x; i < (long long)z.n * kC; i += kAll) {
-        const int c = col + (int)(i % kC);
-        if (c < DV) DT<TO>::store(static_cast<TO*>(A.o) + z.b * A.ob + (long long)z.h * A.oh + (z.lo + i / kC) * A.ol + c, nan);
+    if (word[kFailed]) {
+      // products and copies in flight end by themselves; shared memory and TMEM are given back after them
+      if (warp == kIssuer) {
+        if (elect()) umma::commit(&bar[kDrain]);
+        wait_phase(&bar[kDrain], 0, kWaitClocks);
+      } else if (warp == kLoader && lane < L::nbuf) {
+        constexpr int kTurns = L::nbuf == 1 ? 1 : 2;
+        const int i = max(word[kLast], word[kLast + 1]) - lane;  // the last chunk of one of the buffers
+        if (i >= 0 && i <= word[kLast + i % kTurns]) wait_phase(&bar[kFull + i % L::nbuf], i / L::nbuf & 1, kWaitClocks);
+      } else if (OUT && warp == kLoader + 2 && lane < L::qbuf) {
+        const int i = word[kLast + 2] - lane;
+        if (i >= 0) wait_phase(&bar[kFullQ + i % L::qbuf], i / L::qbuf & 1, kWaitClocks);
       }
-    float* dst = !OUT ? A.seg + (z.bh * A.nseg + z.seg) * A.DK * DV
-                      : A.nseg == 1 && A.finish ? A.finish + z.bh * A.DK * DV : nullptr;
-    if (dst)
-      for (int i = threadIdx.x; i < A.DK * kC; i += kAll) {
-        const int c = col + i % kC;
-        if (c < DV) dst[(long long)(i / kC) * (OUT ? A.srow : DV) + (long long)c * (OUT ? A.scol : 1)] = nan;
-      }
-    if (threadIdx.x == 0) atomicExch(&g_ran_out, 1u);
+      umma::fence_before_sync();
+      __syncthreads();
+      const int col = z.slice * kC, DV = A.DV;
+      const float nan = __int_as_float(0x7fffffff);
+      if (OUT)
+        for (long long i = threadIdx.x; i < (long long)z.n * kC; i += kAll) {
+          const int c = col + (int)(i % kC);
+          if (c < DV) DT<TO>::store(static_cast<TO*>(A.o) + z.b * A.ob + (long long)z.h * A.oh + (z.lo + i / kC) * A.ol + c, nan);
+        }
+      float* dst = !OUT ? A.seg + (z.bh * A.nseg + z.seg) * A.DK * DV
+                        : A.nseg == 1 && A.finish ? A.finish + z.bh * A.DK * DV : nullptr;
+      if (dst)
+        for (int i = threadIdx.x; i < A.DK * kC; i += kAll) {
+          const int c = col + i % kC;
+          if (c < DV) dst[(long long)(i / kC) * (OUT ? A.srow : DV) + (long long)c * (OUT ? A.scol : 1)] = nan;
+        }
+      if (threadIdx.x == 0) atomicExch(&g_ran_out, 1u);
+    } else {
+      scan_by_token<DK, OUT, NT, TO>(A, z, reinterpret_cast<float*>(smem));
+    }
   }
   if (warp == 0) umma::tmem_dealloc(tmem, kTmemCols);
 }

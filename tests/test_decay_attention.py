@@ -487,3 +487,45 @@ def test_waits_that_run_out_leave_nan_and_a_status(shape, dtype):
     for a, b in zip((want[0], want[1], *want[2]), (again[0], again[1], *again[2])):
         assert torch.equal(a, b)
     _lib.check_waits(0)
+
+
+# ---------------------------------------------------------------- infinities and NaN in live tokens
+
+
+def _same_kinds(name, want, got, tol):
+    """NaN and infinities where float64 has them, and the rest right."""
+    want, got = want.detach().double().cpu(), got.detach().double().cpu()
+    assert torch.equal(want.isnan(), got.isnan()), name
+    odd = want.isinf()
+    assert torch.equal(odd, got.isinf()) and torch.equal(want[odd], got[odd]), name
+    ok = want.isfinite()
+    assert rel_l2(want[ok], got[ok]) <= tol, (name, rel_l2(want[ok], got[ok]))
+
+
+@gpu
+@pytest.mark.parametrize("where", ["q", "k", "v", "do", "state", "dstate"])
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")], ids=["inf", "nan"])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("shape", [(40, 150, 4, 2, 64, 64), (2, 600, 2, 2, 64, 72), (1, 530, 2, 1, 128, 128), (2, 30, 2, 2, 64, 64),
+                                   (1, 90, 2, 2, 136, 20)], ids=str)
+def test_bad_values_reach_what_the_recurrence_lets_them_reach(shape, dtype, bad, where):
+    """One infinity or NaN in one live token: earlier tokens, other heads and other sequences are as if it were not there, and an
+    infinity comes out as one. On either path, with the axis cut or not."""
+    B, L, H, Hk, Dk, Dv = shape
+    args = list(_inputs(*shape, dtype))
+    i = ("q", "k", "v", None, "state", "do", "dstate").index(where)
+    t = args[i].clone()
+    if where in ("state", "dstate"):
+        t[B - 1, 1, 3, 5] = bad
+    else:
+        t[B - 1, L * 2 // 3, -1, 5] = bad
+    args[i] = t
+    o, s, grads = _run(*args, learn=False)
+    q, k, v, g, s0, do, ds = args
+    ro, rs = oracle_forward(q, k, v, g, initial_state=s0)
+    ref = decay_attention_grads(q, k, v, g, do, ds, initial_state=s0)
+    _same_kinds("o", ro, o, TOL[dtype])
+    _same_kinds("state", rs, s, TOL[F32])
+    for n, r, x in zip(("dq", "dk", "dv"), ref, grads):
+        _same_kinds(n, r, x, TOL[dtype])
+    _same_kinds("dstate", ref[4], grads[4], TOL[F32])
