@@ -18,7 +18,8 @@
 // Inside a chunk of 16 tokens the state is kept divided by a^i, which takes the decay out of the inner loop: v is
 // multiplied by a^-i and o by a^i, each from a table, and the chunk's a^n is applied once, as the sum of two floats
 // (a rounded a^n would be off by its rounding error times the number of chunks in a head's memory). Heads that
-// forget more than e^-46 within a chunk, where a^-i would overflow, multiply the state for each token.
+// forget more than e^-46 within a chunk, where a^-i would overflow, multiply the state for each token; so does a CTA whose
+// results came out infinite or NaN, once more from the start, in case only the division by a^i made them so.
 // What of this runs on the tensor cores instead (decay_mma.cu) says use_mma below.
 // Few rows and a long axis: the axis is cut into segments; a first pass adds up each segment from a zero
 // state, a small kernel chains the segments' states, and the second pass starts every segment from its own.
@@ -126,55 +127,20 @@ __global__ void __launch_bounds__(32 * KW) decay_scan_kernel(const ScanArgs A) {
 
   const float g = A.log_decay[h];
   const int lag = A.reverse ? 0 : 1;
-  const bool fast = !(fabs((double)g) * kTok > kFastLimit);
-  if (threadIdx.x < kTok) {
-    const int e = threadIdx.x + lag;
-    apow[threadIdx.x] = fast ? (float)(e ? exp((double)g * e) : 1.0) : 1.f;
-    ainv[threadIdx.x] = (fast ? (float)(e ? exp(-(double)g * e) : 1.0) : 1.f) * A.vscale;
-  }
-  const float a1 = expf(g);
-  const double ac = exp((double)g * kTok);
-  float achi, aclo;
-  two_floats(ac, &achi, &aclo);
+  float a1, a1lo, achi, aclo;
+  two_floats(exp((double)g), &a1, &a1lo);
+  two_floats(exp((double)g * kTok), &achi, &aclo);
 
   // rows row0 + 2 p, row0 + 2 p + 1 of column col + c; D: the same of T
   float2 S[RH / 2][4], D[LEARN ? RH / 2 : 1][4];
-#pragma unroll
-  for (int p = 0; p < RH / 2; ++p)
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      S[p][c] = dup(0.f);
-      if (LEARN) D[LEARN ? p : 0][c] = dup(0.f);
-    }
   const long long per_state = (long long)A.DK * A.DV;
-  if (A.o) {
-    const float* src = nullptr;
-    long long sr = A.DV, sc = 1;
-    if (A.nseg > 1) {
-      src = A.seg + (bh * A.nseg + seg) * per_state;
-      sr = A.segrow, sc = A.segcol;
-    } else if (A.start) {
-      src = A.start + bh * per_state;
-      sr = A.srow, sc = A.scol;
-    }
-    const float* srcT = LEARN && A.nseg > 1 ? A.segT + (bh * A.nseg + seg) * per_state : nullptr;
-#pragma unroll
-    for (int r = 0; r < RH; ++r)
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-        if (row0 + r < A.DK && c < left) {
-          if (src) (&S[r >> 1][c].x)[r & 1] = src[(row0 + r) * sr + (c0 + col + c) * sc];
-          if (LEARN && srcT) (&D[LEARN ? r >> 1 : 0][c].x)[r & 1] = srcT[(long long)(row0 + r) * A.DV + c0 + col + c];
-        }
-  }
-
   const T* qp = static_cast<const T*>(A.q.p) + b * A.q.sb + (long long)(h / A.q.group) * A.q.sh;
   const T* kp = static_cast<const T*>(A.k.p) + b * A.k.sb + (long long)(h / A.k.group) * A.k.sh;
   const T* vp = static_cast<const T*>(A.v.p) + b * A.v.sb + (long long)(h / A.v.group) * A.v.sh;
   const T* xp = LEARN ? static_cast<const T*>(A.x.p) + b * A.x.sb + (long long)(h / A.x.group) * A.x.sh : nullptr;
   TO* op = static_cast<TO*>(A.o) + (A.o ? b * A.ob + (long long)h * A.oh + c0 : 0);
   const int step = A.reverse ? -1 : 1;
-  float dg = 0.f;
+  float dg;
 
   // A chunk's tiles: q [kTok][W], k [kTok][W], v [kTok][kCols], x [kTok][kCols].
   const auto fetch = [&](int i0) {
@@ -186,138 +152,198 @@ __global__ void __launch_bounds__(32 * KW) decay_scan_kernel(const ScanArgs A) {
     fetch_tile<T, kCols>(raw + 2 * kTok * W, vp, A.v.sl, n, c0, A.DV, t0, step);
     if (LEARN && A.o) fetch_tile<T, kCols>(raw + 2 * kTok * W + kTok * kCols, xp, A.x.sl, n, c0, A.DV, t0, step);
   };
-  if (A.vec) {
-    if (n_all > 0) fetch(0);
-    asm volatile("cp.async.commit_group;\n" ::: "memory");
-  }
-  for (int i0 = 0; i0 < n_all; i0 += kTok) {
-    const int n = min(kTok, n_all - i0);
-    const long long t0 = A.reverse ? t_hi - 1 - i0 : t_lo + i0;
-    float* tile = smem + (M::wide ? (i0 / kTok & 1) * M::chunk : 0);
-    __syncthreads();  // the last chunk has been read
-    if (A.vec) {
-      if (i0 + kTok < n_all) fetch(i0 + kTok);
-      asm volatile("cp.async.commit_group;\ncp.async.wait_group 1;\n" ::: "memory");
-      if constexpr (!M::wide) {
-        __syncthreads();
-        const T* raw = reinterpret_cast<const T*>(smem + M::raw) + (i0 / kTok & 1) * M::chunk;
-        if (A.o) widen_tile<T, W>(tile, raw, n);
-        widen_tile<T, W>(tile + kTok * W, raw + kTok * W, n);
-        widen_tile<T, kCols>(tile + 2 * kTok * W, raw + 2 * kTok * W, n);
-        if (LEARN && A.o) widen_tile<T, kCols>(tile + 2 * kTok * W + kTok * kCols, raw + 2 * kTok * W + kTok * kCols, n);
-      }
-    } else {
-      if (A.o) load_tile<T, W>(tile, qp, A.q.sl, n, 0, A.DK, t0, step);
-      load_tile<T, W>(tile + kTok * W, kp, A.k.sl, n, 0, A.DK, t0, step);
-      load_tile<T, kCols>(tile + 2 * kTok * W, vp, A.v.sl, n, c0, A.DV, t0, step);
-      if (LEARN && A.o) load_tile<T, kCols>(tile + 2 * kTok * W + kTok * kCols, xp, A.x.sl, n, c0, A.DV, t0, step);
+  // whether a result was infinite or NaN
+  const auto run = [&](auto divided) {
+    constexpr bool fast = divided;
+    float2 odd = dup(0.f);  // NaN once a result was infinite or NaN
+    dg = 0.f;
+    if (threadIdx.x < kTok) {
+      const int e = threadIdx.x + lag;
+      apow[threadIdx.x] = fast ? (float)(e ? exp((double)g * e) : 1.0) : 1.f;
+      ainv[threadIdx.x] = (fast ? (float)(e ? exp(-(double)g * e) : 1.0) : 1.f) * A.vscale;
     }
-    __syncthreads();
-    const float *qs = tile, *ks = tile + kTok * W, *vs = ks + kTok * W, *xs = vs + kTok * kCols;
-    for (int i = 0; i < n; ++i) {
-      const float4 v4 = *reinterpret_cast<const float4*>(vs + i * kCols + col);
-      const float ai = ainv[i];
-      const float2 vj[4] = {dup(v4.x * ai), dup(v4.y * ai), dup(v4.z * ai), dup(v4.w * ai)};
-      const float4* k4 = reinterpret_cast<const float4*>(ks + i * W + row0);
-      const float4* q4 = reinterpret_cast<const float4*>(qs + i * W + row0);
-      if (!fast && lag) {
 #pragma unroll
-        for (int p = 0; p < RH / 2; ++p)
+    for (int p = 0; p < RH / 2; ++p)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        S[p][c] = dup(0.f);
+        if (LEARN) D[LEARN ? p : 0][c] = dup(0.f);
+      }
+    if (A.o) {
+      const float* src = nullptr;
+      long long sr = A.DV, sc = 1;
+      if (A.nseg > 1) {
+        src = A.seg + (bh * A.nseg + seg) * per_state;
+        sr = A.segrow, sc = A.segcol;
+      } else if (A.start) {
+        src = A.start + bh * per_state;
+        sr = A.srow, sc = A.scol;
+      }
+      const float* srcT = LEARN && A.nseg > 1 ? A.segT + (bh * A.nseg + seg) * per_state : nullptr;
+#pragma unroll
+      for (int r = 0; r < RH; ++r)
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          if (row0 + r < A.DK && c < left) {
+            if (src) (&S[r >> 1][c].x)[r & 1] = src[(row0 + r) * sr + (c0 + col + c) * sc];
+            if (LEARN && srcT) (&D[LEARN ? r >> 1 : 0][c].x)[r & 1] = srcT[(long long)(row0 + r) * A.DV + c0 + col + c];
+          }
+    }
+
+    if (A.vec) {
+      if (n_all > 0) fetch(0);
+      asm volatile("cp.async.commit_group;\n" ::: "memory");
+    }
+    for (int i0 = 0; i0 < n_all; i0 += kTok) {
+      const int n = min(kTok, n_all - i0);
+      const long long t0 = A.reverse ? t_hi - 1 - i0 : t_lo + i0;
+      float* tile = smem + (M::wide ? (i0 / kTok & 1) * M::chunk : 0);
+      __syncthreads();  // the last chunk has been read
+      if (A.vec) {
+        if (i0 + kTok < n_all) fetch(i0 + kTok);
+        asm volatile("cp.async.commit_group;\ncp.async.wait_group 1;\n" ::: "memory");
+        if constexpr (!M::wide) {
+          __syncthreads();
+          const T* raw = reinterpret_cast<const T*>(smem + M::raw) + (i0 / kTok & 1) * M::chunk;
+          if (A.o) widen_tile<T, W>(tile, raw, n);
+          widen_tile<T, W>(tile + kTok * W, raw + kTok * W, n);
+          widen_tile<T, kCols>(tile + 2 * kTok * W, raw + 2 * kTok * W, n);
+          if (LEARN && A.o) widen_tile<T, kCols>(tile + 2 * kTok * W + kTok * kCols, raw + 2 * kTok * W + kTok * kCols, n);
+        }
+      } else {
+        if (A.o) load_tile<T, W>(tile, qp, A.q.sl, n, 0, A.DK, t0, step);
+        load_tile<T, W>(tile + kTok * W, kp, A.k.sl, n, 0, A.DK, t0, step);
+        load_tile<T, kCols>(tile + 2 * kTok * W, vp, A.v.sl, n, c0, A.DV, t0, step);
+        if (LEARN && A.o) load_tile<T, kCols>(tile + 2 * kTok * W + kTok * kCols, xp, A.x.sl, n, c0, A.DV, t0, step);
+      }
+      __syncthreads();
+      const float *qs = tile, *ks = tile + kTok * W, *vs = ks + kTok * W, *xs = vs + kTok * kCols;
+      for (int i = 0; i < n; ++i) {
+        const float4 v4 = *reinterpret_cast<const float4*>(vs + i * kCols + col);
+        const float ai = ainv[i];
+        const float2 vj[4] = {dup(v4.x * ai), dup(v4.y * ai), dup(v4.z * ai), dup(v4.w * ai)};
+        const float4* k4 = reinterpret_cast<const float4*>(ks + i * W + row0);
+        const float4* q4 = reinterpret_cast<const float4*>(qs + i * W + row0);
+        if (!fast && lag) {
+#pragma unroll
+          for (int p = 0; p < RH / 2; ++p)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              if (LEARN) {
+                const float2 x = cadd(D[LEARN ? p : 0][c], S[p][c]);
+                D[LEARN ? p : 0][c] = ffma2(x, dup(a1), mul2(x, a1lo));
+              }
+              S[p][c] = ffma2(S[p][c], dup(a1), mul2(S[p][c], a1lo));
+            }
+        }
+        float2 acc[4] = {dup(0.f), dup(0.f), dup(0.f), dup(0.f)};  // of o, or of q T
+#pragma unroll
+        for (int r = 0; r < RH / 4; ++r) {
+          const float4 kk = k4[r];
+          const float2 ka = make_float2(kk.x, kk.y), kb = make_float2(kk.z, kk.w);
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            if (LEARN) D[LEARN ? p : 0][c] = mul2(cadd(D[LEARN ? p : 0][c], S[p][c]), a1);
-            S[p][c] = mul2(S[p][c], a1);
+            if (LEARN && fast) {
+              D[LEARN ? 2 * r : 0][c] = cadd(D[LEARN ? 2 * r : 0][c], S[2 * r][c]);
+              D[LEARN ? 2 * r + 1 : 0][c] = cadd(D[LEARN ? 2 * r + 1 : 0][c], S[2 * r + 1][c]);
+            }
+            S[2 * r][c] = ffma2(ka, vj[c], S[2 * r][c]);
+            S[2 * r + 1][c] = ffma2(kb, vj[c], S[2 * r + 1][c]);
           }
-      }
-      float2 acc[4] = {dup(0.f), dup(0.f), dup(0.f), dup(0.f)};  // of o, or of q T
+          if (A.o) {
+            const float4 qq = q4[r];
+            const float2 qa = make_float2(qq.x, qq.y), qb = make_float2(qq.z, qq.w);
 #pragma unroll
-      for (int r = 0; r < RH / 4; ++r) {
-        const float4 kk = k4[r];
-        const float2 ka = make_float2(kk.x, kk.y), kb = make_float2(kk.z, kk.w);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          if (LEARN && fast) {
-            D[LEARN ? 2 * r : 0][c] = cadd(D[LEARN ? 2 * r : 0][c], S[2 * r][c]);
-            D[LEARN ? 2 * r + 1 : 0][c] = cadd(D[LEARN ? 2 * r + 1 : 0][c], S[2 * r + 1][c]);
+            for (int c = 0; c < 4; ++c) {
+              acc[c] = ffma2(qa, LEARN ? D[LEARN ? 2 * r : 0][c] : S[2 * r][c], acc[c]);
+              acc[c] = ffma2(qb, LEARN ? D[LEARN ? 2 * r + 1 : 0][c] : S[2 * r + 1][c], acc[c]);
+            }
           }
-          S[2 * r][c] = ffma2(ka, vj[c], S[2 * r][c]);
-          S[2 * r + 1][c] = ffma2(kb, vj[c], S[2 * r + 1][c]);
         }
         if (A.o) {
-          const float4 qq = q4[r];
-          const float2 qa = make_float2(qq.x, qq.y), qb = make_float2(qq.z, qq.w);
+          if (LEARN) {
+            const float4 x4 = *reinterpret_cast<const float4*>(xs + i * kCols + col);
+            float s = (acc[0].x + acc[0].y) * x4.x;
+            s = fmaf(acc[1].x + acc[1].y, x4.y, s);
+            s = fmaf(acc[2].x + acc[2].y, x4.z, s);
+            s = fmaf(acc[3].x + acc[3].y, x4.w, s);
+            dg = fmaf(s, apow[i], dg);
+          } else {
+            const float as = apow[i] * A.oscale;
+            float o[4];
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            acc[c] = ffma2(qa, LEARN ? D[LEARN ? 2 * r : 0][c] : S[2 * r][c], acc[c]);
-            acc[c] = ffma2(qb, LEARN ? D[LEARN ? 2 * r + 1 : 0][c] : S[2 * r + 1][c], acc[c]);
-          }
-        }
-      }
-      if (A.o) {
-        if (LEARN) {
-          const float4 x4 = *reinterpret_cast<const float4*>(xs + i * kCols + col);
-          float s = (acc[0].x + acc[0].y) * x4.x;
-          s = fmaf(acc[1].x + acc[1].y, x4.y, s);
-          s = fmaf(acc[2].x + acc[2].y, x4.z, s);
-          s = fmaf(acc[3].x + acc[3].y, x4.w, s);
-          dg = fmaf(s, apow[i], dg);
-        } else {
-          const float as = apow[i] * A.oscale;
-          float o[4];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            o[c] = acc[c].x + acc[c].y;
-            o[c] = (o[c] + __shfl_xor_sync(0xffffffffu, o[c], 16)) * as;
-          }
-          if (lane < 16) {
-            if (KW > 1) {
-              *reinterpret_cast<float4*>(os + (warp * kTok + i) * kCols + col) = make_float4(o[0], o[1], o[2], o[3]);
-            } else {
-              TO* d = op + (t0 + (long long)i * step) * A.ol + col;
-              if (sizeof(TO) == 4 && A.ovec && left > 0) {
-                *reinterpret_cast<float4*>(d) = make_float4(o[0], o[1], o[2], o[3]);
+            for (int c = 0; c < 4; ++c) {
+              o[c] = acc[c].x + acc[c].y;
+              o[c] = (o[c] + __shfl_xor_sync(0xffffffffu, o[c], 16)) * as;
+            }
+            if (fast) {
+              odd = ffma2(make_float2(o[0], o[1]), dup(0.f), odd);
+              odd = ffma2(make_float2(o[2], o[3]), dup(0.f), odd);
+            }
+            if (lane < 16) {
+              if (KW > 1) {
+                *reinterpret_cast<float4*>(os + (warp * kTok + i) * kCols + col) = make_float4(o[0], o[1], o[2], o[3]);
               } else {
+                TO* d = op + (t0 + (long long)i * step) * A.ol + col;
+                if (sizeof(TO) == 4 && A.ovec && left > 0) {
+                  *reinterpret_cast<float4*>(d) = make_float4(o[0], o[1], o[2], o[3]);
+                } else {
 #pragma unroll
-                for (int c = 0; c < 4; ++c)
-                  if (c < left) DT<TO>::store(d + c, o[c]);
+                  for (int c = 0; c < 4; ++c)
+                    if (c < left) DT<TO>::store(d + c, o[c]);
+                }
               }
             }
           }
         }
+        if (!fast && !lag) {
+#pragma unroll
+          for (int p = 0; p < RH / 2; ++p)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) S[p][c] = ffma2(S[p][c], dup(a1), mul2(S[p][c], a1lo));
+        }
       }
-      if (!fast && !lag) {
+      if (fast) {
+        float hi = achi, lo = aclo;
+        if (n != kTok) {
+          two_floats(exp((double)g * n), &hi, &lo);
+        }
 #pragma unroll
         for (int p = 0; p < RH / 2; ++p)
 #pragma unroll
-          for (int c = 0; c < 4; ++c) S[p][c] = mul2(S[p][c], a1);
+          for (int c = 0; c < 4; ++c) {
+            S[p][c] = ffma2(S[p][c], dup(hi), mul2(S[p][c], lo));
+            if (LEARN) D[LEARN ? p : 0][c] = ffma2(D[LEARN ? p : 0][c], dup(hi), mul2(D[LEARN ? p : 0][c], lo));
+          }
+      }
+      if (KW > 1 && A.o && !LEARN) {
+        __syncthreads();
+        for (int i = threadIdx.x; i < n * kCols; i += 32 * KW) {
+          const int r = i / kCols, c = i - r * kCols;
+          if (c0 + c < A.DV) {
+            float o = 0.f;
+#pragma unroll
+            for (int j = 0; j < KW; ++j) o += os[j * kTok * kCols + i];
+            DT<TO>::store(op + (t0 + (long long)r * step) * A.ol + c, o);
+          }
+        }
       }
     }
-    if (fast) {
-      float hi = achi, lo = aclo;
-      if (n != kTok) {
-        two_floats(exp((double)g * n), &hi, &lo);
-      }
+
+    if constexpr (fast) {
 #pragma unroll
       for (int p = 0; p < RH / 2; ++p)
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          S[p][c] = ffma2(S[p][c], dup(hi), mul2(S[p][c], lo));
-          if (LEARN) D[LEARN ? p : 0][c] = ffma2(D[LEARN ? p : 0][c], dup(hi), mul2(D[LEARN ? p : 0][c], lo));
+          odd = ffma2(S[p][c], dup(0.f), odd);
+          if (LEARN) odd = ffma2(D[LEARN ? p : 0][c], dup(0.f), odd);
         }
+      if (LEARN) odd.x = fmaf(dg, 0.f, odd.x);
     }
-    if (KW > 1 && A.o && !LEARN) {
-      __syncthreads();
-      for (int i = threadIdx.x; i < n * kCols; i += 32 * KW) {
-        const int r = i / kCols, c = i - r * kCols;
-        if (c0 + c < A.DV) {
-          float o = 0.f;
-#pragma unroll
-          for (int j = 0; j < KW; ++j) o += os[j * kTok * kCols + i];
-          DT<TO>::store(op + (t0 + (long long)r * step) * A.ol + c, o);
-        }
-      }
-    }
-  }
+    return __syncthreads_or(odd.x != 0.f || odd.y != 0.f) != 0;
+  };
+  const bool fast = !(fabs((double)g) * kTok > kFastLimit);
+  if (!fast || run(std::true_type{})) run(std::false_type{});
 
   if (A.o && !LEARN) {  // tokens past the length: zeros
     const long long z0 = max(t_lo, t_hi);

@@ -915,6 +915,13 @@ struct SplitArgs {
   int B, L, terms;
 };
 
+// The bfloat16 nearest to f; of a finite f never an infinity (float32 reaches a little further: the next term has the rest).
+__device__ __forceinline__ uint32_t finite_bits(float f) {
+  uint32_t u = __bfloat16_as_ushort(__float2bfloat16_rn(f));
+  if ((u & 0x7fff) == 0x7f80 && isfinite(f)) --u;
+  return u;
+}
+
 // x = sum of bfloat16 terms, largest first; an infinity or NaN is the first term alone.
 template <typename T>
 __global__ void __launch_bounds__(256) decay_split_kernel(const SplitArgs A) {
@@ -939,7 +946,7 @@ __global__ void __launch_bounds__(256) decay_split_kernel(const SplitArgs A) {
     uint4 out;
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      const uint32_t p = pack2(f[2 * u], f[2 * u + 1]);
+      const uint32_t p = finite_bits(f[2 * u]) | finite_bits(f[2 * u + 1]) << 16;
       (&out.x)[u] = p;
       const float2 r = unpack2(p);
       f[2 * u] = isfinite(r.x) ? f[2 * u] - r.x : 0.f;

@@ -529,3 +529,17 @@ def test_bad_values_reach_what_the_recurrence_lets_them_reach(shape, dtype, bad,
     for n, r, x in zip(("dq", "dk", "dv"), ref, grads):
         _same_kinds(n, r, x, TOL[dtype])
     _same_kinds("dstate", ref[4], grads[4], TOL[F32])
+
+
+@gpu
+@pytest.mark.parametrize("shape", [(2, 100, 2, 2, 64, 64), (2, 20, 2, 2, 64, 64), (1, 600, 2, 1, 96, 40)], ids=str)
+def test_float32_values_beyond_bfloat16(shape):
+    """The largest float32 is finite, though it rounds to an infinity in 8 bits."""
+    q, k, v, g, _, _, _ = _inputs(*shape, F32)
+    q, k = q * 2.0 ** -40, k * 2.0 ** -4
+    v[0, 30 if shape[1] > 30 else 5, 0, 5] = torch.finfo(F32).max
+    v[0, 10, -1, 7] = -torch.finfo(F32).max
+    o, s = decay_attention(q.cuda(), k.cuda(), v.cuda(), g.cuda(), return_state=True)
+    ro, rs = oracle_forward(q, k, v, g)
+    for col in (5, 7, 9):  # the columns' sizes differ by 2^128
+        assert rel_l2(ro[..., col], o[..., col]) <= TOL[F32] and rel_l2(rs[..., col], s[..., col]) <= TOL[F32]
