@@ -384,7 +384,7 @@ HYFFT_API long long hyfft_launch_count(void);
 /* Kernels that wait for copies or tensor-core products of their own give up after a number of clocks (2^31, about a
  * second): the CTA ends, what it would have written is NaN, and a word on the device says so. hyfft_wait_status waits for
  * the device and returns HYFFT_ERR_WAIT where that has happened since the word was last cleared, else HYFFT_OK.
- * Not to be called while a stream is captured. Covers the decayed linear attention.             */
+ * Not to be called while a stream is captured. Covers the decayed linear attention and the layer norm. */
 HYFFT_API int hyfft_wait_status(int32_t device, int32_t clear);
 /* Sets that number of clocks for the launches that follow, in the whole process (2^31 at most; below 0: leaves it); returns the one before. */
 HYFFT_API long long hyfft_set_wait_clocks(long long clocks);

@@ -55,6 +55,7 @@ int set_error(int code, const char* msg) { return fail(code, "%s", msg); }
 std::atomic<long long> g_launches{0};
 std::atomic<unsigned> g_wait_clocks{1u << 31};  // kWaitClocks of waits.cuh
 int decay_wait_status(bool clear, unsigned* ran_out);  // decay_mma.cu
+int norm_wait_status(bool clear, unsigned* ran_out);   // layer_norm.cu
 
 static int check_launch(const char* what) {
   cudaError_t e = cudaGetLastError();
@@ -1242,11 +1243,14 @@ int hyfft_wait_status(int32_t device, int32_t clear) {
     cudaGetLastError();
     return fail(HYFFT_ERR_CUDA, "wait status: device %d", (int)device);
   }
-  unsigned scan = 0;
-  const bool read = cudaDeviceSynchronize() == cudaSuccess && decay_wait_status(clear != 0, &scan) == HYFFT_OK;
+  unsigned scan = 0, norm = 0;
+  const bool read = cudaDeviceSynchronize() == cudaSuccess && decay_wait_status(clear != 0, &scan) == HYFFT_OK &&
+                    norm_wait_status(clear != 0, &norm) == HYFFT_OK;
   cudaSetDevice(cur);
   if (!read) return fail(HYFFT_ERR_CUDA, "wait status: %s", cudaGetErrorString(cudaGetLastError()));
-  if (scan) return fail(HYFFT_ERR_WAIT, "a wait inside a kernel ran out: decayed linear attention left NaN in its results");
+  if (scan || norm)
+    return fail(HYFFT_ERR_WAIT, "a wait inside a kernel ran out: %s%s%s left NaN in its results",
+                scan ? "decayed linear attention" : "", scan && norm ? ", " : "", norm ? "layer norm" : "");
   return HYFFT_OK;
 }
 

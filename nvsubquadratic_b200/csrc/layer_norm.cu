@@ -27,6 +27,7 @@
 #include "../../include/hyfft.h"
 #include "common.cuh"
 #include "umma.cuh"
+#include "waits.cuh"
 
 namespace hyfft {
 
@@ -47,6 +48,7 @@ struct NormArgs {
   long long rows, xs, ds;  // row strides of x and dy; y and dx are contiguous
   int C, tpr, groups;
   int stages;  // rows in a group's ring
+  unsigned patience;  // clocks after which a wait gives up
   float eps, invC;
 };
 
@@ -112,6 +114,19 @@ __device__ __forceinline__ void init_ring(uint64_t (*full)[kStages]) {
   }
 }
 
+// What a group's fetching thread has in flight once a wait of its own has run out: the rows from `row` on, that one at place
+// `at` in phase `phase` of the ring. It fetches no more, and waits for these before it leaves.
+struct Lost {
+  long long row;
+  int at, phase;
+};
+__device__ __forceinline__ void drain(uint64_t* full, Lost l, int stages, long long step, long long rows) {
+  for (int i = 0; i < stages && l.row + i * step < rows; ++i) {
+    wait_phase(&full[l.at], l.phase, kWaitClocks);
+    if (++l.at == stages) l.at = 0, l.phase ^= 1;
+  }
+}
+
 // A thread's PER elements as PER / 2 pairs, so that the arithmetic runs as packed float32 pairs: element e is column
 // (t + tpr * (e / V)) * V + e % V. Places past C hold zeros (WHOLE: there are none, C = tpr * PER).
 template <typename T>
@@ -158,6 +173,11 @@ __device__ __forceinline__ void load_row(T (&e)[PER], const T* __restrict__ p, i
     else
       DT<T>::store(e + j, in ? DT<T>::load(p + c) : 0.f);
   }
+}
+template <typename T, int PER>
+__device__ __forceinline__ void no_row(T (&e)[PER]) {
+#pragma unroll
+  for (int j = 0; j < PER; ++j) DT<T>::store(e + j, __int_as_float(0x7fffffff));
 }
 template <typename T, int V, int PER, bool WHOLE>
 __device__ __forceinline__ void store_row(T* __restrict__ p, const T (&e)[PER], int t, int tpr, int C) {
@@ -208,10 +228,12 @@ __device__ __forceinline__ void keep_param(P (&f)[PER], const void* p, float non
   }
 }
 
+// 16-bit rows of up to 16 elements a thread: 64 registers, for four CTAs of 256 threads an SM.
 template <typename T, typename P, int V, int PER, bool WHOLE>
-__global__ void __launch_bounds__(512) layer_norm_fwd_kernel(const NormArgs A) {
+__global__ void __launch_bounds__(512, V == 8 && sizeof(P) == 2 && PER <= 16 ? 2 : 1) layer_norm_fwd_kernel(const NormArgs A) {
   extern __shared__ __align__(16) unsigned char ring[];  // [groups, stages, C]
   __shared__ uint64_t full[kMaxGroups][kStages];
+  __shared__ Lost lost[kMaxGroups];
   __shared__ Sums sums;
   clear(sums);
   init_ring(full);
@@ -241,11 +263,18 @@ __global__ void __launch_bounds__(512) layer_norm_fwd_kernel(const NormArgs A) {
     load_row<T, V, PER, WHOLE>(cur, x + row * A.xs, t, A.tpr, A.C);
   }
   int at = 0, phase = 0;
-  bool ok = true;  // false once a wait has run out: NaN in what is written
+  // phase: from 2 on once a wait has run out; this thread's part of a row is NaN then, and so are its group's results
   for (; row < A.rows; row += step) {
     if (kRing) {
-      ok = ok && umma::mbar_wait(&full[group][at], phase);
-      load_row<T, V, PER, WHOLE>(cur, reinterpret_cast<const T*>(mine + (size_t)at * bytes), t, A.tpr, A.C);
+      if (phase < 2 && !wait_phase(&full[group][at], phase, A.patience)) {
+        if (t == 0) lost[group] = {row, at, phase};
+        phase |= 2;
+        atomicExch(&g_ran_out, 1u);
+      }
+      if (phase < 2)
+        load_row<T, V, PER, WHOLE>(cur, reinterpret_cast<const T*>(mine + (size_t)at * bytes), t, A.tpr, A.C);
+      else
+        no_row(cur);
     }
     float2 f[PER / 2], s2 = dup(0.f);
 #pragma unroll
@@ -256,7 +285,7 @@ __global__ void __launch_bounds__(512) layer_norm_fwd_kernel(const NormArgs A) {
     if (!kRing && row + step < A.rows) load_row<T, V, PER, WHOLE>(cur, x + (row + step) * A.xs, t, A.tpr, A.C);
     const float mean = group_sum(s2.x + s2.y, A.tpr, group, sums, slot) * A.invC;
     if (kRing) {  // every thread of the group has read its part of the row
-      if (t == 0 && row + A.stages * step < A.rows) fetch(at, row + A.stages * step);
+      if (t == 0 && phase < 2 && row + A.stages * step < A.rows) fetch(at, row + A.stages * step);
       if (++at == A.stages) at = 0, phase ^= 1;
     }
     s2 = dup(0.f);
@@ -266,7 +295,7 @@ __global__ void __launch_bounds__(512) layer_norm_fwd_kernel(const NormArgs A) {
       s2 = ffma2(f[p], f[p], s2);
     }
     const float var = group_sum(s2.x + s2.y, A.tpr, group, sums, slot) * A.invC;
-    const float rstd = ok ? 1.f / sqrtf(var + A.eps) : __int_as_float(0x7fffffff);
+    const float rstd = 1.f / sqrtf(var + A.eps);
     opaque(w);
     opaque(b);
     alignas(16) T o[PER];
@@ -275,6 +304,7 @@ __global__ void __launch_bounds__(512) layer_norm_fwd_kernel(const NormArgs A) {
     store_row<T, V, PER, WHOLE>(y + row * A.C, o, t, A.tpr, A.C);
     if (t == 0 && A.mean) A.mean[row] = mean, A.rstd[row] = rstd;
   }
+  if (kRing && t == 0 && phase >= 2) drain(full[group], lost[group], A.stages, step, A.rows);
 }
 
 template <typename T, typename P, int V, int PER, bool WHOLE>
@@ -282,6 +312,7 @@ __global__ void __launch_bounds__(512) layer_norm_bwd_kernel(const NormArgs A) {
   extern __shared__ __align__(16) unsigned char ring[];  // [groups, stages, 2, C]; at the end the groups' sums [groups, 2, C]
   float* sums = reinterpret_cast<float*>(ring);
   __shared__ uint64_t full[kMaxGroups][kStages];
+  __shared__ Lost lost[kMaxGroups];
   __shared__ Sums sx, sy;
   clear(sx);
   clear(sy);
@@ -318,14 +349,23 @@ __global__ void __launch_bounds__(512) layer_norm_bwd_kernel(const NormArgs A) {
     load_row<T, V, PER, WHOLE>(cd, dy + row * A.ds, t, A.tpr, A.C);
   }
   int at = 0, phase = 0;
-  bool ok = true;  // false once a wait has run out: NaN in what is written
+  // phase: from 2 on once a wait has run out; this thread's part of a row is NaN then, and so are its group's results
   for (; row < A.rows; row += step) {
     if (kRing) {
-      ok = ok && umma::mbar_wait(&full[group][at], phase);
-      load_row<T, V, PER, WHOLE>(cx, reinterpret_cast<const T*>(mine + (size_t)at * 2 * bytes), t, A.tpr, A.C);
-      load_row<T, V, PER, WHOLE>(cd, reinterpret_cast<const T*>(mine + ((size_t)at * 2 + 1) * bytes), t, A.tpr, A.C);
+      if (phase < 2 && !wait_phase(&full[group][at], phase, A.patience)) {
+        if (t == 0) lost[group] = {row, at, phase};
+        phase |= 2;
+        atomicExch(&g_ran_out, 1u);
+      }
+      if (phase < 2) {
+        load_row<T, V, PER, WHOLE>(cx, reinterpret_cast<const T*>(mine + (size_t)at * 2 * bytes), t, A.tpr, A.C);
+        load_row<T, V, PER, WHOLE>(cd, reinterpret_cast<const T*>(mine + ((size_t)at * 2 + 1) * bytes), t, A.tpr, A.C);
+      } else {
+        no_row(cx);
+        no_row(cd);
+      }
     }
-    const float r = ok ? rstd : __int_as_float(0x7fffffff);
+    const float r = rstd;  // of this row: the next one's is fetched below
     float2 h[PER / 2], g[PER / 2], s1 = dup(0.f), s2 = dup(0.f);
 #pragma unroll
     for (int p = 0; p < PER / 2; ++p) {
@@ -346,7 +386,7 @@ __global__ void __launch_bounds__(512) layer_norm_bwd_kernel(const NormArgs A) {
     }
     float2 s = group_sum(make_float2(s1.x + s1.y, s2.x + s2.y), A.tpr, group, sx, sy, slot);
     if (kRing) {  // every thread of the group has read its part of both rows
-      if (t == 0 && row + A.stages * step < A.rows) fetch(at, row + A.stages * step);
+      if (t == 0 && phase < 2 && row + A.stages * step < A.rows) fetch(at, row + A.stages * step);
       if (++at == A.stages) at = 0, phase ^= 1;
     }
     s.x *= A.invC, s.y *= A.invC;
@@ -358,6 +398,7 @@ __global__ void __launch_bounds__(512) layer_norm_bwd_kernel(const NormArgs A) {
       store_row<T, V, PER, WHOLE>(static_cast<T*>(A.dx) + row * A.C, o, t, A.tpr, A.C);
     }
   }
+  if (kRing && t == 0 && phase >= 2) drain(full[group], lost[group], A.stages, step, A.rows);
   if (!A.part) return;
   __syncthreads();  // the ring is read
   float* out = A.part + (long long)blockIdx.x * 2 * A.C;
@@ -540,6 +581,7 @@ bool aligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 template <typename T, typename P>
 int launch_t(NormArgs& A, NormPlan& p, bool backward, cudaStream_t st) {
   A.tpr = p.tpr, A.groups = p.groups;
+  A.patience = g_wait_clocks.load(std::memory_order_relaxed);
   A.invC = 1.f / (float)A.C;
   if (p.per == 0) {
     if (backward)
@@ -561,6 +603,12 @@ int check_args(int64_t rows, int64_t C, int32_t dtype, int32_t param_dtype) {
     return set_error(HYFFT_ERR_INVALID, "layer norm: weight and bias have x's dtype or float32");
   return HYFFT_OK;
 }
+
+}  // namespace
+
+int norm_wait_status(bool clear, unsigned* ran_out) { return read_ran_out(clear, ran_out) == cudaSuccess ? HYFFT_OK : HYFFT_ERR_CUDA; }
+
+namespace {
 
 int run(NormArgs& A, NormPlan& p, int32_t dtype, int32_t param_dtype, bool backward, cudaStream_t st) {
   if (dtype == HYFFT_F32) return launch_t<float, float>(A, p, backward, st);

@@ -168,3 +168,40 @@ def test_same_bits_every_time():
     x, w, b, dy = (t.cuda().requires_grad_() for t in _case(3000, 768, BF16, BF16))
     runs = [torch.autograd.grad(layer_norm(x, w, b), [x, w, b], dy) for _ in range(2)]
     assert all(torch.equal(p, q) for p, q in zip(*runs))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("shape", [(5000, 64), (3000, 768), (4000, 4096), (40, 8192)], ids=str)
+def test_waits_that_run_out_leave_nan_and_a_status(shape, dtype):
+    """With no patience at all the waits for rows run out: every value is the right one or NaN, the host can tell, and the
+    next call is as ever."""
+    from nvsubquadratic_b200 import _lib
+
+    x, w, b, dy = (t.cuda() for t in _case(*shape, dtype, dtype))
+    args = [t.requires_grad_() for t in (x, w, b)]
+
+    def run():
+        y = layer_norm(*args)
+        return [y.detach(), *torch.autograd.grad(y, args, dy)]
+
+    want = run()
+    _lib.check_waits(0)
+    lib = _lib.load()
+    before = lib.hyfft_set_wait_clocks(0)
+    try:
+        got = run()
+        torch.cuda.synchronize()
+    finally:
+        lib.hyfft_set_wait_clocks(before)
+    # a row may have arrived before it is asked for: there is a status exactly where there is a NaN
+    if any(t.isnan().any() for t in got):
+        with pytest.raises(_lib.HyfftError, match="layer norm"):
+            _lib.check_waits(0)
+    else:
+        assert shape[1] < 4096  # groups that walk over many wide rows do not find every one there
+    _lib.check_waits(0)
+    for p, q in zip(want, got):
+        assert ((p == q) | q.isnan()).all()
+    assert all(torch.equal(p, q) for p, q in zip(want, run()))
+    _lib.check_waits(0)
