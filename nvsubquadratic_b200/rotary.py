@@ -33,7 +33,8 @@ def rotary_turns(rot_dim: int, *, base: float = 10000.0, scaling: str = "none", 
       ``factor`` and leaves the fastest;
     * ``"ramp"``: pairs that turn more than ``fast_turns`` times within ``original_length`` keep their
       frequency, pairs that turn less than ``slow_turns`` times are divided by ``factor``, those between are blended by
-      their index; the amplitude is ``0.1 ln(factor) + 1``.
+      their index (from the whole number below the index that turns ``fast_turns`` times to the one above that of
+      ``slow_turns``, which may lie past the last pair; at most ``rot_dim - 1``); the amplitude is ``0.1 ln(factor) + 1``.
 
     ``turns`` is int64 ``[rot_dim // 2]``, turns per position in units of 2^-64; ``amplitude`` is 1 but for ``"ramp"``.
     """
@@ -52,7 +53,7 @@ def rotary_turns(rot_dim: int, *, base: float = 10000.0, scaling: str = "none", 
         def pair_turning(times):  # the index (a real number) of the pair that turns so often
             return rot_dim * math.log(original_length / (times * 2 * math.pi)) / (2 * math.log(base))
 
-        low, high = max(math.floor(pair_turning(fast_turns)), 0), min(math.ceil(pair_turning(slow_turns)), half - 1)
+        low, high = max(math.floor(pair_turning(fast_turns)), 0), min(math.ceil(pair_turning(slow_turns)), rot_dim - 1)
         for i in range(half):
             keep = 1.0 - min(max((i - low) / max(high - low, 0.001), 0.0), 1.0)
             freq[i] = freq[i] / factor * (1.0 - keep) + freq[i] * keep

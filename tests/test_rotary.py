@@ -150,3 +150,26 @@ def test_strides_alignment_and_missing_k(dtype):
     (g,) = torch.autograd.grad([out[1]], [kd], [dk.cuda()])
     assert rel_l2(oracle(dk, _radians(turns), backward=True), g) <= TOL[dtype]
     assert rotary(views[0][:, :0], views[1][:, :0], t)[0].shape == (B, 0, H, D)
+
+
+@pytest.mark.parametrize("rot,length", [(64, 131072), (64, 1 << 20), (128, 131072), (6, 8192), (8, 8192), (64, 4096), (32, 512)])
+def test_ramp_follows_its_definition(rot, length):
+    """Slowed by 8 below one turn within the original length, not at all above 32, in between by the index: 0 at the whole index below
+    that of 32 turns, 1 at the one above that of one turn, wherever the last pair lies."""
+    ratio = _radians(rotary_turns(rot)[0]) / _radians(rotary_turns(rot, scaling="ramp", factor=8.0, original_length=length)[0])
+    # turns of a pair of index x: length * 10000^(-2 x / rot) / (2 pi)
+    index = lambda turns: rot / 2 * (math.log(length / (2 * math.pi)) - math.log(turns)) / math.log(10000.0)  # noqa: E731
+    low, high = max(math.floor(index(32.0)), 0), math.ceil(index(1.0))
+    for i in range(rot // 2):
+        slowed = min(max((i - low) / (high - low), 0.0), 1.0)
+        assert ratio[i].item() == pytest.approx(1.0 / (1.0 - slowed + slowed / 8.0), rel=1e-12), i
+        turns = length * 10000.0 ** (-2 * i / rot) / (2 * math.pi)
+        if 1.0 < turns < 32.0 and low < i < high:
+            assert 1.0 < ratio[i].item() < 8.0
+
+
+@pytest.mark.parametrize("rot,length,last", [(64, 131072, 2.54), (64, 1 << 20, 1.16)])
+def test_ramp_blends_a_last_pair_that_still_turns(rot, length, last):
+    """Worked out by hand: the last pair (31) of 64 features turns 2.78 and 22 times; it is divided by less than the factor."""
+    plain, ramp = (_radians(rotary_turns(rot, **a)[0]) for a in ({}, dict(scaling="ramp", factor=8.0, original_length=length)))
+    assert (plain[-1] / ramp[-1]).item() == pytest.approx(last, abs=0.01)
