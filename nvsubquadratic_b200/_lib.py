@@ -8,6 +8,7 @@ library is missing or the tensors are not on a CUDA device, calls raise.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 import threading
 from pathlib import Path
@@ -252,6 +253,45 @@ def check_waits(device: torch.device | int = 0, clear: bool = True) -> None:
     such check (the results of that call hold NaN)."""
     index = device if isinstance(device, int) else torch.device(device).index or 0
     check(load().hyfft_wait_status(index, int(clear)), "hyfft_wait_status")
+
+
+def autograd_sees(*tensors: torch.Tensor | None) -> bool:
+    """Whether autograd has to see a call: an input requires a gradient, or carries a forward-mode tangent (which needs no
+    requires_grad; a Function without a jvp refuses it)."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        return True
+    ad = torch.autograd.forward_ad
+    return ad._current_level >= 0 and any(t is not None and ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
+class _Final(torch.autograd.Function):
+    """Its tensors, which nothing can be differentiated through."""
+
+    @staticmethod
+    def forward(ctx, anchor, *tensors):
+        return tuple(t.view_as(t) for t in tensors)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("this operator's gradient has no second derivative")
+
+
+def no_second_derivative(backward):
+    """Decorates a Function's backward whose kernels record no graph: under ``create_graph=True`` differentiating its gradients
+    again is an error. (``once_differentiable`` says so only where the upstream gradient requires a gradient itself; these
+    gradients depend on saved inputs too.)"""
+
+    @functools.wraps(backward)
+    def wrapped(ctx, *upstream):
+        with torch.no_grad():
+            grads = backward(ctx, *upstream)
+        if not torch.is_grad_enabled():
+            return grads
+        anchor = torch.empty(0, requires_grad=True)
+        final = iter(_Final.apply(anchor, *(g for g in grads if g is not None)))
+        return tuple(None if g is None else next(final) for g in grads)
+
+    return wrapped
 
 
 def launch_count() -> int:

@@ -119,6 +119,7 @@ class _DecayFunction(torch.autograd.Function):
         return o, state
 
     @staticmethod
+    @_lib.no_second_derivative
     def backward(ctx, do, dstate):
         q, k, v, g, s0, saved, lengths = ctx.saved_tensors
         dev = q.device
@@ -181,7 +182,7 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay
         lengths = lengths.contiguous()
     scale = Dk ** -0.5 if scale is None else float(scale)
     args = (q, k, v, log_decay, initial_state, lengths, scale, bool(return_state))
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:5]):
+    if _lib.autograd_sees(*args[:5]):
         o, state = _DecayFunction.apply(*args)
     else:
         o, state, _ = _forward(*args, False)
@@ -208,7 +209,7 @@ def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_
     assert state.ndim == 4, f"state must be [N, {H}, {Dk}, {v.shape[-1]}]; got {tuple(state.shape)}"
     N = state.shape[0]
     _check_state("state", state, (N, H, Dk, v.shape[-1]))
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, log_decay, state)):
+    if _lib.autograd_sees(q, k, v, log_decay, state):
         raise NotImplementedError("decay_attention_step records no gradient: call it under torch.no_grad(), "
                                   "or use decay_attention with L = 1")
     out_state = state if out_state is None else out_state

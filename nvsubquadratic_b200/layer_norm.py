@@ -63,6 +63,7 @@ class _LayerNormFunction(torch.autograd.Function):
         return y
 
     @staticmethod
+    @_lib.no_second_derivative
     def backward(ctx, dy):
         x2, w, stats = ctx.saved_tensors
         dev = x2.device
@@ -105,7 +106,7 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
         assert weight.dtype == bias.dtype, f"weight and bias must share a dtype; got {weight.dtype} and {bias.dtype}"
     if x.dtype not in _lib.DTYPE_CODE:
         raise NotImplementedError(f"dtype {x.dtype} is not supported (float32, bfloat16, float16)")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+    if _lib.autograd_sees(x, weight, bias):
         return _LayerNormFunction.apply(x, weight, bias, float(eps))
     return _forward(x, weight, bias, float(eps), False)[0]
 

@@ -122,6 +122,7 @@ class _RotaryFunction(torch.autograd.Function):
         return _call(q, k, turns, positions, amplitude, interleaved, False)
 
     @staticmethod
+    @_lib.no_second_derivative
     def backward(ctx, dq, dk):
         turns, positions = ctx.saved_tensors
         if dq is None and dk is None:
@@ -161,6 +162,6 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, turns: torch.Tensor, *, posi
     if q.dtype not in _lib.DTYPE_CODE:
         raise NotImplementedError(f"dtype {q.dtype} is not supported (float32, bfloat16, float16)")
     args = (q, k, turns.contiguous(), positions, float(amplitude), bool(interleaved))
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+    if _lib.autograd_sees(q, k):
         return _RotaryFunction.apply(*args)
     return _call(*args, False)

@@ -543,3 +543,25 @@ def test_float32_values_beyond_bfloat16(shape):
     ro, rs = oracle_forward(q, k, v, g)
     for col in (5, 7, 9):  # the columns' sizes differ by 2^128
         assert rel_l2(ro[..., col], o[..., col]) <= TOL[F32] and rel_l2(rs[..., col], s[..., col]) <= TOL[F32]
+
+
+@gpu
+def test_second_and_forward_mode_derivatives_are_refused():
+    from torch.autograd import forward_ad
+
+    q, k, v, g, s0, do, ds = (t.cuda() for t in _inputs(1, 40, 2, 1, 64, 64, F32))
+    leaf = q.clone().requires_grad_()
+    (dq,) = torch.autograd.grad(decay_attention(leaf, k, v, g).square().sum(), [leaf], create_graph=True)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        (leaf.sum() + dq.sum()).backward()
+    args = [q, k, v, g]
+    with forward_ad.dual_level():
+        for i in range(5):
+            a = list(args) + [s0]
+            a[i] = forward_ad.make_dual(a[i], torch.ones_like(a[i]))
+            with pytest.raises((RuntimeError, NotImplementedError), match="forward mode AD"):
+                decay_attention(*a[:4], initial_state=a[4])
+        dual = forward_ad.make_dual(q[:, 0].contiguous(), torch.ones_like(q[:, 0]))
+        with pytest.raises(NotImplementedError, match="no gradient"):
+            decay_attention_step(dual, k[:, 0], v[:, 0], g, s0)
+        decay_attention_step(q[:, 0], k[:, 0], v[:, 0], g, s0)

@@ -205,3 +205,65 @@ def test_waits_that_run_out_leave_nan_and_a_status(shape, dtype):
         assert ((p == q) | q.isnan()).all()
     assert all(torch.equal(p, q) for p, q in zip(want, run()))
     _lib.check_waits(0)
+
+
+# ---------------------------------------------------------------- derivatives that are not there
+
+
+def test_autograd_sees_tangents():
+    from torch.autograd import forward_ad
+
+    from nvsubquadratic_b200 import _lib
+
+    plain, leaf = torch.randn(3), torch.randn(3, requires_grad=True)
+    assert _lib.autograd_sees(None, leaf) and not _lib.autograd_sees(plain, None)
+    with torch.no_grad():
+        assert not _lib.autograd_sees(leaf)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(plain, torch.ones(3))
+        assert _lib.autograd_sees(None, dual) and not _lib.autograd_sees(plain)
+        with torch.no_grad():
+            assert _lib.autograd_sees(dual)
+    assert not _lib.autograd_sees(plain)
+
+
+@gpu
+def test_second_and_forward_mode_derivatives_are_refused():
+    """Neither has a kernel: an error, not a result that lacks them."""
+    from torch.autograd import forward_ad
+
+    x, w, b, dy = (t.cuda() for t in _case(5, 64, F32, F32))
+    x.requires_grad_()
+    (dx,) = torch.autograd.grad(layer_norm(x, w, b), [x], dy, create_graph=True)
+    with pytest.raises(RuntimeError, match="second derivative"):  # a penalty beside a loss
+        (x.sum() + dx.square().sum()).backward()
+    x = x.detach()
+    for i in range(3):
+        with forward_ad.dual_level():
+            args = [forward_ad.make_dual(t, torch.ones_like(t)) if i == j else t for j, t in enumerate((x, w, b))]
+            with pytest.raises((RuntimeError, NotImplementedError), match="forward mode AD"):
+                layer_norm(*args)
+            layer_norm(x, w, b)  # nothing to lose
+
+
+def test_gradients_without_a_second_derivative():
+    from nvsubquadratic_b200 import _lib
+
+    class Square(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x, y):
+            ctx.save_for_backward(x)
+            return x.square() + y
+
+        @staticmethod
+        @_lib.no_second_derivative
+        def backward(ctx, g):
+            return 2 * g * ctx.saved_tensors[0], None
+
+    x = torch.randn(3, requires_grad=True)
+    (g,) = torch.autograd.grad(Square.apply(x, torch.zeros(3)).sum(), [x])
+    assert not g.requires_grad and torch.equal(g, 2 * x.detach())
+    (g,) = torch.autograd.grad(Square.apply(x, torch.zeros(3)).sum(), [x], create_graph=True)
+    assert torch.equal(g.detach(), 2 * x.detach())
+    with pytest.raises(RuntimeError, match="second derivative"):
+        (x.sum() + g.sum()).backward()

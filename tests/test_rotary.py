@@ -173,3 +173,20 @@ def test_ramp_blends_a_last_pair_that_still_turns(rot, length, last):
     """Worked out by hand: the last pair (31) of 64 features turns 2.78 and 22 times; it is divided by less than the factor."""
     plain, ramp = (_radians(rotary_turns(rot, **a)[0]) for a in ({}, dict(scaling="ramp", factor=8.0, original_length=length)))
     assert (plain[-1] / ramp[-1]).item() == pytest.approx(last, abs=0.01)
+
+
+@gpu
+def test_second_and_forward_mode_derivatives_are_refused():
+    from torch.autograd import forward_ad
+
+    q, k, dq, dk, _ = (t.cuda() if t is not None else None for t in _case(2, 5, 3, 1, 64, 64, F32, "order"))
+    turns = rotary_turns(64, device="cuda")[0]
+    q.requires_grad_()
+    (g,) = torch.autograd.grad(rotary(q, k, turns)[0].square().sum(), [q], create_graph=True)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        (q.sum() + g.sum()).backward()
+    q = q.detach()
+    with forward_ad.dual_level():
+        for args in ((forward_ad.make_dual(q, dq), k), (q, forward_ad.make_dual(k, dk))):
+            with pytest.raises((RuntimeError, NotImplementedError), match="forward mode AD"):
+                rotary(*args, turns)
