@@ -29,11 +29,14 @@ __all__ = ["DecayCache", "DecayMixerB200", "DecayBlockB200"]
 
 class DecayCache:
     """The states of up to ``slots`` running requests: float32 ``[slots, heads, head_dim, head_dim]`` and the position of
-    each one's next token. Its size does not depend on the requests' lengths."""
+    each one's next token. Its size does not depend on the requests' lengths.
+
+    A slot outside ``0 .. slots - 1`` in a call marks an idle request: nothing of it is read, the mixer's output for it is zero and no
+    state changes, for prompts and for single tokens alike."""
 
     def __init__(self, slots: int, heads: int, head_dim: int, device=None):
         self.slots = slots
-        # one row more than slots: what calls with idle requests gather and scatter in their place
+        # one row more than slots: what calls with idle requests gather and scatter in their place, unchanged
         self.state = torch.zeros((slots + 1, heads, head_dim, head_dim), dtype=torch.float32, device=device)
         self.position = torch.zeros(slots + 1, dtype=torch.int64, device=device)
 
@@ -109,12 +112,15 @@ class DecayMixerB200(torch.nn.Module):
             rows = cache.rows(slots, B)
             start = cache.position[rows]
             q, k = self._turn(q, k, start[:, None] + torch.arange(L, device=start.device))
+            live = None if slots is None else rows < cache.slots
             if L == 1 and lengths is None:
-                live = rows if slots is None else torch.where(rows < cache.slots, rows, -1)
+                owned = rows if live is None else torch.where(live, rows, -1)
                 o = decay_attention_step(q[:, 0], k[:, 0], v[:, 0], self.log_decay, cache.state,
-                                         slots=live.to(torch.int32)).unsqueeze(1)
-                count = torch.ones_like(start)
+                                         slots=owned.to(torch.int32)).unsqueeze(1)
+                count = torch.ones_like(start) if live is None else live.long()
             else:
+                if live is not None:  # an idle request has no tokens
+                    lengths = live.to(torch.int32) * L if lengths is None else lengths.masked_fill(~live, 0)
                 o, state = decay_attention(q, k, v, self.log_decay, lengths=lengths, initial_state=cache.state[rows],
                                            return_state=True)
                 cache.state.index_copy_(0, rows, state.detach())

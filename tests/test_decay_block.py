@@ -127,3 +127,31 @@ def test_runs_in_the_qkv_mixer_and_refuses_context_parallel():
 
     with pytest.raises(NotImplementedError, match="context-parallel"):
         layer(torch.randn(1, 4, 64, device="cuda"), Group())
+
+
+@gpu
+@pytest.mark.parametrize("lengths", [None, [9, 9, 4]], ids=["whole", "ragged"])
+def test_idle_requests_of_a_prompt(lengths):
+    """A slot outside the cache in a prompt call: zero mixer output whatever its tokens and earlier idle calls held, no state or
+    position touched, and the same answer for the others."""
+    torch.manual_seed(0)
+    mixer = DecayMixerB200(64, 2).cuda()
+    q, k, v = (torch.randn(3, 9, 64, device="cuda") for _ in range(3))
+    n = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    cache, want_cache = DecayCache(4, 2, 32, device="cuda"), DecayCache(4, 2, 32, device="cuda")
+    with torch.no_grad():
+        want = mixer(q, k, v, cache=want_cache, slots=torch.tensor([2, 0, 1], device="cuda"), lengths=n)
+        bad = [t.clone() for t in (q, k, v)]
+        for t in bad:
+            t[1] = float("nan")
+        slots = torch.tensor([2, 7, 1], device="cuda")
+        for _ in range(2):  # what an idle request leaves behind must not matter to the next
+            cache.reset(torch.tensor([1, 2], device="cuda"))
+            got = mixer(*bad, cache=cache, slots=slots, lengths=n)
+            assert torch.equal(got[0], want[0]) and torch.equal(got[2], want[2]) and (got[1] == 0).all()
+            slots[1] = -1
+        assert torch.equal(cache.state[1:3], want_cache.state[1:3]) and (cache.state[[0, 3, 4]] == 0).all()
+        assert cache.position.tolist() == [0, lengths[2] if lengths else 9, 9, 0, 0]
+        token = mixer(*(t[:, :1] for t in bad), cache=cache, slots=slots)
+        assert (token[1] == 0).all() and torch.isfinite(token).all() and (cache.state[[0, 3, 4]] == 0).all()
+        assert cache.position.tolist() == [0, (lengths[2] if lengths else 9) + 1, 10, 0, 0]
