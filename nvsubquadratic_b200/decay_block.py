@@ -88,9 +88,11 @@ class DecayMixerB200(torch.nn.Module):
         # the decays stay float32 whatever type the rest of a model is cast to: a decay's rounding error is
         # raised to the power of the distance
         keep = self.log_decay.detach()
+        grad = None if self.log_decay.grad is None else self.log_decay.grad.detach()
         super()._apply(fn, recurse)
-        if self.log_decay.dtype != torch.float32:
-            self.log_decay.data = keep.to(self.log_decay.device)
+        for t, kept in ((self.log_decay, keep), (self.log_decay.grad, grad)):
+            if t is not None and t.dtype != torch.float32:
+                t.data = kept.to(t.device)
         return self
 
     def _turn(self, q, k, positions):

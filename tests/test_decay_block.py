@@ -155,3 +155,14 @@ def test_idle_requests_of_a_prompt(lengths):
         token = mixer(*(t[:, :1] for t in bad), cache=cache, slots=slots)
         assert (token[1] == 0).all() and torch.isfinite(token).all() and (cache.state[[0, 3, 4]] == 0).all()
         assert cache.position.tolist() == [0, (lengths[2] if lengths else 9) + 1, 10, 0, 0]
+
+
+def test_learned_decays_and_their_gradients_keep_their_precision():
+    mixer = DecayMixerB200(64, 4, learn_decay=True)
+    mixer.log_decay.grad = torch.randn(4)
+    value, grad = mixer.log_decay.detach().clone(), mixer.log_decay.grad.clone()
+    mixer.to(torch.bfloat16).half().double()
+    assert mixer.log_decay.dtype == torch.float32 and torch.equal(mixer.log_decay, value)
+    assert mixer.log_decay.grad.dtype == torch.float32 and torch.equal(mixer.log_decay.grad, grad)
+    torch.optim.AdamW(mixer.parameters(), lr=0.1).step()
+    assert not torch.equal(mixer.log_decay, value)
