@@ -227,6 +227,8 @@ def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_
     o = q.new_empty((B, H, v.shape[-1]))
     if B == 0:
         return o
+    if N == 0:  # every request is idle
+        return o.zero_()
     d, _ = _plan(q, k, v, Dk ** -0.5 if scale is None else float(scale))
     rc = _lib.load().hyfft_decay_step(ctypes.byref(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(),
                                       _lib.ptr(slots), N, state.data_ptr(), out_state.data_ptr(), o.data_ptr(),

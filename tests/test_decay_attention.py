@@ -565,3 +565,12 @@ def test_second_and_forward_mode_derivatives_are_refused():
         with pytest.raises(NotImplementedError, match="no gradient"):
             decay_attention_step(dual, k[:, 0], v[:, 0], g, s0)
         decay_attention_step(q[:, 0], k[:, 0], v[:, 0], g, s0)
+
+
+@gpu
+def test_step_without_states():
+    """A pool of no states: every request is idle."""
+    q, k, v = (torch.randn(2, 3, 16, device="cuda") for _ in range(3))
+    state = torch.empty(0, 3, 16, 16, device="cuda")
+    o = decay_attention_step(q, k, v, torch.zeros(3, device="cuda"), state, slots=torch.zeros(2, dtype=torch.int32, device="cuda"))
+    assert o.shape == (2, 3, 16) and (o == 0).all()
