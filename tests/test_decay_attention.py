@@ -574,3 +574,39 @@ def test_step_without_states():
     state = torch.empty(0, 3, 16, 16, device="cuda")
     o = decay_attention_step(q, k, v, torch.zeros(3, device="cuda"), state, slots=torch.zeros(2, dtype=torch.int32, device="cuda"))
     assert o.shape == (2, 3, 16) and (o == 0).all()
+
+
+# ---------------------------------------------------------------- buffers that are used many times over
+
+# Rows that fill the machine and are walked whole (16 chunks and more of 64 tokens), few of them in segments of two dozen chunks,
+# and head sizes of two column slices whose axis is cut. Checked on some of the batch, which the float64 recurrence can afford.
+LONG = [
+    (16, 1023, 12, 4, 64, 64),
+    (38, 700, 4, 4, 128, 96),
+    (40, 650, 4, 2, 72, 64),
+    (25, 3000, 4, 4, 64, 64),
+    (25, 3000, 2, 2, 128, 128),
+    (10, 2600, 4, 2, 96, 128),
+    (1, 1500, 2, 2, 128, 128),
+    (2, 900, 2, 1, 96, 72),
+    (1, 1100, 3, 3, 80, 128),
+    (1, 1037, 4, 2, 100, 100),
+]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("shape", LONG, ids=str)
+def test_many_chunks(shape, dtype):
+    B, L = shape[:2]
+    args = _inputs(*shape, dtype)
+    lengths = None
+    if B > 1:
+        lengths = torch.randint(0, L + 1, (B,), generator=torch.Generator().manual_seed(5), dtype=torch.int32)
+        lengths[0], lengths[-1] = L, L - 1
+    o, s, grads = _run(*args, lengths=lengths, learn=False)
+    some = torch.tensor([0, B - 1] if L > 2000 else sorted({0, B // 2, B - 1}))
+    q, k, v, g, s0, do, ds = args
+    part = [t[some] for t in (q, k, v)] + [g] + [t[some] for t in (s0, do, ds)]
+    got = (o.cpu()[some], s.cpu()[some], [t.cpu()[some] if t is not None else None for t in grads])
+    _compare(part, got, lengths=lengths[some] if lengths is not None else None, dtype=dtype)
