@@ -946,11 +946,18 @@ __global__ void __launch_bounds__(256) decay_split_kernel(const SplitArgs A) {
     uint4 out;
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      const uint32_t p = finite_bits(f[2 * u]) | finite_bits(f[2 * u + 1]) << 16;
+      uint32_t p = pack2(f[2 * u], f[2 * u + 1]);
+      float2 r = unpack2(p);
+      if (!isfinite(r.x) || !isfinite(r.y)) {
+        p = finite_bits(f[2 * u]) | finite_bits(f[2 * u + 1]) << 16;
+        r = unpack2(p);
+        f[2 * u] = isfinite(r.x) ? f[2 * u] - r.x : 0.f;
+        f[2 * u + 1] = isfinite(r.y) ? f[2 * u + 1] - r.y : 0.f;
+      } else {
+        f[2 * u] -= r.x;
+        f[2 * u + 1] -= r.y;
+      }
       (&out.x)[u] = p;
-      const float2 r = unpack2(p);
-      f[2 * u] = isfinite(r.x) ? f[2 * u] - r.x : 0.f;
-      f[2 * u + 1] = isfinite(r.y) ? f[2 * u + 1] - r.y : 0.f;
     }
     *reinterpret_cast<uint4*>(dst + t * per) = out;
   }
