@@ -13,7 +13,7 @@
 // owns four columns of the state and up to 32 of its rows in registers, packed in pairs of rows: a token costs two packed
 // multiply-adds per pair (S += k v, o += q S). q and k are read from shared memory as broadcasts, which the register
 // file takes at 128 bytes a cycle: one 16-byte read serves 16 multiply-adds here (with one column per thread it served four
-// and the reads were the bound: 2.08 ms for 16 x 4096 tokens, 12 heads of 64, float16, instead of 1.00). The two halves of a
+// and the reads were the bound: 2.08 ms for 16 x 4096 tokens, 12 heads of 64, float16, instead of 1.04). The two halves of a
 // warp hold two parts of the rows, their sums meet in one shuffle; states of more than 64 rows take more warps.
 // Inside a chunk of 16 tokens the state is kept divided by a^i, which takes the decay out of the inner loop: v is
 // multiplied by a^-i and o by a^i, each from a table, and the chunk's a^n is applied once, as the sum of two floats
@@ -561,14 +561,14 @@ void scan_shape(int DK, int* rh, int* kw) {
 
 // The tensor cores take every bfloat16 scan whose state has up to 128 rows, and float16 and float32 ones (as sums of
 // bfloat16 terms) from half a chunk of tokens on: below, the scan's time is latency either way and laying out the terms is one
-// launch more (12 heads of 64, float32, multiply-adds: 11 us for 16 tokens, 27 for 64; tensor cores: 10 for 64). All
+// launch more (12 heads of 64, float32, multiply-adds: 11 us for 16 tokens, 28 for 64; tensor cores: 10 for 64). All
 // scans of a call go one way.
 bool use_mma(const hyfft_decay_desc* d, int DK) {
   if (d->dtype == HYFFT_BF16) return DK <= kMmaMaxDK;
   return std::max(d->dk, d->dv) <= kMmaMaxDK && d->length >= kMmaTok / 2;
 }
 // bfloat16 terms of an operand, 0: none are laid out. bfloat16 heads of a size that 16-byte copies cannot take are laid out
-// as one term (8 x 4096 tokens, 8 heads of 65, forward and backward: 0.81 ms; element by element in the scan itself 2.72).
+// as one term (8 x 4096 tokens, 8 heads of 65, forward and backward: 0.94 ms; element by element in the scan itself 4.14).
 int terms(const hyfft_decay_desc* d) {
   if (d->dtype != HYFFT_BF16) return !use_mma(d, d->dk) ? 0 : d->dtype == HYFFT_F16 ? 2 : 3;
   return (d->dk % 8 || d->dv % 8) && std::max(d->dk, d->dv) <= kMmaMaxDK && d->length >= kMmaTok / 2 ? 1 : 0;
@@ -582,9 +582,10 @@ struct Segments {
 };
 
 // All scans of a call cut the axis at the same places, so that one pass over the segments serves several. Tensor
-// cores: as many CTAs as fit; rows alone where they give every SM one or are shorter than eight chunks, else as many segments
+// cores: as many CTAs as fit; rows alone where they give every SM one (200 rows of 4096 tokens of 64: 155 us forwards, as two
+// segments each 204; of 1024 tokens 46 and 79; 150 rows of 4096 153 and 199) or are shorter than eight chunks, else as many segments
 // as there is room for, none shorter than two chunks (1024 tokens, 12 heads of 64, forward and backward: segments of four chunks
-// or more 58 us, of two 48, of one 55; 256 tokens: one segment 38 us, two 44). Else: twelve warps for each SM, segments of
+// or more 63 us, of two 52, of one 59; 256 tokens: one segment 42 us, two 48). Else: twelve warps for each SM, segments of
 // one chunk at least.
 Segments segments(const hyfft_decay_desc* d, bool learn) {
   const long long rows = (long long)d->batch * d->heads;

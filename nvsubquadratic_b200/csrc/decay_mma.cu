@@ -3,7 +3,7 @@
 // float16 and float32 operands come as sums of NT = 2 and 3 bfloat16 terms (8 bits each; a small kernel lays them out
 // first, NT = 1 below is bfloat16 itself). A product of two sums runs the pairs of terms whose order is below NT, 3 or 6 of
 // them, into one float32 accumulator, and what the kernel rounds for a product (P, the state's copy) it keeps to NT terms too, so
-// float32 results are float32's (16 x 4096 tokens, 12 heads of 64: 0.62 ms, multiply-adds take 1.03; float16 0.48 and 1.00).
+// float32 results are float32's (16 x 4096 tokens, 12 heads of 64: 0.62 ms, multiply-adds take 1.06; float16 0.46 and 1.04).
 // The tensor cores' own float16 would do with fewer products but not hold a state beyond 65504.
 //
 // A CTA walks over one row's tokens (or a segment of them) in chunks of 64 and keeps 64 columns of the state. With
@@ -29,9 +29,9 @@
 // length or a head size; two take turns with K and V, one brings Q), one issues the products, eight compute: they decay P,
 // update the state and split the next chunk's V; four write the outputs. Only mbarriers order them. The computing warps' chain
 // of TMEM reads, shared-memory writes and barriers sets the pace, so what need not be in it is not (a pass with outputs
-// over the 128 x 128 grid, 32 rows of 16384 tokens of 64: 134 us with eight warps doing everything, 69 with loads and products
-// issued by others, 58 with the outputs written by others too, Q in several buffers and no register spilled; its traffic
-// at the copy's rate takes 41).
+// over the 128 x 128 grid, 32 rows of 16384 tokens of 64, with P and the state's copy as one term: 134 us with eight warps
+// doing everything, 69 with loads and products issued by others, 58 with the outputs written by others too, Q in several buffers
+// and no register spilled; as two terms 72; its traffic at the copy's rate takes 41).
 // A result that is infinite or NaN is computed again at the end, token by token in scan order (scan_by_token).
 // Registers move from the loading to the computing warps. Two CTAs share an SM (<= 113 KB, 256 TMEM columns each).
 //

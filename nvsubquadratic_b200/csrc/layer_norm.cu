@@ -7,9 +7,9 @@
 // A row is held in the registers of a group of 32 .. 512 threads (kPer = 8, 16 or 32 elements each), so the mean and
 // then the centred squares are summed from registers: two reductions, no cancellation between E[x^2] and
 // E[x]^2. Groups walk over the rows with the weights in registers. Rows that start on 16 bytes come through a ring of up
-// to four in shared memory for each group, filled by bulk copies (65536 rows of 4096 bfloat16: 205 us forwards, 277
+// to four in shared memory for each group, filled by bulk copies (65536 rows of 4096 bfloat16: 210 us forwards, 282
 // backwards; with the next row's loads in registers instead 246 and 330). Other rows are loaded one ahead into registers.
-// Forwards 16-bit weights stay packed, which leaves room for four CTAs an SM instead of three (205 against 227 us); joining
+// Forwards 16-bit weights stay packed, which leaves room for four CTAs an SM instead of three (210 against 228 us); joining
 // the warps' own means and squares with one barrier instead of two cost more instructions than it saved (251).
 // Everything per element runs on packed pairs (element by element, with a test of the column for each, it was 314 and
 // 422 us: instructions were the bound). The weight's and the bias's gradients stay in each thread's registers over
