@@ -14,6 +14,7 @@ import threading
 from pathlib import Path
 
 import torch
+from torch.autograd import forward_ad as _forward_ad
 
 _PKG = Path(__file__).resolve().parent
 _LIB_PATH = _PKG / "libhyfft.so"
@@ -258,10 +259,13 @@ def check_waits(device: torch.device | int = 0, clear: bool = True) -> None:
 def autograd_sees(*tensors: torch.Tensor | None) -> bool:
     """Whether autograd has to see a call: an input requires a gradient, or carries a forward-mode tangent (which needs no
     requires_grad; a Function without a jvp refuses it)."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        return True
-    ad = torch.autograd.forward_ad
-    return ad._current_level >= 0 and any(t is not None and ad.unpack_dual(t).tangent is not None for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    if _forward_ad._current_level < 0:
+        return False
+    return any(t is not None and _forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 class _Final(torch.autograd.Function):
@@ -283,10 +287,10 @@ def no_second_derivative(backward):
 
     @functools.wraps(backward)
     def wrapped(ctx, *upstream):
+        if not torch.is_grad_enabled():
+            return backward(ctx, *upstream)
         with torch.no_grad():
             grads = backward(ctx, *upstream)
-        if not torch.is_grad_enabled():
-            return grads
         anchor = torch.empty(0, requires_grad=True)
         final = iter(_Final.apply(anchor, *(g for g in grads if g is not None)))
         return tuple(None if g is None else next(final) for g in grads)
