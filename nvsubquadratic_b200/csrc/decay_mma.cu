@@ -68,7 +68,8 @@ constexpr int kLoader = kThreads / 32, kIssuer = kLoader + 3;  // first loading 
 constexpr int kWriter = kIssuer + 1, kWriters = 4;
 constexpr int kAll = 32 * (kWriter + kWriters);
 // Registers of a thread: computing, loading and issuing, writing; together those of the launch (64 for each of 512). Chosen
-// so that nothing spills: with the shared memory that is taken here a spilled register comes back from L2.
+// so that little spills (bfloat16 heads of 64: nothing): with the shared memory that is taken here a spilled register comes
+// back from L2.
 // Where all warps have something to run at the end, they take the launch's 64 again: after a barrier, since a warp that
 // did so before the computing warps have got their registers would leave them waiting forever.
 template <int DK, bool OUT>
