@@ -250,6 +250,18 @@ __global__ void __launch_bounds__(32 * KW) decay_scan_kernel(const ScanArgs A) {
             S[2 * r][c] = ffma2(ka, vj[c], S[2 * r][c]);
             S[2 * r + 1][c] = ffma2(kb, vj[c], S[2 * r + 1][c]);
           }
+          if constexpr (!fast) {  // rows past the head's size stay zero, where zero times an infinity does not
+            const int rows = A.DK - row0 - 4 * r;
+            if (rows < 4) {
+#pragma unroll
+              for (int c = 0; c < 4; ++c) {
+                if (rows < 1) S[2 * r][c].x = 0.f;
+                if (rows < 2) S[2 * r][c].y = 0.f;
+                if (rows < 3) S[2 * r + 1][c].x = 0.f;
+                S[2 * r + 1][c].y = 0.f;
+              }
+            }
+          }
           if (A.o) {
             const float4 qq = q4[r];
             const float2 qa = make_float2(qq.x, qq.y), qb = make_float2(qq.z, qq.w);

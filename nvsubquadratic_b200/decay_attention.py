@@ -170,7 +170,7 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay
             ``decay_attention_step`` or another call goes on.
 
     Returns ``o [B, L, H, Dv]`` in q's dtype, or ``(o, state)``. Sums and states are float32. An infinity or a NaN
-    reaches what the recurrence lets it reach: no earlier token, no other head.
+    reaches what the recurrence lets it reach: no earlier token, no other head. First derivatives only.
     """
     _check(q, k, v, log_decay, token=False)
     B, L, H, Dk = q.shape

@@ -95,7 +95,7 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
                eps: float = 1e-5) -> torch.Tensor:
     """``(x - mean) / sqrt(var + eps) * weight + bias`` over the last axis of ``x [..., C]`` (float32, bfloat16 or
     float16). weight and bias ``[C]``, each optional, both of x's dtype or both float32. Statistics and sums are float32;
-    the output is rounded once to x's dtype, the parameters' gradients once to theirs."""
+    the output is rounded once to x's dtype, the parameters' gradients once to theirs. First derivatives only."""
     assert x.ndim >= 1 and x.shape[-1] >= 1, f"x must be [..., C]; got {tuple(x.shape)}"
     C = x.shape[-1]
     for name, p in (("weight", weight), ("bias", bias)):

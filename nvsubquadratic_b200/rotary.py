@@ -144,7 +144,7 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, turns: torch.Tensor, *, posi
         positions: int64 or int32, ``[L]`` or ``[B, L]``; ``0 .. L - 1`` by default.
         interleaved: pairs are neighbours ``(2i, 2i + 1)``; by default the two halves ``(i, i + rot_dim / 2)``.
 
-    Returns ``(q', k')`` (k' None without k), contiguous, computed in float32 and rounded once.
+    Returns ``(q', k')`` (k' None without k), contiguous, computed in float32 and rounded once. First derivatives only.
     """
     assert q.ndim == 4, f"q must be [B, L, H, D]; got {tuple(q.shape)}"
     B, L, H, D = q.shape

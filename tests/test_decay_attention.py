@@ -610,3 +610,25 @@ def test_many_chunks(shape, dtype):
     part = [t[some] for t in (q, k, v)] + [g] + [t[some] for t in (s0, do, ds)]
     got = (o.cpu()[some], s.cpu()[some], [t.cpu()[some] if t is not None else None for t in grads])
     _compare(part, got, lengths=lengths[some] if lengths is not None else None, dtype=dtype)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("shape", [(2, 20, 2, 2, 3, 5), (2, 100, 2, 1, 5, 3), (1, 40, 1, 1, 129, 2), (1, 40, 1, 1, 2, 131)], ids=str)
+def test_infinities_of_heads_smaller_than_their_tiles(shape, dtype):
+    """All else positive, so that the recurrence keeps the sign of an infinity in v or do: the places that pad a head count for nothing."""
+    args = [t.abs() if t.ndim > 1 else t for t in _inputs(*shape, dtype)]
+    for i in (2, 5):
+        bad = list(args)
+        bad[i] = args[i].clone()
+        bad[i][0, 7, 0, 1] = float("-inf")
+        q, k, v, g, s0, do, ds = bad
+        o, s, grads = _run(*bad, learn=False)
+        ro, rs = oracle_forward(q, k, v, g, initial_state=s0)
+        ref = decay_attention_grads(q, k, v, g, do, ds, initial_state=s0)
+        assert (ro.isinf() if i == 2 else ref[0].isinf()).any()
+        _same_kinds("o", ro, o, TOL[dtype])
+        _same_kinds("state", rs, s, TOL[F32])
+        for n, r, x in zip(("dq", "dk", "dv"), ref, grads):
+            _same_kinds(n, r, x, TOL[dtype])
+        _same_kinds("dstate", ref[4], grads[4], TOL[F32])
