@@ -332,7 +332,8 @@ struct Place {
 // The CTA's work once more, strictly token by token, for results that are infinite or NaN. The products above run over
 // all pairs of a chunk's tokens and multiply what is masked by zero, so an infinity or a NaN in one token reaches earlier ones, and
 // a difference of two terms makes a NaN of an infinity. Here neither happens: a value reaches what the recurrence lets it reach.
-// A thread holds DK / 8 rows of one column; slow (about 16 tokens in 2 us), and only such results pay for it.
+// A thread holds DK / 8 rows of one column. Slow, and only CTAs with such results pay for it (with every one of them: 128 x 128 grid
+// training 6.8 ms instead of 0.38, 65536 tokens of 8 heads of 128 10.2 instead of 0.30).
 template <int DK, bool OUT, int NT, typename TO>
 __device__ __forceinline__ void scan_by_token(const ScanArgs& A, const Place& z, float* sm) {
   constexpr int kN = 16, kG = kAll / kC, kR = DK / kG;
