@@ -374,6 +374,46 @@ HYFFT_API int hyfft_layer_norm_backward(const void* x, const void* weight, const
                                         int64_t C, int64_t x_stride, int64_t dy_stride, int32_t dtype,
                                         int32_t param_dtype, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------- gated linear recurrence
+ *   a_t = sigmoid(gate_t) (form LOGIT) or exp(gate_t) (form LOG),  s_t = 1 - a_t (complement) or 1
+ *   h_t = a_t h_{t-1} + s_t x_t,   y_t = h_t, or h_t * silu(out_gate_t) where out_gate is given
+ * x, gate, out_gate [B, L, C] of `dtype`, any batch and token strides (0 among them), unit stride over the channels.
+ * lengths: int32 [B] or NULL (all L): tokens from a sequence's length on are neither read nor counted, their outputs and
+ * gradients are zero (values outside 0 .. L are clamped). States: float32 contiguous [B, C]; initial_state NULL means zero.
+ * y and the gradients are contiguous and overwritten; sums are float32, each output rounded once. An infinity or a NaN
+ * reaches what the recurrence lets it reach: no earlier token, no other channel. No counterpart in the reference.         */
+#define HYFFT_GATED_LOGIT 0
+#define HYFFT_GATED_LOG 1
+typedef struct hyfft_gated_desc {
+  int32_t batch, channels, dtype;
+  int32_t form;
+  int32_t complement;
+  int32_t reserved;
+  int64_t length;
+  int64_t x_stride[2]; /* element strides: batch, token */
+  int64_t gate_stride[2];
+  int64_t out_gate_stride[2];
+  int64_t dy_stride[2]; /* the backward's; the forward's y is contiguous */
+} hyfft_gated_desc;
+
+HYFFT_API int hyfft_gated_saved_size(const hyfft_gated_desc* d, size_t* saved_bytes);
+/* final_state: the state after each sequence's last token, or NULL to skip it. saved: what the backward of the same call
+ * reads, or NULL where there is none. */
+HYFFT_API int hyfft_gated_forward(const hyfft_gated_desc* d, const void* x, const void* gate, const void* out_gate,
+                                  const int32_t* lengths, const float* initial_state, void* y, float* final_state,
+                                  void* saved, size_t saved_bytes, void* stream);
+/* Gradients for dy [B, L, C] and dfinal_state (NULL: zero). dinitial_state may be NULL to skip it; dout_gate is needed
+ * where out_gate is given. */
+HYFFT_API int hyfft_gated_backward(const hyfft_gated_desc* d, const void* x, const void* gate, const void* out_gate,
+                                   const int32_t* lengths, const void* saved, size_t saved_bytes, const void* dy,
+                                   const float* dfinal_state, void* dx, void* dgate, void* dout_gate,
+                                   float* dinitial_state, void* stream);
+/* One token of each request: x, gate, out_gate, y [B, C] (the token strides and `length` are not used). state and
+ * out_state: [pool, C], may be the same memory. Slots as in hyfft_decay_step. */
+HYFFT_API int hyfft_gated_step(const hyfft_gated_desc* d, const void* x, const void* gate, const void* out_gate,
+                               const int32_t* slots, int64_t pool, const float* state, float* out_state, void* y,
+                               void* stream);
+
 /* ---------------------------------------------------------------- misc */
 /* Message of the most recent error on this thread ("" if none). */
 HYFFT_API const char* hyfft_last_error(void);

@@ -126,6 +126,22 @@ class RotaryDesc(ctypes.Structure):
     ]
 
 
+class GatedDesc(ctypes.Structure):
+    _fields_ = [
+        ("batch", ctypes.c_int32),
+        ("channels", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("form", ctypes.c_int32),
+        ("complement", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+        ("length", ctypes.c_int64),
+        ("x_stride", ctypes.c_int64 * 2),
+        ("gate_stride", ctypes.c_int64 * 2),
+        ("out_gate_stride", ctypes.c_int64 * 2),
+        ("dy_stride", ctypes.c_int64 * 2),
+    ]
+
+
 SIGNATURES = {
     "hyfft_conv_workspace_size": [ctypes.POINTER(ConvDesc), ctypes.POINTER(_sz), ctypes.POINTER(_sz)],
     "hyfft_conv_forward": [ctypes.POINTER(ConvDesc), _vp, _vp, _vp, _vp, _vp, _sz, _vp],
@@ -156,6 +172,10 @@ SIGNATURES = {
     "hyfft_layer_norm_workspace_size": [_i64, _i64, ctypes.POINTER(_sz)],
     "hyfft_layer_norm_forward": [_vp] * 6 + [_i64, _i64, _i64, ctypes.c_float, _i32, _i32, _vp],
     "hyfft_layer_norm_backward": [_vp] * 8 + [_i64, _i64, _i64, _i64, _i32, _i32, _vp, _sz, _vp],
+    "hyfft_gated_saved_size": [ctypes.POINTER(GatedDesc), ctypes.POINTER(_sz)],
+    "hyfft_gated_forward": [ctypes.POINTER(GatedDesc)] + [_vp] * 8 + [_sz, _vp],
+    "hyfft_gated_backward": [ctypes.POINTER(GatedDesc)] + [_vp] * 5 + [_sz] + [_vp] * 7,
+    "hyfft_gated_step": [ctypes.POINTER(GatedDesc)] + [_vp] * 4 + [_i64] + [_vp] * 4,
     "hyfft_last_error": [],
     "hyfft_version": [],
     "hyfft_launch_count": [],
