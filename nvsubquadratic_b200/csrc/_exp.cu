@@ -1,0 +1,835 @@
+// Gated linear recurrence over sequences (forward, backward) and for single tokens.
+//
+//   a_t = sigmoid(g_t) or exp(g_t),  u_t = 1 - a_t,  s_t = u_t or 1
+//   h_t = a_t h_{t-1} + s_t x_t,     y_t = h_t  or  h_t * silu(o_t)
+//
+//   dh_t = dy_t (* silu(o_t)),  G_t = dh_t + c_{t+1},  c_t = a_t G_t,  c_{T+1} = the final state's gradient
+//   dx_t = s_t G_t,  dg_t = G_t (h_{t-1} - [s_t = u_t] x_t) * (a_t u_t or a_t),  do_t = dy_t h_t silu'(o_t),  dh_0 = c_1
+//
+// Every channel is a recurrence of its own; there is nothing to share but the loads, so the floor is one read of the inputs and one write
+// of the outputs. A CTA takes 128 bytes of channels (a lane: two of 16 bits or one of 32) and 64 tokens at a time, eight
+// for each warp, copied to shared memory one tile ahead. A warp runs its eight tokens from a zero state, which gives the segment's map
+//   h -> A h + H  (backwards: c -> A c + C),
+// the maps go through shared memory in token order, and the tokens are finished with the state that enters them. The state a segment
+// starts from is kept for the backward pass (four bytes for eight tokens of a channel), which then needs nothing else of the forward's.
+//
+// What is exact: A is carried as P + l. P is the product of the rounded decays, whose relative error grows with every token; l = (1 - P) - D
+// with D = 1 - A accumulated as D += u (1 - D), which keeps the digits of slow decays. So a state that remembers 10^5 tokens
+// is off by the roundings of its 10^4 segments, not by those of its decays. In a segment, eight products of rounded decays. Sums are float32.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <math_constants.h>
+
+#include <algorithm>
+#include <atomic>
+#include <map>
+#include <mutex>
+#include <tuple>
+#include <type_traits>
+
+#include "../../include/hyfft.h"
+#include "common.cuh"
+
+namespace hyfft {
+
+extern std::atomic<long long> g_launches;
+int set_error(int code, const char* msg);  // engine.cu: the message hyfft_last_error returns
+
+namespace {
+
+#ifndef SG
+#define SG 16
+#define WP 4
+#endif
+constexpr int kSeg = SG;               // tokens of a warp's segment, and of one saved state
+constexpr int kWarps = WP;
+constexpr int kThreads = 32 * kWarps;
+constexpr int kTile = kSeg * kWarps;   // tokens of a tile
+constexpr int kWidth = 128;            // bytes of a tile's row
+constexpr int kMaxCluster = 8;
+#ifndef FC
+#define FC 4
+#define BC 3
+#endif
+constexpr int kFwdCtas = FC, kBwdCtas = BC;
+
+struct ScanArgs {
+  const char* in[4];          // x, gate, out_gate, dy
+  long long batch[4], tok[4]; // their strides in bytes
+  char* out[3];               // y; or dx, dgate, dout_gate; contiguous
+  const int* lengths;
+  const float* first;         // the state before the first token; backwards the final state's gradient; or NULL
+  float* last;                // the state after the last token; backwards the initial state's gradient; or NULL
+  float* saved;               // [B, segments, C]: the state that enters each segment; or NULL
+  int L, C, cols, segments, complement;
+};
+
+// ---------------------------------------------------------------- a lane's channels: float2 for 16-bit types, float for float32
+
+template <typename T> struct Lane { using F = float2; static constexpr int N = 2; };
+template <> struct Lane<float> { using F = float; static constexpr int N = 1; };
+
+__device__ __forceinline__ float fma_(float a, float b, float c) { return fmaf(a, b, c); }
+__device__ __forceinline__ float2 fma_(float2 a, float2 b, float2 c) { return ffma2(a, b, c); }
+__device__ __forceinline__ float mul_(float a, float b) { return a * b; }
+__device__ __forceinline__ float2 mul_(float2 a, float2 b) {
+  float2 r;
+  asm("{\n.reg .b64 ra, rb, rd;\nmov.b64 ra, {%2, %3};\nmov.b64 rb, {%4, %5};\nmul.rn.f32x2 rd, ra, rb;\n"
+      "mov.b64 {%0, %1}, rd;\n}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float add_(float a, float b) { return a + b; }
+__device__ __forceinline__ float2 add_(float2 a, float2 b) { return cadd(a, b); }
+__device__ __forceinline__ float sub_(float a, float b) { return a - b; }
+__device__ __forceinline__ float2 sub_(float2 a, float2 b) { return csub(a, b); }
+template <typename F> __device__ __forceinline__ F all_(float v);
+template <> __device__ __forceinline__ float all_<float>(float v) { return v; }
+template <> __device__ __forceinline__ float2 all_<float2>(float v) { return make_float2(v, v); }
+// op on every channel of up to three values
+template <typename Op> __device__ __forceinline__ float each_(float a, Op op) { return op(a); }
+template <typename Op> __device__ __forceinline__ float2 each_(float2 a, Op op) { return make_float2(op(a.x), op(a.y)); }
+template <typename Op> __device__ __forceinline__ float each_(float a, float b, Op op) { return op(a, b); }
+template <typename Op> __device__ __forceinline__ float2 each_(float2 a, float2 b, Op op) {
+  return make_float2(op(a.x, b.x), op(a.y, b.y));
+}
+template <typename Op> __device__ __forceinline__ float each_(float a, float b, float c, Op op) { return op(a, b, c); }
+template <typename Op> __device__ __forceinline__ float2 each_(float2 a, float2 b, float2 c, Op op) {
+  return make_float2(op(a.x, b.x, c.x), op(a.y, b.y, c.y));
+}
+template <typename Op> __device__ __forceinline__ bool any_(float a, Op op) { return op(a); }
+template <typename Op> __device__ __forceinline__ bool any_(float2 a, Op op) { return op(a.x) || op(a.y); }
+
+// 2^x and 1 / x to 2 units in the last place, results below 2^-126 flushed to zero.
+__device__ __forceinline__ float exp2_(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float inverse(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+constexpr float kLog2E = 1.4426950408889634f;
+__device__ __forceinline__ float silu_sigmoid(float o) { return inverse(1.0f + exp2_(-kLog2E * o)); }
+
+// The decay and what it leaves, a + u = 1, each without cancellation.
+template <bool LOG>
+__device__ __forceinline__ void decay_of(float g, float& a, float& u) {
+  if constexpr (LOG) {
+    a = exp2_(kLog2E * g);
+    // 1 - exp(g) near 0 by its series (the rest at 0.35 is below 2e-8 of it)
+    float s = fmaf(g, 1.0f / 7, 1.0f);
+    s = fmaf(s, g * (1.0f / 6), 1.0f);
+    s = fmaf(s, g * (1.0f / 5), 1.0f);
+    s = fmaf(s, g * (1.0f / 4), 1.0f);
+    s = fmaf(s, g * (1.0f / 3), 1.0f);
+    s = fmaf(s, g * (1.0f / 2), 1.0f);
+    u = fabsf(g) < 0.35f ? -g * s : 1.0f - a;
+  } else {
+    const float e = exp2_(-kLog2E * fabsf(g));  // in [0, 1]: nothing overflows
+    const float big = inverse(1.0f + e), small = e * big;
+    a = g >= 0.0f ? big : small;
+    u = g >= 0.0f ? small : big;
+  }
+}
+template <bool LOG> __device__ __forceinline__ void decay_of(float2 g, float2& a, float2& u) {
+  decay_of<LOG>(g.x, a.x, u.x);
+  decay_of<LOG>(g.y, a.y, u.y);
+}
+
+// ---------------------------------------------------------------- maps h -> (P + l) h + H
+
+template <typename F> struct Map { F P, l, H; };
+
+__device__ __forceinline__ bool infinite(float v) { return fabsf(v) == CUDART_INF_F; }
+
+// l is a correction of what P says: it does not touch an infinity (which would become a NaN).
+template <typename F> __device__ __forceinline__ F apply(const Map<F>& m, F h) {
+  const F fin = each_(h, [](float v) { return infinite(v) ? 0.0f : v; });
+  return fma_(m.P, h, fma_(m.l, fin, m.H));
+}
+
+// A product of decays above 0 is above 0: an infinite state stays infinite where the product has underflowed.
+__device__ __forceinline__ float above_zero(float p) { return p == 0.0f ? __int_as_float(1) : p; }
+
+template <typename F> __device__ __forceinline__ Map<F> then(const Map<F>& f, const Map<F>& s) {
+  Map<F> r;
+  r.H = apply(s, f.H);
+  const F p = mul_(f.P, s.P);
+  F e = fma_(f.P, s.P, each_(p, [](float v) { return -v; }));
+  e = fma_(f.P, s.l, fma_(s.P, f.l, e));
+  r.P = each_(p, f.P, s.P, [](float v, float a, float b) { return a > 0.0f && b > 0.0f ? above_zero(v) : v; });
+  r.l = each_(e, p, [](float v, float q) { return fabsf(q) < CUDART_INF_F ? v : 0.0f; });
+  return r;
+}
+
+// l of a segment with the product P of its decays and D = 1 - A. Beyond D = 1/2 P is as exact as it gets.
+template <typename F> __device__ __forceinline__ F low_part(F P, F D) {
+  return each_(P, D, [](float p, float d) { return fabsf(d) < 0.5f ? (1.0f - p) - d : 0.0f; });
+}
+
+// ---------------------------------------------------------------- tiles
+
+__device__ __forceinline__ uint32_t smem_of(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+template <int BYTES> __device__ __forceinline__ void copy_async(uint32_t dst, const char* src, int valid) {
+  if constexpr (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(valid) : "memory");
+}
+
+// Rows of 128 bytes where every row starts on 16 bytes (ALIGNED), else the 32-bit words that cover them: 33, and a pitch of 144 bytes.
+template <bool ALIGNED> constexpr int kPitch = ALIGNED ? kWidth : kWidth + 16;
+template <bool ALIGNED> constexpr int kTileBytes = kTile * kPitch<ALIGNED>;
+
+// `rows` tokens from `src` on (the tile's first channel of its first token), `width` bytes of each.
+template <bool ALIGNED>
+__device__ __forceinline__ void load_tile(unsigned char* tile, const char* src, long long stride, int rows, int width) {
+  const uint32_t to = smem_of(tile);
+  if constexpr (ALIGNED) {
+    const int c = 16 * (threadIdx.x & 7), valid = min(16, width - c);
+    if (valid > 0) {
+#pragma unroll
+      for (int i = 0; i < kTile * 8 / kThreads; ++i) {
+        const int r = (threadIdx.x >> 3) + i * (kThreads / 8);
+        if (r < rows) copy_async<16>(to + r * kWidth + c, src + r * stride + c, valid);
+      }
+    }
+  } else {
+    const int lane = threadIdx.x & 31;
+    for (int r = threadIdx.x >> 5; r < rows; r += kWarps) {
+      const char* p = src + r * stride;
+      const int off = (int)(reinterpret_cast<uintptr_t>(p) & 3);
+      for (int w = 4 * lane; w < off + width; w += 128)
+        copy_async<4>(to + r * kPitch<false> + w, p - off + w, min(4, off + width - w));
+    }
+  }
+}
+
+// A lane's channels of row r; `src` as for load_tile.
+template <typename T, bool ALIGNED>
+__device__ __forceinline__ typename Lane<T>::F lane_of(const unsigned char* tile, const char* src, long long stride, int r) {
+  const unsigned char* p = tile + r * kPitch<ALIGNED> + 4 * (threadIdx.x & 31);
+  if constexpr (std::is_same<T, float>::value) {
+    return *reinterpret_cast<const float*>(p);
+  } else if constexpr (ALIGNED) {
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(p);
+    if constexpr (std::is_same<T, __half>::value)
+      return __half22float2(*reinterpret_cast<const __half2*>(&w));
+    else
+      return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  } else {
+    p += reinterpret_cast<uintptr_t>(src + r * stride) & 2;
+    const T* t = reinterpret_cast<const T*>(p);
+    return make_float2(DT<T>::load(t), DT<T>::load(t + 1));
+  }
+}
+
+// A lane's channels to the output; `have` of them exist.
+template <typename T, bool ALIGNED>
+__device__ __forceinline__ void put(T* p, typename Lane<T>::F v, int have) {
+  if constexpr (std::is_same<T, float>::value) {
+    if (have > 0) *p = v;
+  } else if constexpr (ALIGNED) {
+    if (have > 0) {
+      if constexpr (std::is_same<T, __half>::value)
+        *reinterpret_cast<__half2*>(p) = __floats2half2_rn(v.x, v.y);
+      else
+        *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(v.x, v.y);
+    }
+  } else {
+    if (have > 0) DT<T>::store(p, v.x);
+    if (have > 1) DT<T>::store(p + 1, v.y);
+  }
+}
+__device__ __forceinline__ float get_state(const float* p, int have, float) { return have > 0 ? *p : 0.0f; }
+__device__ __forceinline__ float2 get_state(const float* p, int have, float2) {
+  return make_float2(have > 0 ? p[0] : 0.0f, have > 1 ? p[1] : 0.0f);
+}
+__device__ __forceinline__ void put_state(float* p, int have, float v) {
+  if (have > 0) *p = v;
+}
+__device__ __forceinline__ void put_state(float* p, int have, float2 v) {
+  if (have > 0) p[0] = v.x;
+  if (have > 1) p[1] = v.y;
+}
+
+// ---------------------------------------------------------------- clusters
+
+__device__ __forceinline__ int cluster_size() {
+  int r;
+  asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ int cluster_rank() {
+  int r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_meet() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void store_to(uint32_t at, int rank, float v) {
+  uint32_t p;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(p) : "r"(at), "r"(rank));
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(p), "f"(v) : "memory");
+}
+__device__ __forceinline__ void store_to(uint32_t at, int rank, float2 v) {
+  uint32_t p;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(p) : "r"(at), "r"(rank));
+  asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(p), "f"(v.x), "f"(v.y) : "memory");
+}
+
+// The maps of a step's segments, of all warps of a CTA and of all CTAs of a cluster.
+template <typename F> struct Maps {
+  F P[kWarps][32], l[kWarps][32], H[kWarps][32];
+};
+template <typename F> struct CtaMap {  // of one CTA; two sets of a cluster's, used in turn
+  F P[32], l[32], H[32];
+};
+
+// Hands the warps' maps on. order: this warp's place in the direction of the recurrence (the warp, or counted from the last one
+// backwards), place: the CTA's. state: what enters the step; becomes what leaves it. Returns what enters this warp's segment.
+template <typename F>
+__device__ __forceinline__ F hand_on(Maps<F>& M, CtaMap<F>* X, int n, int place, bool back, int turn, const Map<F>& mine,
+                                     F& state) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int order = back ? kWarps - 1 - warp : warp;
+  M.P[order][lane] = mine.P, M.l[order][lane] = mine.l, M.H[order][lane] = mine.H;
+  __syncthreads();
+  if (n == 1) {
+    F h = state, in = state;
+#pragma unroll
+    for (int j = 0; j < kWarps; ++j) {
+      if (j == order) in = h;
+      h = apply(Map<F>{M.P[j][lane], M.l[j][lane], M.H[j][lane]}, h);
+    }
+    state = h;
+    return in;
+  }
+  Map<F> before{all_<F>(1.0f), all_<F>(0.0f), all_<F>(0.0f)};
+  for (int j = 0; j < order; ++j) before = then(before, Map<F>{M.P[j][lane], M.l[j][lane], M.H[j][lane]});
+  CtaMap<F>* Y = X + (turn & 1) * n;
+  if (order == kWarps - 1) {
+    const Map<F> whole = then(before, mine);
+    for (int r = 0; r < n; ++r) {
+      store_to(smem_of(&Y[place].P[lane]), r, whole.P);
+      store_to(smem_of(&Y[place].l[lane]), r, whole.l);
+      store_to(smem_of(&Y[place].H[lane]), r, whole.H);
+    }
+  }
+  cluster_meet();
+  F h = state, in = state;
+  for (int j = 0; j < n; ++j) {
+    if (j == place) in = h;
+    h = apply(Map<F>{Y[j].P[lane], Y[j].l[lane], Y[j].H[lane]}, h);
+  }
+  state = h;
+  return apply(before, in);
+}
+
+// ---------------------------------------------------------------- the passes
+
+// Where a CTA works: one batch row and 128 bytes of channels; the CTAs of a cluster share them and take tiles in turn.
+struct Place {
+  int n, rank, b, col, ch, have, len, steps;
+};
+template <typename T> __device__ __forceinline__ Place place_of(const ScanArgs& A) {
+  Place p;
+  p.n = cluster_size(), p.rank = cluster_rank();
+  const int row = blockIdx.x / p.n;
+  p.b = row / A.cols, p.col = row % A.cols;
+  p.ch = (p.col * 32 + (threadIdx.x & 31)) * Lane<T>::N;
+  p.have = A.C - p.ch;
+  p.len = A.lengths ? min(max(A.lengths[p.b], 0), A.L) : A.L;
+  const int tokens = p.n * kTile;
+  p.steps = (p.len + tokens - 1) / tokens;
+  return p;
+}
+
+// Tokens past the last step's: zeros.
+template <typename T, bool ALIGNED, int OUTS>
+__device__ __forceinline__ void zeros_behind(const ScanArgs& A, const Place& p) {
+  for (int t = p.steps * p.n * kTile + p.rank * kWarps + (threadIdx.x >> 5); t < A.L; t += p.n * kWarps)
+#pragma unroll
+    for (int k = 0; k < OUTS; ++k)
+      put<T, ALIGNED>(reinterpret_cast<T*>(A.out[k]) + ((long long)p.b * A.L + t) * A.C + p.ch, all_<typename Lane<T>::F>(0.0f),
+                      p.have);
+}
+
+template <typename T, bool LOG, bool GATE, bool COMP, bool ALIGNED>
+__global__ void __launch_bounds__(kThreads, kFwdCtas) gated_fwd_kernel(const ScanArgs A) {
+  using F = typename Lane<T>::F;
+  constexpr int K = GATE ? 3 : 2, TB = kTileBytes<ALIGNED>;
+  extern __shared__ __align__(128) unsigned char smem[];
+  Maps<F>& M = *reinterpret_cast<Maps<F>*>(smem + 2 * K * TB);
+  CtaMap<F>* X = reinterpret_cast<CtaMap<F>*>(smem + 2 * K * TB + sizeof(Maps<F>));
+  const Place p = place_of<T>(A);
+  const int warp = threadIdx.x >> 5, width = min(kWidth, A.C * (int)sizeof(T) - p.col * kWidth);
+  const char* in[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) in[k] = A.in[k] + p.b * A.batch[k] + p.col * kWidth;
+  const auto fetch = [&](int step) {
+    const int t = (step * p.n + p.rank) * kTile, rows = min(kTile, p.len - t);
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+      load_tile<ALIGNED>(smem + ((step & 1) * K + k) * TB, in[k] + t * A.tok[k], A.tok[k], rows, width);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  F state = all_<F>(0.0f);
+  if (A.first) state = get_state(A.first + (long long)p.b * A.C + p.ch, p.have, state);
+  if (p.n > 1) cluster_meet();  // the others run, their shared memory can be written
+  if (p.steps > 0) fetch(0);
+  for (int step = 0; step < p.steps; ++step) {
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();
+    if (step + 1 < p.steps) fetch(step + 1);
+    const unsigned char* tile = smem + (step & 1) * K * TB;
+    const int tile0 = (step * p.n + p.rank) * kTile, r0 = warp * kSeg, t0 = tile0 + r0;
+    const int live = min(kSeg, p.len - t0);  // below 1: none
+    const auto value = [&](int k, int i) {
+      return lane_of<T, ALIGNED>(tile + k * TB, in[k] + tile0 * A.tok[k], A.tok[k], r0 + i);
+    };
+    const auto token = [&](int i, F& a, F& u, F& b) {
+      const F x = value(0, i);
+      decay_of<LOG>(value(1, i), a, u);
+      b = COMP ? mul_(u, x) : x;
+    };
+    F hl[kSeg], Pl[kSeg];
+    F h = all_<F>(0.0f), P = all_<F>(1.0f), D = all_<F>(0.0f);
+    const auto gather = [&](auto whole) {  // a branch for each token would keep the tokens' latencies apart
+#pragma unroll
+      for (int i = 0; i < kSeg; ++i) {
+        if (decltype(whole)::value || i < live) {
+          F a, u, b;
+          token(i, a, u, b);
+          h = fma_(a, h, b);
+          P = mul_(P, a);
+          D = fma_(u, sub_(all_<F>(1.0f), D), D);
+        }
+        hl[i] = h, Pl[i] = P;
+      }
+    };
+    if (live >= kSeg)
+      gather(std::true_type{});
+    else
+      gather(std::false_type{});
+    if (any_(P, [](float v) { return v == 0.0f; })) {  // underflow, or a decay of exactly 0?
+      F least = all_<F>(1.0f);
+      for (int i = 0; i < live; ++i) {
+        F a, u, b;
+        token(i, a, u, b);
+        least = each_(least, a, [](float v, float w) { return fminf(v, w); });
+      }
+      P = each_(P, least, [](float v, float w) { return w > 0.0f ? above_zero(v) : v; });
+    }
+    const F enter = hand_on<F>(M, X, p.n, p.rank, false, step, Map<F>{P, low_part(P, D), h}, state);
+    F carry = enter;
+    if (any_(carry, infinite)) {  // token by token, so that an infinity stays one
+      F full = carry;
+#pragma unroll
+      for (int i = 0; i < kSeg; ++i) {
+        if (i < live) {
+          F a, u, b;
+          token(i, a, u, b);
+          full = fma_(a, full, b);
+        }
+        hl[i] = each_(hl[i], full, carry, [](float v, float w, float c) { return infinite(c) ? w : v; });
+        Pl[i] = each_(Pl[i], carry, [](float v, float c) { return infinite(c) ? 0.0f : v; });
+      }
+      carry = each_(carry, [](float v) { return infinite(v) ? 0.0f : v; });
+    }
+    if (A.saved && live > 0) put_state(A.saved + ((long long)p.b * A.segments + t0 / kSeg) * A.C + p.ch, p.have, enter);
+    T* y = reinterpret_cast<T*>(A.out[0]) + ((long long)p.b * A.L + t0) * A.C + p.ch;
+    const auto finish = [&](auto whole) {
+#pragma unroll
+      for (int i = 0; i < kSeg; ++i) {
+        if (decltype(whole)::value || t0 + i < A.L) {
+          F v = all_<F>(0.0f);
+          if (decltype(whole)::value || i < live) {
+            v = fma_(Pl[i], carry, hl[i]);
+            if constexpr (GATE) {
+              const F o = value(2, i);
+              v = mul_(v, mul_(o, each_(o, silu_sigmoid)));
+            }
+          }
+          put<T, ALIGNED>(y + (long long)i * A.C, v, p.have);
+        }
+      }
+    };
+    if (live >= kSeg)
+      finish(std::true_type{});
+    else
+      finish(std::false_type{});
+  }
+  if (A.last && warp == 0 && p.rank == 0) put_state(A.last + (long long)p.b * A.C + p.ch, p.have, state);
+  zeros_behind<T, ALIGNED, 1>(A, p);
+}
+
+template <typename T, bool LOG, bool GATE, bool COMP, bool ALIGNED>
+__global__ void __launch_bounds__(kThreads, kBwdCtas) gated_bwd_kernel(const ScanArgs A) {
+  using F = typename Lane<T>::F;
+  constexpr int K = GATE ? 4 : 3, TB = kTileBytes<ALIGNED>;
+  constexpr int kDy = K - 1;  // x, gate, (out_gate,) dy
+  extern __shared__ __align__(128) unsigned char smem[];
+  Maps<F>& M = *reinterpret_cast<Maps<F>*>(smem + 2 * K * TB);
+  CtaMap<F>* X = reinterpret_cast<CtaMap<F>*>(smem + 2 * K * TB + sizeof(Maps<F>));
+  const Place p = place_of<T>(A);
+  const int warp = threadIdx.x >> 5, width = min(kWidth, A.C * (int)sizeof(T) - p.col * kWidth);
+  const char* in[K];
+  long long tok[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int from = k == kDy ? 3 : k;
+    in[k] = A.in[from] + p.b * A.batch[from] + p.col * kWidth;
+    tok[k] = A.tok[from];
+  }
+  const auto fetch = [&](int step) {
+    const int t = (step * p.n + p.rank) * kTile, rows = min(kTile, p.len - t);
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+      load_tile<ALIGNED>(smem + ((step & 1) * K + k) * TB, in[k] + t * tok[k], tok[k], rows, width);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  F state = all_<F>(0.0f);
+  if (A.first) state = get_state(A.first + (long long)p.b * A.C + p.ch, p.have, state);
+  if (p.n > 1) cluster_meet();
+  if (p.steps > 0) fetch(p.steps - 1);
+  for (int step = p.steps - 1; step >= 0; --step) {
+    const int tile0 = (step * p.n + p.rank) * kTile, r0 = warp * kSeg, t0 = tile0 + r0;
+    const int live = min(kSeg, p.len - t0);
+    F before[kSeg + 1];  // before[i]: the state that enters token i
+    before[0] = all_<F>(0.0f);
+    if (live > 0) before[0] = get_state(A.saved + ((long long)p.b * A.segments + t0 / kSeg) * A.C + p.ch, p.have, before[0]);
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();
+    if (step > 0) fetch(step - 1);
+    const unsigned char* tile = smem + (step & 1) * K * TB;
+    const auto value = [&](int k, int i) {
+      return lane_of<T, ALIGNED>(tile + k * TB, in[k] + tile0 * tok[k], tok[k], r0 + i);
+    };
+    F a[kSeg], u[kSeg], sig[kSeg];
+    F c = all_<F>(0.0f), P = all_<F>(1.0f), D = all_<F>(0.0f), least = all_<F>(1.0f);
+    const auto gather = [&](auto whole) {
+#pragma unroll
+      for (int i = 0; i < kSeg; ++i) {
+        before[i + 1] = before[i];
+        if (decltype(whole)::value || i < live) {
+          const F x = value(0, i);
+          decay_of<LOG>(value(1, i), a[i], u[i]);
+          before[i + 1] = fma_(a[i], before[i], COMP ? mul_(u[i], x) : x);
+        }
+      }
+#pragma unroll
+      for (int i = kSeg - 1; i >= 0; --i) {
+        if (decltype(whole)::value || i < live) {
+          F dh = value(kDy, i);
+          if constexpr (GATE) {
+            const F o = value(2, i);
+            sig[i] = each_(o, silu_sigmoid);
+            dh = mul_(dh, mul_(o, sig[i]));
+          }
+          c = mul_(a[i], add_(dh, c));
+          P = mul_(P, a[i]);
+          D = fma_(u[i], sub_(all_<F>(1.0f), D), D);
+        }
+      }
+    };
+    if (live >= kSeg)
+      gather(std::true_type{});
+    else
+      gather(std::false_type{});
+    if (any_(P, [](float v) { return v == 0.0f; })) {
+#pragma unroll
+      for (int i = 0; i < kSeg; ++i)
+        if (i < live) least = each_(least, a[i], [](float v, float w) { return fminf(v, w); });
+      P = each_(P, least, [](float v, float w) { return w > 0.0f ? above_zero(v) : v; });
+    }
+    c = hand_on<F>(M, X, p.n, p.n - 1 - p.rank, true, step, Map<F>{P, low_part(P, D), c}, state);
+    const long long at = ((long long)p.b * A.L + t0) * A.C + p.ch;
+    const auto finish = [&](auto whole) {
+#pragma unroll
+      for (int i = kSeg - 1; i >= 0; --i) {
+        if (decltype(whole)::value || t0 + i < A.L) {
+          F dx = all_<F>(0.0f), dg = dx;
+          [[maybe_unused]] F dO = dx;
+          if (decltype(whole)::value || i < live) {
+            const F dy = value(kDy, i), x = value(0, i);
+            F dh = dy;
+            if constexpr (GATE) {
+              const F o = value(2, i);
+              dh = mul_(dy, mul_(o, sig[i]));
+              // silu'(o) = sig + o sig (1 - sig)
+              const F slope = mul_(sig[i], fma_(o, sub_(all_<F>(1.0f), sig[i]), all_<F>(1.0f)));
+              dO = mul_(mul_(dy, before[i + 1]), slope);
+            }
+            const F G = add_(dh, c);
+            c = mul_(a[i], G);
+            dx = COMP ? mul_(u[i], G) : G;
+            const F da = mul_(G, COMP ? sub_(before[i], x) : before[i]);
+            dg = mul_(da, LOG ? a[i] : mul_(a[i], u[i]));
+          }
+          const long long to = at + (long long)i * A.C;
+          put<T, ALIGNED>(reinterpret_cast<T*>(A.out[0]) + to, dx, p.have);
+          put<T, ALIGNED>(reinterpret_cast<T*>(A.out[1]) + to, dg, p.have);
+          if constexpr (GATE) put<T, ALIGNED>(reinterpret_cast<T*>(A.out[2]) + to, dO, p.have);
+        }
+      }
+    };
+    if (live >= kSeg)
+      finish(std::true_type{});
+    else
+      finish(std::false_type{});
+  }
+  if (A.last && warp == 0 && p.rank == 0) put_state(A.last + (long long)p.b * A.C + p.ch, p.have, state);
+  zeros_behind<T, ALIGNED, GATE ? 3 : 2>(A, p);
+}
+
+// ---------------------------------------------------------------- single tokens
+
+struct StepArgs {
+  const void *x, *g, *o;
+  long long xb, gb, ob;  // element strides of the batch
+  const int* slots;
+  const float* state;
+  float* out_state;
+  void* y;
+  long long pool;
+  int B, C, complement, units;
+};
+
+// One thread for V neighbouring channels of a request.
+template <typename T, bool LOG, int V>
+__global__ void __launch_bounds__(256) gated_step_kernel(const StepArgs A) {
+  const long long id = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (id >= (long long)A.B * A.units) return;
+  const int b = (int)(id / A.units), c = (int)(id % A.units) * V;
+  struct alignas(V * sizeof(T)) Row { T e[V]; };
+  struct alignas(V * 4) State { float e[V]; };
+  Row& y = *reinterpret_cast<Row*>(static_cast<T*>(A.y) + (long long)b * A.C + c);
+  const long long slot = A.slots ? A.slots[b] : b;
+  Row out;
+  if (slot < 0 || slot >= A.pool) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) DT<T>::store(&out.e[i], 0.0f);
+    y = out;
+    return;
+  }
+  const Row x = *reinterpret_cast<const Row*>(static_cast<const T*>(A.x) + b * A.xb + c);
+  const Row g = *reinterpret_cast<const Row*>(static_cast<const T*>(A.g) + b * A.gb + c);
+  Row o{};
+  if (A.o) o = *reinterpret_cast<const Row*>(static_cast<const T*>(A.o) + b * A.ob + c);
+  State h = *reinterpret_cast<const State*>(A.state + slot * A.C + c);
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    float a, u;
+    decay_of<LOG>(DT<T>::load(&g.e[i]), a, u);
+    const float xi = DT<T>::load(&x.e[i]);
+    h.e[i] = fmaf(a, h.e[i], A.complement ? u * xi : xi);
+    float v = h.e[i];
+    if (A.o) {
+      const float oi = DT<T>::load(&o.e[i]);
+      v *= oi * silu_sigmoid(oi);
+    }
+    DT<T>::store(&out.e[i], v);
+  }
+  *reinterpret_cast<State*>(A.out_state + slot * A.C + c) = h;
+  y = out;
+}
+
+// ---------------------------------------------------------------- host
+
+using Kernel = void (*)(ScanArgs);
+
+template <typename T, bool LOG, bool GATE, bool COMP> Kernel pick3(bool back, bool aligned) {
+  if (back) return aligned ? gated_bwd_kernel<T, LOG, GATE, COMP, true> : gated_bwd_kernel<T, LOG, GATE, COMP, false>;
+  return aligned ? gated_fwd_kernel<T, LOG, GATE, COMP, true> : gated_fwd_kernel<T, LOG, GATE, COMP, false>;
+}
+template <typename T, bool LOG, bool GATE> Kernel pick2(bool back, bool complement, bool aligned) {
+  return complement ? pick3<T, LOG, GATE, true>(back, aligned) : pick3<T, LOG, GATE, false>(back, aligned);
+}
+template <typename T> Kernel pick(bool back, bool log, bool gate, bool complement, bool aligned) {
+  if (log) return gate ? pick2<T, true, true>(back, complement, aligned) : pick2<T, true, false>(back, complement, aligned);
+  return gate ? pick2<T, false, true>(back, complement, aligned) : pick2<T, false, false>(back, complement, aligned);
+}
+
+// Clusters of n CTAs that can run at once (0: unknown), asked once for each kernel, size and device.
+int room_for(Kernel fn, int n, size_t smem) {
+  static std::mutex mu;
+  static std::map<std::tuple<const void*, int, int>, int> known;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  std::lock_guard<std::mutex> lock(mu);
+  const auto key = std::make_tuple(reinterpret_cast<const void*>(fn), n, dev);
+  const auto it = known.find(key);
+  if (it != known.end()) return it->second;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(n), cfg.blockDim = dim3(kThreads), cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim.x = n, at.val.clusterDim.y = 1, at.val.clusterDim.z = 1;
+  cfg.attrs = &at, cfg.numAttrs = 1;
+  int room = 0;
+  if (cudaOccupancyMaxActiveClusters(&room, reinterpret_cast<const void*>(fn), &cfg) != cudaSuccess) {
+    cudaGetLastError();
+    room = 0;
+  }
+  known[key] = room;
+  return room;
+}
+
+int check_desc(const hyfft_gated_desc* d, const char* null_msg) {
+  if (!d) return set_error(HYFFT_ERR_INVALID, null_msg);
+  if (d->batch < 1 || d->length < 1 || d->channels < 1)
+    return set_error(HYFFT_ERR_INVALID, "gated scan: every extent must be positive");
+  if (d->dtype < HYFFT_F32 || d->dtype > HYFFT_F16) return set_error(HYFFT_ERR_INVALID, "gated scan: bad dtype");
+  if (d->form != HYFFT_GATED_LOGIT && d->form != HYFFT_GATED_LOG)
+    return set_error(HYFFT_ERR_INVALID, "gated scan: bad form");
+  // token numbers and the cluster's tiles past the end are 32-bit
+  if (d->length > (1ll << 30) || d->channels > (1 << 28) || (long long)d->batch * ((d->channels + 31) / 32) > (1ll << 27))
+    return set_error(HYFFT_ERR_UNSUPPORTED, "gated scan: too many tokens, channels or rows");
+  return HYFFT_OK;
+}
+
+int run_scan(const hyfft_gated_desc* d, ScanArgs A, bool back, cudaStream_t st) {
+  const int e = d->dtype == HYFFT_F32 ? 4 : 2;
+  const bool gate = A.in[2] != nullptr;
+  A.L = (int)d->length, A.C = d->channels, A.complement = d->complement ? 1 : 0;
+  A.cols = (int)(((long long)A.C * e + kWidth - 1) / kWidth);
+  A.segments = (A.L + kSeg - 1) / kSeg;
+  const int64_t* strides[4] = {d->x_stride, d->gate_stride, d->out_gate_stride, d->dy_stride};
+  bool aligned = (long long)A.C * e % 4 == 0;
+  for (int k = 0; k < 4; ++k) {
+    if (!A.in[k]) continue;
+    A.batch[k] = strides[k][0] * e, A.tok[k] = strides[k][1] * e;
+    aligned = aligned && reinterpret_cast<uintptr_t>(A.in[k]) % 16 == 0 && A.batch[k] % 16 == 0 && A.tok[k] % 16 == 0;
+  }
+  for (int k = 0; k < 3; ++k) aligned = aligned && reinterpret_cast<uintptr_t>(A.out[k]) % 4 == 0;
+  const bool log = d->form == HYFFT_GATED_LOG;
+  const Kernel fn = d->dtype == HYFFT_F32    ? pick<float>(back, log, gate, A.complement, aligned)
+                    : d->dtype == HYFFT_BF16 ? pick<__nv_bfloat16>(back, log, gate, A.complement, aligned)
+                                             : pick<__half>(back, log, gate, A.complement, aligned);
+  const size_t tile = aligned ? kTileBytes<true> : kTileBytes<false>;
+  const size_t one = e == 4 ? sizeof(Maps<float>) : sizeof(Maps<float2>);
+  const size_t cta = 2 * (e == 4 ? sizeof(CtaMap<float>) : sizeof(CtaMap<float2>));
+  const auto smem_for = [&](int n) { return 2 * tile * ((gate ? 3 : 2) + (back ? 1 : 0)) + one + (n > 1 ? n * cta : 0); };
+  if (!kernel_smem_once(reinterpret_cast<const void*>(fn), smem_for(kMaxCluster), true))
+    return set_error(HYFFT_ERR_CUDA, "gated scan: shared memory");
+  // As many CTAs for a row as the machine can run at once for all rows, and as the row has tiles.
+  const long long rows = (long long)d->batch * A.cols;
+  int n = kMaxCluster;
+  while (n > 1 && ((long long)(n / 2) * kTile >= A.L || room_for(fn, n, smem_for(n)) < rows)) n /= 2;
+#ifdef FORCE_N
+  if (getenv("FN")) n = atoi(getenv("FN"));
+#endif
+  if (n > 1) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(rows * n)), cfg.blockDim = dim3(kThreads), cfg.dynamicSmemBytes = smem_for(n), cfg.stream = st;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = n, at.val.clusterDim.y = 1, at.val.clusterDim.z = 1;
+    cfg.attrs = &at, cfg.numAttrs = 1;
+    if (cudaLaunchKernelEx(&cfg, fn, A) != cudaSuccess) {
+      cudaGetLastError();
+      return set_error(HYFFT_ERR_CUDA, "gated scan: kernel launch failed");
+    }
+  } else {
+    fn<<<(unsigned)rows, kThreads, smem_for(1), st>>>(A);
+  }
+  if (cudaGetLastError() != cudaSuccess) return set_error(HYFFT_ERR_CUDA, "gated scan: kernel launch failed");
+  g_launches.fetch_add(1, std::memory_order_relaxed);
+  return HYFFT_OK;
+}
+
+template <typename T, bool LOG> int launch_step(StepArgs A, cudaStream_t st) {
+  // 16 bytes of state and 4 elements at once where all rows start on their boundaries
+  constexpr int V = 4;
+  bool wide = A.C % V == 0 && A.xb % V == 0 && A.gb % V == 0 && (!A.o || A.ob % V == 0);
+  for (const void* p : {A.x, A.g, A.o, (const void*)A.y}) wide = wide && reinterpret_cast<uintptr_t>(p) % (V * sizeof(T)) == 0;
+  for (const void* p : {(const void*)A.state, (const void*)A.out_state}) wide = wide && reinterpret_cast<uintptr_t>(p) % 16 == 0;
+  A.units = wide ? A.C / V : A.C;
+  const long long ctas = ((long long)A.B * A.units + 255) / 256;
+  if (ctas > 0x7fffffffLL) return set_error(HYFFT_ERR_UNSUPPORTED, "gated step: too many elements");
+  if (wide)
+    gated_step_kernel<T, LOG, V><<<(unsigned)ctas, 256, 0, st>>>(A);
+  else
+    gated_step_kernel<T, LOG, 1><<<(unsigned)ctas, 256, 0, st>>>(A);
+  if (cudaGetLastError() != cudaSuccess) return set_error(HYFFT_ERR_CUDA, "gated step: kernel launch failed");
+  g_launches.fetch_add(1, std::memory_order_relaxed);
+  return HYFFT_OK;
+}
+template <typename T> int launch_step(const StepArgs& A, bool log, cudaStream_t st) {
+  return log ? launch_step<T, true>(A, st) : launch_step<T, false>(A, st);
+}
+
+}  // namespace
+}  // namespace hyfft
+
+using namespace hyfft;
+
+extern "C" int hyfft_gated_saved_size(const hyfft_gated_desc* d, size_t* saved_bytes) {
+  if (int rc = check_desc(d, "gated scan: null descriptor")) return rc;
+  if (!saved_bytes) return set_error(HYFFT_ERR_INVALID, "gated scan: null size");
+  *saved_bytes = sizeof(float) * (size_t)d->batch * (size_t)((d->length + kSeg - 1) / kSeg) * (size_t)d->channels;
+  return HYFFT_OK;
+}
+
+extern "C" int hyfft_gated_forward(const hyfft_gated_desc* d, const void* x, const void* gate, const void* out_gate,
+                                   const int32_t* lengths, const float* initial_state, void* y, float* final_state,
+                                   void* saved, size_t saved_bytes, void* stream) {
+  if (int rc = check_desc(d, "gated scan: null descriptor")) return rc;
+  if (!x || !gate || !y) return set_error(HYFFT_ERR_INVALID, "gated scan: null tensor");
+  size_t need = 0;
+  if (int rc = hyfft_gated_saved_size(d, &need)) return rc;
+  if (saved && saved_bytes < need) return set_error(HYFFT_ERR_WORKSPACE, "gated scan: saved buffer too small");
+  if (bind_device_of(x) != HYFFT_OK) return set_error(HYFFT_ERR_CUDA, "gated scan: device");
+  ScanArgs A{};
+  A.in[0] = static_cast<const char*>(x), A.in[1] = static_cast<const char*>(gate);
+  A.in[2] = static_cast<const char*>(out_gate);
+  A.out[0] = static_cast<char*>(y);
+  A.lengths = lengths, A.first = initial_state, A.last = final_state, A.saved = static_cast<float*>(saved);
+  return run_scan(d, A, false, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int hyfft_gated_backward(const hyfft_gated_desc* d, const void* x, const void* gate, const void* out_gate,
+                                    const int32_t* lengths, const void* saved, size_t saved_bytes, const void* dy,
+                                    const float* dfinal_state, void* dx, void* dgate, void* dout_gate,
+                                    float* dinitial_state, void* stream) {
+  if (int rc = check_desc(d, "gated scan: null descriptor")) return rc;
+  if (!x || !gate || !dy || !dx || !dgate || (out_gate && !dout_gate))
+    return set_error(HYFFT_ERR_INVALID, "gated scan: null tensor");
+  size_t need = 0;
+  if (int rc = hyfft_gated_saved_size(d, &need)) return rc;
+  if (!saved || saved_bytes < need) return set_error(HYFFT_ERR_WORKSPACE, "gated scan: saved buffer missing or too small");
+  if (bind_device_of(x) != HYFFT_OK) return set_error(HYFFT_ERR_CUDA, "gated scan: device");
+  ScanArgs A{};
+  A.in[0] = static_cast<const char*>(x), A.in[1] = static_cast<const char*>(gate);
+  A.in[2] = static_cast<const char*>(out_gate), A.in[3] = static_cast<const char*>(dy);
+  A.out[0] = static_cast<char*>(dx), A.out[1] = static_cast<char*>(dgate);
+  A.out[2] = out_gate ? static_cast<char*>(dout_gate) : nullptr;
+  A.lengths = lengths, A.first = dfinal_state, A.last = dinitial_state;
+  A.saved = const_cast<float*>(static_cast<const float*>(saved));
+  return run_scan(d, A, true, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int hyfft_gated_step(const hyfft_gated_desc* d, const void* x, const void* gate, const void* out_gate,
+                                const int32_t* slots, int64_t pool, const float* state, float* out_state, void* y,
+                                void* stream) {
+  if (int rc = check_desc(d, "gated step: null descriptor")) return rc;
+  if (!x || !gate || !state || !out_state || !y) return set_error(HYFFT_ERR_INVALID, "gated step: null tensor");
+  if (pool < 1 || (!slots && pool < d->batch)) return set_error(HYFFT_ERR_INVALID, "gated step: too few states");
+  if (bind_device_of(x) != HYFFT_OK) return set_error(HYFFT_ERR_CUDA, "gated step: device");
+  StepArgs A{};
+  A.x = x, A.g = gate, A.o = out_gate, A.slots = slots, A.state = state, A.out_state = out_state, A.y = y;
+  A.xb = d->x_stride[0], A.gb = d->gate_stride[0], A.ob = d->out_gate_stride[0];
+  A.pool = pool, A.B = d->batch, A.C = d->channels, A.complement = d->complement ? 1 : 0;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool log = d->form == HYFFT_GATED_LOG;
+  if (d->dtype == HYFFT_F32) return launch_step<float>(A, log, st);
+  if (d->dtype == HYFFT_BF16) return launch_step<__nv_bfloat16>(A, log, st);
+  return launch_step<__half>(A, log, st);
+}

@@ -7,11 +7,18 @@
 //   dx_t = s_t G_t,  dg_t = G_t (h_{t-1} - [s_t = u_t] x_t) * (a_t u_t or a_t),  do_t = dy_t h_t silu'(o_t),  dh_0 = c_1
 //
 // Every channel is a recurrence of its own; there is nothing to share but the loads, so the floor is one read of the inputs and one write
-// of the outputs. A CTA takes 128 bytes of channels (a lane: two of 16 bits or one of 32) and 64 tokens at a time, eight
-// for each warp, copied to shared memory one tile ahead. A warp runs its eight tokens from a zero state, which gives the segment's map
+// of the outputs. A CTA takes 128 bytes of channels (a lane: two of 16 bits or one of 32) and 64 tokens at a time, 16 (backwards 8)
+// for each warp, copied to shared memory one tile ahead. A warp runs its tokens from a zero state, which gives the segment's map
 //   h -> A h + H  (backwards: c -> A c + C),
-// the maps go through shared memory in token order, and the tokens are finished with the state that enters them. The state a segment
-// starts from is kept for the backward pass (four bytes for eight tokens of a channel), which then needs nothing else of the forward's.
+// the maps go through shared memory in token order, and the tokens are finished with the state that enters them. Every eighth token's
+// state is kept for the backward pass (four bytes for eight tokens of a channel), which then needs nothing else of the forward's.
+//
+// Where there are fewer rows (batch x 128 bytes of channels) than CTAs that fit the machine, the CTAs of a cluster take a row's tiles in
+// turn: each passes the state that leaves its tile on to the next one's shared memory. In steady state a CTA has its tile's map
+// before the state arrives, so a hop is a wait, one map and one remote store (0.26 us), and the data still goes through once. 65536
+// tokens of 4096 channels, bfloat16, with output gates: one CTA a row 1.54 ms, eight in a cluster 0.49 ms (all of a
+// cluster's maps exchanged behind a barrier: 0.73); 64 x 2048 tokens of 1024 channels, one CTA a row, 193 us (8 bytes an element: 85% of
+// a copy's rate). What is left is instruction issue: about 35 an element forwards and 52 backwards, two of them roundings' unpacking.
 //
 // What is exact: A is carried as P + l. P is the product of the rounded decays, whose relative error grows with every token; l = (1 - P) - D
 // with D = 1 - A accumulated as D += u (1 - D), which keeps the digits of slow decays. So a state that remembers 10^5 tokens
@@ -26,9 +33,11 @@
 #include <map>
 #include <mutex>
 #include <tuple>
+#include <type_traits>
 
 #include "../../include/hyfft.h"
 #include "common.cuh"
+#include "waits.cuh"
 
 namespace hyfft {
 
@@ -37,12 +46,16 @@ int set_error(int code, const char* msg);  // engine.cu: the message hyfft_last_
 
 namespace {
 
-constexpr int kSeg = 8;                // tokens of a warp's segment, and of one saved state
-constexpr int kWarps = 8;
-constexpr int kThreads = 32 * kWarps;
-constexpr int kTile = kSeg * kWarps;   // tokens of a tile
+// A pass's tile: SEG tokens for each of WARPS warps, and how many CTAs of it an SM holds at least.
+template <int SEG, int WARPS, int CTAS> struct Shape {
+  static constexpr int kSeg = SEG, kWarps = WARPS, kCtas = CTAS, kThreads = 32 * WARPS, kTile = SEG * WARPS;
+};
+using Fwd = Shape<16, 4, 4>;
+using Bwd = Shape<8, 8, 2>;
+constexpr int kSaved = Bwd::kSeg;      // tokens from one saved state to the next
+static_assert(Fwd::kSeg % kSaved == 0, "the forward pass has the saved states at hand");
 constexpr int kWidth = 128;            // bytes of a tile's row
-constexpr int kMaxCluster = 8;
+constexpr int kMaxCluster = 16;       // above 8 by a kernel attribute
 
 struct ScanArgs {
   const char* in[4];          // x, gate, out_gate, dy
@@ -53,6 +66,8 @@ struct ScanArgs {
   float* last;                // the state after the last token; backwards the initial state's gradient; or NULL
   float* saved;               // [B, segments, C]: the state that enters each segment; or NULL
   int L, C, cols, segments, complement;
+  int n;                      // CTAs of a cluster
+  unsigned patience;          // clocks that a wait may take
 };
 
 // ---------------------------------------------------------------- a lane's channels: float2 for 16-bit types, float for float32
@@ -92,31 +107,42 @@ template <typename Op> __device__ __forceinline__ float2 each_(float2 a, float2 
 template <typename Op> __device__ __forceinline__ bool any_(float a, Op op) { return op(a); }
 template <typename Op> __device__ __forceinline__ bool any_(float2 a, Op op) { return op(a.x) || op(a.y); }
 
-__device__ __forceinline__ float silu_sigmoid(float o) { return __fdividef(1.0f, 1.0f + __expf(-o)); }
+// 2^x and 1 / x to 2 units in the last place, results below 2^-126 flushed to zero.
+__device__ __forceinline__ float exp2_(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float inverse(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+constexpr float kLog2E = 1.4426950408889634f;
+template <typename F> __device__ __forceinline__ F sigmoid_of(F o) {
+  const F e = each_(mul_(o, all_<F>(-kLog2E)), exp2_);
+  return each_(add_(e, all_<F>(1.0f)), inverse);
+}
 
 // The decay and what it leaves, a + u = 1, each without cancellation.
-template <bool LOG>
-__device__ __forceinline__ void decay_of(float g, float& a, float& u) {
+template <bool LOG, typename F> __device__ __forceinline__ void decay_of(F g, F& a, F& u) {
   if constexpr (LOG) {
-    a = __expf(g);
+    a = each_(mul_(g, all_<F>(kLog2E)), exp2_);
     // 1 - exp(g) near 0 by its series (the rest at 0.35 is below 2e-8 of it)
-    float s = fmaf(g, 1.0f / 7, 1.0f);
-    s = fmaf(s, g * (1.0f / 6), 1.0f);
-    s = fmaf(s, g * (1.0f / 5), 1.0f);
-    s = fmaf(s, g * (1.0f / 4), 1.0f);
-    s = fmaf(s, g * (1.0f / 3), 1.0f);
-    s = fmaf(s, g * (1.0f / 2), 1.0f);
-    u = fabsf(g) < 0.35f ? -g * s : 1.0f - a;
+    const F one = all_<F>(1.0f);
+    F s = fma_(g, all_<F>(1.0f / 7), one);
+    s = fma_(s, mul_(g, all_<F>(1.0f / 6)), one);
+    s = fma_(s, mul_(g, all_<F>(1.0f / 5)), one);
+    s = fma_(s, mul_(g, all_<F>(1.0f / 4)), one);
+    s = fma_(s, mul_(g, all_<F>(1.0f / 3)), one);
+    s = fma_(s, mul_(g, all_<F>(1.0f / 2)), one);
+    u = each_(g, mul_(g, s), sub_(one, a), [](float v, float near, float far) { return fabsf(v) < 0.35f ? -near : far; });
   } else {
-    const float e = __expf(-fabsf(g));  // in (0, 1]: nothing overflows
-    const float big = __fdividef(1.0f, 1.0f + e), small = e * big;
-    a = g >= 0.0f ? big : small;
-    u = g >= 0.0f ? small : big;
+    const F e = each_(mul_(g, all_<F>(-kLog2E)), exp2_);
+    a = each_(add_(e, all_<F>(1.0f)), inverse);
+    // e a, which is 1 - a; where e has overflowed and a is 0 that is a NaN or 0, and 1 - 2 a is 1 (below 1 - a everywhere)
+    u = each_(mul_(e, a), fma_(a, all_<F>(-2.0f), all_<F>(1.0f)), [](float v, float w) { return fmaxf(v, w); });
   }
-}
-template <bool LOG> __device__ __forceinline__ void decay_of(float2 g, float2& a, float2& u) {
-  decay_of<LOG>(g.x, a.x, u.x);
-  decay_of<LOG>(g.y, a.y, u.y);
 }
 
 // ---------------------------------------------------------------- maps h -> (P + l) h + H
@@ -125,18 +151,20 @@ template <typename F> struct Map { F P, l, H; };
 
 __device__ __forceinline__ bool infinite(float v) { return fabsf(v) == CUDART_INF_F; }
 
-// l is a correction of what P says: it does not touch an infinity (which would become a NaN).
-template <typename F> __device__ __forceinline__ F apply(const Map<F>& m, F h) {
-  const F fin = each_(h, [](float v) { return infinite(v) ? 0.0f : v; });
-  return fma_(m.P, h, fma_(m.l, fin, m.H));
+template <typename F> __device__ __forceinline__ F apply(const Map<F>& m, F h) { return fma_(m.P, h, fma_(m.l, h, m.H)); }
+// l is a correction of what P says: it leaves an infinity alone (which would become a NaN).
+template <typename F> __device__ __forceinline__ F apply_to_infinity(const Map<F>& m, F h) {
+  return fma_(m.P, h, fma_(m.l, each_(h, [](float v) { return infinite(v) ? 0.0f : v; }), m.H));
 }
 
 // A product of decays above 0 is above 0: an infinite state stays infinite where the product has underflowed.
 __device__ __forceinline__ float above_zero(float p) { return p == 0.0f ? __int_as_float(1) : p; }
 
+// First f, then s.
 template <typename F> __device__ __forceinline__ Map<F> then(const Map<F>& f, const Map<F>& s) {
   Map<F> r;
   r.H = apply(s, f.H);
+  if (any_(r.H, [](float v) { return v != v; })) r.H = apply_to_infinity(s, f.H);
   const F p = mul_(f.P, s.P);
   F e = fma_(f.P, s.P, each_(p, [](float v) { return -v; }));
   e = fma_(f.P, s.l, fma_(s.P, f.l, e));
@@ -162,24 +190,24 @@ template <int BYTES> __device__ __forceinline__ void copy_async(uint32_t dst, co
 
 // Rows of 128 bytes where every row starts on 16 bytes (ALIGNED), else the 32-bit words that cover them: 33, and a pitch of 144 bytes.
 template <bool ALIGNED> constexpr int kPitch = ALIGNED ? kWidth : kWidth + 16;
-template <bool ALIGNED> constexpr int kTileBytes = kTile * kPitch<ALIGNED>;
+template <typename S, bool ALIGNED> constexpr int kTileBytes = S::kTile * kPitch<ALIGNED>;
 
 // `rows` tokens from `src` on (the tile's first channel of its first token), `width` bytes of each.
-template <bool ALIGNED>
+template <typename S, bool ALIGNED>
 __device__ __forceinline__ void load_tile(unsigned char* tile, const char* src, long long stride, int rows, int width) {
   const uint32_t to = smem_of(tile);
   if constexpr (ALIGNED) {
     const int c = 16 * (threadIdx.x & 7), valid = min(16, width - c);
     if (valid > 0) {
 #pragma unroll
-      for (int i = 0; i < kTile * 8 / kThreads; ++i) {
-        const int r = (threadIdx.x >> 3) + i * (kThreads / 8);
+      for (int i = 0; i < S::kTile * 8 / S::kThreads; ++i) {
+        const int r = (threadIdx.x >> 3) + i * (S::kThreads / 8);
         if (r < rows) copy_async<16>(to + r * kWidth + c, src + r * stride + c, valid);
       }
     }
   } else {
     const int lane = threadIdx.x & 31;
-    for (int r = threadIdx.x >> 5; r < rows; r += kWarps) {
+    for (int r = threadIdx.x >> 5; r < rows; r += S::kWarps) {
       const char* p = src + r * stride;
       const int off = (int)(reinterpret_cast<uintptr_t>(p) & 3);
       for (int w = 4 * lane; w < off + width; w += 128)
@@ -207,21 +235,24 @@ __device__ __forceinline__ typename Lane<T>::F lane_of(const unsigned char* tile
   }
 }
 
-// A lane's channels to the output; `have` of them exist.
+// base + i * stride (elements): the compiler keeps the three bases and one stride of the backward pass in registers.
+template <typename T> __device__ __forceinline__ T* row_at(T* base, unsigned stride, unsigned i) {
+  T* r;
+  asm("mad.wide.u32 %0, %1, %2, %3;" : "=l"(r) : "r"(stride), "r"(i * (unsigned)sizeof(T)), "l"(base));
+  return r;
+}
+// A lane's channels to the output; `have` (1 at least) of them exist.
 template <typename T, bool ALIGNED>
 __device__ __forceinline__ void put(T* p, typename Lane<T>::F v, int have) {
   if constexpr (std::is_same<T, float>::value) {
-    if (have > 0) *p = v;
-  } else if constexpr (ALIGNED) {
-    if (have > 0) {
-      if constexpr (std::is_same<T, __half>::value)
-        *reinterpret_cast<__half2*>(p) = __floats2half2_rn(v.x, v.y);
-      else
-        *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(v.x, v.y);
-    }
-  } else {
-    if (have > 0) DT<T>::store(p, v.x);
+    *p = v;
+  } else if constexpr (!ALIGNED) {
+    DT<T>::store(p, v.x);
     if (have > 1) DT<T>::store(p + 1, v.y);
+  } else if constexpr (std::is_same<T, __half>::value) {
+    *reinterpret_cast<__half2*>(p) = __floats2half2_rn(v.x, v.y);
+  } else {
+    *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(v.x, v.y);
   }
 }
 __device__ __forceinline__ float get_state(const float* p, int have, float) { return have > 0 ? *p : 0.0f; }
@@ -236,157 +267,230 @@ __device__ __forceinline__ void put_state(float* p, int have, float2 v) {
   if (have > 1) p[1] = v.y;
 }
 
-// ---------------------------------------------------------------- clusters
+// ---------------------------------------------------------------- a row's tiles among the CTAs of a cluster
 
-__device__ __forceinline__ int cluster_size() {
-  int r;
-  asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ int cluster_rank() {
-  int r;
-  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
 __device__ __forceinline__ void cluster_meet() {
   asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ void store_to(uint32_t at, int rank, float v) {
+__device__ __forceinline__ uint32_t at_rank(uint32_t own, int rank) {
   uint32_t p;
-  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(p) : "r"(at), "r"(rank));
-  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(p), "f"(v) : "memory");
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(p) : "r"(own), "r"(rank));
+  return p;
 }
-__device__ __forceinline__ void store_to(uint32_t at, int rank, float2 v) {
-  uint32_t p;
-  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(p) : "r"(at), "r"(rank));
-  asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(p), "f"(v.x), "f"(v.y) : "memory");
+// Writes to another CTA's shared memory and counts the bytes at a barrier there.
+__device__ __forceinline__ void send(uint32_t to, uint32_t bar, float v) {
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(to),
+               "r"(__float_as_uint(v)), "r"(bar)
+               : "memory");
+}
+__device__ __forceinline__ void send(uint32_t to, uint32_t bar, float2 v) {
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.b32 [%0], {%1, %2}, [%3];" ::"r"(to),
+               "r"(__float_as_uint(v.x)), "r"(__float_as_uint(v.y)), "r"(bar)
+               : "memory");
+}
+__device__ __forceinline__ void arm(uint32_t bar, int bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ bool try_message(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n.reg .pred p;\nmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(done)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return done != 0;
+}
+__device__ __forceinline__ bool test_message(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n.reg .pred p;\nmbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(done)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return done != 0;
+}
+// Waits for a message; false after `patience` clocks (0: without waiting).
+__device__ __forceinline__ bool wait_message(uint32_t bar, uint32_t parity, unsigned patience) {
+  if (patience ? try_message(bar, parity) : test_message(bar, parity)) return true;
+  const unsigned t0 = (unsigned)clock64();
+  do {
+    if ((unsigned)clock64() - t0 >= patience) return false;
+  } while (!try_message(bar, parity));
+  return true;
 }
 
-// The maps of a step's segments, of all warps of a CTA and of all CTAs of a cluster.
-template <typename F> struct Maps {
-  F P[kWarps][32], l[kWarps][32], H[kWarps][32];
+// The maps of a tile's segments, and the states that enter tiles: two, used in turn. Where another CTA has the tile before, it sends
+// them. The next one into a place is written only after this CTA's last warp has handed on the one in between, so after all warps have read it.
+template <typename F, int WARPS> struct Board {
+  F P[WARPS][32], l[WARPS][32], H[WARPS][32];
+  F inbox[2][32];
+  unsigned long long full[2];
 };
-template <typename F> struct CtaMaps {  // two of them, used in turn
-  F P[kMaxCluster][32], l[kMaxCluster][32], H[kMaxCluster][32];
-};
 
-// Hands the warps' maps on. order: this warp's place in the direction of the recurrence (the warp, or counted from the last one
-// backwards), place: the CTA's. state: what enters the step; becomes what leaves it. Returns what enters this warp's segment.
-template <typename F>
-__device__ __forceinline__ F hand_on(Maps<F>& M, CtaMaps<F>* X, int n, int place, bool back, int turn, const Map<F>& mine,
-                                     F& state) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int order = back ? kWarps - 1 - warp : warp;
-  M.P[order][lane] = mine.P, M.l[order][lane] = mine.l, M.H[order][lane] = mine.H;
-  __syncthreads();
-  if (n == 1) {
-    F h = state, in = state;
-#pragma unroll
-    for (int j = 0; j < kWarps; ++j) {
-      if (j == order) in = h;
-      h = apply(Map<F>{M.P[j][lane], M.l[j][lane], M.H[j][lane]}, h);
-    }
-    state = h;
-    return in;
-  }
-  Map<F> before{all_<F>(1.0f), all_<F>(0.0f), all_<F>(0.0f)};
-  for (int j = 0; j < order; ++j) before = then(before, Map<F>{M.P[j][lane], M.l[j][lane], M.H[j][lane]});
-  CtaMaps<F>& Y = X[turn & 1];
-  if (order == kWarps - 1) {
-    const Map<F> whole = then(before, mine);
-    for (int r = 0; r < n; ++r) {
-      store_to(smem_of(&Y.P[place][lane]), r, whole.P);
-      store_to(smem_of(&Y.l[place][lane]), r, whole.l);
-      store_to(smem_of(&Y.H[place][lane]), r, whole.H);
-    }
-  }
-  cluster_meet();
-  F h = state, in = state;
-  for (int j = 0; j < n; ++j) {
-    if (j == place) in = h;
-    h = apply(Map<F>{Y.P[j][lane], Y.l[j][lane], Y.H[j][lane]}, h);
-  }
-  state = h;
-  return apply(before, in);
-}
-
-// ---------------------------------------------------------------- the passes
-
-// Where a CTA works: one batch row and 128 bytes of channels; the CTAs of a cluster share them and take tiles in turn.
+// Where a CTA works: one batch row and 128 bytes of channels. The n CTAs of a cluster take the row's tiles in turn, each passing the
+// state that leaves its tile to the next.
 struct Place {
-  int n, rank, b, col, ch, have, len, steps;
+  int n, rank, b, col, ch, have, len, tiles;
 };
-template <typename T> __device__ __forceinline__ Place place_of(const ScanArgs& A) {
+template <typename T, typename S> __device__ __forceinline__ Place place_of(const ScanArgs& A) {
   Place p;
-  p.n = cluster_size(), p.rank = cluster_rank();
-  const int row = blockIdx.x / p.n;
+  p.n = A.n, p.rank = blockIdx.x % A.n;  // a cluster's CTAs are neighbours
+  const int row = blockIdx.x / A.n;
   p.b = row / A.cols, p.col = row % A.cols;
   p.ch = (p.col * 32 + (threadIdx.x & 31)) * Lane<T>::N;
   p.have = A.C - p.ch;
   p.len = A.lengths ? min(max(A.lengths[p.b], 0), A.L) : A.L;
-  const int tokens = p.n * kTile;
-  p.steps = (p.len + tokens - 1) / tokens;
+  p.tiles = (p.len + S::kTile - 1) / S::kTile;
   return p;
 }
 
-// Tokens past the last step's: zeros.
-template <typename T, bool ALIGNED, int OUTS>
-__device__ __forceinline__ void zeros_behind(const ScanArgs& A, const Place& p) {
-  for (int t = p.steps * p.n * kTile + p.rank * kWarps + (threadIdx.x >> 5); t < A.L; t += p.n * kWarps)
-#pragma unroll
-    for (int k = 0; k < OUTS; ++k)
-      put<T, ALIGNED>(reinterpret_cast<T*>(A.out[k]) + ((long long)p.b * A.L + t) * A.C + p.ch, all_<typename Lane<T>::F>(0.0f),
-                      p.have);
+template <typename F, int WARPS> __device__ __forceinline__ void open_board(Board<F, WARPS>& B, const Place& p) {
+  if (p.n == 1) return;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_of(&B.full[i])) : "memory");
+      arm(smem_of(&B.full[i]), 32 * sizeof(F));
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  cluster_meet();  // the others run, and their barriers are there
+}
+// No CTA leaves while another may still write to it. A CTA that has given up on a message gives those on their way time to land.
+__device__ __forceinline__ void close_board(const Place& p, bool lost) {
+  if (p.n == 1) return;
+  cluster_meet();
+  if (lost)
+    for (const unsigned t0 = (unsigned)clock64(); (unsigned)clock64() - t0 < (1u << 20);) {
+    }
 }
 
-template <typename T, bool LOG, bool GATE, bool ALIGNED>
-__global__ void __launch_bounds__(kThreads) gated_fwd_kernel(const ScanArgs A) {
+// Hands the maps of a tile's segments on. k: the tile's number in the order of the recurrence, step: how many this CTA has done
+// before; order: this warp's place within the tile. state: what enters the first tile; in the last warp, what leaves each. Returns what
+// enters this warp's segment: NaN from the first message on that did not come (lost).
+template <typename F, int WARPS>
+__device__ __forceinline__ F hand_on(Board<F, WARPS>& B, const Place& p, int k, int step, int order, const Map<F>& mine, F& state,
+                                     unsigned patience, bool& lost) {
+  const int lane = threadIdx.x & 31;
+  B.P[order][lane] = mine.P, B.l[order][lane] = mine.l, B.H[order][lane] = mine.H;
+  __syncthreads();
+  const auto map_of = [&](int j) { return Map<F>{B.P[j][lane], B.l[j][lane], B.H[j][lane]}; };
+  const auto through = [&](const Map<F>& m, F h) {
+    const F r = apply(m, h);
+    return any_(r, [](float v) { return v != v; }) ? apply_to_infinity(m, h) : r;
+  };
+  // What leaves the tile goes by one map over all of it, which is there before the message is: the next CTA waits for nothing else.
+  const bool last = order == WARPS - 1;
+  Map<F> whole = mine;
+  if (last && p.n > 1) {
+    Map<F> m = map_of(0);
+#pragma unroll 1
+    for (int j = 1; j < WARPS - 1; ++j) m = then(m, map_of(j));
+    whole = then(m, mine);
+  }
+  if (p.n == 1 && WARPS <= 4) {
+    F h = state, in = state;
+#pragma unroll
+    for (int j = 0; j < WARPS; ++j) {
+      if (j == order) in = h;
+      h = through(map_of(j), h);
+    }
+    state = h;
+    return in;
+  }
+  F h = state;
+  if (k > 0) {
+    // the message's number: the first CTA of a cluster gets none for its first tile, a CTA alone leaves them to itself
+    const int m = p.rank > 0 ? step : step - 1;
+    if (p.n > 1) {
+      const uint32_t bar = smem_of(&B.full[m & 1]);
+      if (!lost) lost = !__all_sync(0xffffffffu, wait_message(bar, (m >> 1) & 1, patience));
+      if (threadIdx.x == 0 && !lost) arm(bar, 32 * sizeof(F));
+      if (lost && lane == 0) atomicExch(&g_ran_out, 1u);
+    }
+    h = lost ? all_<F>(CUDART_NAN_F) : B.inbox[m & 1][lane];
+  }
+  if (last && p.n > 1) {
+    state = through(whole, h);
+    if (k + 1 < p.tiles) {
+      const int next = p.rank + 1 == p.n ? 0 : p.rank + 1;
+      send(at_rank(smem_of(&B.inbox[step & 1][lane]), next), at_rank(smem_of(&B.full[step & 1]), next), state);
+    }
+  }
+  F in = h;
+#pragma unroll 1
+  for (int j = 0; j < order; ++j) in = apply(map_of(j), in);
+  if (any_(in, [](float v) { return v != v; })) {  // an infinity on the way?
+    in = h;
+#pragma unroll 1
+    for (int j = 0; j < order; ++j) in = apply_to_infinity(map_of(j), in);
+  }
+  if (last && p.n == 1) B.inbox[step & 1][lane] = state = through(mine, in);
+  return in;
+}
+
+// ---------------------------------------------------------------- the passes
+
+// Tokens past the last tile: zeros.
+template <typename T, typename S, bool ALIGNED, int OUTS>
+__device__ __forceinline__ void zeros_behind(const ScanArgs& A, const Place& p) {
+  if (p.have < 1) return;
+  for (int t = p.tiles * S::kTile + p.rank * S::kWarps + (threadIdx.x >> 5); t < A.L; t += p.n * S::kWarps)
+#pragma unroll
+    for (int k = 0; k < OUTS; ++k)
+      put<T, ALIGNED>(reinterpret_cast<T*>(A.out[k]) + ((long long)p.b * A.L + t) * A.C + p.ch, all_<typename Lane<T>::F>(0.0f), p.have);
+}
+
+template <typename T, bool LOG, bool GATE, bool COMP, bool ALIGNED>
+__global__ void __launch_bounds__(Fwd::kThreads, Fwd::kCtas) gated_fwd_kernel(const ScanArgs A) {
   using F = typename Lane<T>::F;
-  constexpr int K = GATE ? 3 : 2, TB = kTileBytes<ALIGNED>;
+  using S = Fwd;
+  constexpr int K = GATE ? 3 : 2, TB = kTileBytes<S, ALIGNED>, kSeg = S::kSeg;
   extern __shared__ __align__(128) unsigned char smem[];
-  Maps<F>& M = *reinterpret_cast<Maps<F>*>(smem + 2 * K * TB);
-  CtaMaps<F>* X = reinterpret_cast<CtaMaps<F>*>(smem + 2 * K * TB + sizeof(Maps<F>));
-  const Place p = place_of<T>(A);
+  auto& B = *reinterpret_cast<Board<F, S::kWarps>*>(smem + 2 * K * TB);
+  const Place p = place_of<T, S>(A);
   const int warp = threadIdx.x >> 5, width = min(kWidth, A.C * (int)sizeof(T) - p.col * kWidth);
   const char* in[K];
 #pragma unroll
   for (int k = 0; k < K; ++k) in[k] = A.in[k] + p.b * A.batch[k] + p.col * kWidth;
-  const auto fetch = [&](int step) {
-    const int t = (step * p.n + p.rank) * kTile, rows = min(kTile, p.len - t);
+  const auto fetch = [&](int step, int tile) {
+    const int t = tile * S::kTile, rows = min(S::kTile, p.len - t);
 #pragma unroll
     for (int k = 0; k < K; ++k)
-      load_tile<ALIGNED>(smem + ((step & 1) * K + k) * TB, in[k] + t * A.tok[k], A.tok[k], rows, width);
+      load_tile<S, ALIGNED>(smem + ((step & 1) * K + k) * TB, in[k] + t * A.tok[k], A.tok[k], rows, width);
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
   F state = all_<F>(0.0f);
   if (A.first) state = get_state(A.first + (long long)p.b * A.C + p.ch, p.have, state);
-  if (p.n > 1) cluster_meet();  // the others run, their shared memory can be written
-  if (p.steps > 0) fetch(0);
-  for (int step = 0; step < p.steps; ++step) {
+  bool lost = false;
+  open_board(B, p);
+  if (p.rank < p.tiles) fetch(0, p.rank);
+  // Whole tiles, and the tile that the row ends in, are apart from each other: a test for each token keeps the tokens' latencies apart too.
+  const auto run = [&](int k, int step, auto all_live) {
+    constexpr bool whole = decltype(all_live)::value;
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();
-    if (step + 1 < p.steps) fetch(step + 1);
+    if (k + p.n < p.tiles) fetch(step + 1, k + p.n);
     const unsigned char* tile = smem + (step & 1) * K * TB;
-    const int tile0 = (step * p.n + p.rank) * kTile, r0 = warp * kSeg, t0 = tile0 + r0;
-    const int live = min(kSeg, p.len - t0);  // below 1: none
+    const int tile0 = k * S::kTile, r0 = warp * kSeg, t0 = tile0 + r0;
+    const int live = whole ? kSeg : min(kSeg, p.len - t0);  // below 1: none
     const auto value = [&](int k, int i) {
       return lane_of<T, ALIGNED>(tile + k * TB, in[k] + tile0 * A.tok[k], A.tok[k], r0 + i);
     };
     const auto token = [&](int i, F& a, F& u, F& b) {
       const F x = value(0, i);
       decay_of<LOG>(value(1, i), a, u);
-      b = A.complement ? mul_(u, x) : x;
+      b = COMP ? mul_(u, x) : x;
     };
     F hl[kSeg], Pl[kSeg];
     F h = all_<F>(0.0f), P = all_<F>(1.0f), D = all_<F>(0.0f);
 #pragma unroll
     for (int i = 0; i < kSeg; ++i) {
-      if (i < live) {
+      if (whole || i < live) {
         F a, u, b;
         token(i, a, u, b);
         h = fma_(a, h, b);
+        D = fma_(u, P, D);
         P = mul_(P, a);
-        D = fma_(u, sub_(all_<F>(1.0f), D), D);
       }
       hl[i] = h, Pl[i] = P;
     }
@@ -399,52 +503,70 @@ __global__ void __launch_bounds__(kThreads) gated_fwd_kernel(const ScanArgs A) {
       }
       P = each_(P, least, [](float v, float w) { return w > 0.0f ? above_zero(v) : v; });
     }
-    const F enter = hand_on<F>(M, X, p.n, p.rank, false, step, Map<F>{P, low_part(P, D), h}, state);
-    F carry = enter;
-    if (any_(carry, infinite)) {  // token by token, so that an infinity stays one
+    const F carry = hand_on(B, p, k, step, warp, Map<F>{P, low_part(P, D), h}, state, A.patience, lost);
+    if (p.have < 1) return;
+    T* const y = reinterpret_cast<T*>(A.out[0]) + ((long long)p.b * A.L + t0) * A.C + p.ch;
+    float* const s = A.saved + ((long long)p.b * A.segments + t0 / kSaved) * A.C + p.ch;
+    if (any_(carry, infinite)) {  // token by token, so that an infinity stays one; apart from the rest, which keeps its registers
       F full = carry;
-#pragma unroll
-      for (int i = 0; i < kSeg; ++i) {
-        if (i < live) {
-          F a, u, b;
-          token(i, a, u, b);
-          full = fma_(a, full, b);
-        }
-        hl[i] = each_(hl[i], full, carry, [](float v, float w, float c) { return infinite(c) ? w : v; });
-        Pl[i] = each_(Pl[i], carry, [](float v, float c) { return infinite(c) ? 0.0f : v; });
-      }
-      carry = each_(carry, [](float v) { return infinite(v) ? 0.0f : v; });
-    }
-    if (A.saved && live > 0) put_state(A.saved + ((long long)p.b * A.segments + t0 / kSeg) * A.C + p.ch, p.have, enter);
-    T* y = reinterpret_cast<T*>(A.out[0]) + ((long long)p.b * A.L + t0) * A.C + p.ch;
-#pragma unroll
-    for (int i = 0; i < kSeg; ++i, y += A.C) {
-      if (t0 + i < A.L) {
+#pragma unroll 1
+      for (int i = 0; i < kSeg && t0 + i < A.L; ++i) {
         F v = all_<F>(0.0f);
         if (i < live) {
+          if (A.saved && i % kSaved == 0) put_state(s + (long long)(i / kSaved) * A.C, p.have, full);
+          F a, u, b;
+          token(i, a, u, b);
+          v = full = fma_(a, full, b);
+          if constexpr (GATE) {
+            const F o = value(2, i);
+            v = mul_(v, mul_(o, sigmoid_of(o)));
+          }
+        }
+        put<T, ALIGNED>(y + (long long)i * A.C, v, p.have);
+      }
+      return;
+    }
+    if (A.saved) {
+#pragma unroll
+      for (int i = 0; i < kSeg; i += kSaved)
+        if (whole || i < live)
+          put_state(s + (long long)(i / kSaved) * A.C, p.have, i ? fma_(Pl[i ? i - 1 : 0], carry, hl[i ? i - 1 : 0]) : carry);
+    }
+#pragma unroll
+    for (int i = 0; i < kSeg; ++i) {
+      if (whole || t0 + i < A.L) {
+        F v = all_<F>(0.0f);
+        if (whole || i < live) {
           v = fma_(Pl[i], carry, hl[i]);
           if constexpr (GATE) {
             const F o = value(2, i);
-            v = mul_(v, mul_(o, each_(o, silu_sigmoid)));
+            v = mul_(v, mul_(o, sigmoid_of(o)));
           }
         }
-        put<T, ALIGNED>(y, v, p.have);
+        put<T, ALIGNED>(y + (long long)i * A.C, v, p.have);
       }
     }
-  }
-  if (A.last && warp == 0 && p.rank == 0) put_state(A.last + (long long)p.b * A.C + p.ch, p.have, state);
-  zeros_behind<T, ALIGNED, 1>(A, p);
+  };
+  const int full = p.len / S::kTile;
+  int k = p.rank, step = 0;
+  for (; k < full; k += p.n, ++step) run(k, step, std::true_type{});
+  if (k < p.tiles) run(k, step, std::false_type{});
+  // the last tile's CTA has the state in its last warp; a row without tokens keeps what it was given
+  if (A.last && warp == S::kWarps - 1 && p.rank == max(p.tiles - 1, 0) % p.n)
+    put_state(A.last + (long long)p.b * A.C + p.ch, p.have, state);
+  zeros_behind<T, S, ALIGNED, 1>(A, p);
+  close_board(p, lost);
 }
 
-template <typename T, bool LOG, bool GATE, bool ALIGNED>
-__global__ void __launch_bounds__(kThreads) gated_bwd_kernel(const ScanArgs A) {
+template <typename T, bool LOG, bool GATE, bool COMP, bool ALIGNED>
+__global__ void __launch_bounds__(Bwd::kThreads, Bwd::kCtas) gated_bwd_kernel(const ScanArgs A) {
   using F = typename Lane<T>::F;
-  constexpr int K = GATE ? 4 : 3, TB = kTileBytes<ALIGNED>;
+  using S = Bwd;
+  constexpr int K = GATE ? 4 : 3, TB = kTileBytes<S, ALIGNED>, kSeg = S::kSeg;
   constexpr int kDy = K - 1;  // x, gate, (out_gate,) dy
   extern __shared__ __align__(128) unsigned char smem[];
-  Maps<F>& M = *reinterpret_cast<Maps<F>*>(smem + 2 * K * TB);
-  CtaMaps<F>* X = reinterpret_cast<CtaMaps<F>*>(smem + 2 * K * TB + sizeof(Maps<F>));
-  const Place p = place_of<T>(A);
+  auto& B = *reinterpret_cast<Board<F, S::kWarps>*>(smem + 2 * K * TB);
+  const Place p = place_of<T, S>(A);
   const int warp = threadIdx.x >> 5, width = min(kWidth, A.C * (int)sizeof(T) - p.col * kWidth);
   const char* in[K];
   long long tok[K];
@@ -454,69 +576,79 @@ __global__ void __launch_bounds__(kThreads) gated_bwd_kernel(const ScanArgs A) {
     in[k] = A.in[from] + p.b * A.batch[from] + p.col * kWidth;
     tok[k] = A.tok[from];
   }
-  const auto fetch = [&](int step) {
-    const int t = (step * p.n + p.rank) * kTile, rows = min(kTile, p.len - t);
+  const auto fetch = [&](int step, int tile) {
+    const int t = tile * S::kTile, rows = min(S::kTile, p.len - t);
 #pragma unroll
     for (int k = 0; k < K; ++k)
-      load_tile<ALIGNED>(smem + ((step & 1) * K + k) * TB, in[k] + t * tok[k], tok[k], rows, width);
+      load_tile<S, ALIGNED>(smem + ((step & 1) * K + k) * TB, in[k] + t * tok[k], tok[k], rows, width);
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
+  unsigned stride = A.C;
+  asm volatile("" : "+r"(stride));  // in a register, not fetched again for each store
   F state = all_<F>(0.0f);
   if (A.first) state = get_state(A.first + (long long)p.b * A.C + p.ch, p.have, state);
-  if (p.n > 1) cluster_meet();
-  if (p.steps > 0) fetch(p.steps - 1);
-  for (int step = p.steps - 1; step >= 0; --step) {
-    const int tile0 = (step * p.n + p.rank) * kTile, r0 = warp * kSeg, t0 = tile0 + r0;
-    const int live = min(kSeg, p.len - t0);
+  bool lost = false;
+  open_board(B, p);
+  if (p.rank < p.tiles) fetch(0, p.tiles - 1 - p.rank);
+  const auto run = [&](int k, int step, auto all_live) {
+    constexpr bool whole = decltype(all_live)::value;
+    const int tile0 = (p.tiles - 1 - k) * S::kTile, r0 = warp * kSeg, t0 = tile0 + r0;
+    const int live = whole ? kSeg : min(kSeg, p.len - t0);
     F before[kSeg + 1];  // before[i]: the state that enters token i
     before[0] = all_<F>(0.0f);
-    if (live > 0) before[0] = get_state(A.saved + ((long long)p.b * A.segments + t0 / kSeg) * A.C + p.ch, p.have, before[0]);
+    if (live > 0) before[0] = get_state(A.saved + ((long long)p.b * A.segments + t0 / kSaved) * A.C + p.ch, p.have, before[0]);
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();
-    if (step > 0) fetch(step - 1);
+    if (k + p.n < p.tiles) fetch(step + 1, p.tiles - 1 - k - p.n);
     const unsigned char* tile = smem + (step & 1) * K * TB;
     const auto value = [&](int k, int i) {
       return lane_of<T, ALIGNED>(tile + k * TB, in[k] + tile0 * tok[k], tok[k], r0 + i);
     };
     F a[kSeg], u[kSeg], sig[kSeg];
+    F c = all_<F>(0.0f), P = all_<F>(1.0f), D = all_<F>(0.0f);
 #pragma unroll
     for (int i = 0; i < kSeg; ++i) {
       before[i + 1] = before[i];
-      if (i < live) {
+      if (whole || i < live) {
         const F x = value(0, i);
         decay_of<LOG>(value(1, i), a[i], u[i]);
-        before[i + 1] = fma_(a[i], before[i], A.complement ? mul_(u[i], x) : x);
+        before[i + 1] = fma_(a[i], before[i], COMP ? mul_(u[i], x) : x);
       }
     }
-    F c = all_<F>(0.0f), P = all_<F>(1.0f), D = all_<F>(0.0f), least = all_<F>(1.0f);
 #pragma unroll
     for (int i = kSeg - 1; i >= 0; --i) {
-      if (i < live) {
+      if (whole || i < live) {
         F dh = value(kDy, i);
         if constexpr (GATE) {
           const F o = value(2, i);
-          sig[i] = each_(o, silu_sigmoid);
+          sig[i] = sigmoid_of(o);
           dh = mul_(dh, mul_(o, sig[i]));
         }
         c = mul_(a[i], add_(dh, c));
+        D = fma_(u[i], P, D);
         P = mul_(P, a[i]);
-        D = fma_(u[i], sub_(all_<F>(1.0f), D), D);
       }
     }
     if (any_(P, [](float v) { return v == 0.0f; })) {
+      F least = all_<F>(1.0f);
 #pragma unroll
       for (int i = 0; i < kSeg; ++i)
         if (i < live) least = each_(least, a[i], [](float v, float w) { return fminf(v, w); });
       P = each_(P, least, [](float v, float w) { return w > 0.0f ? above_zero(v) : v; });
     }
-    c = hand_on<F>(M, X, p.n, p.n - 1 - p.rank, true, step, Map<F>{P, low_part(P, D), c}, state);
+    c = hand_on(B, p, k, step, S::kWarps - 1 - warp, Map<F>{P, low_part(P, D), c}, state, A.patience, lost);
     const long long at = ((long long)p.b * A.L + t0) * A.C + p.ch;
+    T* const dx_at = reinterpret_cast<T*>(A.out[0]) + at;
+    T* const dg_at = reinterpret_cast<T*>(A.out[1]) + at;
+    [[maybe_unused]] T* const do_at = reinterpret_cast<T*>(A.out[2]) + at;
+    if (p.have < 1) return;
 #pragma unroll
     for (int i = kSeg - 1; i >= 0; --i) {
-      if (t0 + i < A.L) {
-        F dx = all_<F>(0.0f), dg = dx, dO = dx;
-        if (i < live) {
-          const F dy = value(kDy, i), x = value(0, i);
+      if (whole || t0 + i < A.L) {
+        F dx = all_<F>(0.0f), dg = dx;
+        [[maybe_unused]] F dO = dx;
+        if (whole || i < live) {
+          const F dy = value(kDy, i);
           F dh = dy;
           if constexpr (GATE) {
             const F o = value(2, i);
@@ -527,19 +659,26 @@ __global__ void __launch_bounds__(kThreads) gated_bwd_kernel(const ScanArgs A) {
           }
           const F G = add_(dh, c);
           c = mul_(a[i], G);
-          dx = A.complement ? mul_(u[i], G) : G;
-          const F da = mul_(G, A.complement ? sub_(before[i], x) : before[i]);
+          dx = COMP ? mul_(u[i], G) : G;
+          const F da = mul_(G, COMP ? sub_(before[i], value(0, i)) : before[i]);
           dg = mul_(da, LOG ? a[i] : mul_(a[i], u[i]));
         }
-        const long long to = at + (long long)i * A.C;
-        put<T, ALIGNED>(reinterpret_cast<T*>(A.out[0]) + to, dx, p.have);
-        put<T, ALIGNED>(reinterpret_cast<T*>(A.out[1]) + to, dg, p.have);
-        if constexpr (GATE) put<T, ALIGNED>(reinterpret_cast<T*>(A.out[2]) + to, dO, p.have);
+        put<T, ALIGNED>(row_at(dx_at, stride, i), dx, p.have);
+        put<T, ALIGNED>(row_at(dg_at, stride, i), dg, p.have);
+        if constexpr (GATE) put<T, ALIGNED>(row_at(do_at, stride, i), dO, p.have);
       }
     }
+  };
+  int k = p.rank, step = 0;
+  if (k == 0 && p.len % S::kTile) {
+    run(k, step, std::false_type{});
+    k += p.n, ++step;
   }
-  if (A.last && warp == 0 && p.rank == 0) put_state(A.last + (long long)p.b * A.C + p.ch, p.have, state);
-  zeros_behind<T, ALIGNED, GATE ? 3 : 2>(A, p);
+  for (; k < p.tiles; k += p.n, ++step) run(k, step, std::true_type{});
+  if (A.last && warp == 0 && p.rank == max(p.tiles - 1, 0) % p.n)
+    put_state(A.last + (long long)p.b * A.C + p.ch, p.have, state);
+  zeros_behind<T, S, ALIGNED, GATE ? 3 : 2>(A, p);
+  close_board(p, lost);
 }
 
 // ---------------------------------------------------------------- single tokens
@@ -586,7 +725,7 @@ __global__ void __launch_bounds__(256) gated_step_kernel(const StepArgs A) {
     float v = h.e[i];
     if (A.o) {
       const float oi = DT<T>::load(&o.e[i]);
-      v *= oi * silu_sigmoid(oi);
+      v *= oi * sigmoid_of(oi);
     }
     DT<T>::store(&out.e[i], v);
   }
@@ -598,17 +737,20 @@ __global__ void __launch_bounds__(256) gated_step_kernel(const StepArgs A) {
 
 using Kernel = void (*)(ScanArgs);
 
-template <typename T, bool LOG, bool ALIGNED> Kernel pick_gate(bool back, bool gate) {
-  if (back) return gate ? gated_bwd_kernel<T, LOG, true, ALIGNED> : gated_bwd_kernel<T, LOG, false, ALIGNED>;
-  return gate ? gated_fwd_kernel<T, LOG, true, ALIGNED> : gated_fwd_kernel<T, LOG, false, ALIGNED>;
+template <typename T, bool LOG, bool GATE, bool COMP> Kernel pick3(bool back, bool aligned) {
+  if (back) return aligned ? gated_bwd_kernel<T, LOG, GATE, COMP, true> : gated_bwd_kernel<T, LOG, GATE, COMP, false>;
+  return aligned ? gated_fwd_kernel<T, LOG, GATE, COMP, true> : gated_fwd_kernel<T, LOG, GATE, COMP, false>;
 }
-template <typename T> Kernel pick(bool back, bool log, bool gate, bool aligned) {
-  if (log) return aligned ? pick_gate<T, true, true>(back, gate) : pick_gate<T, true, false>(back, gate);
-  return aligned ? pick_gate<T, false, true>(back, gate) : pick_gate<T, false, false>(back, gate);
+template <typename T, bool LOG, bool GATE> Kernel pick2(bool back, bool complement, bool aligned) {
+  return complement ? pick3<T, LOG, GATE, true>(back, aligned) : pick3<T, LOG, GATE, false>(back, aligned);
+}
+template <typename T> Kernel pick(bool back, bool log, bool gate, bool complement, bool aligned) {
+  if (log) return gate ? pick2<T, true, true>(back, complement, aligned) : pick2<T, true, false>(back, complement, aligned);
+  return gate ? pick2<T, false, true>(back, complement, aligned) : pick2<T, false, false>(back, complement, aligned);
 }
 
 // Clusters of n CTAs that can run at once (0: unknown), asked once for each kernel, size and device.
-int room_for(Kernel fn, int n, size_t smem) {
+int room_for(Kernel fn, int n, int threads, size_t smem) {
   static std::mutex mu;
   static std::map<std::tuple<const void*, int, int>, int> known;
   int dev = 0;
@@ -618,12 +760,13 @@ int room_for(Kernel fn, int n, size_t smem) {
   const auto it = known.find(key);
   if (it != known.end()) return it->second;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(n), cfg.blockDim = dim3(kThreads), cfg.dynamicSmemBytes = smem;
+  cfg.gridDim = dim3(n), cfg.blockDim = dim3(threads), cfg.dynamicSmemBytes = smem;
   cudaLaunchAttribute at{};
   at.id = cudaLaunchAttributeClusterDimension;
   at.val.clusterDim.x = n, at.val.clusterDim.y = 1, at.val.clusterDim.z = 1;
   cfg.attrs = &at, cfg.numAttrs = 1;
   int room = 0;
+  if (n > 8) cudaFuncSetAttribute(reinterpret_cast<const void*>(fn), cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   if (cudaOccupancyMaxActiveClusters(&room, reinterpret_cast<const void*>(fn), &cfg) != cudaSuccess) {
     cudaGetLastError();
     room = 0;
@@ -650,7 +793,7 @@ int run_scan(const hyfft_gated_desc* d, ScanArgs A, bool back, cudaStream_t st) 
   const bool gate = A.in[2] != nullptr;
   A.L = (int)d->length, A.C = d->channels, A.complement = d->complement ? 1 : 0;
   A.cols = (int)(((long long)A.C * e + kWidth - 1) / kWidth);
-  A.segments = (A.L + kSeg - 1) / kSeg;
+  A.segments = (A.L + kSaved - 1) / kSaved;
   const int64_t* strides[4] = {d->x_stride, d->gate_stride, d->out_gate_stride, d->dy_stride};
   bool aligned = (long long)A.C * e % 4 == 0;
   for (int k = 0; k < 4; ++k) {
@@ -660,16 +803,35 @@ int run_scan(const hyfft_gated_desc* d, ScanArgs A, bool back, cudaStream_t st) 
   }
   for (int k = 0; k < 3; ++k) aligned = aligned && reinterpret_cast<uintptr_t>(A.out[k]) % 4 == 0;
   const bool log = d->form == HYFFT_GATED_LOG;
-  const Kernel fn = d->dtype == HYFFT_F32    ? pick<float>(back, log, gate, aligned)
-                    : d->dtype == HYFFT_BF16 ? pick<__nv_bfloat16>(back, log, gate, aligned)
-                                             : pick<__half>(back, log, gate, aligned);
-  const size_t tile = aligned ? kTileBytes<true> : kTileBytes<false>;
-  const size_t one = e == 4 ? sizeof(Maps<float>) : sizeof(Maps<float2>);
-  const size_t smem = 2 * tile * ((gate ? 3 : 2) + (back ? 1 : 0)) + one;
+  const Kernel fn = d->dtype == HYFFT_F32    ? pick<float>(back, log, gate, A.complement, aligned)
+                    : d->dtype == HYFFT_BF16 ? pick<__nv_bfloat16>(back, log, gate, A.complement, aligned)
+                                             : pick<__half>(back, log, gate, A.complement, aligned);
+  const int tile = back ? Bwd::kTile : Fwd::kTile, threads = back ? Bwd::kThreads : Fwd::kThreads;
+  const size_t board = back ? (e == 4 ? sizeof(Board<float, Bwd::kWarps>) : sizeof(Board<float2, Bwd::kWarps>))
+                            : (e == 4 ? sizeof(Board<float, Fwd::kWarps>) : sizeof(Board<float2, Fwd::kWarps>));
+  const size_t smem = 2 * (size_t)tile * (aligned ? kPitch<true> : kPitch<false>)*((gate ? 3 : 2) + (back ? 1 : 0)) + board;
+  A.patience = g_wait_clocks.load(std::memory_order_relaxed);
   if (!kernel_smem_once(reinterpret_cast<const void*>(fn), smem, true))
     return set_error(HYFFT_ERR_CUDA, "gated scan: shared memory");
+  // As many CTAs for a row as the machine can run at once for all rows, and as the row has tiles.
   const long long rows = (long long)d->batch * A.cols;
-  fn<<<(unsigned)rows, kThreads, smem, st>>>(A);
+  int n = (int)std::min<long long>(kMaxCluster, (A.L + tile - 1) / tile);
+  while (n > 1 && room_for(fn, n, threads, smem) < rows) --n;
+  A.n = n;
+  if (n > 1) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(rows * n)), cfg.blockDim = dim3(threads), cfg.dynamicSmemBytes = smem, cfg.stream = st;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = n, at.val.clusterDim.y = 1, at.val.clusterDim.z = 1;
+    cfg.attrs = &at, cfg.numAttrs = 1;
+    if (cudaLaunchKernelEx(&cfg, fn, A) != cudaSuccess) {
+      cudaGetLastError();
+      return set_error(HYFFT_ERR_CUDA, "gated scan: kernel launch failed");
+    }
+  } else {
+    fn<<<(unsigned)rows, threads, smem, st>>>(A);
+  }
   if (cudaGetLastError() != cudaSuccess) return set_error(HYFFT_ERR_CUDA, "gated scan: kernel launch failed");
   g_launches.fetch_add(1, std::memory_order_relaxed);
   return HYFFT_OK;
@@ -699,12 +861,16 @@ template <typename T> int launch_step(const StepArgs& A, bool log, cudaStream_t 
 }  // namespace
 }  // namespace hyfft
 
+namespace hyfft {
+int gated_wait_status(bool clear, unsigned* ran_out) { return read_ran_out(clear, ran_out) == cudaSuccess ? HYFFT_OK : HYFFT_ERR_CUDA; }
+}  // namespace hyfft
+
 using namespace hyfft;
 
 extern "C" int hyfft_gated_saved_size(const hyfft_gated_desc* d, size_t* saved_bytes) {
   if (int rc = check_desc(d, "gated scan: null descriptor")) return rc;
   if (!saved_bytes) return set_error(HYFFT_ERR_INVALID, "gated scan: null size");
-  *saved_bytes = sizeof(float) * (size_t)d->batch * (size_t)((d->length + kSeg - 1) / kSeg) * (size_t)d->channels;
+  *saved_bytes = sizeof(float) * (size_t)d->batch * (size_t)((d->length + kSaved - 1) / kSaved) * (size_t)d->channels;
   return HYFFT_OK;
 }
 

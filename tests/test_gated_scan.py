@@ -380,6 +380,43 @@ def test_streams_and_graphs():
         assert torch.equal(a, b)
 
 
+@gpu
+@DTYPES
+def test_more_rows_than_the_machine_runs_at_once(dtype):
+    """Rows that one CTA each takes from end to end (few rows share theirs among several)."""
+    B, L, C = 40, 150, 2048
+    c = _case(B, L, C, dtype)
+    some = torch.randint(0, C, (40,), generator=torch.Generator().manual_seed(2))
+    few = {k: t[..., some] for k, t in c.items()}
+    for want, got in zip(_want(few, "logit", True), _run(c, "logit", True)):
+        close(want, got[..., some.cuda()], got.dtype)
+
+
+@gpu
+def test_waits_that_run_out():
+    """A CTA that gives up on its neighbour's message leaves NaN from there on and a status for the host; the next call is sound."""
+    from nvsubquadratic_b200 import _lib
+
+    c = _case(2, 3000, 64, BF16)
+    want = _run(c, "logit", True)
+    _lib.check_waits(0)
+    lib = _lib.load()
+    before = lib.hyfft_set_wait_clocks(0)
+    try:
+        got = _run(c, "logit", True)
+        torch.cuda.synchronize()
+    finally:
+        lib.hyfft_set_wait_clocks(before)
+    if any(t.isnan().any() for t in got):
+        with pytest.raises(_lib.HyfftError, match="gated scan"):
+            _lib.check_waits(0)
+    _lib.check_waits(0)
+    for i in (0, 1):  # a message that came in time is the one that it is otherwise
+        assert ((got[i] == want[i]) | got[i].isnan()).all()
+    assert all(torch.equal(p, q) for p, q in zip(want, _run(c, "logit", True)))
+    _lib.check_waits(0)
+
+
 # ---------------------------------------------------------------- single tokens
 
 
