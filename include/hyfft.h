@@ -414,6 +414,34 @@ HYFFT_API int hyfft_gated_step(const hyfft_gated_desc* d, const void* x, const v
                                const int32_t* slots, int64_t pool, const float* state, float* out_state, void* y,
                                void* stream);
 
+/* ---------------------------------------------------------------- norm of each head, and rotary positions
+ * h = x / sqrt(mean(x^2) + eps) * weight over the features of every head of q [B, L, H, D] and k [B, L, Hk, D] (kv_heads 0: no
+ * k), then turned as by hyfft_rotary (rot_dim 0: not turned). Any batch, token and head strides; outputs contiguous. q_weight,
+ * k_weight [D] of `dtype` or float32 (weight_dtype), NULL: 1. D <= 256 (HYFFT_ERR_UNSUPPORTED above). Sums are float32, the
+ * weights' gradients summed over tokens and heads in a fixed order; each output rounded once. */
+typedef struct hyfft_qk_norm_desc {
+  int32_t batch, heads, kv_heads, dim, rot_dim, dtype, weight_dtype;
+  int32_t interleaved, pos_int32;
+  float amplitude, eps;
+  int32_t reserved;
+  int64_t length;
+  int64_t q_stride[3]; /* element strides: batch, token, head */
+  int64_t k_stride[3];
+  int64_t dq_stride[3]; /* of the gradients that the backward is given */
+  int64_t dk_stride[3];
+  int64_t pos_stride[2];
+} hyfft_qk_norm_desc;
+
+HYFFT_API int hyfft_qk_norm_workspace_size(const hyfft_qk_norm_desc* d, size_t* bwd_bytes);
+HYFFT_API int hyfft_qk_norm_forward(const hyfft_qk_norm_desc* d, const void* q, const void* k, const void* q_weight,
+                                    const void* k_weight, const int64_t* turns, const void* positions, void* out_q,
+                                    void* out_k, void* stream);
+/* Gradients for dout_q, dout_k; dq_weight and dk_weight may be NULL (then the workspace may be NULL too). */
+HYFFT_API int hyfft_qk_norm_backward(const hyfft_qk_norm_desc* d, const void* q, const void* k, const void* q_weight,
+                                     const void* k_weight, const int64_t* turns, const void* positions,
+                                     const void* dout_q, const void* dout_k, void* dq, void* dk, void* dq_weight,
+                                     void* dk_weight, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---------------------------------------------------------------- misc */
 /* Message of the most recent error on this thread ("" if none). */
 HYFFT_API const char* hyfft_last_error(void);

@@ -142,6 +142,29 @@ class GatedDesc(ctypes.Structure):
     ]
 
 
+class QkNormDesc(ctypes.Structure):
+    _fields_ = [
+        ("batch", ctypes.c_int32),
+        ("heads", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32),
+        ("dim", ctypes.c_int32),
+        ("rot_dim", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("weight_dtype", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32),
+        ("pos_int32", ctypes.c_int32),
+        ("amplitude", ctypes.c_float),
+        ("eps", ctypes.c_float),
+        ("reserved", ctypes.c_int32),
+        ("length", ctypes.c_int64),
+        ("q_stride", ctypes.c_int64 * 3),
+        ("k_stride", ctypes.c_int64 * 3),
+        ("dq_stride", ctypes.c_int64 * 3),
+        ("dk_stride", ctypes.c_int64 * 3),
+        ("pos_stride", ctypes.c_int64 * 2),
+    ]
+
+
 SIGNATURES = {
     "hyfft_conv_workspace_size": [ctypes.POINTER(ConvDesc), ctypes.POINTER(_sz), ctypes.POINTER(_sz)],
     "hyfft_conv_forward": [ctypes.POINTER(ConvDesc), _vp, _vp, _vp, _vp, _vp, _sz, _vp],
@@ -176,6 +199,9 @@ SIGNATURES = {
     "hyfft_gated_forward": [ctypes.POINTER(GatedDesc)] + [_vp] * 8 + [_sz, _vp],
     "hyfft_gated_backward": [ctypes.POINTER(GatedDesc)] + [_vp] * 5 + [_sz] + [_vp] * 7,
     "hyfft_gated_step": [ctypes.POINTER(GatedDesc)] + [_vp] * 4 + [_i64] + [_vp] * 4,
+    "hyfft_qk_norm_workspace_size": [ctypes.POINTER(QkNormDesc), ctypes.POINTER(_sz)],
+    "hyfft_qk_norm_forward": [ctypes.POINTER(QkNormDesc)] + [_vp] * 9,
+    "hyfft_qk_norm_backward": [ctypes.POINTER(QkNormDesc)] + [_vp] * 13 + [_sz, _vp],
     "hyfft_last_error": [],
     "hyfft_version": [],
     "hyfft_launch_count": [],
