@@ -29,7 +29,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxDim = 256;
-constexpr int kMaxCtas = 592;  // partial rows of the weights' gradients: four CTAs an SM
+constexpr int kMaxCtas = 296;  // partial rows of a weight's gradient: two CTAs an SM
 
 struct QkArgs {
   const void* x[2];
@@ -45,8 +45,9 @@ struct QkArgs {
   int pos32, w32;                 // the weights are float32
   float amplitude, eps;
   float* partial;                 // [2][CTAs][D]
-  int D, half, groups, per, want_dw;
-  long long L, tokens, items;     // items: (token, group of heads)
+  int D, half, want_dw;
+  int groups[2], ctas[2];         // groups of heads of a token; CTAs (q's first)
+  long long L, tokens, items[2];  // items: (token, group of heads)
 };
 
 // Where the features of lane j are: U units of 2 V features. A unit of pairs is two runs of V (halves) or one of 2 V (neighbours);
@@ -57,9 +58,6 @@ template <typename T, int R>
 __device__ __forceinline__ void move_run(T* dst, const T* src) {
   if constexpr (R * sizeof(T) == 16) {
     *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(src);
-  } else if constexpr (R * sizeof(T) == 32) {
-    reinterpret_cast<uint4*>(dst)[0] = reinterpret_cast<const uint4*>(src)[0];
-    reinterpret_cast<uint4*>(dst)[1] = reinterpret_cast<const uint4*>(src)[1];
   } else {
     static_assert(R <= 2, "longer runs are aligned");
 #pragma unroll
@@ -95,42 +93,43 @@ struct Rows {
   // places of the runs' features within the unit
   static constexpr int kFirst = INTER ? 2 * V : V;
 
-  template <typename S>
-  static __device__ __forceinline__ void load(const QkArgs& A, const S* row, int unit, float* v) {
+  static constexpr bool kWide = V > 1;
+  static __device__ __forceinline__ void fetch(const QkArgs& A, const T* row, int unit, Unit<T, V>& d) {
     int c[2], n[2];
     runs(A, unit, c, n);
-    constexpr bool wide = V * sizeof(S) * (INTER ? 2 : 1) % 16 == 0;
-    if constexpr (wide) {
-      Unit<S, V> d{};
-      if (n[0]) move_run<S, kFirst>(d.e, row + c[0]);
+    if constexpr (kWide) {
+      if (n[0]) move_run<T, kFirst>(d.e, row + c[0]);
       if constexpr (!INTER)
-        if (n[1]) move_run<S, V>(d.e + V, row + c[1]);
-#pragma unroll
-      for (int u = 0; u < V; ++u) {
-        float2 f;
-        if constexpr (std::is_same<S, float>::value)
-          f = make_float2(d.e[2 * u], d.e[2 * u + 1]);
-        else if constexpr (std::is_same<S, __half>::value)
-          f = __half22float2(*reinterpret_cast<const __half2*>(d.e + 2 * u));
-        else {
-          const uint32_t w = *reinterpret_cast<const uint32_t*>(d.e + 2 * u);
-          f = make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
-        }
-        v[2 * u] = f.x, v[2 * u + 1] = f.y;
-      }
+        if (n[1]) move_run<T, V>(d.e + V, row + c[1]);
     } else {
 #pragma unroll
-      for (int u = 0; u < kFirst; ++u) v[u] = u < n[0] ? DT<S>::load(row + c[0] + u) : 0.0f;
+      for (int u = 0; u < kFirst; ++u)
+        if (u < n[0]) d.e[u] = row[c[0] + u];
       if constexpr (!INTER)
 #pragma unroll
-        for (int u = 0; u < V; ++u) v[V + u] = u < n[1] ? DT<S>::load(row + c[1] + u) : 0.0f;
+        for (int u = 0; u < V; ++u)
+          if (u < n[1]) d.e[V + u] = row[c[1] + u];
+    }
+  }
+  static __device__ __forceinline__ void unpack(const Unit<T, V>& d, float* v) {
+#pragma unroll
+    for (int u = 0; u < V; ++u) {
+      float2 f;
+      if constexpr (std::is_same<T, float>::value) {
+        f = make_float2(d.e[2 * u], d.e[2 * u + 1]);
+      } else if constexpr (std::is_same<T, __half>::value) {
+        f = __half22float2(*reinterpret_cast<const __half2*>(d.e + 2 * u));
+      } else {
+        const uint32_t w = *reinterpret_cast<const uint32_t*>(d.e + 2 * u);
+        f = make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+      }
+      v[2 * u] = f.x, v[2 * u + 1] = f.y;
     }
   }
   static __device__ __forceinline__ void store(const QkArgs& A, T* row, int unit, const float* v) {
     int c[2], n[2];
     runs(A, unit, c, n);
-    constexpr bool wide = V * sizeof(T) * (INTER ? 2 : 1) % 16 == 0;
-    if constexpr (wide) {
+    if constexpr (kWide) {
       Unit<T, V> d;
 #pragma unroll
       for (int u = 0; u < V; ++u) {
@@ -189,44 +188,78 @@ template <int E, int G> __device__ __forceinline__ float of_large(const float (&
   return ss == CUDART_INF_F && m < CUDART_INF_F ? rsqrtf(fmaf(s, inv, eps / m / m)) / m : r;
 }
 
-// Groups of G lanes walk over the items. HB rows of one tensor at a time, so that their loads are in flight together.
+// Groups of G lanes walk over the items of one tensor (q's CTAs and k's are apart: one set of weights and of their sums in registers). The
+// next HB rows' loads are in flight while HB are worked on. 65536 tokens of 32 + 32 heads of 128, bfloat16: 412 us forwards (80%
+// of a copy's rate) and 672 backwards (73%); without the loads ahead 424 with four rows at once, and 789 with two backwards; with 8
+// bytes a run instead of 16, twice the lanes of a row, 449 and 812. Neighbouring pairs have 8 features a lane, and room for three
+// CTAs an SM instead of two forwards (32 + 8 heads: 277 against 338 us).
 template <typename T, int V, int U, int G, bool INTER, bool BACK>
-__global__ void __launch_bounds__(kThreads) qk_norm_kernel(const QkArgs A) {
+__global__ void __launch_bounds__(kThreads, BACK || 2 * V * U > 8 ? 2 : 3) qk_norm_kernel(const QkArgs A) {
   using R = Rows<T, V, U, INTER, BACK>;
-  constexpr int E = R::E, HB = E <= 4 ? 4 : 2;
+  constexpr int E = R::E, HB = BACK ? 1 : 2;
   const int lane = threadIdx.x % G;
-  float w[2][E], dw[BACK ? 2 : 1][BACK ? E : 1];
+  const int k = blockIdx.x >= A.ctas[0];
+  const int cta = blockIdx.x - (k ? A.ctas[0] : 0), ctas = A.ctas[k], heads = A.heads[k], groups = A.groups[k];
+  const long long items = A.items[k];
+  float w[E], dw[BACK ? E : 1];
 #pragma unroll
-  for (int k = 0; k < 2; ++k)
+  for (int n = 0; n < U; ++n) {
+    int c[2], m[2];
+    R::runs(A, lane + n * G, c, m);
 #pragma unroll
-    for (int n = 0; n < U; ++n) {
-      int c[2], m[2];
-      R::runs(A, lane + n * G, c, m);
-#pragma unroll
-      for (int e = 0; e < 2 * V; ++e) {  // one by one: the weights' alignment is not known, and they are read once
-        const int run = e < R::kFirst ? 0 : 1, at = e - run * R::kFirst;
-        float& to = w[k][n * 2 * V + e];
-        to = 1.0f;
-        if (A.w[k] && at < m[run])
-          to = A.w32 ? static_cast<const float*>(A.w[k])[c[run] + at] : DT<T>::load(static_cast<const T*>(A.w[k]) + c[run] + at);
-      }
+    for (int e = 0; e < 2 * V; ++e) {  // one by one: the weights' alignment is not known, and they are read once
+      const int run = e < R::kFirst ? 0 : 1, at = e - run * R::kFirst;
+      float& to = w[n * 2 * V + e];
+      to = 1.0f;
+      if (A.w[k] && at < m[run])
+        to = A.w32 ? static_cast<const float*>(A.w[k])[c[run] + at] : DT<T>::load(static_cast<const T*>(A.w[k]) + c[run] + at);
     }
+  }
   if constexpr (BACK) {
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
-#pragma unroll
-      for (int e = 0; e < E; ++e) dw[k][e] = 0.0f;
+    for (int e = 0; e < E; ++e) dw[e] = 0.0f;
   }
   const float inv = 1.0f / A.D;
-  const long long stride = (long long)gridDim.x * (kThreads / G);
+  const long long stride = (long long)ctas * (kThreads / G);
+  const long long xh = A.xh[k], dh = BACK ? A.dh[k] : 0;
   // all lanes of a warp take the same number of turns (the sums are over whole warps)
-  const long long base = (long long)blockIdx.x * (kThreads / G) + threadIdx.x / 32 * (32 / G);
-  for (long long first = base; first < A.items; first += stride) {
+  const long long base = (long long)cta * (kThreads / G) + threadIdx.x / 32 * (32 / G);
+  for (long long first = base; first < items; first += stride) {
     const long long item = first + threadIdx.x % 32 / G;
-    const bool live = item < A.items;
-    const long long tok = live ? item / A.groups : 0;
-    const int grp = live ? (int)(item % A.groups) : 0;
-    const long long b = tok / A.L, l = tok - b * A.L;
+    const bool live = item < items;
+    long long tok = 0, b = 0;
+    if (live && items < (1ll << 31) && A.L < (1ll << 31)) {  // a 64-bit division costs as much as a row
+      tok = (unsigned)item / (unsigned)groups;
+      b = (unsigned)tok / (unsigned)A.L;
+    } else if (live) {
+      tok = item / groups;
+      b = tok / A.L;
+    }
+    const int grp = live ? (int)(item - tok * groups) : heads;
+    const long long l = tok - b * A.L;
+    const T* x = static_cast<const T*>(A.x[k]) + b * A.xb[k] + l * A.xl[k];
+    const T* dy = BACK ? static_cast<const T*>(A.dy[k]) + b * A.db[k] + l * A.dl[k] : nullptr;
+    T* out = static_cast<T*>(A.out[k]) + tok * heads * (long long)A.D;
+    struct Raw {
+      Unit<T, V> x[HB][U], d[BACK ? HB : 1][U];
+    };
+    const auto fetch = [&](int h0, Raw& raw) {  // heads h0, h0 + groups, ...
+#pragma unroll
+      for (int j = 0; j < HB; ++j) {
+        const int h = h0 + j * groups;
+#pragma unroll
+        for (int n = 0; n < U; ++n) {
+          raw.x[j][n] = Unit<T, V>{};
+          if constexpr (BACK) raw.d[j][n] = Unit<T, V>{};
+          if (h < heads) {
+            R::fetch(A, x + h * xh, lane + n * G, raw.x[j][n]);
+            if constexpr (BACK) R::fetch(A, dy + h * dh, lane + n * G, raw.d[j][n]);
+          }
+        }
+      }
+    };
+    Raw raw, ahead;
+    fetch(grp, raw);
     float cs[U][V], sn[U][V];
     {
       long long p = l;
@@ -249,114 +282,93 @@ __global__ void __launch_bounds__(kThreads) qk_norm_kernel(const QkArgs A) {
           }
         }
     }
+    const int rounds = (heads + groups - 1) / groups;
+#pragma unroll 2
+    for (int i = 0; i < rounds; i += HB) {
+      const int h0 = grp + i * groups;
+      if (i + HB < rounds) fetch(h0 + HB * groups, ahead);  // while these are worked on
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      // this group's heads: grp, grp + groups, ...
-      const T* x = static_cast<const T*>(A.x[k]) + b * A.xb[k] + l * A.xl[k];
-      const T* dy = BACK ? static_cast<const T*>(A.dy[k]) + b * A.db[k] + l * A.dl[k] : nullptr;
-      T* out = static_cast<T*>(A.out[k]) + tok * A.heads[k] * (long long)A.D;
-      for (int h0 = 0; h0 < (A.heads[k] + A.groups - 1) / A.groups; h0 += HB) {
-        float v[HB][E], t[BACK ? HB : 1][BACK ? E : 1];
+      for (int j = 0; j < HB; ++j) {
+        const int h = h0 + j * groups;
+        const bool on = h < heads;
+        float v[E];
 #pragma unroll
-        for (int j = 0; j < HB; ++j) {
-          const int h = grp + (h0 + j) * A.groups;
-          const bool on = live && h < A.heads[k];
+        for (int n = 0; n < U; ++n) R::unpack(raw.x[j][n], v + n * 2 * V);
+        float ss = 0.0f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) ss = fmaf(v[e], v[e], ss);
+        ss = sum_of<G>(ss);
+        float r = rsqrtf(fmaf(ss, inv, A.eps));
+        if (__any_sync(0xffffffffu, ss == CUDART_INF_F)) r = of_large<E, G>(v, ss, r, inv, A.eps);
+        if (!on) r = 0.0f;
+        if constexpr (!BACK) {
+#pragma unroll
+          for (int e = 0; e < E; ++e) v[e] = v[e] * r * w[e];
 #pragma unroll
           for (int n = 0; n < U; ++n) {
-            if (on) {
-              R::load(A, x + h * A.xh[k], lane + n * G, &v[j][n * 2 * V]);
-              if constexpr (BACK) R::load(A, dy + h * A.dh[k], lane + n * G, &t[j][n * 2 * V]);
-            } else {
-#pragma unroll
-              for (int e = 0; e < 2 * V; ++e) {
-                v[j][n * 2 * V + e] = 0.0f;
-                if constexpr (BACK) t[j][n * 2 * V + e] = 0.0f;
-              }
-            }
+            if ((lane + n * G) * V < A.half) turn<V, INTER>(v + n * 2 * V, cs[n], sn[n]);
+            if (on) R::store(A, out + (long long)h * A.D, lane + n * G, v + n * 2 * V);
           }
-        }
+        } else {
+          float t[E], gh = 0.0f;
 #pragma unroll
-        for (int j = 0; j < HB; ++j) {
-          const int h = grp + (h0 + j) * A.groups;
-          const bool on = live && h < A.heads[k];
-          float ss = 0.0f;
-#pragma unroll
-          for (int e = 0; e < E; ++e) ss = fmaf(v[j][e], v[j][e], ss);
-          ss = sum_of<G>(ss);
-          float r = rsqrtf(fmaf(ss, inv, A.eps));
-          if (__any_sync(0xffffffffu, ss == CUDART_INF_F)) r = of_large<E, G>(v[j], ss, r, inv, A.eps);
-          if (!on) r = 0.0f;
-          if constexpr (!BACK) {
-#pragma unroll
-            for (int e = 0; e < E; ++e) v[j][e] = v[j][e] * r * w[k][e];
-#pragma unroll
-            for (int n = 0; n < U; ++n) {
-              if ((lane + n * G) * V < A.half) turn<V, INTER>(&v[j][n * 2 * V], cs[n], sn[n]);
-              if (on) R::store(A, out + (long long)h * A.D, lane + n * G, &v[j][n * 2 * V]);
-            }
-          } else {
-            float gh = 0.0f;
-#pragma unroll
-            for (int n = 0; n < U; ++n)
-              if ((lane + n * G) * V < A.half) turn<V, INTER>(&t[j][n * 2 * V], cs[n], sn[n]);
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-              v[j][e] *= r;
-              dw[k][e] = fmaf(t[j][e], v[j][e], dw[k][e]);
-              t[j][e] *= w[k][e];
-              gh = fmaf(t[j][e], v[j][e], gh);
-            }
-            gh = sum_of<G>(gh) * inv;
-#pragma unroll
-            for (int e = 0; e < E; ++e) v[j][e] = r * fmaf(-gh, v[j][e], t[j][e]);
-#pragma unroll
-            for (int n = 0; n < U; ++n)
-              if (on) R::store(A, out + (long long)h * A.D, lane + n * G, &v[j][n * 2 * V]);
+          for (int n = 0; n < U; ++n) {
+            R::unpack(raw.d[j][n], t + n * 2 * V);
+            if ((lane + n * G) * V < A.half) turn<V, INTER>(t + n * 2 * V, cs[n], sn[n]);
           }
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
+            v[e] *= r;
+            dw[e] = fmaf(t[e], v[e], dw[e]);
+            t[e] *= w[e];
+            gh = fmaf(t[e], v[e], gh);
+          }
+          gh = sum_of<G>(gh) * inv;
+#pragma unroll
+          for (int e = 0; e < E; ++e) v[e] = r * fmaf(-gh, v[e], t[e]);
+#pragma unroll
+          for (int n = 0; n < U; ++n)
+            if (on) R::store(A, out + (long long)h * A.D, lane + n * G, v + n * 2 * V);
         }
       }
+      raw = ahead;
     }
   }
   if constexpr (BACK) {
-    if (!A.want_dw) return;
+    if (!A.want_dw || !A.w[k]) return;
     // this CTA's sums over its groups, in their order
-    extern __shared__ float part[];  // [groups of the CTA][D], one tensor at a time
-    constexpr int groups = kThreads / G;
+    extern __shared__ float part[];  // [groups of the CTA][D]
+    float* mine = part + threadIdx.x / G * A.D;
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      if (!A.w[k] || !A.heads[k]) continue;
-      __syncthreads();
-      float* mine = part + threadIdx.x / G * A.D;
+    for (int n = 0; n < U; ++n) {
+      int c[2], m[2];
+      R::runs(A, lane + n * G, c, m);
 #pragma unroll
-      for (int n = 0; n < U; ++n) {
-        int c[2], m[2];
-        R::runs(A, lane + n * G, c, m);
-#pragma unroll
-        for (int e = 0; e < 2 * V; ++e) {
-          const int run = e < R::kFirst ? 0 : 1, at = e - run * R::kFirst;
-          if (at < m[run]) mine[c[run] + at] = dw[k][n * 2 * V + e];
-        }
+      for (int e = 0; e < 2 * V; ++e) {
+        const int run = e < R::kFirst ? 0 : 1, at = e - run * R::kFirst;
+        if (at < m[run]) mine[c[run] + at] = dw[n * 2 * V + e];
       }
-      __syncthreads();
-      for (int c = threadIdx.x; c < A.D; c += kThreads) {
-        float s = 0.0f;
-        for (int i = 0; i < groups; ++i) s += part[i * A.D + c];
-        A.partial[((long long)k * gridDim.x + blockIdx.x) * A.D + c] = s;
-      }
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < A.D; c += kThreads) {
+      float s = 0.0f;
+      for (int i = 0; i < kThreads / G; ++i) s += part[i * A.D + c];
+      A.partial[((long long)k * kMaxCtas + cta) * A.D + c] = s;
     }
   }
 }
 
 // dw[k][c]: column c of the partial rows, in a fixed order. Eight columns (a sector) for each CTA.
 template <typename W>
-__global__ void __launch_bounds__(256) qk_norm_reduce_kernel(const float* partial, W* dwq, W* dwk, int D, int rows) {
+__global__ void __launch_bounds__(256) qk_norm_reduce_kernel(const float* partial, W* dwq, W* dwk, int D, int rows_q, int rows_k) {
   W* dw = blockIdx.y ? dwk : dwq;
   if (!dw) return;
+  const int rows = blockIdx.y ? rows_k : rows_q;
   const int c = blockIdx.x * 8 + threadIdx.x % 8, i0 = threadIdx.x / 8;
   __shared__ float part[32][9];
   float s = 0.0f;
   if (c < D) {
-    const float* p = partial + (long long)blockIdx.y * rows * D + c;
+    const float* p = partial + (long long)blockIdx.y * kMaxCtas * D + c;
 #pragma unroll 4
     for (int i = i0; i < rows; i += 32) s += p[(long long)i * D];
   }
@@ -371,18 +383,27 @@ __global__ void __launch_bounds__(256) qk_norm_reduce_kernel(const float* partia
 
 template <typename T, int V, int U, int G, bool INTER, bool BACK>
 int launch(QkArgs A, int* ctas, cudaStream_t st) {
-  const int nh = std::max(A.heads[0], A.heads[1]);
-  // heads a group takes at one token: as many as share the turned angles, while there are two thousand threads for each SM
-  int per = std::min(nh, 16);
-  while (per > 1 && A.tokens * G * ((nh + per - 1) / per) < 148ll * 2048) per = (per + 1) / 2;
-  A.groups = (nh + per - 1) / per;
-  A.items = A.tokens * A.groups;
-  const long long blocks = (A.items + kThreads / G - 1) / (kThreads / G);
+  for (int k = 0; k < 2; ++k) {
+    const int nh = A.heads[k];
+    if (!nh) continue;
+    // heads a group takes at one token: as many as share the turned angles, while there are 512 threads for each SM
+    int per = std::min(nh, 16);
+    while (per > 1 && A.tokens * G * ((nh + per - 1) / per) < 148ll * 512) per = (per + 1) / 2;
+    A.groups[k] = (nh + per - 1) / per;
+    A.items[k] = A.tokens * A.groups[k];
+  }
+  const long long most = kMaxCtas, all = A.heads[0] + A.heads[1];
+  long long grid = 0;
+  for (int k = 0; k < 2; ++k) {
+    if (!A.heads[k]) continue;
+    long long n = (A.items[k] + kThreads / G - 1) / (kThreads / G);
+    // backwards the weights' sums stay in registers over many tokens: the CTAs that run at once, shared by the heads
+    if (BACK) n = std::min(n, std::max(1ll, most * A.heads[k] / all));
+    if (n > 0x3fffffffLL) return set_error(HYFFT_ERR_UNSUPPORTED, "qk norm: too many elements");
+    A.ctas[k] = (int)n, grid += n;
+  }
+  if (ctas) ctas[0] = A.ctas[0], ctas[1] = A.ctas[1];
   const size_t smem = BACK ? sizeof(float) * (kThreads / G) * A.D : 0;
-  long long grid = blocks;
-  if (BACK) grid = std::min<long long>(blocks, kMaxCtas);  // the weights' gradients stay in registers over many tokens
-  if (grid > 0x7fffffffLL) return set_error(HYFFT_ERR_UNSUPPORTED, "qk norm: too many elements");
-  if (ctas) *ctas = (int)grid;
   const auto fn = qk_norm_kernel<T, V, U, G, INTER, BACK>;
   if (smem > 48 * 1024 && !kernel_smem_once(reinterpret_cast<const void*>(fn), smem))
     return set_error(HYFFT_ERR_CUDA, "qk norm: shared memory");
@@ -401,14 +422,14 @@ int launch_lanes(const QkArgs& A, int lanes, int* ctas, cudaStream_t st) {
 }
 
 template <typename T, bool INTER, bool BACK> int launch_t(const QkArgs& A, int* ctas, cudaStream_t st) {
-  constexpr int E = 16 / (int)sizeof(T), V = INTER ? E / 2 : E;
+  constexpr int V = (INTER ? 8 : 16) / (int)sizeof(T), E = INTER ? 2 * V : V;  // pairs of a unit, elements of a run
   // runs of 16 bytes where every run of every row starts on a 16-byte boundary, pairs of elements otherwise
   bool al = A.D % E == 0 && (INTER ? (2 * A.half) % E == 0 : A.half % E == 0);
   for (int k = 0; k < 2; ++k) {
     if (!A.heads[k]) continue;
-    al = al && reinterpret_cast<uintptr_t>(A.x[k]) % 16 == 0 && reinterpret_cast<uintptr_t>(A.out[k]) % 16 == 0 &&
+    al = al && reinterpret_cast<uintptr_t>(A.x[k]) % (E * sizeof(T)) == 0 && reinterpret_cast<uintptr_t>(A.out[k]) % (E * sizeof(T)) == 0 &&
          A.xb[k] % E == 0 && A.xl[k] % E == 0 && A.xh[k] % E == 0;
-    if (BACK) al = al && reinterpret_cast<uintptr_t>(A.dy[k]) % 16 == 0 && A.db[k] % E == 0 && A.dl[k] % E == 0 && A.dh[k] % E == 0;
+    if (BACK) al = al && reinterpret_cast<uintptr_t>(A.dy[k]) % (E * sizeof(T)) == 0 && A.db[k] % E == 0 && A.dl[k] % E == 0 && A.dh[k] % E == 0;
   }
   const int v = al ? V : 1;
   const int units = (A.half + v - 1) / v + (A.D - 2 * A.half + 2 * v - 1) / (2 * v);
@@ -500,17 +521,17 @@ extern "C" int hyfft_qk_norm_backward(const hyfft_qk_norm_desc* d, const void* q
   A.db[1] = d->dk_stride[0], A.dl[1] = d->dk_stride[1], A.dh[1] = d->dk_stride[2];
   A.partial = static_cast<float*>(workspace), A.want_dw = want;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  int ctas = 0;
-  if (int rc = run<true>(d, A, &ctas, st)) return rc;
+  int ctas[2] = {0, 0};
+  if (int rc = run<true>(d, A, ctas, st)) return rc;
   if (!want) return HYFFT_OK;
   const dim3 grid((d->dim + 7) / 8, 2);
   if (d->weight_dtype == HYFFT_F32)
-    qk_norm_reduce_kernel<float><<<grid, 256, 0, st>>>(A.partial, (float*)dq_weight, (float*)dk_weight, A.D, ctas);
+    qk_norm_reduce_kernel<float><<<grid, 256, 0, st>>>(A.partial, (float*)dq_weight, (float*)dk_weight, A.D, ctas[0], ctas[1]);
   else if (d->weight_dtype == HYFFT_BF16)
     qk_norm_reduce_kernel<__nv_bfloat16>
-        <<<grid, 256, 0, st>>>(A.partial, (__nv_bfloat16*)dq_weight, (__nv_bfloat16*)dk_weight, A.D, ctas);
+        <<<grid, 256, 0, st>>>(A.partial, (__nv_bfloat16*)dq_weight, (__nv_bfloat16*)dk_weight, A.D, ctas[0], ctas[1]);
   else
-    qk_norm_reduce_kernel<__half><<<grid, 256, 0, st>>>(A.partial, (__half*)dq_weight, (__half*)dk_weight, A.D, ctas);
+    qk_norm_reduce_kernel<__half><<<grid, 256, 0, st>>>(A.partial, (__half*)dq_weight, (__half*)dk_weight, A.D, ctas[0], ctas[1]);
   if (cudaGetLastError() != cudaSuccess) return set_error(HYFFT_ERR_CUDA, "qk norm: kernel launch failed");
   g_launches.fetch_add(1, std::memory_order_relaxed);
   return HYFFT_OK;
