@@ -442,6 +442,30 @@ HYFFT_API int hyfft_qk_norm_backward(const hyfft_qk_norm_desc* d, const void* q,
                                      const void* dout_q, const void* dout_k, void* dq, void* dk, void* dq_weight,
                                      void* dk_weight, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------- slots of pools of states
+ * A pool: `slots` rows of row_bytes bytes, contiguous; up to HYFFT_MAX_POOLS pools of the same number of slots go through one call
+ * (they must not overlap).
+ * hyfft_pool_copy: row target[i] becomes what row source[i] held before the call, for all moves at once (a source may be
+ * another move's target: chains, cycles and exchanges come out as they would in a second buffer). A source outside 0 .. slots - 1
+ * means zeros, a move whose target is outside is not made, and of several moves into one slot the last is. At most 12800
+ * moves (HYFFT_ERR_UNSUPPORTED above).
+ * hyfft_pool_compact: live [slots] (0 or not): which slots hold running requests. Those in the highest slots are moved into the
+ * lowest free ones, in order, so that the running requests take slots 0 .. (their number) - 1; the rows they leave are left as
+ * they were. moved int32 [slots]: each slot's request's new slot, -1 for a free one.
+ * source, target, live, moved and the workspace are in device memory. No counterpart in the reference.                  */
+#define HYFFT_MAX_POOLS 16
+typedef struct hyfft_pool {
+  void* data;
+  int64_t row_bytes;
+} hyfft_pool;
+
+HYFFT_API int hyfft_pool_workspace_size(int64_t slots, int64_t moves, size_t* copy_bytes, size_t* compact_bytes);
+HYFFT_API int hyfft_pool_copy(const hyfft_pool* pools, int32_t n, int64_t slots, const int32_t* source,
+                              const int32_t* target, int64_t moves, void* workspace, size_t workspace_bytes,
+                              void* stream);
+HYFFT_API int hyfft_pool_compact(const hyfft_pool* pools, int32_t n, int64_t slots, const uint8_t* live, int32_t* moved,
+                                 void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---------------------------------------------------------------- misc */
 /* Message of the most recent error on this thread ("" if none). */
 HYFFT_API const char* hyfft_last_error(void);

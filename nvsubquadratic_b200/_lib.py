@@ -165,6 +165,10 @@ class QkNormDesc(ctypes.Structure):
     ]
 
 
+class Pool(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("row_bytes", ctypes.c_int64)]
+
+
 SIGNATURES = {
     "hyfft_conv_workspace_size": [ctypes.POINTER(ConvDesc), ctypes.POINTER(_sz), ctypes.POINTER(_sz)],
     "hyfft_conv_forward": [ctypes.POINTER(ConvDesc), _vp, _vp, _vp, _vp, _vp, _sz, _vp],
@@ -202,6 +206,9 @@ SIGNATURES = {
     "hyfft_qk_norm_workspace_size": [ctypes.POINTER(QkNormDesc), ctypes.POINTER(_sz)],
     "hyfft_qk_norm_forward": [ctypes.POINTER(QkNormDesc)] + [_vp] * 9,
     "hyfft_qk_norm_backward": [ctypes.POINTER(QkNormDesc)] + [_vp] * 13 + [_sz, _vp],
+    "hyfft_pool_workspace_size": [_i64, _i64, ctypes.POINTER(_sz), ctypes.POINTER(_sz)],
+    "hyfft_pool_copy": [ctypes.POINTER(Pool), _i32, _i64, _vp, _vp, _i64, _vp, _sz, _vp],
+    "hyfft_pool_compact": [ctypes.POINTER(Pool), _i32, _i64, _vp, _vp, _vp, _sz, _vp],
     "hyfft_last_error": [],
     "hyfft_version": [],
     "hyfft_launch_count": [],

@@ -26,7 +26,7 @@ STAMP = PKG / ".libhyfft.stamp"
 
 SOURCES = ["engine.cu", "cp.cu", "fused.cu", "toeplitz.cu", "big2d.cu", "shortconv.cu", "transpose_tma.cu", "fft_long.cu", "siren.cu",
            "decay_attn.cu", "decay_mma.cu", "rotary.cu", "layer_norm.cu",
-           "gated_scan.cu", "qk_norm.cu"]
+           "gated_scan.cu", "qk_norm.cu", "state_pool.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
