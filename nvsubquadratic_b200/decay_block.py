@@ -21,18 +21,20 @@ import torch
 
 from .decay_attention import decay_attention, decay_attention_step
 from .layer_norm import LayerNormB200, layer_norm
+from .qk_norm import qk_norm_rotary
 from .rotary import rotary, rotary_turns
 from .sequence_mixer import QKVSequenceMixerB200
+from .state_pool import SlotCache
 
 __all__ = ["DecayCache", "DecayMixerB200", "DecayBlockB200"]
 
 
-class DecayCache:
+class DecayCache(SlotCache):
     """The states of up to ``slots`` running requests: float32 ``[slots, heads, head_dim, head_dim]`` and the position of
     each one's next token. Its size does not depend on the requests' lengths.
 
     A slot outside ``0 .. slots - 1`` in a call marks an idle request: nothing of it is read, the mixer's output for it is zero and no
-    state changes, for prompts and for single tokens alike."""
+    state changes, for prompts and for single tokens alike. ``fork`` and ``compact`` copy and move requests between slots."""
 
     def __init__(self, slots: int, heads: int, head_dim: int, device=None):
         self.slots = slots
@@ -46,14 +48,8 @@ class DecayCache:
         self.state.index_fill_(0, rows, 0.0)
         self.position.index_fill_(0, rows, 0)
 
-    def rows(self, slots: torch.Tensor | None, batch: int) -> torch.Tensor:
-        """Rows of ``state`` for ``batch`` requests; idle ones (slots outside 0 .. slots - 1) get the spare row."""
-        if slots is None:
-            assert batch <= self.slots, f"{batch} requests need as many slots; the cache has {self.slots}"
-            return torch.arange(batch, device=self.position.device)
-        assert tuple(slots.shape) == (batch,), f"slots must be [{batch}]; got {tuple(slots.shape)}"
-        slots = slots.long()
-        return torch.where((slots >= 0) & (slots < self.slots), slots, self.slots)
+    def tensors(self) -> list[torch.Tensor]:
+        return [self.state, self.position]
 
 
 class DecayMixerB200(torch.nn.Module):
@@ -65,10 +61,12 @@ class DecayMixerB200(torch.nn.Module):
         learn_decay: make the decays' logarithms parameters (they are a buffer by default).
         rot_dim: features of each head that rotary positions turn (all of them by default, 0: none).
         rotary_args: further arguments of ``rotary_turns`` (base, scaling, factor, original_length).
+        qk_norm: divide each head of queries and keys by its root mean square and scale it by learned weights, in the pass
+            that turns them (``qk_norm_rotary``).
     """
 
     def __init__(self, hidden_dim: int, heads: int, *, learn_decay: bool = False, rot_dim: int | None = None,
-                 interleaved: bool = False, eps: float = 1e-5, rotary_args: dict | None = None):
+                 interleaved: bool = False, eps: float = 1e-5, rotary_args: dict | None = None, qk_norm: bool = False):
         super().__init__()
         assert hidden_dim % heads == 0, f"hidden_dim {hidden_dim} must be a multiple of heads {heads}"
         self.heads, self.head_dim, self.eps, self.interleaved = heads, hidden_dim // heads, eps, interleaved
@@ -83,6 +81,8 @@ class DecayMixerB200(torch.nn.Module):
         if rot_dim:
             turns, self.amplitude = rotary_turns(rot_dim, **(rotary_args or {}))
         self.register_buffer("turns", turns, persistent=False)
+        self.q_norm = torch.nn.Parameter(torch.ones(self.head_dim)) if qk_norm else None
+        self.k_norm = torch.nn.Parameter(torch.ones(self.head_dim)) if qk_norm else None
 
     def _apply(self, fn, recurse=True):
         # the decays stay float32 whatever type the rest of a model is cast to: a decay's rounding error is
@@ -96,6 +96,9 @@ class DecayMixerB200(torch.nn.Module):
         return self
 
     def _turn(self, q, k, positions):
+        if self.q_norm is not None:
+            return qk_norm_rotary(q, k, self.q_norm, self.k_norm, self.turns, positions=None if self.turns is None else positions,
+                                  amplitude=self.amplitude, interleaved=self.interleaved)
         if self.turns is None:
             return q, k
         return rotary(q, k, self.turns, positions=positions, amplitude=self.amplitude, interleaved=self.interleaved)

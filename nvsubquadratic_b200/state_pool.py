@@ -16,7 +16,7 @@ import torch
 
 from . import _lib
 
-__all__ = ["copy_slots", "compact_slots"]
+__all__ = ["copy_slots", "compact_slots", "SlotCache"]
 
 MAX_POOLS = 16
 
@@ -98,3 +98,36 @@ def compact_slots(pools: torch.Tensor | Sequence[torch.Tensor], live: torch.Tens
                                         _lib.stream_ptr(dev))
     _lib.check(rc, "hyfft_pool_compact")
     return moved
+
+
+class SlotCache:
+    """What caches of running requests share: ``slots`` rows of some tensors (``tensors()``), and one row more that calls with idle
+    requests gather and scatter in their place. A slot outside ``0 .. slots - 1`` marks an idle request."""
+
+    slots: int
+
+    def tensors(self) -> list[torch.Tensor]:
+        raise NotImplementedError
+
+    def pools(self) -> list[torch.Tensor]:
+        """The rows of the slots, without the spare one."""
+        return [t[:self.slots] for t in self.tensors()]
+
+    def fork(self, source: torch.Tensor, target: torch.Tensor) -> None:
+        """Slots ``target`` go on from where slots ``source`` are, all at once (see ``copy_slots``); int32 lists."""
+        copy_slots(self.pools(), source, target)
+
+    def compact(self, live: torch.Tensor) -> torch.Tensor:
+        """Moves the requests of the slots in ``live`` (bool ``[slots]``) into the lowest ones; returns where each is now (see
+        ``compact_slots``)."""
+        return compact_slots(self.pools(), live)
+
+    def rows(self, slots: torch.Tensor | None, batch: int) -> torch.Tensor:
+        """Rows for ``batch`` requests; idle ones (slots outside 0 .. slots - 1) get the spare row."""
+        device = self.tensors()[0].device
+        if slots is None:
+            assert batch <= self.slots, f"{batch} requests need as many slots; the cache has {self.slots}"
+            return torch.arange(batch, device=device)
+        assert tuple(slots.shape) == (batch,), f"slots must be [{batch}]; got {tuple(slots.shape)}"
+        slots = slots.long()
+        return torch.where((slots >= 0) & (slots < self.slots), slots, self.slots)
