@@ -7,22 +7,25 @@
 //   dx_t = s_t G_t,  dg_t = G_t (h_{t-1} - [s_t = u_t] x_t) * (a_t u_t or a_t),  do_t = dy_t h_t silu'(o_t),  dh_0 = c_1
 //
 // Every channel is a recurrence of its own; there is nothing to share but the loads, so the floor is one read of the inputs and one write
-// of the outputs. A CTA takes 128 bytes of channels (a lane: two of 16 bits or one of 32) and 64 tokens at a time, 16 (backwards 8)
-// for each warp, copied to shared memory one tile ahead. A warp runs its tokens from a zero state, which gives the segment's map
+// of the outputs. A CTA takes a row of 128 bytes of channels (a lane: two of 16 bits or one of 32) and 64 tokens at a time, 16 (backwards
+// 8) for each warp, copied to shared memory one tile ahead. A lane runs its tokens from a zero state, which gives the segment's map
 //   h -> A h + H  (backwards: c -> A c + C),
 // the maps go through shared memory in token order, and the tokens are finished with the state that enters them. Every eighth token's
 // state is kept for the backward pass (four bytes for eight tokens of a channel), which then needs nothing else of the forward's.
 //
-// Where there are fewer rows (batch x 128 bytes of channels) than CTAs that fit the machine, the CTAs of a cluster take a row's tiles in
-// turn: each passes the state that leaves its tile on to the next one's shared memory. In steady state a CTA has its tile's map
-// before the state arrives, so a hop is a wait, one map and one remote store (0.26 us), and the data still goes through once. 65536
-// tokens of 4096 channels, bfloat16, with output gates: one CTA a row 1.54 ms, eight in a cluster 0.49 ms (all of a
-// cluster's maps exchanged behind a barrier: 0.73); 64 x 2048 tokens of 1024 channels, one CTA a row, 193 us (8 bytes an element: 85% of
-// a copy's rate). What is left is instruction issue: about 35 an element forwards and 52 backwards, two of them roundings' unpacking.
+// Where there are fewer rows than CTAs that fit the machine, the CTAs of a cluster take a row's tiles in turn: each passes the state that
+// leaves its tile on to the next one's shared memory. In steady state a CTA has its tile's map before the state arrives, so a hop is a
+// wait, one map and one remote store (0.25 us), and the data still goes through once; no workspace, no order of arrival in the results.
+//
+// Measured, bfloat16 with output gates (8 bytes an element forwards, 14 backwards): 64 x 2048 tokens of 1024 channels, one CTA a row,
+// 193 us forwards (85% of a copy's rate) and 354 backwards (81%); 65536 tokens of 4096 channels, 8 and 4 CTAs a cluster, 490 us (67%; one CTA a
+// row 1.54 ms, all of a cluster's maps exchanged behind a barrier 0.73) and 924 us (62%). float32: 97% and 93% of the same rate on the first.
+// What is left is instructions: 38 an element forwards and 55 backwards, of which a third are moves and unpacking, on a machine that has
+// time for 44 and 77 at a copy's rate; and with clusters the turns of the tiles.
 //
 // What is exact: A is carried as P + l. P is the product of the rounded decays, whose relative error grows with every token; l = (1 - P) - D
-// with D = 1 - A accumulated as D += u (1 - D), which keeps the digits of slow decays. So a state that remembers 10^5 tokens
-// is off by the roundings of its 10^4 segments, not by those of its decays. In a segment, eight products of rounded decays. Sums are float32.
+// with D = 1 - A, accumulated as D += u P, which keeps the digits of slow decays. So a state that remembers 10^5 tokens is off by the
+// roundings of its 10^4 segments, not by those of its decays; within a segment, by 16 products of rounded decays. Sums are float32.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -46,16 +49,17 @@ int set_error(int code, const char* msg);  // engine.cu: the message hyfft_last_
 
 namespace {
 
-// A pass's tile: SEG tokens for each of WARPS warps, and how many CTAs of it an SM holds at least.
-template <int SEG, int WARPS, int CTAS> struct Shape {
-  static constexpr int kSeg = SEG, kWarps = WARPS, kCtas = CTAS, kThreads = 32 * WARPS, kTile = SEG * WARPS;
+// A pass's tile: SEG tokens for each of a row's lanes, LANES lanes a row (a warp has 32 / LANES segments, one behind the other), WARPS
+// warps, and how many CTAs of it an SM holds at least.
+template <int SEG, int WARPS, int CTAS, int LANES> struct Shape {
+  static constexpr int kSeg = SEG, kWarps = WARPS, kCtas = CTAS, kLanes = LANES, kThreads = 32 * WARPS;
+  static constexpr int kSegs = WARPS * 32 / LANES, kTile = SEG * kSegs, kWidth = 4 * LANES;  // bytes of a tile's row
 };
-using Fwd = Shape<16, 4, 4>;
-using Bwd = Shape<8, 8, 2>;
-constexpr int kSaved = Bwd::kSeg;      // tokens from one saved state to the next
-static_assert(Fwd::kSeg % kSaved == 0, "the forward pass has the saved states at hand");
-constexpr int kWidth = 128;            // bytes of a tile's row
-constexpr int kMaxCluster = 16;       // above 8 by a kernel attribute
+template <int LANES> using Fwd = Shape<16, 4, 4, LANES>;
+template <int LANES> using Bwd = Shape<8, 8, 2, LANES>;
+constexpr int kSaved = 8;              // tokens from one saved state to the next: the backward pass's segments
+static_assert(Fwd<32>::kSeg % kSaved == 0 && Bwd<32>::kSeg == kSaved, "both passes have the saved states at hand");
+constexpr int kMaxCluster = 16;        // above 8 by a kernel attribute
 
 struct ScanArgs {
   const char* in[4];          // x, gate, out_gate, dy
@@ -119,15 +123,26 @@ __device__ __forceinline__ float inverse(float x) {
   return r;
 }
 constexpr float kLog2E = 1.4426950408889634f;
+// exp(s g), s = 1 or -1. 16-bit inputs: off by the exponent's rounding, 2^-24 of s g, and by exp2_ (what is left of both in a 16-bit result is
+// below its rounding). float32: the rest of the exponent's product too, as a factor 1 + rest.
+template <int SIGN> __device__ __forceinline__ float2 exp_of(float2 g) {
+  return each_(mul_(g, all_<float2>(SIGN * kLog2E)), exp2_);
+}
+template <int SIGN> __device__ __forceinline__ float exp_of(float g) {
+  constexpr float kLow = 1.925963e-8f;  // log2(e) - kLog2E
+  const float t = SIGN * kLog2E * g;
+  const float rest = fmaf(SIGN * kLow, g, fmaf(SIGN * kLog2E, g, -t)), e = exp2_(t);
+  return fabsf(t) < 126.0f ? fmaf(e * 0.6931472f, rest, e) : e;
+}
 template <typename F> __device__ __forceinline__ F sigmoid_of(F o) {
-  const F e = each_(mul_(o, all_<F>(-kLog2E)), exp2_);
+  const F e = exp_of<-1>(o);
   return each_(add_(e, all_<F>(1.0f)), inverse);
 }
 
 // The decay and what it leaves, a + u = 1, each without cancellation.
 template <bool LOG, typename F> __device__ __forceinline__ void decay_of(F g, F& a, F& u) {
   if constexpr (LOG) {
-    a = each_(mul_(g, all_<F>(kLog2E)), exp2_);
+    a = exp_of<1>(g);
     // 1 - exp(g) near 0 by its series (the rest at 0.35 is below 2e-8 of it)
     const F one = all_<F>(1.0f);
     F s = fma_(g, all_<F>(1.0f / 7), one);
@@ -138,7 +153,7 @@ template <bool LOG, typename F> __device__ __forceinline__ void decay_of(F g, F&
     s = fma_(s, mul_(g, all_<F>(1.0f / 2)), one);
     u = each_(g, mul_(g, s), sub_(one, a), [](float v, float near, float far) { return fabsf(v) < 0.35f ? -near : far; });
   } else {
-    const F e = each_(mul_(g, all_<F>(-kLog2E)), exp2_);
+    const F e = exp_of<-1>(g);
     a = each_(add_(e, all_<F>(1.0f)), inverse);
     // e a, which is 1 - a; where e has overflowed and a is 0 that is a NaN or 0, and 1 - 2 a is 1 (below 1 - a everywhere)
     u = each_(mul_(e, a), fma_(a, all_<F>(-2.0f), all_<F>(1.0f)), [](float v, float w) { return fmaxf(v, w); });
@@ -188,21 +203,27 @@ template <int BYTES> __device__ __forceinline__ void copy_async(uint32_t dst, co
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(valid) : "memory");
 }
 
-// Rows of 128 bytes where every row starts on 16 bytes (ALIGNED), else the 32-bit words that cover them: 33, and a pitch of 144 bytes.
-template <bool ALIGNED> constexpr int kPitch = ALIGNED ? kWidth : kWidth + 16;
-template <typename S, bool ALIGNED> constexpr int kTileBytes = S::kTile * kPitch<ALIGNED>;
+// Rows of S::kWidth bytes where every row starts on 16 bytes (ALIGNED), else the 32-bit words that cover them: one more, and a pitch of 16
+// bytes more. The halves of a warp that has two segments read rows a segment apart: 64 bytes between segments keep their banks apart.
+template <typename S, bool ALIGNED> struct Tile {
+  static constexpr int kPitch = S::kWidth + (ALIGNED ? 0 : 16), kPad = S::kLanes < 32 ? 64 : 0;
+  static constexpr int kBytes = S::kTile * kPitch + S::kSegs * kPad;
+  static __device__ __forceinline__ int row(int r) { return r * kPitch + (kPad ? r / S::kSeg * kPad : 0); }
+};
 
 // `rows` tokens from `src` on (the tile's first channel of its first token), `width` bytes of each.
 template <typename S, bool ALIGNED>
 __device__ __forceinline__ void load_tile(unsigned char* tile, const char* src, long long stride, int rows, int width) {
+  using L = Tile<S, ALIGNED>;
   const uint32_t to = smem_of(tile);
   if constexpr (ALIGNED) {
-    const int c = 16 * (threadIdx.x & 7), valid = min(16, width - c);
+    constexpr int kChunks = S::kWidth / 16;
+    const int c = 16 * (threadIdx.x % kChunks), valid = min(16, width - c);
     if (valid > 0) {
 #pragma unroll
-      for (int i = 0; i < S::kTile * 8 / S::kThreads; ++i) {
-        const int r = (threadIdx.x >> 3) + i * (S::kThreads / 8);
-        if (r < rows) copy_async<16>(to + r * kWidth + c, src + r * stride + c, valid);
+      for (int i = 0; i < S::kTile * kChunks / S::kThreads; ++i) {
+        const int r = threadIdx.x / kChunks + i * (S::kThreads / kChunks);
+        if (r < rows) copy_async<16>(to + L::row(r) + c, src + r * stride + c, valid);
       }
     }
   } else {
@@ -210,16 +231,14 @@ __device__ __forceinline__ void load_tile(unsigned char* tile, const char* src, 
     for (int r = threadIdx.x >> 5; r < rows; r += S::kWarps) {
       const char* p = src + r * stride;
       const int off = (int)(reinterpret_cast<uintptr_t>(p) & 3);
-      for (int w = 4 * lane; w < off + width; w += 128)
-        copy_async<4>(to + r * kPitch<false> + w, p - off + w, min(4, off + width - w));
+      for (int w = 4 * lane; w < off + width; w += 128) copy_async<4>(to + L::row(r) + w, p - off + w, min(4, off + width - w));
     }
   }
 }
 
-// A lane's channels of row r; `src` as for load_tile.
+// A lane's channels at p in the tile, of row r; `src` as for load_tile.
 template <typename T, bool ALIGNED>
-__device__ __forceinline__ typename Lane<T>::F lane_of(const unsigned char* tile, const char* src, long long stride, int r) {
-  const unsigned char* p = tile + r * kPitch<ALIGNED> + 4 * (threadIdx.x & 31);
+__device__ __forceinline__ typename Lane<T>::F lane_of(const unsigned char* p, const char* src, long long stride, int r) {
   if constexpr (std::is_same<T, float>::value) {
     return *reinterpret_cast<const float*>(p);
   } else if constexpr (ALIGNED) {
@@ -321,35 +340,37 @@ __device__ __forceinline__ bool wait_message(uint32_t bar, uint32_t parity, unsi
 
 // The maps of a tile's segments, and the states that enter tiles: two, used in turn. Where another CTA has the tile before, it sends
 // them. The next one into a place is written only after this CTA's last warp has handed on the one in between, so after all warps have read it.
-template <typename F, int WARPS> struct Board {
-  F P[WARPS][32], l[WARPS][32], H[WARPS][32];
-  F inbox[2][32];
+template <typename F, typename S> struct Board {
+  F P[S::kSegs][S::kLanes], l[S::kSegs][S::kLanes], H[S::kSegs][S::kLanes];
+  F inbox[2][S::kLanes];
   unsigned long long full[2];
 };
 
-// Where a CTA works: one batch row and 128 bytes of channels. The n CTAs of a cluster take the row's tiles in turn, each passing the
+// Where a CTA works: one batch row and S::kWidth bytes of channels. The n CTAs of a cluster take the row's tiles in turn, each passing the
 // state that leaves its tile to the next.
 struct Place {
   int n, rank, b, col, ch, have, len, tiles;
+  int seg;  // this lane's segment of a tile
 };
 template <typename T, typename S> __device__ __forceinline__ Place place_of(const ScanArgs& A) {
   Place p;
   p.n = A.n, p.rank = blockIdx.x % A.n;  // a cluster's CTAs are neighbours
   const int row = blockIdx.x / A.n;
   p.b = row / A.cols, p.col = row % A.cols;
-  p.ch = (p.col * 32 + (threadIdx.x & 31)) * Lane<T>::N;
+  p.ch = (p.col * S::kLanes + threadIdx.x % S::kLanes) * Lane<T>::N;
+  p.seg = threadIdx.x / S::kLanes;
   p.have = A.C - p.ch;
   p.len = A.lengths ? min(max(A.lengths[p.b], 0), A.L) : A.L;
   p.tiles = (p.len + S::kTile - 1) / S::kTile;
   return p;
 }
 
-template <typename F, int WARPS> __device__ __forceinline__ void open_board(Board<F, WARPS>& B, const Place& p) {
+template <typename F, typename S> __device__ __forceinline__ void open_board(Board<F, S>& B, const Place& p) {
   if (p.n == 1) return;
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_of(&B.full[i])) : "memory");
-      arm(smem_of(&B.full[i]), 32 * sizeof(F));
+      arm(smem_of(&B.full[i]), sizeof(B.inbox[0]));
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -365,12 +386,12 @@ __device__ __forceinline__ void close_board(const Place& p, bool lost) {
 }
 
 // Hands the maps of a tile's segments on. k: the tile's number in the order of the recurrence, step: how many this CTA has done
-// before; order: this warp's place within the tile. state: what enters the first tile; in the last warp, what leaves each. Returns what
-// enters this warp's segment: NaN from the first message on that did not come (lost).
-template <typename F, int WARPS>
-__device__ __forceinline__ F hand_on(Board<F, WARPS>& B, const Place& p, int k, int step, int order, const Map<F>& mine, F& state,
+// before; order: this lane's segment's place within the tile. state: what enters the first tile; in the last segment, what leaves each.
+// Returns what enters this lane's segment: NaN from the first message on that did not come (lost).
+template <typename F, typename S>
+__device__ __forceinline__ F hand_on(Board<F, S>& B, const Place& p, int k, int step, int order, const Map<F>& mine, F& state,
                                      unsigned patience, bool& lost) {
-  const int lane = threadIdx.x & 31;
+  const int lane = threadIdx.x % S::kLanes;
   B.P[order][lane] = mine.P, B.l[order][lane] = mine.l, B.H[order][lane] = mine.H;
   __syncthreads();
   const auto map_of = [&](int j) { return Map<F>{B.P[j][lane], B.l[j][lane], B.H[j][lane]}; };
@@ -379,18 +400,18 @@ __device__ __forceinline__ F hand_on(Board<F, WARPS>& B, const Place& p, int k, 
     return any_(r, [](float v) { return v != v; }) ? apply_to_infinity(m, h) : r;
   };
   // What leaves the tile goes by one map over all of it, which is there before the message is: the next CTA waits for nothing else.
-  const bool last = order == WARPS - 1;
+  const bool last = order == S::kSegs - 1;
   Map<F> whole = mine;
   if (last && p.n > 1) {
     Map<F> m = map_of(0);
 #pragma unroll 1
-    for (int j = 1; j < WARPS - 1; ++j) m = then(m, map_of(j));
+    for (int j = 1; j < S::kSegs - 1; ++j) m = then(m, map_of(j));
     whole = then(m, mine);
   }
-  if (p.n == 1 && WARPS <= 4) {
+  if (p.n == 1 && S::kSegs <= 4) {  // few enough for every warp to go through all of them
     F h = state, in = state;
 #pragma unroll
-    for (int j = 0; j < WARPS; ++j) {
+    for (int j = 0; j < S::kSegs; ++j) {
       if (j == order) in = h;
       h = through(map_of(j), h);
     }
@@ -404,8 +425,8 @@ __device__ __forceinline__ F hand_on(Board<F, WARPS>& B, const Place& p, int k, 
     if (p.n > 1) {
       const uint32_t bar = smem_of(&B.full[m & 1]);
       if (!lost) lost = !__all_sync(0xffffffffu, wait_message(bar, (m >> 1) & 1, patience));
-      if (threadIdx.x == 0 && !lost) arm(bar, 32 * sizeof(F));
-      if (lost && lane == 0) atomicExch(&g_ran_out, 1u);
+      if (threadIdx.x == 0 && !lost) arm(bar, sizeof(B.inbox[0]));
+      if (lost && threadIdx.x % 32 == 0) atomicExch(&g_ran_out, 1u);
     }
     h = lost ? all_<F>(CUDART_NAN_F) : B.inbox[m & 1][lane];
   }
@@ -434,24 +455,24 @@ __device__ __forceinline__ F hand_on(Board<F, WARPS>& B, const Place& p, int k, 
 template <typename T, typename S, bool ALIGNED, int OUTS>
 __device__ __forceinline__ void zeros_behind(const ScanArgs& A, const Place& p) {
   if (p.have < 1) return;
-  for (int t = p.tiles * S::kTile + p.rank * S::kWarps + (threadIdx.x >> 5); t < A.L; t += p.n * S::kWarps)
+  for (int t = p.tiles * S::kTile + p.rank * S::kSegs + p.seg; t < A.L; t += p.n * S::kSegs)
 #pragma unroll
     for (int k = 0; k < OUTS; ++k)
       put<T, ALIGNED>(reinterpret_cast<T*>(A.out[k]) + ((long long)p.b * A.L + t) * A.C + p.ch, all_<typename Lane<T>::F>(0.0f), p.have);
 }
 
-template <typename T, bool LOG, bool GATE, bool COMP, bool ALIGNED>
-__global__ void __launch_bounds__(Fwd::kThreads, Fwd::kCtas) gated_fwd_kernel(const ScanArgs A) {
+template <typename T, int LANES, bool LOG, bool GATE, bool COMP, bool ALIGNED>
+__global__ void __launch_bounds__(Fwd<LANES>::kThreads, Fwd<LANES>::kCtas) gated_fwd_kernel(const ScanArgs A) {
   using F = typename Lane<T>::F;
-  using S = Fwd;
-  constexpr int K = GATE ? 3 : 2, TB = kTileBytes<S, ALIGNED>, kSeg = S::kSeg;
+  using S = Fwd<LANES>;
+  constexpr int K = GATE ? 3 : 2, TB = Tile<S, ALIGNED>::kBytes, kSeg = S::kSeg;
   extern __shared__ __align__(128) unsigned char smem[];
-  auto& B = *reinterpret_cast<Board<F, S::kWarps>*>(smem + 2 * K * TB);
+  auto& B = *reinterpret_cast<Board<F, S>*>(smem + 2 * K * TB);
   const Place p = place_of<T, S>(A);
-  const int warp = threadIdx.x >> 5, width = min(kWidth, A.C * (int)sizeof(T) - p.col * kWidth);
+  const int width = min(S::kWidth, A.C * (int)sizeof(T) - p.col * S::kWidth);
   const char* in[K];
 #pragma unroll
-  for (int k = 0; k < K; ++k) in[k] = A.in[k] + p.b * A.batch[k] + p.col * kWidth;
+  for (int k = 0; k < K; ++k) in[k] = A.in[k] + p.b * A.batch[k] + p.col * S::kWidth;
   const auto fetch = [&](int step, int tile) {
     const int t = tile * S::kTile, rows = min(S::kTile, p.len - t);
 #pragma unroll
@@ -471,10 +492,11 @@ __global__ void __launch_bounds__(Fwd::kThreads, Fwd::kCtas) gated_fwd_kernel(co
     __syncthreads();
     if (k + p.n < p.tiles) fetch(step + 1, k + p.n);
     const unsigned char* tile = smem + (step & 1) * K * TB;
-    const int tile0 = k * S::kTile, r0 = warp * kSeg, t0 = tile0 + r0;
+    const int tile0 = k * S::kTile, r0 = p.seg * kSeg, t0 = tile0 + r0;
     const int live = whole ? kSeg : min(kSeg, p.len - t0);  // below 1: none
+    const unsigned char* mine = tile + Tile<S, ALIGNED>::row(r0) + 4 * (threadIdx.x % LANES);
     const auto value = [&](int k, int i) {
-      return lane_of<T, ALIGNED>(tile + k * TB, in[k] + tile0 * A.tok[k], A.tok[k], r0 + i);
+      return lane_of<T, ALIGNED>(mine + k * TB + i * Tile<S, ALIGNED>::kPitch, in[k] + tile0 * A.tok[k], A.tok[k], r0 + i);
     };
     const auto token = [&](int i, F& a, F& u, F& b) {
       const F x = value(0, i);
@@ -503,7 +525,7 @@ __global__ void __launch_bounds__(Fwd::kThreads, Fwd::kCtas) gated_fwd_kernel(co
       }
       P = each_(P, least, [](float v, float w) { return w > 0.0f ? above_zero(v) : v; });
     }
-    const F carry = hand_on(B, p, k, step, warp, Map<F>{P, low_part(P, D), h}, state, A.patience, lost);
+    const F carry = hand_on(B, p, k, step, p.seg, Map<F>{P, low_part(P, D), h}, state, A.patience, lost);
     if (p.have < 1) return;
     T* const y = reinterpret_cast<T*>(A.out[0]) + ((long long)p.b * A.L + t0) * A.C + p.ch;
     float* const s = A.saved + ((long long)p.b * A.segments + t0 / kSaved) * A.C + p.ch;
@@ -551,29 +573,29 @@ __global__ void __launch_bounds__(Fwd::kThreads, Fwd::kCtas) gated_fwd_kernel(co
   int k = p.rank, step = 0;
   for (; k < full; k += p.n, ++step) run(k, step, std::true_type{});
   if (k < p.tiles) run(k, step, std::false_type{});
-  // the last tile's CTA has the state in its last warp; a row without tokens keeps what it was given
-  if (A.last && warp == S::kWarps - 1 && p.rank == max(p.tiles - 1, 0) % p.n)
+  // the last tile's CTA has the state in its last segment; a row without tokens keeps what it was given
+  if (A.last && p.seg == S::kSegs - 1 && p.rank == max(p.tiles - 1, 0) % p.n)
     put_state(A.last + (long long)p.b * A.C + p.ch, p.have, state);
   zeros_behind<T, S, ALIGNED, 1>(A, p);
   close_board(p, lost);
 }
 
-template <typename T, bool LOG, bool GATE, bool COMP, bool ALIGNED>
-__global__ void __launch_bounds__(Bwd::kThreads, Bwd::kCtas) gated_bwd_kernel(const ScanArgs A) {
+template <typename T, int LANES, bool LOG, bool GATE, bool COMP, bool ALIGNED>
+__global__ void __launch_bounds__(Bwd<LANES>::kThreads, Bwd<LANES>::kCtas) gated_bwd_kernel(const ScanArgs A) {
   using F = typename Lane<T>::F;
-  using S = Bwd;
-  constexpr int K = GATE ? 4 : 3, TB = kTileBytes<S, ALIGNED>, kSeg = S::kSeg;
+  using S = Bwd<LANES>;
+  constexpr int K = GATE ? 4 : 3, TB = Tile<S, ALIGNED>::kBytes, kSeg = S::kSeg;
   constexpr int kDy = K - 1;  // x, gate, (out_gate,) dy
   extern __shared__ __align__(128) unsigned char smem[];
-  auto& B = *reinterpret_cast<Board<F, S::kWarps>*>(smem + 2 * K * TB);
+  auto& B = *reinterpret_cast<Board<F, S>*>(smem + 2 * K * TB);
   const Place p = place_of<T, S>(A);
-  const int warp = threadIdx.x >> 5, width = min(kWidth, A.C * (int)sizeof(T) - p.col * kWidth);
+  const int width = min(S::kWidth, A.C * (int)sizeof(T) - p.col * S::kWidth);
   const char* in[K];
   long long tok[K];
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     const int from = k == kDy ? 3 : k;
-    in[k] = A.in[from] + p.b * A.batch[from] + p.col * kWidth;
+    in[k] = A.in[from] + p.b * A.batch[from] + p.col * S::kWidth;
     tok[k] = A.tok[from];
   }
   const auto fetch = [&](int step, int tile) {
@@ -592,7 +614,7 @@ __global__ void __launch_bounds__(Bwd::kThreads, Bwd::kCtas) gated_bwd_kernel(co
   if (p.rank < p.tiles) fetch(0, p.tiles - 1 - p.rank);
   const auto run = [&](int k, int step, auto all_live) {
     constexpr bool whole = decltype(all_live)::value;
-    const int tile0 = (p.tiles - 1 - k) * S::kTile, r0 = warp * kSeg, t0 = tile0 + r0;
+    const int tile0 = (p.tiles - 1 - k) * S::kTile, r0 = p.seg * kSeg, t0 = tile0 + r0;
     const int live = whole ? kSeg : min(kSeg, p.len - t0);
     F before[kSeg + 1];  // before[i]: the state that enters token i
     before[0] = all_<F>(0.0f);
@@ -601,8 +623,9 @@ __global__ void __launch_bounds__(Bwd::kThreads, Bwd::kCtas) gated_bwd_kernel(co
     __syncthreads();
     if (k + p.n < p.tiles) fetch(step + 1, p.tiles - 1 - k - p.n);
     const unsigned char* tile = smem + (step & 1) * K * TB;
+    const unsigned char* mine = tile + Tile<S, ALIGNED>::row(r0) + 4 * (threadIdx.x % LANES);
     const auto value = [&](int k, int i) {
-      return lane_of<T, ALIGNED>(tile + k * TB, in[k] + tile0 * tok[k], tok[k], r0 + i);
+      return lane_of<T, ALIGNED>(mine + k * TB + i * Tile<S, ALIGNED>::kPitch, in[k] + tile0 * tok[k], tok[k], r0 + i);
     };
     F a[kSeg], u[kSeg], sig[kSeg];
     F c = all_<F>(0.0f), P = all_<F>(1.0f), D = all_<F>(0.0f);
@@ -636,7 +659,7 @@ __global__ void __launch_bounds__(Bwd::kThreads, Bwd::kCtas) gated_bwd_kernel(co
         if (i < live) least = each_(least, a[i], [](float v, float w) { return fminf(v, w); });
       P = each_(P, least, [](float v, float w) { return w > 0.0f ? above_zero(v) : v; });
     }
-    c = hand_on(B, p, k, step, S::kWarps - 1 - warp, Map<F>{P, low_part(P, D), c}, state, A.patience, lost);
+    c = hand_on(B, p, k, step, S::kSegs - 1 - p.seg, Map<F>{P, low_part(P, D), c}, state, A.patience, lost);
     const long long at = ((long long)p.b * A.L + t0) * A.C + p.ch;
     T* const dx_at = reinterpret_cast<T*>(A.out[0]) + at;
     T* const dg_at = reinterpret_cast<T*>(A.out[1]) + at;
@@ -675,7 +698,7 @@ __global__ void __launch_bounds__(Bwd::kThreads, Bwd::kCtas) gated_bwd_kernel(co
     k += p.n, ++step;
   }
   for (; k < p.tiles; k += p.n, ++step) run(k, step, std::true_type{});
-  if (A.last && warp == 0 && p.rank == max(p.tiles - 1, 0) % p.n)
+  if (A.last && p.seg == 0 && p.rank == max(p.tiles - 1, 0) % p.n)
     put_state(A.last + (long long)p.b * A.C + p.ch, p.have, state);
   zeros_behind<T, S, ALIGNED, GATE ? 3 : 2>(A, p);
   close_board(p, lost);
@@ -737,16 +760,23 @@ __global__ void __launch_bounds__(256) gated_step_kernel(const StepArgs A) {
 
 using Kernel = void (*)(ScanArgs);
 
-template <typename T, bool LOG, bool GATE, bool COMP> Kernel pick3(bool back, bool aligned) {
-  if (back) return aligned ? gated_bwd_kernel<T, LOG, GATE, COMP, true> : gated_bwd_kernel<T, LOG, GATE, COMP, false>;
-  return aligned ? gated_fwd_kernel<T, LOG, GATE, COMP, true> : gated_fwd_kernel<T, LOG, GATE, COMP, false>;
+struct Form {
+  bool back, log, gate, complement, aligned;
+};
+template <typename T, int LANES, bool LOG, bool GATE, bool COMP> Kernel pick3(const Form& f) {
+  if (f.back) return f.aligned ? gated_bwd_kernel<T, LANES, LOG, GATE, COMP, true> : gated_bwd_kernel<T, LANES, LOG, GATE, COMP, false>;
+  return f.aligned ? gated_fwd_kernel<T, LANES, LOG, GATE, COMP, true> : gated_fwd_kernel<T, LANES, LOG, GATE, COMP, false>;
 }
-template <typename T, bool LOG, bool GATE> Kernel pick2(bool back, bool complement, bool aligned) {
-  return complement ? pick3<T, LOG, GATE, true>(back, aligned) : pick3<T, LOG, GATE, false>(back, aligned);
+template <typename T, int LANES, bool LOG, bool GATE> Kernel pick2(const Form& f) {
+  return f.complement ? pick3<T, LANES, LOG, GATE, true>(f) : pick3<T, LANES, LOG, GATE, false>(f);
 }
-template <typename T> Kernel pick(bool back, bool log, bool gate, bool complement, bool aligned) {
-  if (log) return gate ? pick2<T, true, true>(back, complement, aligned) : pick2<T, true, false>(back, complement, aligned);
-  return gate ? pick2<T, false, true>(back, complement, aligned) : pick2<T, false, false>(back, complement, aligned);
+template <typename T, int LANES> Kernel pick1(const Form& f) {
+  if (f.log) return f.gate ? pick2<T, LANES, true, true>(f) : pick2<T, LANES, true, false>(f);
+  return f.gate ? pick2<T, LANES, false, true>(f) : pick2<T, LANES, false, false>(f);
+}
+template <int LANES> Kernel pick(int dtype, const Form& f) {
+  if (dtype == HYFFT_F32) return pick1<float, LANES>(f);
+  return dtype == HYFFT_BF16 ? pick1<__nv_bfloat16, LANES>(f) : pick1<__half, LANES>(f);
 }
 
 // Clusters of n CTAs that can run at once (0: unknown), asked once for each kernel, size and device.
@@ -775,6 +805,19 @@ int room_for(Kernel fn, int n, int threads, size_t smem) {
   return room;
 }
 
+struct Bytes {
+  int tile, threads;
+  size_t smem;
+};
+template <int LANES> Bytes bytes_of(const Form& f, int e) {
+  const auto of = [&](auto shape, int tensors) {
+    using S = decltype(shape);
+    const size_t tile = f.aligned ? Tile<S, true>::kBytes : Tile<S, false>::kBytes;
+    return Bytes{S::kTile, S::kThreads, 2 * tile * tensors + (e == 4 ? sizeof(Board<float, S>) : sizeof(Board<float2, S>))};
+  };
+  return f.back ? of(Bwd<LANES>{}, f.gate ? 4 : 3) : of(Fwd<LANES>{}, f.gate ? 3 : 2);
+}
+
 int check_desc(const hyfft_gated_desc* d, const char* null_msg) {
   if (!d) return set_error(HYFFT_ERR_INVALID, null_msg);
   if (d->batch < 1 || d->length < 1 || d->channels < 1)
@@ -792,7 +835,6 @@ int run_scan(const hyfft_gated_desc* d, ScanArgs A, bool back, cudaStream_t st) 
   const int e = d->dtype == HYFFT_F32 ? 4 : 2;
   const bool gate = A.in[2] != nullptr;
   A.L = (int)d->length, A.C = d->channels, A.complement = d->complement ? 1 : 0;
-  A.cols = (int)(((long long)A.C * e + kWidth - 1) / kWidth);
   A.segments = (A.L + kSaved - 1) / kSaved;
   const int64_t* strides[4] = {d->x_stride, d->gate_stride, d->out_gate_stride, d->dy_stride};
   bool aligned = (long long)A.C * e % 4 == 0;
@@ -802,19 +844,22 @@ int run_scan(const hyfft_gated_desc* d, ScanArgs A, bool back, cudaStream_t st) 
     aligned = aligned && reinterpret_cast<uintptr_t>(A.in[k]) % 16 == 0 && A.batch[k] % 16 == 0 && A.tok[k] % 16 == 0;
   }
   for (int k = 0; k < 3; ++k) aligned = aligned && reinterpret_cast<uintptr_t>(A.out[k]) % 4 == 0;
-  const bool log = d->form == HYFFT_GATED_LOG;
-  const Kernel fn = d->dtype == HYFFT_F32    ? pick<float>(back, log, gate, A.complement, aligned)
-                    : d->dtype == HYFFT_BF16 ? pick<__nv_bfloat16>(back, log, gate, A.complement, aligned)
-                                             : pick<__half>(back, log, gate, A.complement, aligned);
-  const int tile = back ? Bwd::kTile : Fwd::kTile, threads = back ? Bwd::kThreads : Fwd::kThreads;
-  const size_t board = back ? (e == 4 ? sizeof(Board<float, Bwd::kWarps>) : sizeof(Board<float2, Bwd::kWarps>))
-                            : (e == 4 ? sizeof(Board<float, Fwd::kWarps>) : sizeof(Board<float2, Fwd::kWarps>));
-  const size_t smem = 2 * (size_t)tile * (aligned ? kPitch<true> : kPitch<false>)*((gate ? 3 : 2) + (back ? 1 : 0)) + board;
+  const Form form{back, d->form == HYFFT_GATED_LOG, gate, d->complement != 0, aligned};
+  const auto rows_of = [&](int width) { return (long long)d->batch * (((long long)A.C * e + width - 1) / width); };
+  // Few rows: half as wide ones, so twice as many, of tiles with twice the tokens, so half the hops. Measured, bfloat16 with output gates,
+  // wide against narrow: rows of 128 bytes 4 (1 x 65536 x 256): 249 | 119 us forwards, 305 | 163 backwards; 16 (4 x 16384 x 256): 73 | 48, 94 | 85;
+  // 32 (8 x 16384 x 256): 85 | 75, 130 | 155; 48 (3 x 8192 x 1024): 58 | 61, 101 | 151; 64 (1 x 65536 x 4096): 490 | 528, 924 | 1137.
+  const bool narrow = rows_of(128) < (back ? 24 : 48);
+  const Kernel fn = narrow ? pick<16>(d->dtype, form) : pick<32>(d->dtype, form);
+  const long long rows = rows_of(narrow ? 64 : 128);
+  A.cols = (int)(rows / d->batch);
+  const Bytes by = narrow ? bytes_of<16>(form, e) : bytes_of<32>(form, e);
+  const int tile = by.tile, threads = by.threads;
+  const size_t smem = by.smem;
   A.patience = g_wait_clocks.load(std::memory_order_relaxed);
   if (!kernel_smem_once(reinterpret_cast<const void*>(fn), smem, true))
     return set_error(HYFFT_ERR_CUDA, "gated scan: shared memory");
   // As many CTAs for a row as the machine can run at once for all rows, and as the row has tiles.
-  const long long rows = (long long)d->batch * A.cols;
   int n = (int)std::min<long long>(kMaxCluster, (A.L + tile - 1) / tile);
   while (n > 1 && room_for(fn, n, threads, smem) < rows) --n;
   A.n = n;
