@@ -167,9 +167,12 @@ template <typename F> struct Map { F P, l, H; };
 __device__ __forceinline__ bool infinite(float v) { return fabsf(v) == CUDART_INF_F; }
 
 template <typename F> __device__ __forceinline__ F apply(const Map<F>& m, F h) { return fma_(m.P, h, fma_(m.l, h, m.H)); }
-// l is a correction of what P says: it leaves an infinity alone (which would become a NaN).
+// The same where a product overflows or h is infinite: l, a correction of what P says, leaves an infinity alone (which would become a
+// NaN), and a state of zero stays zero under decays above 1 whose product is infinite.
 template <typename F> __device__ __forceinline__ F apply_to_infinity(const Map<F>& m, F h) {
-  return fma_(m.P, h, fma_(m.l, each_(h, [](float v) { return infinite(v) ? 0.0f : v; }), m.H));
+  const F fin = each_(h, [](float v) { return infinite(v) ? 0.0f : v; });
+  const F ph = each_(m.P, h, [](float p, float v) { return v == 0.0f && p == p ? 0.0f : p * v; });
+  return add_(ph, fma_(m.l, fin, m.H));
 }
 
 // A product of decays above 0 is above 0: an infinite state stays infinite where the product has underflowed.
@@ -529,7 +532,8 @@ __global__ void __launch_bounds__(Fwd<LANES>::kThreads, Fwd<LANES>::kCtas) gated
     if (p.have < 1) return;
     T* const y = reinterpret_cast<T*>(A.out[0]) + ((long long)p.b * A.L + t0) * A.C + p.ch;
     float* const s = A.saved + ((long long)p.b * A.segments + t0 / kSaved) * A.C + p.ch;
-    if (any_(carry, infinite)) {  // token by token, so that an infinity stays one; apart from the rest, which keeps its registers
+    // token by token, so that an infinity stays one; apart from the rest, which keeps its registers
+    if (any_(carry, infinite) || any_(P, infinite)) {
       F full = carry;
 #pragma unroll 1
       for (int i = 0; i < kSeg && t0 + i < A.L; ++i) {

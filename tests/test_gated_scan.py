@@ -302,6 +302,25 @@ def test_growing_log_decays():
 
 
 @gpu
+def test_decays_above_one_whose_product_overflows():
+    """exp(3) for each token: a state of zero stays zero however long, and what is put in grows as far as float32 goes."""
+    L = 400
+    x, g = torch.zeros(1, L, 8, device="cuda"), torch.full((1, L, 8), 3.0, device="cuda")
+    y, s = gated_scan(x, g, form="log", complement=False, return_state=True)
+    assert (y == 0).all() and (s == 0).all()
+    x[0, 380, 1] = 1.0
+    y, s = gated_scan(x, g, form="log", complement=False, return_state=True)
+    want, end = oracle(x, g, form="log", complement=False)
+    for ch in range(8):
+        close(want[..., ch], y[..., ch], F32)
+    close(end, s, F32)
+    x[0, 100, 2] = 1.0
+    y = gated_scan(x, g, form="log", complement=False)
+    assert (y[0, :100, 2] == 0).all() and (y[0, 200:, 2] == float("inf")).all()
+    assert (y[..., 3:] == 0).all() and torch.isfinite(y[..., :2]).all()
+
+
+@gpu
 def test_a_sequence_in_pieces_is_the_sequence():
     c = _case(2, 200, 48, F32)
     x, g, o = (c[k].cuda() for k in ("x", "gate", "out_gate"))
