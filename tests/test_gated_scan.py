@@ -412,6 +412,22 @@ def test_more_rows_than_the_machine_runs_at_once(dtype):
 
 
 @gpu
+@pytest.mark.parametrize("C", [2048, 2101])
+@DTYPES
+def test_rows_that_clusters_share(dtype, C):
+    """Rows enough to be 128 bytes wide and few enough for several CTAs each; ragged, on and off 16 bytes."""
+    B, L, lengths = 3, 333, [333, 64, 200]
+    if dtype is F32:
+        C //= 2
+    c = _case(B, L, C, dtype)
+    some = torch.randint(0, C, (30,), generator=torch.Generator().manual_seed(2))
+    some[:2] = torch.tensor([0, C - 1])
+    few = {k: t[..., some] for k, t in c.items()}
+    for want, got in zip(_want(few, "logit", True, lengths), _run(c, "logit", True, lengths)):
+        close(want, got[..., some.cuda()], got.dtype)
+
+
+@gpu
 def test_waits_that_run_out():
     """A CTA that gives up on its neighbour's message leaves NaN from there on and a status for the host; the next call is sound."""
     from nvsubquadratic_b200 import _lib
