@@ -50,8 +50,8 @@ struct QkArgs {
   long long L, tokens, items[2];  // items: (token, group of heads)
 };
 
-// Where the features of lane j are: U units of 2 V features. A unit of pairs is two runs of V (halves) or one of 2 V (neighbours);
-// units past the pairs hold the features that are not turned, 2 V a unit.
+// Where the features of lane j are: U units of 2 V features, two runs of V (halves; units past the pairs hold the features that are not
+// turned) or one of 2 V (neighbours).
 template <typename T, int V> struct alignas(16) Unit { T e[2 * V]; };
 
 template <typename T, int R>
@@ -70,22 +70,17 @@ template <typename T, int V, int U, bool INTER, bool BACK>
 struct Rows {
   static constexpr int E = 2 * V * U;  // features of a lane
 
-  // the first feature of each run of unit n, and how many features it has; runs: 2, or 1 where the features are neighbours
+  // The first feature of each run of a unit, and how many features it has. Neighbours: one run, whether its pairs are turned or not.
   static __device__ __forceinline__ void runs(const QkArgs& A, int unit, int (&c)[2], int (&n)[2]) {
-    const int pairs = (A.half + V - 1) / V;
-    if (unit < pairs) {
-      const int p = unit * V, k = min(V, A.half - p);
-      if constexpr (INTER) {
-        c[0] = 2 * p, n[0] = 2 * k, c[1] = 0, n[1] = 0;
-      } else {
-        c[0] = p, n[0] = k, c[1] = p + A.half, n[1] = k;
-      }
+    if constexpr (INTER) {
+      c[0] = unit * 2 * V, n[0] = min(max(A.D - c[0], 0), 2 * V), c[1] = 0, n[1] = 0;
     } else {
-      const int p = 2 * A.half + (unit - pairs) * 2 * V;
-      const int left = max(min(2 * V, A.D - p), 0);
-      if constexpr (INTER) {
-        c[0] = p, n[0] = left, c[1] = 0, n[1] = 0;
+      const int pairs = (A.half + V - 1) / V;
+      if (unit < pairs) {
+        const int p = unit * V, k = min(V, A.half - p);
+        c[0] = p, n[0] = k, c[1] = p + A.half, n[1] = k;
       } else {
+        const int p = 2 * A.half + (unit - pairs) * 2 * V, left = max(min(2 * V, A.D - p), 0);
         c[0] = p, n[0] = min(V, left), c[1] = p + V, n[1] = left - n[0];
       }
     }
@@ -156,15 +151,22 @@ struct Rows {
   }
 };
 
-// The pairs of a unit turned (back: turned back); places (2 u, 2 u + 1) or (u, V + u).
+// The pairs of a unit turned (back: turned back), the first `on` of them; places (2 u, 2 u + 1) or (u, V + u).
 template <int V, bool INTER>
-__device__ __forceinline__ void turn(float* v, const float* cs, const float* sn) {
-#pragma unroll
-  for (int u = 0; u < V; ++u) {
+__device__ __forceinline__ void turn(float* v, const float* cs, const float* sn, int on) {
+  const auto one = [&](int u) {
     float &a = v[INTER ? 2 * u : u], &b = v[INTER ? 2 * u + 1 : V + u];
     const float x = a, y = b;
     a = fmaf(x, cs[u], -y * sn[u]);
     b = fmaf(x, sn[u], y * cs[u]);
+  };
+  if (on >= V) {
+#pragma unroll
+    for (int u = 0; u < V; ++u) one(u);
+  } else if (INTER && V > 1 && on > 0) {  // a unit that the turned features end in
+#pragma unroll
+    for (int u = 0; u < V; ++u)
+      if (u < on) one(u);
   }
 }
 
@@ -192,7 +194,8 @@ template <int E, int G> __device__ __forceinline__ float of_large(const float (&
 // next HB rows' loads are in flight while HB are worked on. 65536 tokens of 32 + 32 heads of 128, bfloat16: 412 us forwards (80%
 // of a copy's rate) and 672 backwards (73%); without the loads ahead 424 with four rows at once, and 789 with two backwards; with 8
 // bytes a run instead of 16, twice the lanes of a row, 449 and 812. Neighbouring pairs have 8 features a lane, and room for three
-// CTAs an SM instead of two forwards (32 + 8 heads: 277 against 338 us).
+// CTAs an SM instead of two forwards (32 + 8 heads: 269 against 338 us); turned or not they lie side by side, so their runs are aligned
+// wherever the turned features end (26 x 3238 tokens, 2 + 2 heads of 128, 18 turned, training: 476 -> 195 us).
 template <typename T, int V, int U, int G, bool INTER, bool BACK>
 __global__ void __launch_bounds__(kThreads, BACK || 2 * V * U > 8 ? 2 : 3) qk_norm_kernel(const QkArgs A) {
   using R = Rows<T, V, U, INTER, BACK>;
@@ -306,7 +309,7 @@ __global__ void __launch_bounds__(kThreads, BACK || 2 * V * U > 8 ? 2 : 3) qk_no
           for (int e = 0; e < E; ++e) v[e] = v[e] * r * w[e];
 #pragma unroll
           for (int n = 0; n < U; ++n) {
-            if ((lane + n * G) * V < A.half) turn<V, INTER>(v + n * 2 * V, cs[n], sn[n]);
+            turn<V, INTER>(v + n * 2 * V, cs[n], sn[n], A.half - (lane + n * G) * V);
             if (on) R::store(A, out + (long long)h * A.D, lane + n * G, v + n * 2 * V);
           }
         } else {
@@ -314,7 +317,7 @@ __global__ void __launch_bounds__(kThreads, BACK || 2 * V * U > 8 ? 2 : 3) qk_no
 #pragma unroll
           for (int n = 0; n < U; ++n) {
             R::unpack(raw.d[j][n], t + n * 2 * V);
-            if ((lane + n * G) * V < A.half) turn<V, INTER>(t + n * 2 * V, cs[n], sn[n]);
+            turn<V, INTER>(t + n * 2 * V, cs[n], sn[n], A.half - (lane + n * G) * V);
           }
 #pragma unroll
           for (int e = 0; e < E; ++e) {
@@ -424,7 +427,7 @@ int launch_lanes(const QkArgs& A, int lanes, int* ctas, cudaStream_t st) {
 template <typename T, bool INTER, bool BACK> int launch_t(const QkArgs& A, int* ctas, cudaStream_t st) {
   constexpr int V = (INTER ? 8 : 16) / (int)sizeof(T), E = INTER ? 2 * V : V;  // pairs of a unit, elements of a run
   // runs of 16 bytes where every run of every row starts on a 16-byte boundary, pairs of elements otherwise
-  bool al = A.D % E == 0 && (INTER ? (2 * A.half) % E == 0 : A.half % E == 0);
+  bool al = A.D % E == 0 && (INTER || A.half % E == 0);
   for (int k = 0; k < 2; ++k) {
     if (!A.heads[k]) continue;
     al = al && reinterpret_cast<uintptr_t>(A.x[k]) % (E * sizeof(T)) == 0 && reinterpret_cast<uintptr_t>(A.out[k]) % (E * sizeof(T)) == 0 &&
@@ -432,7 +435,7 @@ template <typename T, bool INTER, bool BACK> int launch_t(const QkArgs& A, int* 
     if (BACK) al = al && reinterpret_cast<uintptr_t>(A.dy[k]) % (E * sizeof(T)) == 0 && A.db[k] % E == 0 && A.dl[k] % E == 0 && A.dh[k] % E == 0;
   }
   const int v = al ? V : 1;
-  const int units = (A.half + v - 1) / v + (A.D - 2 * A.half + 2 * v - 1) / (2 * v);
+  const int units = INTER ? (A.D + 2 * v - 1) / (2 * v) : (A.half + v - 1) / v + (A.D - 2 * A.half + 2 * v - 1) / (2 * v);
   if (al) {
     if constexpr (V * 2 * 32 < kMaxDim)
       if (units > 32) return launch<T, V, 2, 32, INTER, BACK>(A, ctas, st);

@@ -101,7 +101,8 @@ def test_refusals():
 
 # B, L, H, Hk, D, rot
 SHAPES = [(1, 1, 1, 1, 1, 0), (1, 1, 1, 1, 2, 2), (2, 5, 3, 1, 64, 64), (2, 17, 4, 4, 128, 64), (1, 9, 2, 2, 80, 50), (3, 7, 5, 5, 33, 32),
-          (2, 4, 1, 1, 256, 256), (1, 300, 20, 3, 64, 16), (2, 3, 2, 2, 7, 6), (1, 6, 2, 1, 255, 100), (2, 3, 2, 1, 96, 0), (1, 4, 3, 3, 200, 128)]
+          (2, 4, 1, 1, 256, 256), (1, 300, 20, 3, 64, 16), (2, 3, 2, 2, 7, 6), (1, 6, 2, 1, 255, 100), (2, 3, 2, 1, 96, 0), (1, 4, 3, 3, 200, 128),
+          (2, 5, 2, 2, 128, 18), (1, 3, 2, 1, 72, 70)]
 
 
 def _case(B, L, H, Hk, D, rot, dtype, where, seed=0):
