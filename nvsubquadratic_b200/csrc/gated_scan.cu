@@ -20,7 +20,7 @@
 // Measured, bfloat16 with output gates (8 bytes an element forwards, 14 backwards): 64 x 2048 tokens of 1024 channels, one CTA a row,
 // 193 us forwards (85% of a copy's rate) and 354 backwards (81%); 65536 tokens of 4096 channels, 8 and 4 CTAs a cluster, 490 us (67%; one CTA a
 // row 1.54 ms, all of a cluster's maps exchanged behind a barrier 0.73) and 924 us (62%). float32: 97% and 93% of the same rate on the first.
-// What is left is instructions: 38 an element forwards and 55 backwards, of which a third are moves and unpacking, on a machine that has
+// What is left is instructions: 32 an element forwards and 59 backwards, of which a third are moves and unpacking, on a machine that has
 // time for 44 and 77 at a copy's rate; and with clusters the turns of the tiles.
 //
 // What is exact: A is carried as P + l. P is the product of the rounded decays, whose relative error grows with every token; l = (1 - P) - D

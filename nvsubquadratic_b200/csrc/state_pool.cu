@@ -6,8 +6,9 @@
 // cycles, so every source has to be read before its row is written. A CTA takes the same few bytes of every row that takes part: it copies
 // them to shared memory, waits, and writes them out, so nothing crosses HBM twice and no second buffer is needed. A kernel of one CTA
 // comes first and drops what is not to be copied: targets outside the pool, and all but the last move into a slot.
-// 224 rows of 2 MB in another order: 162 us (89% of a copy's rate); 2000 rows of 16 KB: 25 us (41%: the list of moves takes 5 us, and
-// every CTA reads it; 56 us with one unit looked up at a time).
+// 224 rows of 2 MB in another order: 157 us (91% of a copy's rate); 2000 rows of 16 KB: 26 us (38%: the list of moves takes 5 us to make, and
+// every CTA reads it; 56 us with one unit looked up at a time). Rows off 16 bytes go 4 at a time: 195 rows of 355 KB cleared in 54
+// us instead of 25.
 // Compaction fills the lowest free slots with the highest running requests; sources and targets are apart, and rows are copied through
 // registers.
 #include <cuda_runtime.h>
@@ -29,7 +30,7 @@ constexpr int kThreads = 256;
 constexpr int kPlanThreads = 1024;
 constexpr size_t kStageBytes = 64 * 1024;       // of shared memory for a CTA where that is enough
 constexpr size_t kStageMost = 200 * 1024;
-constexpr int kSkip = -2;                        // a move that is not made; -1: zeros
+constexpr int kSkip = -2;
 
 struct PoolArgs {
   char* base[HYFFT_MAX_POOLS];
@@ -38,15 +39,16 @@ struct PoolArgs {
   int width[HYFFT_MAX_POOLS];        // bytes of a row that a CTA takes
   int first[HYFFT_MAX_POOLS + 1];    // a pool's first CTA
   int pools;
-  const int* source;                 // of each move
-  const int* target;
+  const int* source;                 // the row that each move reads, kSkip for none
+  const int* target;                 // the row that it writes, or what plan_copy_kernel says
   const int* count;                  // moves, on the device (compaction); or NULL
   int moves;
 };
 
-// A move's source: kSkip where it is not made. owner [slots]: the last move into each slot.
+// from [moves]: the row that each move reads, to [moves]: the row that it writes; kSkip where it does not, and rows that become zeros are
+// counted down from kSkip - 1. owner [slots]: the last move into each slot.
 __global__ void __launch_bounds__(kPlanThreads) plan_copy_kernel(const int* source, const int* target, int moves, int slots, int* owner,
-                                                                 int* plan) {
+                                                                 int* from, int* to) {
   for (int i = threadIdx.x; i < moves; i += kPlanThreads) {
     const int t = target[i];
     if (t >= 0 && t < slots) owner[t] = -1;
@@ -60,7 +62,9 @@ __global__ void __launch_bounds__(kPlanThreads) plan_copy_kernel(const int* sour
   for (int i = threadIdx.x; i < moves; i += kPlanThreads) {
     const int t = target[i], s = source[i];
     const bool made = t >= 0 && t < slots && atomicMax(owner + t, -1) == i && s != t;
-    plan[i] = !made ? kSkip : s >= 0 && s < slots ? s : -1;
+    const bool row = s >= 0 && s < slots;
+    from[i] = made && row ? s : kSkip;
+    to[i] = !made ? kSkip : row ? t : kSkip - 1 - t;
   }
 }
 
@@ -113,17 +117,16 @@ __global__ void __launch_bounds__(kPlanThreads) plan_compact_kernel(const unsign
   for (int k = threadIdx.x; k < m; k += kPlanThreads) moved[movers[k]] = holes[k];
 }
 
-template <int U> __device__ __forceinline__ void to_shared(unsigned char* dst, const char* src, bool zero) {
+template <int U> __device__ __forceinline__ void to_shared(unsigned char* dst, const char* src) {
   const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst);
-  const int n = zero ? 0 : U;
   if constexpr (U == 16)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(src), "r"(n) : "memory");
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d), "l"(src) : "memory");
   else if constexpr (U == 8)
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(d), "l"(src), "r"(n) : "memory");
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(d), "l"(src) : "memory");
   else if constexpr (U == 4)
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(d), "l"(src), "r"(n) : "memory");
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(d), "l"(src) : "memory");
   else
-    *dst = zero ? 0 : *reinterpret_cast<const unsigned char*>(src);
+    *dst = *reinterpret_cast<const unsigned char*>(src);
 }
 template <int U> struct Word;
 template <> struct Word<16> { using T = uint4; };
@@ -155,11 +158,15 @@ template <int U> __device__ __forceinline__ void copy_slice(const PoolArgs& A, c
     }
   };
   each([&](int m) { return A.source[m]; },
-       [&](int m, int u, int s) { to_shared<U>(stage + m * width + u, base + (s < 0 ? 0 : s) * row + u, s < 0); });
+       [&](int m, int u, int s) { to_shared<U>(stage + m * width + u, base + s * row + u); });
   asm volatile("cp.async.wait_all;" ::: "memory");
   __syncthreads();
-  each([&](int m) { return A.source[m] == kSkip ? kSkip : A.target[m]; },
-       [&](int m, int u, int t) { *reinterpret_cast<W*>(base + t * row + u) = *reinterpret_cast<const W*>(stage + m * width + u); });
+  each([&](int m) { return A.target[m]; },
+       [&](int m, int u, int t) {
+         W w{};
+         if (t >= 0) w = *reinterpret_cast<const W*>(stage + m * width + u);
+         *reinterpret_cast<W*>(base + (t >= 0 ? t : kSkip - 1 - t) * row + u) = w;
+       });
 }
 
 __global__ void __launch_bounds__(kThreads) pool_copy_kernel(const PoolArgs A) {
@@ -243,7 +250,7 @@ using namespace hyfft;
 extern "C" int hyfft_pool_workspace_size(int64_t slots, int64_t moves, size_t* copy_bytes, size_t* compact_bytes) {
   if (slots < 1 || moves < 0) return set_error(HYFFT_ERR_INVALID, "slots: bad sizes");
   if (!copy_bytes || !compact_bytes) return set_error(HYFFT_ERR_INVALID, "slots: null size");
-  *copy_bytes = sizeof(int) * (size_t)(slots + moves);
+  *copy_bytes = sizeof(int) * (size_t)(slots + 2 * moves);
   *compact_bytes = sizeof(int) * (size_t)(2 * slots + 1);
   return HYFFT_OK;
 }
@@ -261,8 +268,9 @@ extern "C" int hyfft_pool_copy(const hyfft_pool* pools, int32_t n, int64_t slots
   if (bind_device_of(pools[0].data) != HYFFT_OK) return set_error(HYFFT_ERR_CUDA, "slots: device");
   PoolArgs A = args_of(pools, n);
   int* owner = static_cast<int*>(workspace);
-  int* plan = owner + slots;
-  A.source = plan, A.target = target, A.moves = (int)moves;
+  int* from = owner + slots;
+  int* to = from + moves;
+  A.source = from, A.target = to, A.moves = (int)moves;
   // As wide a slice of the rows as a CTA's share of shared memory holds, and narrow enough for two CTAs an SM
   long long total = 0;
   for (int p = 0; p < n; ++p) total += A.row[p];
@@ -282,7 +290,7 @@ extern "C" int hyfft_pool_copy(const hyfft_pool* pools, int32_t n, int64_t slots
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (smem > 48 * 1024 && !kernel_smem_once(reinterpret_cast<const void*>(pool_copy_kernel), kStageMost))
     return set_error(HYFFT_ERR_CUDA, "slots: shared memory");
-  plan_copy_kernel<<<1, kPlanThreads, 0, st>>>(source, target, (int)moves, (int)slots, owner, plan);
+  plan_copy_kernel<<<1, kPlanThreads, 0, st>>>(source, target, (int)moves, (int)slots, owner, from, to);
   pool_copy_kernel<<<(unsigned)ctas, kThreads, smem, st>>>(A);
   if (cudaGetLastError() != cudaSuccess) return set_error(HYFFT_ERR_CUDA, "slots: kernel launch failed");
   g_launches.fetch_add(2, std::memory_order_relaxed);
