@@ -110,6 +110,35 @@ def test_refusals():
         gated_scan_step(t.clone().requires_grad_(), t, s)
 
 
+def test_library_refusals():
+    """At the C entry, on the host, before anything is launched."""
+    import ctypes
+
+    from nvsubquadratic_b200 import _lib
+
+    lib, p, size = _lib.load(), ctypes.c_void_p(16), ctypes.c_size_t()
+
+    def desc(**kw):
+        d = _lib.GatedDesc()
+        d.batch, d.length, d.channels, d.dtype = 2, 20, 8, _lib.BF16
+        for k, v in kw.items():
+            setattr(d, k, v)
+        return ctypes.byref(d)
+
+    assert lib.hyfft_gated_saved_size(desc(), ctypes.byref(size)) == 0 and size.value == 4 * 2 * 3 * 8
+    for bad in (dict(batch=0), dict(length=0), dict(channels=0), dict(dtype=3), dict(form=2)):
+        assert lib.hyfft_gated_saved_size(desc(**bad), ctypes.byref(size)) == _lib.HYFFT_ERR_INVALID
+    assert lib.hyfft_gated_saved_size(desc(length=1 << 31), ctypes.byref(size)) == _lib.HYFFT_ERR_UNSUPPORTED
+    assert lib.hyfft_gated_saved_size(None, ctypes.byref(size)) == _lib.HYFFT_ERR_INVALID
+    assert lib.hyfft_gated_forward(desc(), None, p, None, None, None, p, None, None, 0, None) == _lib.HYFFT_ERR_INVALID
+    assert lib.hyfft_gated_forward(desc(), p, p, None, None, None, p, None, p, 8, None) == _lib.HYFFT_ERR_WORKSPACE
+    args = [p, p, None, None]
+    assert lib.hyfft_gated_backward(desc(), *args, None, 0, p, None, p, p, None, None, None) == _lib.HYFFT_ERR_WORKSPACE
+    args[2] = p  # an output gate without a place for its gradient
+    assert lib.hyfft_gated_backward(desc(), *args, p, 1 << 20, p, None, p, p, None, None, None) == _lib.HYFFT_ERR_INVALID
+    assert lib.hyfft_gated_step(desc(), p, p, None, None, 1, p, p, p, None) == _lib.HYFFT_ERR_INVALID  # two requests, one state
+
+
 # ---------------------------------------------------------------- GPU
 
 # B, L, C: single tokens and channels, tiles and segments cut in every place, columns of 128 bytes cut, rows on and off 16 bytes

@@ -97,6 +97,33 @@ def test_refusals():
         qk_norm_rotary(q.double(), k.double())
 
 
+def test_library_refusals():
+    """At the C entry, on the host, before anything is launched."""
+    import ctypes
+
+    from nvsubquadratic_b200 import _lib
+
+    lib, p, size = _lib.load(), ctypes.c_void_p(16), ctypes.c_size_t()
+
+    def desc(**kw):
+        d = _lib.QkNormDesc()
+        d.batch, d.length, d.heads, d.kv_heads, d.dim, d.rot_dim, d.dtype, d.weight_dtype = 2, 3, 4, 2, 16, 8, _lib.BF16, _lib.BF16
+        for k, v in kw.items():
+            setattr(d, k, v)
+        return ctypes.byref(d)
+
+    assert lib.hyfft_qk_norm_workspace_size(desc(), ctypes.byref(size)) == 0 and size.value > 0
+    for bad in (dict(heads=0), dict(kv_heads=-1), dict(rot_dim=7), dict(rot_dim=18), dict(dtype=5), dict(weight_dtype=_lib.F16)):
+        assert lib.hyfft_qk_norm_workspace_size(desc(**bad), ctypes.byref(size)) == _lib.HYFFT_ERR_INVALID, bad
+    assert lib.hyfft_qk_norm_workspace_size(desc(dim=257), ctypes.byref(size)) == _lib.HYFFT_ERR_UNSUPPORTED
+    assert lib.hyfft_qk_norm_forward(desc(), p, p, None, None, None, None, p, p, None) == _lib.HYFFT_ERR_INVALID  # no turns
+    assert lib.hyfft_qk_norm_forward(desc(), p, None, None, None, p, None, p, p, None) == _lib.HYFFT_ERR_INVALID  # no k
+    back = [p, p, None, None, p, None, p, p, p, p]
+    assert lib.hyfft_qk_norm_backward(desc(), *back, p, None, p, 1 << 30, None) == _lib.HYFFT_ERR_INVALID  # no such weight
+    back[2] = p
+    assert lib.hyfft_qk_norm_backward(desc(), *back, p, None, p, 8, None) == _lib.HYFFT_ERR_WORKSPACE
+
+
 # ---------------------------------------------------------------- GPU
 
 # B, L, H, Hk, D, rot
