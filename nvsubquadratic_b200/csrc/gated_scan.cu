@@ -24,7 +24,7 @@
 // time for 44 and 77 at a copy's rate; and with clusters the turns of the tiles.
 //
 // What is exact: A is carried as P + l. P is the product of the rounded decays, whose relative error grows with every token; l = (1 - P) - D
-// with D = 1 - A, accumulated as D += u P, which keeps the digits of slow decays. So a state that remembers 10^5 tokens is off by the
+// with D = 1 - A, accumulated as D += u P, which keeps the digits of slow decays (0 where decays above 1 made P large on the way, and D inexact). So a state that remembers 10^5 tokens is off by the
 // roundings of its 10^4 segments, not by those of its decays; within a segment, by 16 products of rounded decays. Sums are float32.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -110,6 +110,8 @@ template <typename Op> __device__ __forceinline__ float2 each_(float2 a, float2 
 }
 template <typename Op> __device__ __forceinline__ bool any_(float a, Op op) { return op(a); }
 template <typename Op> __device__ __forceinline__ bool any_(float2 a, Op op) { return op(a.x) || op(a.y); }
+template <typename Op> __device__ __forceinline__ bool any_(float a, float b, Op op) { return op(a, b); }
+template <typename Op> __device__ __forceinline__ bool any_(float2 a, float2 b, Op op) { return op(a.x, b.x) || op(a.y, b.y); }
 
 // 2^x and 1 / x to 2 units in the last place, results below 2^-126 flushed to zero.
 __device__ __forceinline__ float exp2_(float x) {
@@ -150,8 +152,9 @@ template <bool LOG, typename F> __device__ __forceinline__ void decay_of(F g, F&
     s = fma_(s, mul_(g, all_<F>(1.0f / 5)), one);
     s = fma_(s, mul_(g, all_<F>(1.0f / 4)), one);
     s = fma_(s, mul_(g, all_<F>(1.0f / 3)), one);
-    s = fma_(s, mul_(g, all_<F>(1.0f / 2)), one);
-    u = each_(g, mul_(g, s), sub_(one, a), [](float v, float near, float far) { return fabsf(v) < 0.35f ? -near : far; });
+    s = fma_(s, mul_(g, all_<F>(-1.0f / 2)), all_<F>(-1.0f));
+    // below 0 for decays above 1 alone: a gate of 0 leaves +0
+    u = each_(g, fma_(g, s, all_<F>(0.0f)), sub_(one, a), [](float v, float near, float far) { return fabsf(v) < 0.35f ? near : far; });
   } else {
     const F e = exp_of<-1>(g);
     a = each_(add_(e, all_<F>(1.0f)), inverse);
@@ -164,36 +167,65 @@ template <bool LOG, typename F> __device__ __forceinline__ void decay_of(F g, F&
 
 template <typename F> struct Map { F P, l, H; };
 
-__device__ __forceinline__ bool infinite(float v) { return fabsf(v) == CUDART_INF_F; }
-
-template <typename F> __device__ __forceinline__ F apply(const Map<F>& m, F h) { return fma_(m.P, h, fma_(m.l, h, m.H)); }
-// The same where a product overflows or h is infinite: l, a correction of what P says, leaves an infinity alone (which would become a
-// NaN), and a state of zero stays zero under decays above 1 whose product is infinite.
-template <typename F> __device__ __forceinline__ F apply_to_infinity(const Map<F>& m, F h) {
-  const F fin = each_(h, [](float v) { return infinite(v) ? 0.0f : v; });
-  const F ph = each_(m.P, h, [](float p, float v) { return v == 0.0f && p == p ? 0.0f : p * v; });
-  return add_(ph, fma_(m.l, fin, m.H));
-}
-
-// A product of decays above 0 is above 0: an infinite state stays infinite where the product has underflowed.
+// Where a map does not give what the recurrence holds in float32, its result is NaN and the tokens are run one by one instead:
+// a product of decays or a state from zero that overflows (what enters may be small, or of the other sign); and, where decays may be above
+// 1 (form log) and make small states large again, a product that has lost digits (below kLeast: off by up to 2^-149) and grows, or is
+// most of a result. A product of 0 has a decay of exactly 0 in it and loses nothing. A decay of 1 at most needs no such care: what a
+// product below kLeast leaves of a state is 2^-100 of it.
+constexpr float kLeast = 7.888609e-31f;  // 2^-100
+constexpr float kLost = 9.403955e-38f;   // 2^-123: 2^-149 of what enters is at most a quarter of a result's last place
 __device__ __forceinline__ float above_zero(float p) { return p == 0.0f ? __int_as_float(1) : p; }
 
+__device__ __forceinline__ bool infinite(float v) { return fabsf(v) == CUDART_INF_F; }
+__device__ __forceinline__ bool finite(float v) { return fabsf(v) < CUDART_INF_F; }
+template <typename F> __device__ __forceinline__ F held(F P, F H) {
+  return each_(P, H, [](float p, float h) { return finite(p) && finite(h) ? p : CUDART_NAN_F; });
+}
+template <typename F> __device__ __forceinline__ F apply(const Map<F>& m, F h) { return fma_(m.P, h, fma_(m.l, h, m.H)); }
+__device__ __forceinline__ bool lossy(float P) { return P > 0.0f && P < kLeast; }
+// r = P h + H, NaN where it needs digits of P that are not there.
+template <typename F> __device__ __forceinline__ F checked(F r, F P, F h) {
+  return each_(r, P, h, [](float v, float p, float w) { return lossy(p) && fabsf(w) * kLost > fabsf(v) ? CUDART_NAN_F : v; });
+}
+// Whether a map made a NaN of what was none.
+template <typename F> __device__ __forceinline__ bool fresh_nan(F to, F from) {
+  return any_(to, from, [](float t, float f) { return t != t && f == f; });
+}
+
 // First f, then s.
-template <typename F> __device__ __forceinline__ Map<F> then(const Map<F>& f, const Map<F>& s) {
+template <bool LOG, typename F> __device__ __forceinline__ Map<F> then(const Map<F>& f, const Map<F>& s) {
   Map<F> r;
   r.H = apply(s, f.H);
-  if (any_(r.H, [](float v) { return v != v; })) r.H = apply_to_infinity(s, f.H);
   const F p = mul_(f.P, s.P);
-  F e = fma_(f.P, s.P, each_(p, [](float v) { return -v; }));
-  e = fma_(f.P, s.l, fma_(s.P, f.l, e));
-  r.P = each_(p, f.P, s.P, [](float v, float a, float b) { return a > 0.0f && b > 0.0f ? above_zero(v) : v; });
-  r.l = each_(e, p, [](float v, float q) { return fabsf(q) < CUDART_INF_F ? v : 0.0f; });
+  const F e = fma_(f.P, s.P, each_(p, [](float v) { return -v; }));
+  r.l = fma_(f.P, s.l, fma_(s.P, f.l, e));
+  r.P = p;
+  if constexpr (LOG) {
+    const F of_some = each_(p, f.P, s.P, [](float v, float a, float b) { return a > 0.0f && b > 0.0f ? above_zero(v) : v; });
+    r.P = each_(of_some, f.P, s.P, [](float v, float a, float b) { return b > 1.0f && lossy(a) ? CUDART_NAN_F : v; });
+  }
+  r.P = held(r.P, r.H);
   return r;
 }
 
 // l of a segment with the product P of its decays and D = 1 - A. Beyond D = 1/2 P is as exact as it gets.
 template <typename F> __device__ __forceinline__ F low_part(F P, F D) {
   return each_(P, D, [](float p, float d) { return fabsf(d) < 0.5f ? (1.0f - p) - d : 0.0f; });
+}
+// The sign bits of what decays leave: set where a decay is above 1.
+__device__ __forceinline__ int signs_of(float u) { return __float_as_int(u); }
+__device__ __forceinline__ int signs_of(float2 u) { return __float_as_int(u.x) | __float_as_int(u.y); }
+// The map of a segment that has decays above 1, for each product on the way and the one before it. D has the roundings of the largest
+// product, so it corrects nothing where that is far above 1.
+template <typename F> __device__ __forceinline__ void grown(Map<F>& m, F P, F before) {
+  m.l = each_(m.l, P, [](float v, float p) { return p > 2.0f ? 0.0f : v; });
+  m.P = each_(m.P, P, before, [](float v, float p, float q) { return q < kLeast && p >= q ? CUDART_NAN_F : v; });
+}
+// Nothing in the channels that are not there (what a tile holds in their place is not defined).
+__device__ __forceinline__ float there(float v, int have) { return have > 0 ? v : 0.0f; }
+__device__ __forceinline__ float2 there(float2 v, int have) { return make_float2(have > 0 ? v.x : 0.0f, have > 1 ? v.y : 0.0f); }
+template <typename F> __device__ __forceinline__ Map<F> there(const Map<F>& m, int have) {
+  return Map<F>{there(m.P, have), there(m.l, have), there(m.H, have)};
 }
 
 // ---------------------------------------------------------------- tiles
@@ -390,33 +422,55 @@ __device__ __forceinline__ void close_board(const Place& p, bool lost) {
 
 // Hands the maps of a tile's segments on. k: the tile's number in the order of the recurrence, step: how many this CTA has done
 // before; order: this lane's segment's place within the tile. state: what enters the first tile; in the last segment, what leaves each.
+// tokens(j, h): the state that leaves the segment in place j, by its tokens, where h enters it.
 // Returns what enters this lane's segment: NaN from the first message on that did not come (lost).
-template <typename F, typename S>
+template <bool LOG, typename F, typename S, typename Tokens>
 __device__ __forceinline__ F hand_on(Board<F, S>& B, const Place& p, int k, int step, int order, const Map<F>& mine, F& state,
-                                     unsigned patience, bool& lost) {
+                                     unsigned patience, bool& lost, const Tokens& tokens) {
   const int lane = threadIdx.x % S::kLanes;
   B.P[order][lane] = mine.P, B.l[order][lane] = mine.l, B.H[order][lane] = mine.H;
-  __syncthreads();
+  // Maps of lost digits are looked at one by one, where a tile has any (looked for in every chain, 64 x 2048 tokens of 1024
+  // channels in bfloat16 took 392 us backwards instead of 377).
+  bool careful = false;
+  if constexpr (LOG)
+    careful = __syncthreads_or(any_(mine.P, lossy)) != 0;
+  else
+    __syncthreads();
   const auto map_of = [&](int j) { return Map<F>{B.P[j][lane], B.l[j][lane], B.H[j][lane]}; };
-  const auto through = [&](const Map<F>& m, F h) {
-    const F r = apply(m, h);
-    return any_(r, [](float v) { return v != v; }) ? apply_to_infinity(m, h) : r;
+  const auto through = [&](int j, F h) {
+    const Map<F> m = map_of(j);
+    F r = apply(m, h);
+    if constexpr (LOG) r = checked(r, m.P, h);
+    if (!fresh_nan(r, h)) return r;
+    return each_(r, tokens(j, h), [](float v, float t) { return v != v ? t : v; });
   };
   // What leaves the tile goes by one map over all of it, which is there before the message is: the next CTA waits for nothing else.
-  const bool last = order == S::kSegs - 1;
+  const bool last = order == S::kSegs - 1, sends = last && p.n > 1;
   Map<F> whole = mine;
-  if (last && p.n > 1) {
-    Map<F> m = map_of(0);
+  if (sends) {
+    whole = map_of(0);
 #pragma unroll 1
-    for (int j = 1; j < S::kSegs - 1; ++j) m = then(m, map_of(j));
-    whole = then(m, mine);
+    for (int j = 1; j < S::kSegs; ++j) {
+      const Map<F> m = map_of(j), both = then<LOG>(whole, m);
+      const F h = whole.H;
+      whole = both;
+      if (careful) whole.P = each_(both.P, checked(both.H, m.P, h), [](float v, float w) { return w != w ? w : v; });
+    }
   }
   if (p.n == 1 && S::kSegs <= 4) {  // few enough for every warp to go through all of them
     F h = state, in = state;
 #pragma unroll
     for (int j = 0; j < S::kSegs; ++j) {
       if (j == order) in = h;
-      h = through(map_of(j), h);
+      h = apply(map_of(j), h);
+    }
+    if (careful || fresh_nan(h, state)) {
+      h = in = state;
+#pragma unroll 1
+      for (int j = 0; j < S::kSegs; ++j) {
+        if (j == order) in = h;
+        h = through(j, h);
+      }
     }
     state = h;
     return in;
@@ -433,22 +487,29 @@ __device__ __forceinline__ F hand_on(Board<F, S>& B, const Place& p, int k, int 
     }
     h = lost ? all_<F>(CUDART_NAN_F) : B.inbox[m & 1][lane];
   }
-  if (last && p.n > 1) {
-    state = through(whole, h);
+  const auto pass_on = [&] {
     if (k + 1 < p.tiles) {
       const int next = p.rank + 1 == p.n ? 0 : p.rank + 1;
       send(at_rank(smem_of(&B.inbox[step & 1][lane]), next), at_rank(smem_of(&B.full[step & 1]), next), state);
     }
+  };
+  bool late = false;
+  if (sends) {
+    state = apply(whole, h);
+    late = fresh_nan(LOG ? checked(state, whole.P, h) : state, h);
+    if (!late) pass_on();
   }
   F in = h;
 #pragma unroll 1
   for (int j = 0; j < order; ++j) in = apply(map_of(j), in);
-  if (any_(in, [](float v) { return v != v; })) {  // an infinity on the way?
+  if (late || careful || fresh_nan(in, h)) {
     in = h;
 #pragma unroll 1
-    for (int j = 0; j < order; ++j) in = apply_to_infinity(map_of(j), in);
+    for (int j = 0; j < order; ++j) in = through(j, in);
   }
-  if (last && p.n == 1) B.inbox[step & 1][lane] = state = through(mine, in);
+  if (late || (last && p.n == 1)) state = through(order, in);
+  if (late) pass_on();
+  if (last && p.n == 1) B.inbox[step & 1][lane] = state;
   return in;
 }
 
@@ -508,6 +569,7 @@ __global__ void __launch_bounds__(Fwd<LANES>::kThreads, Fwd<LANES>::kCtas) gated
     };
     F hl[kSeg], Pl[kSeg];
     F h = all_<F>(0.0f), P = all_<F>(1.0f), D = all_<F>(0.0f);
+    [[maybe_unused]] int signs = 0;
 #pragma unroll
     for (int i = 0; i < kSeg; ++i) {
       if (whole || i < live) {
@@ -516,24 +578,50 @@ __global__ void __launch_bounds__(Fwd<LANES>::kThreads, Fwd<LANES>::kCtas) gated
         h = fma_(a, h, b);
         D = fma_(u, P, D);
         P = mul_(P, a);
+        if constexpr (LOG) signs |= signs_of(u);
       }
       hl[i] = h, Pl[i] = P;
     }
-    if (any_(P, [](float v) { return v == 0.0f; })) {  // underflow, or a decay of exactly 0?
-      F least = all_<F>(1.0f);
-      for (int i = 0; i < live; ++i) {
-        F a, u, b;
-        token(i, a, u, b);
-        least = each_(least, a, [](float v, float w) { return fminf(v, w); });
+    Map<F> map{P, low_part(P, D), h};
+    if constexpr (LOG) {
+      if (signs < 0) {  // a decay above 1
+#pragma unroll
+        for (int i = 0; i < kSeg; ++i) grown(map, Pl[i], i ? Pl[i ? i - 1 : 0] : all_<F>(1.0f));
       }
-      P = each_(P, least, [](float v, float w) { return w > 0.0f ? above_zero(v) : v; });
+      if (any_(P, [](float v) { return v == 0.0f; })) {  // lost, or a decay of 0?
+        F least = all_<F>(1.0f);
+#pragma unroll 1
+        for (int i = 0; i < live; ++i) {
+          F a, u;
+          decay_of<LOG>(value(1, i), a, u);
+          least = each_(least, a, [](float v, float w) { return fminf(v, w); });
+        }
+        map.P = each_(map.P, least, [](float v, float w) { return w > 0.0f ? above_zero(v) : v; });
+      }
     }
-    const F carry = hand_on(B, p, k, step, p.seg, Map<F>{P, low_part(P, D), h}, state, A.patience, lost);
+    map.P = held(map.P, map.H);
+    map = there(map, p.have);
+    const auto tokens = [&](int seg, F state) {
+      const int r = seg * kSeg, n = min(kSeg, p.len - tile0 - r);
+      const unsigned char* at = tile + Tile<S, ALIGNED>::row(r) + 4 * (threadIdx.x % LANES);
+#pragma unroll 1
+      for (int i = 0; i < n; ++i, at += Tile<S, ALIGNED>::kPitch) {
+        const F x = lane_of<T, ALIGNED>(at, in[0] + tile0 * A.tok[0], A.tok[0], r + i);
+        F a, u;
+        decay_of<LOG>(lane_of<T, ALIGNED>(at + TB, in[1] + tile0 * A.tok[1], A.tok[1], r + i), a, u);
+        state = fma_(a, state, COMP ? mul_(u, x) : x);
+      }
+      return state;
+    };
+    const F carry = hand_on<LOG>(B, p, k, step, p.seg, map, state, A.patience, lost, tokens);
     if (p.have < 1) return;
     T* const y = reinterpret_cast<T*>(A.out[0]) + ((long long)p.b * A.L + t0) * A.C + p.ch;
     float* const s = A.saved + ((long long)p.b * A.segments + t0 / kSaved) * A.C + p.ch;
-    // token by token, so that an infinity stays one; apart from the rest, which keeps its registers
-    if (any_(carry, infinite) || any_(P, infinite)) {
+    bool alone = any_(carry, infinite) || any_(map.P, [](float v) { return v != v; });
+    if constexpr (LOG)
+      if (any_(map.P, lossy)) alone = alone || fresh_nan(checked(apply(map, carry), map.P, carry), carry);
+    // token by token, as the recurrence has it; apart from the rest, which keeps its registers
+    if (alone) {
       F full = carry;
 #pragma unroll 1
       for (int i = 0; i < kSeg && t0 + i < A.L; ++i) {
@@ -633,6 +721,7 @@ __global__ void __launch_bounds__(Bwd<LANES>::kThreads, Bwd<LANES>::kCtas) gated
     };
     F a[kSeg], u[kSeg], sig[kSeg];
     F c = all_<F>(0.0f), P = all_<F>(1.0f), D = all_<F>(0.0f);
+    [[maybe_unused]] int signs = 0;
 #pragma unroll
     for (int i = 0; i < kSeg; ++i) {
       before[i + 1] = before[i];
@@ -654,16 +743,50 @@ __global__ void __launch_bounds__(Bwd<LANES>::kThreads, Bwd<LANES>::kCtas) gated
         c = mul_(a[i], add_(dh, c));
         D = fma_(u[i], P, D);
         P = mul_(P, a[i]);
+        if constexpr (LOG) signs |= signs_of(u[i]);
       }
     }
-    if (any_(P, [](float v) { return v == 0.0f; })) {
-      F least = all_<F>(1.0f);
+    Map<F> map{P, low_part(P, D), c};
+    if constexpr (LOG) {
+      if (signs < 0) {  // a decay above 1
+        F q = all_<F>(1.0f);
+#pragma unroll 1
+        for (int i = live - 1; i >= 0; --i) {
+          const F before_it = q;
+          F decay, left;
+          decay_of<LOG>(value(1, i), decay, left);
+          q = mul_(q, decay);
+          grown(map, q, before_it);
+        }
+      }
+      if (any_(P, [](float v) { return v == 0.0f; })) {  // lost, or a decay of 0?
+        F least = all_<F>(1.0f);
 #pragma unroll
-      for (int i = 0; i < kSeg; ++i)
-        if (i < live) least = each_(least, a[i], [](float v, float w) { return fminf(v, w); });
-      P = each_(P, least, [](float v, float w) { return w > 0.0f ? above_zero(v) : v; });
+        for (int i = 0; i < kSeg; ++i)
+          if (whole || i < live) least = each_(least, a[i], [](float v, float w) { return fminf(v, w); });
+        map.P = each_(map.P, least, [](float v, float w) { return w > 0.0f ? above_zero(v) : v; });
+      }
     }
-    c = hand_on(B, p, k, step, S::kSegs - 1 - p.seg, Map<F>{P, low_part(P, D), c}, state, A.patience, lost);
+    map.P = held(map.P, map.H);
+    map = there(map, p.have);
+    const auto tokens = [&](int place, F state) {
+      const int r = (S::kSegs - 1 - place) * kSeg, n = min(kSeg, p.len - tile0 - r);
+      const unsigned char* first = tile + Tile<S, ALIGNED>::row(r) + 4 * (threadIdx.x % LANES);
+#pragma unroll 1
+      for (int i = n - 1; i >= 0; --i) {
+        const unsigned char* at = first + i * Tile<S, ALIGNED>::kPitch;
+        const auto of = [&](int j) { return lane_of<T, ALIGNED>(at + j * TB, in[j] + tile0 * tok[j], tok[j], r + i); };
+        F a, u, dh = of(kDy);
+        decay_of<LOG>(of(1), a, u);
+        if constexpr (GATE) {
+          const F o = of(2);
+          dh = mul_(dh, mul_(o, sigmoid_of(o)));
+        }
+        state = mul_(a, add_(dh, state));
+      }
+      return state;
+    };
+    c = hand_on<LOG>(B, p, k, step, S::kSegs - 1 - p.seg, map, state, A.patience, lost, tokens);
     const long long at = ((long long)p.b * A.L + t0) * A.C + p.ch;
     T* const dx_at = reinterpret_cast<T*>(A.out[0]) + at;
     T* const dg_at = reinterpret_cast<T*>(A.out[1]) + at;
