@@ -60,6 +60,7 @@ template <int LANES> using Bwd = Shape<8, 8, 2, LANES>;
 constexpr int kSaved = 8;              // tokens from one saved state to the next: the backward pass's segments
 static_assert(Fwd<32>::kSeg % kSaved == 0 && Bwd<32>::kSeg == kSaved, "both passes have the saved states at hand");
 constexpr int kMaxCluster = 16;        // above 8 by a kernel attribute
+constexpr unsigned kLanding = 1u << 24; // clocks for a message that has been sent (about 0.25 us) to land
 
 struct ScanArgs {
   const char* in[4];          // x, gate, out_gate, dy
@@ -411,13 +412,24 @@ template <typename F, typename S> __device__ __forceinline__ void open_board(Boa
   }
   cluster_meet();  // the others run, and their barriers are there
 }
-// No CTA leaves while another may still write to it. A CTA that has given up on a message gives those on their way time to land.
-__device__ __forceinline__ void close_board(const Place& p, bool lost) {
+// What a warp has heard of its CTA's messages. After one that did not come in time (lost) it takes none.
+struct Mail {
+  int heard = 0;
+  bool lost = false;
+};
+// Messages that come late after all: their barriers are armed again, so that what the next ones count stays in range.
+template <typename F, typename S> __device__ __forceinline__ void hear(Board<F, S>& B, Mail& mail, int messages, unsigned patience) {
+  while (mail.heard < messages && wait_message(smem_of(&B.full[mail.heard & 1]), (mail.heard >> 1) & 1, patience)) {
+    arm(smem_of(&B.full[mail.heard & 1]), sizeof(B.inbox[0]));
+    ++mail.heard;
+  }
+}
+// No CTA leaves while another may still write to it: behind the barrier all messages are sent, and one that has given up waits for those
+// that it has not heard. steps: the tiles that this CTA has handed on.
+template <typename F, typename S> __device__ __forceinline__ void close_board(Board<F, S>& B, const Place& p, Mail& mail, int steps) {
   if (p.n == 1) return;
   cluster_meet();
-  if (lost)
-    for (const unsigned t0 = (unsigned)clock64(); (unsigned)clock64() - t0 < (1u << 20);) {
-    }
+  if (threadIdx.x == 0 && mail.lost) hear(B, mail, steps - (p.rank == 0 && steps > 0 ? 1 : 0), kLanding);
 }
 
 // Hands the maps of a tile's segments on. k: the tile's number in the order of the recurrence, step: how many this CTA has done
@@ -426,7 +438,7 @@ __device__ __forceinline__ void close_board(const Place& p, bool lost) {
 // Returns what enters this lane's segment: NaN from the first message on that did not come (lost).
 template <bool LOG, typename F, typename S, typename Tokens>
 __device__ __forceinline__ F hand_on(Board<F, S>& B, const Place& p, int k, int step, int order, const Map<F>& mine, F& state,
-                                     unsigned patience, bool& lost, const Tokens& tokens) {
+                                     unsigned patience, Mail& mail, const Tokens& tokens) {
   const int lane = threadIdx.x % S::kLanes;
   B.P[order][lane] = mine.P, B.l[order][lane] = mine.l, B.H[order][lane] = mine.H;
   // Maps of lost digits are looked at one by one, where a tile has any (looked for in every chain, 64 x 2048 tokens of 1024
@@ -481,11 +493,16 @@ __device__ __forceinline__ F hand_on(Board<F, S>& B, const Place& p, int k, int 
     const int m = p.rank > 0 ? step : step - 1;
     if (p.n > 1) {
       const uint32_t bar = smem_of(&B.full[m & 1]);
-      if (!lost) lost = !__all_sync(0xffffffffu, wait_message(bar, (m >> 1) & 1, patience));
-      if (threadIdx.x == 0 && !lost) arm(bar, sizeof(B.inbox[0]));
-      if (lost && threadIdx.x % 32 == 0) atomicExch(&g_ran_out, 1u);
+      if (!mail.lost) mail.lost = !__all_sync(0xffffffffu, wait_message(bar, (m >> 1) & 1, patience));
+      if (!mail.lost) {
+        if (threadIdx.x == 0) arm(bar, sizeof(B.inbox[0]));
+        mail.heard = m + 1;
+      } else if (threadIdx.x % 32 == 0) {
+        atomicExch(&g_ran_out, 1u);
+        if (threadIdx.x == 0) hear(B, mail, m + 1, 0);
+      }
     }
-    h = lost ? all_<F>(CUDART_NAN_F) : B.inbox[m & 1][lane];
+    h = mail.lost ? all_<F>(CUDART_NAN_F) : B.inbox[m & 1][lane];
   }
   const auto pass_on = [&] {
     if (k + 1 < p.tiles) {
@@ -546,7 +563,7 @@ __global__ void __launch_bounds__(Fwd<LANES>::kThreads, Fwd<LANES>::kCtas) gated
   };
   F state = all_<F>(0.0f);
   if (A.first) state = get_state(A.first + (long long)p.b * A.C + p.ch, p.have, state);
-  bool lost = false;
+  Mail mail;
   open_board(B, p);
   if (p.rank < p.tiles) fetch(0, p.rank);
   // Whole tiles, and the tile that the row ends in, are apart from each other: a test for each token keeps the tokens' latencies apart too.
@@ -613,7 +630,7 @@ __global__ void __launch_bounds__(Fwd<LANES>::kThreads, Fwd<LANES>::kCtas) gated
       }
       return state;
     };
-    const F carry = hand_on<LOG>(B, p, k, step, p.seg, map, state, A.patience, lost, tokens);
+    const F carry = hand_on<LOG>(B, p, k, step, p.seg, map, state, A.patience, mail, tokens);
     if (p.have < 1) return;
     T* const y = reinterpret_cast<T*>(A.out[0]) + ((long long)p.b * A.L + t0) * A.C + p.ch;
     float* const s = A.saved + ((long long)p.b * A.segments + t0 / kSaved) * A.C + p.ch;
@@ -664,12 +681,15 @@ __global__ void __launch_bounds__(Fwd<LANES>::kThreads, Fwd<LANES>::kCtas) gated
   const int full = p.len / S::kTile;
   int k = p.rank, step = 0;
   for (; k < full; k += p.n, ++step) run(k, step, std::true_type{});
-  if (k < p.tiles) run(k, step, std::false_type{});
+  if (k < p.tiles) {
+    run(k, step, std::false_type{});
+    ++step;
+  }
   // the last tile's CTA has the state in its last segment; a row without tokens keeps what it was given
   if (A.last && p.seg == S::kSegs - 1 && p.rank == max(p.tiles - 1, 0) % p.n)
     put_state(A.last + (long long)p.b * A.C + p.ch, p.have, state);
   zeros_behind<T, S, ALIGNED, 1>(A, p);
-  close_board(p, lost);
+  close_board(B, p, mail, step);
 }
 
 template <typename T, int LANES, bool LOG, bool GATE, bool COMP, bool ALIGNED>
@@ -701,7 +721,7 @@ __global__ void __launch_bounds__(Bwd<LANES>::kThreads, Bwd<LANES>::kCtas) gated
   asm volatile("" : "+r"(stride));  // in a register, not fetched again for each store
   F state = all_<F>(0.0f);
   if (A.first) state = get_state(A.first + (long long)p.b * A.C + p.ch, p.have, state);
-  bool lost = false;
+  Mail mail;
   open_board(B, p);
   if (p.rank < p.tiles) fetch(0, p.tiles - 1 - p.rank);
   const auto run = [&](int k, int step, auto all_live) {
@@ -786,7 +806,7 @@ __global__ void __launch_bounds__(Bwd<LANES>::kThreads, Bwd<LANES>::kCtas) gated
       }
       return state;
     };
-    c = hand_on<LOG>(B, p, k, step, S::kSegs - 1 - p.seg, map, state, A.patience, lost, tokens);
+    c = hand_on<LOG>(B, p, k, step, S::kSegs - 1 - p.seg, map, state, A.patience, mail, tokens);
     const long long at = ((long long)p.b * A.L + t0) * A.C + p.ch;
     T* const dx_at = reinterpret_cast<T*>(A.out[0]) + at;
     T* const dg_at = reinterpret_cast<T*>(A.out[1]) + at;
@@ -828,7 +848,7 @@ __global__ void __launch_bounds__(Bwd<LANES>::kThreads, Bwd<LANES>::kCtas) gated
   if (A.last && p.seg == 0 && p.rank == max(p.tiles - 1, 0) % p.n)
     put_state(A.last + (long long)p.b * A.C + p.ch, p.have, state);
   zeros_behind<T, S, ALIGNED, GATE ? 3 : 2>(A, p);
-  close_board(p, lost);
+  close_board(B, p, mail, step);
 }
 
 // ---------------------------------------------------------------- single tokens

@@ -529,3 +529,34 @@ def test_step_follows_the_sequence_and_reads_views():
     assert gated_scan_step(empty, empty, state).shape == (0, 64)
     idle = torch.full((4,), -1, dtype=torch.int32, device="cuda")
     assert (gated_scan_step(x[:, 0], g[:, 0], empty, slots=idle) == 0).all()
+
+
+@gpu
+@pytest.mark.parametrize("B,L,C", [(2, 3000, 64), (3, 3000, 2048)], ids=["rows of 64 bytes", "rows of 128 bytes"])
+def test_a_wait_that_runs_out_is_told(B, L, C):
+    """With no patience at all some wait does run out: results and gradients are NaN from there on and what they are otherwise before,
+    the status says so once, and the calls after it are sound."""
+    from nvsubquadratic_b200 import _lib
+
+    c = _case(B, L, C, BF16)
+    want = _run(c, "logit", True)
+    _lib.check_waits(0)
+    lib, told = _lib.load(), 0
+    before = lib.hyfft_set_wait_clocks(0)
+    try:
+        for _ in range(20):
+            got = _run(c, "logit", True)
+            torch.cuda.synchronize()
+            for w, g in zip(want, got):
+                assert ((g == w) | g.isnan()).all()
+            if any(g.isnan().any() for g in got):
+                with pytest.raises(_lib.HyfftError, match="gated scan"):
+                    _lib.check_waits(0)
+                told += 1
+            _lib.check_waits(0)
+    finally:
+        lib.hyfft_set_wait_clocks(before)
+    assert told > 0
+    for _ in range(3):
+        assert all(torch.equal(p, q) for p, q in zip(want, _run(c, "logit", True)))
+    _lib.check_waits(0)
