@@ -22,7 +22,7 @@ import torch
 from .gated_scan import gated_scan, gated_scan_step
 from .layer_norm import LayerNormB200
 from .sequence_mixer import QKVSequenceMixerB200
-from .state_pool import SlotCache, copy_slots
+from .state_pool import MAX_MOVES, SlotCache, copy_slots
 
 __all__ = ["GatedCache", "GatedMixerB200", "GatedBlockB200"]
 
@@ -42,8 +42,9 @@ class GatedCache(SlotCache):
 
     def reset(self, slots: torch.Tensor) -> None:
         """Forgets what the given slots held, for new requests."""
-        slots = slots.to(torch.int32)
-        copy_slots(self.pools(), torch.full_like(slots, -1), slots)
+        rows = self.rows(slots, slots.numel()).to(torch.int32)  # the spare row is no slot of the pool: idle requests clear nothing
+        for part in rows.split(MAX_MOVES):
+            copy_slots(self.pools(), torch.full_like(part, -1), part)
 
 
 class GatedMixerB200(torch.nn.Module):

@@ -19,6 +19,7 @@ from . import _lib
 __all__ = ["copy_slots", "compact_slots", "SlotCache"]
 
 MAX_POOLS = 16
+MAX_MOVES = 12800
 
 
 def _pools(pools: torch.Tensor | Sequence[torch.Tensor]):

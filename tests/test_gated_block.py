@@ -181,3 +181,16 @@ def test_decay_mixer_with_normed_queries_and_keys(rot_dim):
     assert rel_l2(want, out) <= 256 * 2.0 ** -24
     grads = torch.autograd.grad((out * torch.randn_like(out)).sum(), [mixer.q_norm, mixer.k_norm])
     assert all(torch.isfinite(g).all() and g.abs().max() > 0 for g in grads)
+
+
+@gpu
+def test_any_number_of_slots_is_reset():
+    """More slots than one call of copy_slots takes; slots outside the cache, past 32 bits too, clear nothing."""
+    cache = GatedCache(20001, 4, device="cuda")
+    cache.state.fill_(3)
+    cache.reset(torch.arange(20000, device="cuda"))
+    assert (cache.state[:20000] == 0).all() and (cache.state[20000:] == 3).all()
+    cache.state.fill_(3)
+    cache.reset(torch.tensor([-1, 5, 20001, 1 << 32, (1 << 32) + 7], device="cuda"))
+    assert (cache.state[5] == 0).all() and cache.state.sum().item() == 3 * 4 * 20001
+    cache.reset(torch.zeros(0, dtype=torch.int64, device="cuda"))
