@@ -176,18 +176,22 @@ template <int G> __device__ __forceinline__ float sum_of(float v) {
   return v;
 }
 
-// 1 / sqrt(mean + eps) of a row whose squares overflow although its features do not: of the row over its largest feature.
-template <int E, int G> __device__ __forceinline__ float of_large(const float (&v)[E], float ss, float r, float inv, float eps) {
+// Squares below this have fewer digits, or none, in the sum: mean + eps of a row that needs them.
+constexpr float kSmallMean = 8.0779357e-28f;  // 2^-90
+// 1 / sqrt(mean + eps) of a row whose squares leave float32's range although its features do not: of the row times 2^-100 or 2^100.
+template <int E, int G> __device__ __forceinline__ float of_extreme(const float (&v)[E], float ss, float r, float inv, float eps) {
   float m = 0.0f, s = 0.0f;
 #pragma unroll
   for (int e = 0; e < E; ++e) m = fmaxf(m, fabsf(v[e]));
 #pragma unroll
   for (int d = 1; d < G; d *= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-  const float one_over = 1.0f / m;  // m is 1e19 at least where this is used
+  const float up = m > 1.0f ? 7.8886091e-31f : 1.2676506e30f;
 #pragma unroll
-  for (int e = 0; e < E; ++e) s = fmaf(v[e] * one_over, v[e] * one_over, s);
+  for (int e = 0; e < E; ++e) s = fmaf(v[e] * up, v[e] * up, s);
   s = sum_of<G>(s);
-  return ss == CUDART_INF_F && m < CUDART_INF_F ? rsqrtf(fmaf(s, inv, eps / m / m)) / m : r;
+  const bool large = ss == CUDART_INF_F && m < CUDART_INF_F, small = fmaf(ss, inv, eps) < kSmallMean && m > 0.0f;
+  // below 2^-126 a row counts as if it were there
+  return large || small ? fminf(rsqrtf(fmaf(s, inv, eps * up * up)) * up, 3.4028235e38f) : r;
 }
 
 // Groups of G lanes walk over the items of one tensor (q's CTAs and k's are apart: one set of weights and of their sums in registers). The
@@ -301,8 +305,9 @@ __global__ void __launch_bounds__(kThreads, BACK || 2 * V * U > 8 ? 2 : 3) qk_no
 #pragma unroll
         for (int e = 0; e < E; ++e) ss = fmaf(v[e], v[e], ss);
         ss = sum_of<G>(ss);
-        float r = rsqrtf(fmaf(ss, inv, A.eps));
-        if (__any_sync(0xffffffffu, ss == CUDART_INF_F)) r = of_large<E, G>(v, ss, r, inv, A.eps);
+        const float mean = fmaf(ss, inv, A.eps);
+        float r = rsqrtf(mean);
+        if (__any_sync(0xffffffffu, mean < kSmallMean || ss == CUDART_INF_F)) r = of_extreme<E, G>(v, ss, r, inv, A.eps);
         if (!on) r = 0.0f;
         if constexpr (!BACK) {
 #pragma unroll

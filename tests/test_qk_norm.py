@@ -347,3 +347,37 @@ def test_streams_and_graphs():
     torch.cuda.synchronize()
     kept = [g.clone() for g in got]
     assert all(torch.equal(a, b) for a, b in zip(kept, step()))
+
+
+@gpu
+@pytest.mark.parametrize("D", [64, 33, 256])
+@pytest.mark.parametrize("size", [1e-13, 1e-20, 1e-30, 1e-36])
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+def test_small_rows_without_eps(dtype, size, D):
+    """Features whose squares are below float32's range, eps = 0 or of their squares' size: normed like others."""
+    q, k, dq, dk, wq, wk, _ = _case(2, 5, 3, 2, D, 0, dtype, "order")
+    q, k = (q.float() * size).to(dtype), (k.float() * size).to(dtype)
+    q[0, 1] = (q[0, 1].float() / size).to(dtype)  # among ordinary rows
+    for eps in (0.0, size * size if size > 1e-19 else 0.0):
+        leaves = [t.cuda().requires_grad_() for t in (q, k, wq, wk)]
+        out = qk_norm_rotary(*leaves, eps=eps)
+        grads = torch.autograd.grad(out, leaves, [dq.cuda(), dk.cuda()])
+        for i, (x, d, w) in enumerate(((q, dq, wq), (k, dk, wk))):
+            y, dx, _ = oracle(x, w, eps=torch.tensor(eps, dtype=F32).double().item(), dy=d)
+            assert rel_l2(y, out[i]) <= TOL[dtype]
+            _check_dx(dx, grads[i], x, d, w, dtype, eps=eps)
+            assert torch.isfinite(grads[2 + i]).all()
+    zeros = torch.zeros(1, 2, 1, D, device="cuda", dtype=dtype)
+    assert (qk_norm_rotary(zeros, None, eps=1e-30)[0] == 0).all()
+
+
+@gpu
+def test_rows_from_large_to_small_in_one_call():
+    """Every size of float32 that has all its digits, in rows that share warps; features of one row as far apart as they go."""
+    g = torch.Generator().manual_seed(0)
+    x = torch.randn(1, 40, 6, 48, generator=g) * 10.0 ** torch.linspace(-37, 37, 240).view(1, 40, 6, 1)
+    x[0, ::7, :, 1::2] *= 1e-3
+    for eps in (0.0, 1e-30, 1e-6):
+        y, _ = qk_norm_rotary(x.cuda(), None, eps=eps)
+        want = oracle(x, eps=torch.tensor(eps, dtype=F32).double().item())
+        assert ((want - y.double().cpu()).norm(dim=-1) <= TOL[F32] * want.norm(dim=-1) + 2.0 ** -126).all()
