@@ -965,15 +965,16 @@ template <int LANES> Bytes bytes_of(const Form& f, int e) {
   return f.back ? of(Bwd<LANES>{}, f.gate ? 4 : 3) : of(Fwd<LANES>{}, f.gate ? 3 : 2);
 }
 
-int check_desc(const hyfft_gated_desc* d, const char* null_msg) {
+// step: a single token of each request, whose descriptor has no length.
+int check_desc(const hyfft_gated_desc* d, const char* null_msg, bool step = false) {
   if (!d) return set_error(HYFFT_ERR_INVALID, null_msg);
-  if (d->batch < 1 || d->length < 1 || d->channels < 1)
+  if (d->batch < 1 || (!step && d->length < 1) || d->channels < 1)
     return set_error(HYFFT_ERR_INVALID, "gated scan: every extent must be positive");
   if (d->dtype < HYFFT_F32 || d->dtype > HYFFT_F16) return set_error(HYFFT_ERR_INVALID, "gated scan: bad dtype");
   if (d->form != HYFFT_GATED_LOGIT && d->form != HYFFT_GATED_LOG)
     return set_error(HYFFT_ERR_INVALID, "gated scan: bad form");
   // token numbers and the cluster's tiles past the end are 32-bit
-  if (d->length > (1ll << 30) || d->channels > (1 << 28) || (long long)d->batch * ((d->channels + 31) / 32) > (1ll << 27))
+  if ((!step && d->length > (1ll << 30)) || d->channels > (1 << 28) || (long long)d->batch * ((d->channels + 31) / 32) > (1ll << 27))
     return set_error(HYFFT_ERR_UNSUPPORTED, "gated scan: too many tokens, channels or rows");
   return HYFFT_OK;
 }
@@ -1107,7 +1108,7 @@ extern "C" int hyfft_gated_backward(const hyfft_gated_desc* d, const void* x, co
 extern "C" int hyfft_gated_step(const hyfft_gated_desc* d, const void* x, const void* gate, const void* out_gate,
                                 const int32_t* slots, int64_t pool, const float* state, float* out_state, void* y,
                                 void* stream) {
-  if (int rc = check_desc(d, "gated step: null descriptor")) return rc;
+  if (int rc = check_desc(d, "gated step: null descriptor", true)) return rc;
   if (!x || !gate || !state || !out_state || !y) return set_error(HYFFT_ERR_INVALID, "gated step: null tensor");
   if (pool < 1 || (!slots && pool < d->batch)) return set_error(HYFFT_ERR_INVALID, "gated step: too few states");
   if (bind_device_of(x) != HYFFT_OK) return set_error(HYFFT_ERR_CUDA, "gated step: device");

@@ -560,3 +560,37 @@ def test_a_wait_that_runs_out_is_told(B, L, C):
     for _ in range(3):
         assert all(torch.equal(p, q) for p, q in zip(want, _run(c, "logit", True)))
     _lib.check_waits(0)
+
+
+@pytest.mark.parametrize("length", [0, -1, 1 << 40])
+def test_the_length_of_a_steps_descriptor_is_not_used(length):
+    """The C entry goes on to what it does look at: here two requests and one state, and no output."""
+    import ctypes
+
+    from nvsubquadratic_b200 import _lib
+
+    lib, p, d = _lib.load(), ctypes.c_void_p(16), _lib.GatedDesc()
+    d.batch, d.channels, d.dtype, d.length = 2, 8, _lib.F32, length
+    assert lib.hyfft_gated_step(ctypes.byref(d), p, p, None, None, 1, p, p, p, None) == _lib.HYFFT_ERR_INVALID
+    assert b"too few states" in lib.hyfft_last_error()
+    assert lib.hyfft_gated_step(ctypes.byref(d), p, p, None, None, 2, p, p, None, None) == _lib.HYFFT_ERR_INVALID
+    assert b"null tensor" in lib.hyfft_last_error()
+
+
+@gpu
+def test_a_step_through_the_c_entry_without_a_length():
+    import ctypes
+
+    from nvsubquadratic_b200 import _lib
+
+    c = _case(3, 1, 8, F32)
+    x, g, state, y = c["x"][:, 0].cuda(), c["gate"][:, 0].cuda(), c["initial_state"].cuda(), torch.empty(3, 8, device="cuda")
+    d = _lib.GatedDesc()  # all zeros but what the step reads
+    d.batch, d.channels, d.dtype, d.complement = 3, 8, _lib.F32, 1
+    d.x_stride[0] = d.gate_stride[0] = 8
+    rc = _lib.load().hyfft_gated_step(ctypes.byref(d), x.data_ptr(), g.data_ptr(), None, None, 3, state.data_ptr(), state.data_ptr(),
+                                      y.data_ptr(), _lib.stream_ptr(x.device))
+    _lib.check(rc, "hyfft_gated_step")
+    want, end = oracle(c["x"], c["gate"], initial_state=c["initial_state"])
+    close(want[:, 0], y, F32)
+    close(end, state, F32)
