@@ -8,9 +8,11 @@ from nvsubquadratic_b200.decay_block import DecayBlockB200, DecayCache, DecayMix
 from nvsubquadratic_b200.gated_block import GatedBlockB200, GatedCache, GatedMixerB200
 from nvsubquadratic_b200.sequence_mixer import QKVSequenceMixerB200
 from oracle.decay_attention import decay_attention as attention_oracle
+from oracle.decay_attention import decay_attention_grads as attention_grads
 from oracle.gated_scan import gated_scan as scan_oracle
 from oracle.layer_norm import layer_norm as norm_oracle
 from oracle.qk_norm import qk_norm_rotary as qk_oracle
+from oracle.rotary import rotary as rotary_oracle
 from tests.conftest import rel_l2
 
 gpu = pytest.mark.gpu
@@ -194,3 +196,79 @@ def test_any_number_of_slots_is_reset():
     cache.reset(torch.tensor([-1, 5, 20001, 1 << 32, (1 << 32) + 7], device="cuda"))
     assert (cache.state[5] == 0).all() and cache.state.sum().item() == 3 * 4 * 20001
     cache.reset(torch.zeros(0, dtype=torch.int64, device="cuda"))
+
+
+@gpu
+def test_gradients_of_the_norms_of_queries_and_keys():
+    """Through the decayed mixer, against the oracles' formulas one after the other. A weight's gradient is a sum of n terms, (n + 128)
+    units of their sizes, and what comes to it has gone through the layer norm's and the attention's, 256 units each way."""
+    torch.manual_seed(0)
+    B, L, H, D = 2, 70, 3, 32
+    mixer = DecayMixerB200(H * D, H, rot_dim=20, qk_norm=True).cuda()
+    with torch.no_grad():
+        mixer.q_norm.add_(0.2 * torch.randn_like(mixer.q_norm)), mixer.k_norm.add_(0.2 * torch.randn_like(mixer.k_norm))
+    q, k, v, dy = (torch.randn(B, L, H * D, device="cuda") for _ in range(4))
+    grads = torch.autograd.grad(mixer(q, k, v), [mixer.q_norm, mixer.k_norm], dy)
+    q, k, v, dy = (t.cpu().unflatten(-1, (H, D)) for t in (q, k, v, dy))
+    freq = mixer.turns.double().cpu() / 2.0 ** 64 * 2 * torch.pi
+    a, b = qk_oracle(q, mixer.q_norm, freq), qk_oracle(k, mixer.k_norm, freq)
+    o, _ = attention_oracle(a, b, v, mixer.log_decay)
+    do = norm_oracle(o, eps=mixer.eps, dy=dy)[1]
+    ups = attention_grads(a, b, v, mixer.log_decay, do)[:2]
+    for x, w, up, got in zip((q, k), (mixer.q_norm, mixer.k_norm), ups, grads):
+        want = qk_oracle(x, w, freq, dy=up)[2]
+        h = x.double() / x.double().square().mean(-1, keepdim=True).add(1e-6).sqrt()
+        sizes = (rotary_oracle(up, freq, backward=True) * h).abs().sum((0, 1, 2))
+        assert (want - got.double().cpu()).norm() <= (B * L * H + 128 + 4 * 256) * 2.0 ** -24 * sizes.norm()
+
+
+@gpu
+@pytest.mark.parametrize("kind,make,hold", _blocks(), ids=[b[0] for b in _blocks()])
+def test_training_on_ragged_sequences(kind, make, hold):
+    """A padded batch gives the gradients of its sequences one by one; padding passes the residual on and nothing else. Either side is good
+    to four operators of 128 units each."""
+    torch.manual_seed(0)
+    block, lengths = make().cuda(), [90, 0, 33, 1]
+    x, dy = (torch.randn(4, 90, 128, device="cuda") for _ in range(2))
+    for b, n in enumerate(lengths):
+        dy[b, n:] = 0
+    leaves = [x.requires_grad_(), *block.parameters()]
+    y = block(x, lengths=torch.tensor(lengths, dtype=torch.int32, device="cuda"))
+    got = torch.autograd.grad(y, leaves, dy)
+    want = [torch.zeros_like(t, dtype=torch.float64) for t in leaves]
+    for b, n in enumerate(lengths):
+        assert torch.equal(y[b, n:], x[b, n:])
+        if n:
+            alone = block(x[b:b + 1, :n])
+            assert rel_l2(alone[0], y[b, :n]) <= 256 * 2.0 ** -24
+            for w, g in zip(want, torch.autograd.grad(alone, leaves, dy[b:b + 1, :n])):
+                w += g
+    bad = [(i, rel_l2(w, g)) for i, (w, g) in enumerate(zip(want, got)) if not rel_l2(w, g) <= 2 * 4 * 128 * 2.0 ** -24]
+    assert not bad, bad
+
+
+class _PlainScan(torch.nn.Module):
+    """The gated mixer in float64, rounded where GatedMixerB200 rounds."""
+
+    def forward(self, query, key, value, cp_group=None, **kw):
+        a, u, s, out = torch.sigmoid(key.double()), torch.sigmoid(-key.double()), 0, []
+        for t in range(key.shape[1]):
+            s = a[:, t] * s + u[:, t] * value[:, t].double()
+            out.append(s)
+        return (torch.stack(out, 1) * torch.nn.functional.silu(query.double())).to(value.dtype)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "f16"])
+def test_16_bit_gradients_of_the_block(dtype):
+    """Against the same block with the scan written out. Both round the scan's output and its three gradients, to the same or to
+    neighbouring numbers: four times a step, 2 eps / 2 each."""
+    torch.manual_seed(0)
+    block = GatedBlockB200(64).cuda().to(dtype)
+    x, dy = (torch.randn(2, 40, 64, device="cuda", dtype=dtype) for _ in range(2))
+    leaves = [x.requires_grad_(), *block.parameters()]
+    got = torch.autograd.grad(block(x), leaves, dy)
+    block.mixer.mixer = _PlainScan()
+    want = torch.autograd.grad(block(x), leaves, dy)
+    bad = [(i, rel_l2(w, g)) for i, (w, g) in enumerate(zip(want, got)) if not rel_l2(w, g) <= 4 * torch.finfo(dtype).eps]
+    assert not bad, bad

@@ -594,3 +594,18 @@ def test_a_step_through_the_c_entry_without_a_length():
     want, end = oracle(c["x"], c["gate"], initial_state=c["initial_state"])
     close(want[:, 0], y, F32)
     close(end, state, F32)
+
+
+@gpu
+@FORMS
+@DTYPES
+@pytest.mark.parametrize("B,L,C,copies", [(1, 9003, 40, 1), (2, 3001, 40, 40)], ids=["rows of 64 bytes", "rows of 128 bytes"])
+def test_long_rows_that_many_CTAs_take_in_turn(B, L, C, copies, dtype, form):
+    """Tens of tiles for each CTA of a cluster, with output gates, states at both ends and every gradient; many rows are copies."""
+    c = _case(B, L, C, dtype, form)
+    lengths = [L, 2 * L // 3][:B]
+    wide = {k: t.repeat(*[1] * (t.ndim - 1), copies) for k, t in c.items()}
+    for want, got in zip(_want(c, form, True, lengths), _run(wide, form, True, lengths)):
+        got = got.unflatten(-1, (copies, C))
+        assert torch.equal(got, got[..., :1, :].expand_as(got))
+        close(want, got[..., 0, :], got.dtype)
