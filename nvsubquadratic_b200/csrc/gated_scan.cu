@@ -179,8 +179,9 @@ __device__ __forceinline__ float above_zero(float p) { return p == 0.0f ? __int_
 
 __device__ __forceinline__ bool infinite(float v) { return fabsf(v) == CUDART_INF_F; }
 __device__ __forceinline__ bool finite(float v) { return fabsf(v) < CUDART_INF_F; }
-template <typename F> __device__ __forceinline__ F held(F P, F H) {
-  return each_(P, H, [](float p, float h) { return finite(p) && finite(h) ? p : CUDART_NAN_F; });
+// P, or NaN. A product of decays that are 1 at most does not overflow.
+template <bool LOG, typename F> __device__ __forceinline__ F held(F P, F H) {
+  return each_(P, H, [](float p, float h) { return (!LOG || finite(p)) && finite(h) ? p : CUDART_NAN_F; });
 }
 template <typename F> __device__ __forceinline__ F apply(const Map<F>& m, F h) { return fma_(m.P, h, fma_(m.l, h, m.H)); }
 __device__ __forceinline__ bool lossy(float P) { return P > 0.0f && P < kLeast; }
@@ -205,7 +206,7 @@ template <bool LOG, typename F> __device__ __forceinline__ Map<F> then(const Map
     const F of_some = each_(p, f.P, s.P, [](float v, float a, float b) { return a > 0.0f && b > 0.0f ? above_zero(v) : v; });
     r.P = each_(of_some, f.P, s.P, [](float v, float a, float b) { return b > 1.0f && lossy(a) ? CUDART_NAN_F : v; });
   }
-  r.P = held(r.P, r.H);
+  r.P = held<LOG>(r.P, r.H);
   return r;
 }
 
@@ -459,6 +460,7 @@ __device__ __forceinline__ F hand_on(Board<F, S>& B, const Place& p, int k, int 
   // What leaves the tile goes by one map over all of it, which is there before the message is: the next CTA waits for nothing else.
   const bool last = order == S::kSegs - 1, sends = last && p.n > 1;
   Map<F> whole = mine;
+  bool digits = false;  // that whole has lost
   if (sends) {
     whole = map_of(0);
 #pragma unroll 1
@@ -468,6 +470,7 @@ __device__ __forceinline__ F hand_on(Board<F, S>& B, const Place& p, int k, int 
       whole = both;
       if (careful) whole.P = each_(both.P, checked(both.H, m.P, h), [](float v, float w) { return w != w ? w : v; });
     }
+    digits = LOG && any_(whole.P, lossy);
   }
   if (p.n == 1 && S::kSegs <= 4) {  // few enough for every warp to go through all of them
     F h = state, in = state;
@@ -513,7 +516,7 @@ __device__ __forceinline__ F hand_on(Board<F, S>& B, const Place& p, int k, int 
   bool late = false;
   if (sends) {
     state = apply(whole, h);
-    late = fresh_nan(LOG ? checked(state, whole.P, h) : state, h);
+    late = fresh_nan(digits ? checked(state, whole.P, h) : state, h);
     if (!late) pass_on();
   }
   F in = h;
@@ -524,9 +527,15 @@ __device__ __forceinline__ F hand_on(Board<F, S>& B, const Place& p, int k, int 
 #pragma unroll 1
     for (int j = 0; j < order; ++j) in = through(j, in);
   }
-  if (late || (last && p.n == 1)) state = through(order, in);
-  if (late) pass_on();
-  if (last && p.n == 1) B.inbox[step & 1][lane] = state;
+  if (last && p.n == 1) {
+    state = apply(mine, in);
+    if (careful || fresh_nan(state, in)) state = through(order, in);
+    B.inbox[step & 1][lane] = state;
+  }
+  if (late) {
+    state = through(order, in);
+    pass_on();
+  }
   return in;
 }
 
@@ -616,8 +625,8 @@ __global__ void __launch_bounds__(Fwd<LANES>::kThreads, Fwd<LANES>::kCtas) gated
         map.P = each_(map.P, least, [](float v, float w) { return w > 0.0f ? above_zero(v) : v; });
       }
     }
-    map.P = held(map.P, map.H);
-    map = there(map, p.have);
+    map.P = held<LOG>(map.P, map.H);
+    if (p.have < Lane<T>::N) map = there(map, p.have);
     const auto tokens = [&](int seg, F state) {
       const int r = seg * kSeg, n = min(kSeg, p.len - tile0 - r);
       const unsigned char* at = tile + Tile<S, ALIGNED>::row(r) + 4 * (threadIdx.x % LANES);
@@ -787,8 +796,8 @@ __global__ void __launch_bounds__(Bwd<LANES>::kThreads, Bwd<LANES>::kCtas) gated
         map.P = each_(map.P, least, [](float v, float w) { return w > 0.0f ? above_zero(v) : v; });
       }
     }
-    map.P = held(map.P, map.H);
-    map = there(map, p.have);
+    map.P = held<LOG>(map.P, map.H);
+    if (p.have < Lane<T>::N) map = there(map, p.have);
     const auto tokens = [&](int place, F state) {
       const int r = (S::kSegs - 1 - place) * kSeg, n = min(kSeg, p.len - tile0 - r);
       const unsigned char* first = tile + Tile<S, ALIGNED>::row(r) + 4 * (threadIdx.x % LANES);
