@@ -17,15 +17,17 @@
 // leaves its tile on to the next one's shared memory. In steady state a CTA has its tile's map before the state arrives, so a hop is a
 // wait, one map and one remote store (0.25 us), and the data still goes through once; no workspace, no order of arrival in the results.
 //
-// Measured, bfloat16 with output gates (8 bytes an element forwards, 14 backwards): 64 x 2048 tokens of 1024 channels, one CTA a row,
-// 193 us forwards (85% of a copy's rate) and 354 backwards (81%); 65536 tokens of 4096 channels, 8 and 4 CTAs a cluster, 490 us (67%; one CTA a
-// row 1.54 ms, all of a cluster's maps exchanged behind a barrier 0.73) and 924 us (62%). float32: 97% and 93% of the same rate on the first.
-// What is left is instructions: 32 an element forwards and 59 backwards, of which a third are moves and unpacking, on a machine that has
-// time for 44 and 77 at a copy's rate; and with clusters the turns of the tiles.
+// Measured, bfloat16 with output gates and logits (8 bytes an element forwards, 14 backwards): 64 x 2048 tokens of 1024 channels, one CTA a
+// row, 184 us forwards (89% of a copy's rate) and 358 backwards (80%); 65536 tokens of 4096 channels, 8 and 4 CTAs a cluster, 477 us (69%; one
+// CTA a row 1.54 ms, all of a cluster's maps exchanged behind a barrier 0.73) and 923 us (62%). On the first: logs 213 and 375, float16 192 and
+// 363, float32 344 (95%) and 624 (92%). What is left in 16 bits is latency: 31 instructions an element forwards and 59 backwards keep the issue
+// slots busy for 54 to 61% of the time, DRAM for 47 to 57%, and the registers leave room for 4 warps a scheduler, which wait for their own
+// arithmetic more than for anything else; and with clusters the turns of the tiles.
 //
 // What is exact: A is carried as P + l. P is the product of the rounded decays, whose relative error grows with every token; l = (1 - P) - D
-// with D = 1 - A, accumulated as D += u P, which keeps the digits of slow decays (0 where decays above 1 made P large on the way, and D inexact). So a state that remembers 10^5 tokens is off by the
-// roundings of its 10^4 segments, not by those of its decays; within a segment, by 16 products of rounded decays. Sums are float32.
+// with D = 1 - A, accumulated as D += u P, which keeps the digits of slow decays (0 where decays above 1 made P large on the way, and D
+// inexact). So a state that remembers 10^5 tokens is off by the roundings of its 10^4 segments, not by those of its decays; within a segment,
+// by 16 products of rounded decays. Sums are float32.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -1004,8 +1006,11 @@ int run_scan(const hyfft_gated_desc* d, ScanArgs A, bool back, cudaStream_t st) 
   const Form form{back, d->form == HYFFT_GATED_LOG, gate, d->complement != 0, aligned};
   const auto rows_of = [&](int width) { return (long long)d->batch * (((long long)A.C * e + width - 1) / width); };
   // Few rows: half as wide ones, so twice as many, of tiles with twice the tokens, so half the hops. Measured, bfloat16 with output gates,
-  // wide against narrow: rows of 128 bytes 4 (1 x 65536 x 256): 249 | 119 us forwards, 305 | 163 backwards; 16 (4 x 16384 x 256): 73 | 48, 94 | 85;
-  // 32 (8 x 16384 x 256): 85 | 75, 130 | 155; 48 (3 x 8192 x 1024): 58 | 61, 101 | 151; 64 (1 x 65536 x 4096): 490 | 528, 924 | 1137.
+  // wide | narrow, us forwards and backwards: rows of 128 bytes 4 (1 x 65536 x 256): 248 | 127, 298 | 165; 16 (4 x 16384 x 256): 73 | 48, 92 | 86;
+  // 32 (8 x 16384 x 256): 83 | 73, 127 | 147; 48 (3 x 8192 x 1024): 57 | 59, 99 | 141; 64 (1 x 65536 x 4096): 476 | 517, 921 | 1055. The same
+  // rows in float32 (half the channels): 217 | 105, 208 | 126; 64 | 41, 70 | 70; 70 | 58, 97 | 116; 45 | 47, 78 | 114; 370 | 400, 692 | 848; in
+  // bfloat16 without output gates: 238 | 126, 236 | 129; 68 | 43, 74 | 63; 77 | 57, 95 | 115; 45 | 47, 77 | 113; 355 | 395, 677 | 838. Rows of one
+  // tile take the same rule (47 x 60 x 64: 6.3 | 8.2).
   const bool narrow = rows_of(128) < (back ? 24 : 48);
   const Kernel fn = narrow ? pick<16>(d->dtype, form) : pick<32>(d->dtype, form);
   const long long rows = rows_of(narrow ? 64 : 128);

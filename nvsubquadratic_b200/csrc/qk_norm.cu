@@ -195,11 +195,12 @@ template <int E, int G> __device__ __forceinline__ float of_extreme(const float 
 }
 
 // Groups of G lanes walk over the items of one tensor (q's CTAs and k's are apart: one set of weights and of their sums in registers). The
-// next HB rows' loads are in flight while HB are worked on. 65536 tokens of 32 + 32 heads of 128, bfloat16: 412 us forwards (80%
-// of a copy's rate) and 672 backwards (73%); without the loads ahead 424 with four rows at once, and 789 with two backwards; with 8
-// bytes a run instead of 16, twice the lanes of a row, 449 and 812. Neighbouring pairs have 8 features a lane, and room for three
-// CTAs an SM instead of two forwards (32 + 8 heads: 269 against 338 us); turned or not they lie side by side, so their runs are aligned
-// wherever the turned features end (26 x 3238 tokens, 2 + 2 heads of 128, 18 turned, training: 476 -> 195 us).
+// next HB rows' loads are in flight while HB are worked on. 65536 tokens of 32 + 32 heads of 128, bfloat16: 414 us forwards (79%
+// of a copy's rate) and 652 backwards (75%; the 16-bit kernels with 8 pairs a lane are at their 128 registers and spill 52 to 68 bytes); without
+// the loads ahead 424 with four rows at once, and 789 with two backwards; with 8 bytes a run instead of 16, twice the lanes of a row, 449 and 812.
+// Neighbouring pairs have 8 features a lane, and room for three CTAs an SM instead of two forwards (32 + 8 heads: 265 against 338 us); turned or
+// not they lie side by side, so their runs are aligned wherever the turned features end (26 x 3238 tokens, 2 + 2 heads of 128, 18 turned,
+// training: 476 -> 189 us).
 template <typename T, int V, int U, int G, bool INTER, bool BACK>
 __global__ void __launch_bounds__(kThreads, BACK || 2 * V * U > 8 ? 2 : 3) qk_norm_kernel(const QkArgs A) {
   using R = Rows<T, V, U, INTER, BACK>;
@@ -431,7 +432,9 @@ int launch_lanes(const QkArgs& A, int lanes, int* ctas, cudaStream_t st) {
 
 template <typename T, bool INTER, bool BACK> int launch_t(const QkArgs& A, int* ctas, cudaStream_t st) {
   constexpr int V = (INTER ? 8 : 16) / (int)sizeof(T), E = INTER ? 2 * V : V;  // pairs of a unit, elements of a run
-  // runs of 16 bytes where every run of every row starts on a 16-byte boundary, pairs of elements otherwise
+  // Runs of 16 bytes where every run of every row starts on a 16-byte boundary, pairs of elements otherwise. 4 x 4096 tokens, 8 + 8 heads,
+  // us forwards and backwards: 128 features turned of 128, bfloat16 39 and 88, float32 51 and 89; 24 of 96 (halves on 8 bytes, and on 16 in
+  // float32) 98 and 185, 52 and 89; 76 of 77 82 and 160, 71 and 117.
   bool al = A.D % E == 0 && (INTER || A.half % E == 0);
   for (int k = 0; k < 2; ++k) {
     if (!A.heads[k]) continue;

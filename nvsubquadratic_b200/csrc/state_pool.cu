@@ -6,9 +6,10 @@
 // cycles, so every source has to be read before its row is written. A CTA takes the same few bytes of every row that takes part: it copies
 // them to shared memory, waits, and writes them out, so nothing crosses HBM twice and no second buffer is needed. A kernel of one CTA
 // comes first and drops what is not to be copied: targets outside the pool, and all but the last move into a slot.
-// 224 rows of 2 MB in another order: 157 us (91% of a copy's rate); 2000 rows of 16 KB: 26 us (38%: the list of moves takes 5 us to make, and
-// every CTA reads it; 56 us with one unit looked up at a time). Rows off 16 bytes go 4 at a time: 195 rows of 355 KB cleared in 54
-// us instead of 25.
+// 224 rows of 2 MB in another order: 155 us (93% of a copy's rate); 2000 rows of 16 KB: 18.6 us in a graph, 24.7 among other passes (54 and 41%;
+// 56 us with one unit looked up at a time): the list takes 5 us to make by one CTA, and 64 bytes of 2000 rows fill an SM's shared memory, so
+// 257 CTAs take two waves, each reading all before it writes. Rows are copied 16 bytes at a time where all of them start on 16 bytes, else 8, 4 or 1:
+// those 2000 rows with 8188, 8190 and 8191 elements of 16 bits instead of 8192 take 33, 53 and 232 us.
 // Compaction fills the lowest free slots with the highest running requests; sources and targets are apart, and rows are copied through
 // registers.
 #include <cuda_runtime.h>

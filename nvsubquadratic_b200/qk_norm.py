@@ -124,6 +124,7 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor | None, q_weight: torch.Tens
         q ``[B, L, H, D]``, k ``[B, L, Hk, D]`` or None: float32, bfloat16 or float16, any batch, token and head strides. D <= 256.
         q_weight, k_weight: ``[D]`` each, shared by the heads, both of q's dtype or both float32; None: 1.
         turns, amplitude: from ``rotary_turns``; ``2 * len(turns)`` features are turned, the others are normed alone. None: no turn.
+        eps: 0 or more; with 0 a row of zeros is NaN, and one whose features are all below 2^-126 is not normed.
         positions: int64 or int32, ``[L]`` or ``[B, L]``; ``0 .. L - 1`` by default.
         interleaved: pairs are neighbours ``(2i, 2i + 1)``; by default the two halves ``(i, i + rot_dim / 2)``.
 
