@@ -646,8 +646,14 @@ __global__ void __launch_bounds__(Fwd<LANES>::kThreads, Fwd<LANES>::kCtas) gated
     T* const y = reinterpret_cast<T*>(A.out[0]) + ((long long)p.b * A.L + t0) * A.C + p.ch;
     float* const s = A.saved + ((long long)p.b * A.segments + t0 / kSaved) * A.C + p.ch;
     bool alone = any_(carry, infinite) || any_(map.P, [](float v) { return v != v; });
-    if constexpr (LOG)
-      if (any_(map.P, lossy)) alone = alone || fresh_nan(checked(apply(map, carry), map.P, carry), carry);
+    if constexpr (LOG) {
+      if (any_(P, [](float v) { return v < kLeast; })) {  // digits lost on the way: does an output need them?
+        F low = all_<F>(3.4e38f);
+#pragma unroll
+        for (int i = 0; i < kSeg; ++i) low = each_(low, fma_(Pl[i], carry, hl[i]), [](float v, float w) { return fminf(v, fabsf(w)); });
+        alone = alone || any_(low, carry, [](float v, float c) { return fabsf(c) * kLost > v; });
+      }
+    }
     // token by token, as the recurrence has it; apart from the rest, which keeps its registers
     if (alone) {
       F full = carry;

@@ -33,6 +33,8 @@ CASES = {
     "forgets, then grows": ([-0.1] * 40 + [-INF] + [0.75] * 110, 1.0, 0.0, 1e-20, 0.0),
     "forgets, then overflows": ([-0.1] * 40 + [-INF] + [6.0] * 20 + [-0.5] * 70, 1.0, 0.0, 1e-25, 1e-30),
     "overflows, then forgets": ([6.0] * 20 + [-INF] + [0.25] * 100, 0.0, 0.0, 1e-3, 1e-30),
+    # outputs and states far below what they come from, between a peak and a decay of zero
+    "shrinks far, then forgets": (([5.0] * 10 + [0.0] * 6 + [-50.0] * 2 + [-INF] + [-0.1] * 13) * 4, 1e5, 0.0, 1e-5, 1e-5),
     "slow and fast": (([1e-3] * 30 + [-1e-3] * 30) * 4, 1.0, 1.0, 1.0, 1.0),
 }
 # copies of eight channels side by side: rows of 64 bytes that CTAs share, rows of 128 bytes that CTAs share, a CTA for each row
