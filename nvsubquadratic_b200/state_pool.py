@@ -92,8 +92,9 @@ def compact_slots(pools: torch.Tensor | Sequence[torch.Tensor], live: torch.Tens
     if not slots:
         return moved
     table, count = _table(pools)
-    if not count:  # rows of no bytes: the numbers alone
-        table, count = _table([torch.empty(slots, dtype=torch.uint8, device=dev)])
+    if not count:  # rows of no bytes: the numbers alone, beside rows that nobody reads
+        pools = [torch.empty(slots, dtype=torch.uint8, device=dev)]  # kept until the call has been made
+        table, count = _table(pools)
     ws = _lib.workspace(_workspaces(slots, 0)[1], dev)
     rc = _lib.load().hyfft_pool_compact(table, count, slots, live.data_ptr(), moved.data_ptr(), ws.data_ptr(), ws.numel(),
                                         _lib.stream_ptr(dev))

@@ -205,3 +205,46 @@ def test_graphs_and_streams():
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(g.cpu(), want[0]) and moved.tolist() == new
+
+
+def test_what_stands_in_for_rows_of_no_bytes_lives_through_the_call(monkeypatch):
+    """On the host, with a library that only looks: every tensor whose address it is given is still there."""
+    import weakref
+
+    from nvsubquadratic_b200 import _lib, state_pool
+
+    given, alive = [], []
+
+    class Looks:
+        def hyfft_pool_workspace_size(self, slots, moves, copy, compact):
+            copy._obj.value, compact._obj.value = 4 * (slots + 2 * moves), 4 * (2 * slots + 1)
+            return 0
+
+        def hyfft_pool_compact(self, table, count, *rest):
+            assert count == 1
+            alive.append(all(t() is not None and t().data_ptr() == table[0].data for t in given))
+            return 0
+
+    table = state_pool._table
+
+    def remembered(pools):
+        given[:] = [weakref.ref(t) for t in pools if t.numel()]
+        return table(pools)
+
+    monkeypatch.setattr(state_pool, "_table", remembered)
+    monkeypatch.setattr(_lib, "load", Looks)
+    monkeypatch.setattr(_lib, "require_cuda", lambda *t: torch.device("cpu"))
+    monkeypatch.setattr(_lib, "stream_ptr", lambda dev: 0)
+    for pool in (torch.zeros(50, 0), torch.zeros(50, 3)):
+        compact_slots(pool, torch.ones(50, dtype=torch.bool))
+    assert alive == [True, True]
+
+
+@gpu
+def test_compaction_of_many_slots_of_no_bytes():
+    g = torch.Generator().manual_seed(0)
+    for slots in (1500, 20000, 50000):
+        live = torch.rand(slots, generator=g) < 0.5
+        want = _compacted([], live.tolist())[1]
+        for _ in range(3):
+            assert compact_slots(torch.zeros(slots, 0, device="cuda"), live.cuda()).tolist() == want
