@@ -381,7 +381,8 @@ HYFFT_API int hyfft_layer_norm_backward(const void* x, const void* weight, const
  * lengths: int32 [B] or NULL (all L): tokens from a sequence's length on are neither read nor counted, their outputs and
  * gradients are zero (values outside 0 .. L are clamped). States: float32 contiguous [B, C]; initial_state NULL means zero.
  * y and the gradients are contiguous and overwritten; sums are float32, each output rounded once. An infinity or a NaN
- * reaches what the recurrence lets it reach: no earlier token, no other channel. No counterpart in the reference.         */
+ * reaches what the recurrence lets it reach: no earlier token, no other channel. Decays above 1 (form LOG) are taken as they
+ * are; decays below 2^-126 are 0. No counterpart in the reference. */
 #define HYFFT_GATED_LOGIT 0
 #define HYFFT_GATED_LOG 1
 typedef struct hyfft_gated_desc {

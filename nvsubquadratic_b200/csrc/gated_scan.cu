@@ -176,7 +176,7 @@ template <typename F> struct Map { F P, l, H; };
 // most of a result. A product of 0 has a decay of exactly 0 in it and loses nothing. A decay of 1 at most needs no such care: what a
 // product below kLeast leaves of a state is 2^-100 of it.
 constexpr float kLeast = 7.888609e-31f;  // 2^-100
-constexpr float kLost = 9.403955e-38f;   // 2^-123: 2^-149 of what enters is at most a quarter of a result's last place
+constexpr float kLost = 9.403955e-38f;   // 2^-123: 2^-149 of what enters is at most a quarter of a larger result's last place
 __device__ __forceinline__ float above_zero(float p) { return p == 0.0f ? __int_as_float(1) : p; }
 
 __device__ __forceinline__ bool infinite(float v) { return fabsf(v) == CUDART_INF_F; }

@@ -148,8 +148,9 @@ def gated_scan(x: torch.Tensor, gate: torch.Tensor, *, out_gate: torch.Tensor | 
             ``gated_scan_step`` or another call goes on.
 
     Returns ``y [B, L, C]`` in x's dtype, or ``(y, state)``. Sums and states are float32, ``1 - a`` is computed without
-    cancellation. Decays above 1 are taken as they are: what float32 holds of a growing state comes out. An infinity or a NaN
-    reaches what the recurrence lets it reach: no earlier token, no other channel. First derivatives only.
+    cancellation. Decays above 1 are taken as they are: what float32 holds of a growing state comes out; decays below 2^-126 are
+    0. An infinity or a NaN reaches what the recurrence lets it reach: no earlier token, no other channel. First
+    derivatives only.
     """
     _check(x, gate, out_gate, form, token=False)
     B, L, C = x.shape
